@@ -1,0 +1,403 @@
+// Attention over the paged KV cache (x100_paged.h).
+//
+// o = sum_p softmax_p(scale q.K_p) V_p over the positions p <= the row's own, online: running maximum
+// m and sum l per row, O rescaled when m rises.  The query heads of a KV head are rows of one tile:
+// row i of a sequence and KV head is token i / G, head i % G (G query heads per KV head), so that a
+// K and V row is read once for all of them.
+//
+// Scores come transposed, S^T = K Q^T (a lane holds one query row and several positions), which is the
+// operand layout of O^T = V^T P^T: the weights go from the first product to the second in the
+// registers they were made in.  The cache keeps V in blocks of 8 positions per element for the same
+// reason: a lane's operand of V^T is one 16-byte load (16 bits) or one word (4 bits).
+#include <algorithm>
+
+#include "paged.h"
+#include "x100_internal.h"
+
+namespace {
+
+constexpr float NEG_INF = -__builtin_inff();
+
+struct AttnArgs {
+    x100_kv_cfg c;
+    x100_kv_batch b;
+    const uint16_t *q;
+    int64_t ldq;
+    const uint8_t *kp, *vp;
+    float scale2;        // scale * log2(e): weights are powers of two
+    uint16_t *out;
+    int64_t ldo;
+    float *part;         // [row][head][split][HD + 2]: m, l, then O (not divided by l)
+    int split, n_split;  // positions per split (a multiple of 128), splits
+};
+
+template <int T> struct Mfma16;
+template <> struct Mfma16<X100_T_F16> {
+    static X100_DEV v4f mul(v4u a, v4u b, v4f c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    }
+};
+template <> struct Mfma16<X100_T_BF16> {
+    static X100_DEV v4f mul(v4u a, v4u b, v4f c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+    }
+};
+
+// The tile's power of two 2^-e that brings a row's largest element (in size) to 1 .. 2: bf16 queries
+// become fp16 that way without loss (elements below 2^-24 of the largest aside), whatever their size.
+X100_DEV int row_exponent(float amax)
+{
+    const int e = (int)(__float_as_uint(amax) >> 23) - 127;
+    return amax > 0.0f && e < 128 ? e : 0;
+}
+
+// One block: 16 rows (token, head) of a sequence and KV head, one split of the positions; its 4 waves
+// take tiles of 32 positions in turn and merge at the end.
+// Lane (c = lane % 16, g = lane / 16): query row c; of a tile the positions 8 g .. 8 g + 7.
+template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256) void k_attn_tile(const AttnArgs a)
+{
+    constexpr int MT = Q4 ? X100_T_F16 : AT;   // type on the matrix cores
+    constexpr int KS = HD / 32, NJ = HD / 16;  // steps of K Q^T, element tiles of V^T P^T
+    __shared__ float s_o[4][16][HD + 4];
+    __shared__ float s_m[4][16], s_l[4][16];
+    const int lane = threadIdx.x & 63, w = wave_id(), c = lane & 15, g = lane >> 4;
+    const int sp = blockIdx.x % a.n_split, tile = blockIdx.x / a.n_split, kvh = blockIdx.y, s = blockIdx.z;
+    const int G = a.c.n_head / a.c.n_head_kv, page = a.c.page;
+    const PagedSeq q = paged_seq(a.b, s);
+    const int n_rows = q.q_len * G, i0 = tile * 16;
+    if (i0 >= n_rows) return;
+    const int pos0 = q.kv_len - q.q_len;                       // position of token 0
+    const int vis = pos0 + (min(i0 + 15, n_rows - 1)) / G + 1;  // positions that the tile's last row sees
+    const int ns = max(1, (vis + a.split - 1) / a.split);
+    if (sp >= ns) return;
+    const int t0 = sp * a.split, t1 = min(t0 + a.split, vis);
+
+    const int i = min(i0 + c, n_rows - 1), tok = i / G, head = kvh * G + i % G;
+    const int pos = pos0 + tok;
+    const int pos_lo = pos0 + i0 / G;                          // the tile's first row's
+
+    v4u qf[KS];
+    float sc2 = a.scale2;
+    {
+        const uint16_t *qr = a.q + (size_t)(q.q0 + tok) * a.ldq + (size_t)head * HD;
+#pragma unroll
+        for (int j = 0; j < KS; j++) qf[j] = *(const v4u *)(qr + (Q4 ? g * (HD / 4) + 8 * j : 32 * j + 8 * g));
+        if constexpr (Q4 && AT == X100_T_BF16) {
+            float mx = 0.0f;
+#pragma unroll
+            for (int j = 0; j < KS; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    mx = fmaxf(mx, fmaxf(fabsf(bf2f(qf[j][e] & 0xffffu)), fabsf(__uint_as_float(qf[j][e] & 0xffff0000u))));
+            mx = fmaxf(mx, xor16_f(mx));
+            mx = fmaxf(mx, xor32_f(mx));
+            const int ex = row_exponent(mx);
+            sc2 = ldexpf(sc2, ex);
+#pragma unroll
+            for (int j = 0; j < KS; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const v2h h = {(_Float16)ldexpf(bf2f(qf[j][e] & 0xffffu), -ex),
+                                   (_Float16)ldexpf(__uint_as_float(qf[j][e] & 0xffff0000u), -ex)};
+                    qf[j][e] = __builtin_bit_cast(uint32_t, h);
+                }
+        }
+    }
+
+    v4f o[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) o[j] = v4f{0, 0, 0, 0};
+    float m = NEG_INF, msub = 0.0f, l = 0.0f;
+    const size_t head_bytes = page_head_bytes<HD, Q4>(page);
+    const int psh = __builtin_ctz(page);
+    const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
+
+    for (int t = t0 + 32 * w; t < t1; t += 128) {
+        // pages of the two 8-position blocks this lane reads: K rows 8 (c / 4) .., V block 8 g
+        const int kb = t + 8 * (c >> 2), vb = t + 8 * g;
+        const int kpg = kb < t1 ? tab[kb >> psh] : -1, vpg = vb < t1 ? tab[vb >> psh] : -1;
+        const bool kok = kpg >= 0 && kpg < a.c.n_pages, vok = vpg >= 0 && vpg < a.c.n_pages;
+        const uint8_t *kpage = a.kp + ((size_t)(kok ? kpg : 0) * a.c.n_head_kv + kvh) * head_bytes;
+        const uint8_t *vpage = a.vp + ((size_t)(vok ? vpg : 0) * a.c.n_head_kv + kvh) * head_bytes;
+        const int koff = (kb & (page - 1)) + (c & 3), vblk = (vb & (page - 1)) >> 3;
+
+        // S^T: tile row r of half h is position 8 (r / 4) + 4 h + r % 4, so that lane (c, g) receives
+        // positions 8 g + 4 h .. + 3 of row c
+        v4f sc[2] = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}};
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if constexpr (!Q4) {
+                const uint16_t *kr = (const uint16_t *)kpage + (size_t)(koff + 4 * h) * HD;
+#pragma unroll
+                for (int j = 0; j < KS; j++) sc[h] = Mfma16<MT>::mul(*(const v4u *)(kr + 32 * j + 8 * g), qf[j], sc[h]);
+            } else {
+                const uint32_t *kr = (const uint32_t *)kpage + (size_t)(koff + 4 * h) * (HD / 8) + g * KS;
+                const uint32_t ds = ((const uint32_t *)(kpage + page * HD / 2))[(size_t)(koff + 4 * h) * (HD / 32) + g * HD / 128];
+                const _Float16 d1 = __builtin_bit_cast(_Float16, (uint16_t)ds), m1 = __builtin_bit_cast(_Float16, (uint16_t)(ds >> 16));
+                const v2h d2 = {d1, d1}, m2 = {m1, m1};
+#pragma unroll
+                for (int j = 0; j < KS; j++) {
+                    v2h n[4];
+                    q4_unpack(kr[j], n);
+                    v4u k;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) k[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n[e], d2, m2));
+                    sc[h] = Mfma16<MT>::mul(k, qf[j], sc[h]);
+                }
+            }
+        }
+        // weights
+        float x[8];
+        float mx = NEG_INF;
+        const bool whole = t + 31 <= pos_lo && __all(vok);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            x[e] = sc[e >> 2][e & 3] * sc2;
+            if (!whole && !(vok && vb + e <= pos)) x[e] = NEG_INF;
+            mx = fmaxf(mx, x[e]);
+        }
+        // The maximum may stay up to 8 (a factor of 256) behind: every sum is relative to it
+        if (__any(mx > m + 8.0f)) {
+            mx = fmaxf(mx, xor16_f(mx));
+            mx = fmaxf(mx, xor32_f(mx));
+            const float mn = fmaxf(m, mx);
+            const float f = __builtin_amdgcn_exp2f(mn == NEG_INF ? 0.0f : m - mn);
+            m = mn;
+            msub = mn == NEG_INF ? 0.0f : mn;
+            l *= f;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) o[j] *= f;
+        }
+        v4u p;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float p0 = __builtin_amdgcn_exp2f(x[2 * e] - msub), p1 = __builtin_amdgcn_exp2f(x[2 * e + 1] - msub);
+            l += p0 + p1;
+            p[e] = f2act<MT>(p0) | f2act<MT>(p1) << 16;
+        }
+        // positions that no row of the sequence has, and those of a page that is none: V as zeros
+        uint32_t keep[4];
+        {
+            const int n = vok ? q.kv_len - vb : 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) keep[e] = n >= 2 * e + 2 ? ~0u : (n == 2 * e + 1 ? 0xffffu : 0u);
+        }
+        // O^T += V^T P^T
+        v4u vf[NJ];
+        if constexpr (!Q4) {
+            const uint16_t *vr = (const uint16_t *)vpage + (size_t)vblk * HD * 8;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) vf[j] = *(const v4u *)(vr + (16 * j + c) * 8);
+        } else {
+            const uint32_t *vr = (const uint32_t *)vpage + (size_t)vblk * HD;
+            const uint8_t *vs = vpage + page * HD / 2 + (size_t)vblk * (HD / 32) * 32;
+#pragma unroll
+            for (int u = 0; u < HD / 64; u++) {   // elements 64 u + 4 c .. + 3, of group 2 u + c / 8
+                const v4u wd = *(const v4u *)(vr + 64 * u + 4 * c);
+                v4u d = *(const v4u *)(vs + (2 * u + (c >> 3)) * 32), mm = *(const v4u *)(vs + (2 * u + (c >> 3)) * 32 + 16);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    d[e] &= keep[e];
+                    mm[e] &= keep[e];
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    v2h n[4];
+                    q4_unpack(wd[k], n);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        vf[4 * u + k][e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n[e], as_h2(d[e]), as_h2(mm[e])));
+                }
+            }
+        }
+        if constexpr (!Q4)
+            if (!whole)
+#pragma unroll
+                for (int j = 0; j < NJ; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) vf[j][e] &= keep[e];
+        // An element that is not finite, in a position that only some of the tile's rows see, must not
+        // meet the others' zero weights: such elements are taken out, and added as infinities (both
+        // signs: a NaN) to the rows that see them.
+        bool odd = false;
+        if (!whole) {
+            constexpr uint32_t EXP = MT == X100_T_F16 ? 0x7c00u : 0x7f80u;
+            uint32_t any = 0;
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    any |= (uint32_t)((vf[j][e] & EXP) == EXP) | (uint32_t)((vf[j][e] & (EXP << 16)) == EXP << 16);
+            odd = __any(any);
+            if (odd) {
+                constexpr uint32_t ONE = MT == X100_T_F16 ? 0x3c00u : 0x3f80u;
+                v4u see;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    see[e] = (vok && vb + 2 * e <= pos ? ONE : 0u) | (vok && vb + 2 * e + 1 <= pos ? ONE << 16 : 0u);
+#pragma unroll
+                for (int j = 0; j < NJ; j++) {
+                    v4u up, dn;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        uint32_t u = 0, dd = 0, fine = vf[j][e];
+#pragma unroll
+                        for (int b = 0; b < 32; b += 16) {
+                            const uint32_t v = vf[j][e] >> b & 0xffffu, ex = v & EXP;
+                            if (ex == EXP) {
+                                const bool nan = (v & 0x7fffu) != EXP;
+                                if (nan || !(v & 0x8000u)) u |= ONE << b;
+                                if (nan || (v & 0x8000u)) dd |= ONE << b;
+                                fine &= ~(0xffffu << b);
+                            }
+                        }
+                        up[e] = u;
+                        dn[e] = dd;
+                        vf[j][e] = fine;
+                    }
+                    const v4f z = {0, 0, 0, 0};
+                    const v4f nu = Mfma16<MT>::mul(up, see, z), nd = Mfma16<MT>::mul(dn, see, z);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if (nu[e] > 0.0f) o[j][e] += __builtin_inff();
+                        if (nd[e] > 0.0f) o[j][e] -= __builtin_inff();
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; j++) o[j] = Mfma16<MT>::mul(vf[j], p, o[j]);
+    }
+
+    // the 4 lane groups hold parts of l; then the 4 waves' m, l, O are merged
+    l += xor16_f(l);
+    l += xor32_f(l);
+    if (g == 0) {
+        s_m[w][c] = m;
+        s_l[w][c] = l;
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int el = Q4 ? 4 * (4 * g + e) + (j & 3) + 64 * (j >> 2) : 16 * j + 4 * g + e;
+            s_o[w][c][el] = o[j][e];
+        }
+    __syncthreads();
+    for (int u = threadIdx.x; u < 16 * (HD / 2); u += 256) {
+        const int r = u / (HD / 2), el = u % (HD / 2) * 2;
+        if (i0 + r >= n_rows) continue;
+        float mm = NEG_INF;
+#pragma unroll
+        for (int k = 0; k < 4; k++) mm = fmaxf(mm, s_m[k][r]);
+        const float ms = mm == NEG_INF ? 0.0f : mm;
+        float ls = 0.0f, y0 = 0.0f, y1 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float f = __builtin_amdgcn_exp2f(s_m[k][r] - ms);
+            if (s_m[k][r] == NEG_INF) continue;
+            ls = __builtin_fmaf(s_l[k][r], f, ls);
+            y0 = __builtin_fmaf(s_o[k][r][el], f, y0);
+            y1 = __builtin_fmaf(s_o[k][r][el + 1], f, y1);
+        }
+        const int tk = (i0 + r) / G, hh = kvh * G + (i0 + r) % G;
+        if (ns == 1) {
+            const float f = ls == 0.0f ? 0.0f : 1.0f / ls;
+            const uint32_t b = ls == 0.0f ? 0u : f2act<AT>(y0 * f) | f2act<AT>(y1 * f) << 16;
+            *(uint32_t *)(a.out + (size_t)(q.q0 + tk) * a.ldo + (size_t)hh * HD + el) = b;
+        } else {
+            float *p = a.part + (((size_t)(q.q0 + tk) * a.c.n_head + hh) * a.n_split + sp) * (HD + 2);
+            p[2 + el] = y0;
+            p[3 + el] = y1;
+            if (el == 0) {
+                p[0] = mm;
+                p[1] = ls;
+            }
+        }
+    }
+}
+
+// Merges the splits of rows that have more than one: a wave per (row, head), HD / 64 elements per lane.
+template <int HD, int AT> __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a)
+{
+    const int lane = threadIdx.x & 63, head = blockIdx.y * 4 + wave_id(), row = blockIdx.x;
+    if (head >= a.c.n_head) return;
+    const int s = paged_find(a.b, row);
+    if (s >= a.b.n_seq) return;
+    const PagedSeq q = paged_seq(a.b, s);
+    if (q.q_len <= 0 || row < q.q0) return;
+    const int G = a.c.n_head / a.c.n_head_kv, n_rows = q.q_len * G;
+    const int i = (row - q.q0) * G + head % G;
+    const int vis = q.kv_len - q.q_len + min(i / 16 * 16 + 15, n_rows - 1) / G + 1;
+    const int ns = (vis + a.split - 1) / a.split;
+    if (ns <= 1) return;
+    const float *p = a.part + ((size_t)row * a.c.n_head + head) * a.n_split * (HD + 2);
+    float m = NEG_INF;
+    for (int k = 0; k < ns; k++) m = fmaxf(m, p[(size_t)k * (HD + 2)]);
+    const float ms = m == NEG_INF ? 0.0f : m;
+    float l = 0.0f, y[HD / 64] = {};
+    for (int k = 0; k < ns; k++) {
+        const float *pk = p + (size_t)k * (HD + 2);
+        if (pk[0] == NEG_INF) continue;
+        const float f = __builtin_amdgcn_exp2f(pk[0] - ms);
+        l = __builtin_fmaf(pk[1], f, l);
+#pragma unroll
+        for (int e = 0; e < HD / 64; e++) y[e] = __builtin_fmaf(pk[2 + lane * (HD / 64) + e], f, y[e]);
+    }
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t *o = a.out + (size_t)row * a.ldo + (size_t)head * HD + lane * (HD / 64);
+#pragma unroll
+    for (int e = 0; e < HD / 64; e++) o[e] = l == 0.0f ? 0 : (uint16_t)f2act<AT>(y[e] * f);
+}
+
+struct Plan {
+    int tiles, split, n_split;
+};
+
+// Positions per split: as many splits as give the chip four blocks per CU, of 256 positions or more.
+Plan plan_of(const x100_kv_cfg &c, const x100_kv_batch &b)
+{
+    Plan p;
+    const int G = c.n_head / c.n_head_kv;
+    p.tiles = (int)(((int64_t)b.max_q * G + 15) / 16);
+    const int64_t base = std::max<int64_t>(1, std::min<int64_t>((int64_t)p.tiles * b.n_seq, (int64_t)b.n_rows * G)) * c.n_head_kv;
+    const int64_t want = std::max<int64_t>(1, 1024 / base);
+    int64_t split = (b.max_kv + want - 1) / want;
+    split = std::max<int64_t>(256, (split + 127) / 128 * 128);
+    p.split = (int)std::min<int64_t>(split, ((int64_t)b.max_kv + 127) / 128 * 128);
+    p.n_split = (int)(((int64_t)b.max_kv + p.split - 1) / p.split);
+    return p;
+}
+
+template <int HD, int AT> hipError_t attn_as(const AttnArgs &a, const Plan &p, hipStream_t s)
+{
+    const dim3 grid((unsigned)(p.tiles * p.n_split), a.c.n_head_kv, a.b.n_seq);
+    if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true><<<grid, 256, 0, s>>>(a);
+    else k_attn_tile<HD, AT, false><<<grid, 256, 0, s>>>(a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.n_split == 1) return e;
+    k_attn_join<HD, AT><<<dim3(a.b.n_rows, (a.c.n_head + 3) / 4), 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+size_t x100_attn_paged_workspace(const x100_kv_cfg &c, const x100_kv_batch &b)
+{
+    const Plan p = plan_of(c, b);
+    return p.n_split == 1 ? 0 : (size_t)b.n_rows * c.n_head * p.n_split * (c.head_dim + 2) * sizeof(float);
+}
+
+hipError_t x100_attn_paged_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const void *q, int64_t ldq,
+                                  const void *kp, const void *vp, float scale, void *out, int64_t ldo, void *ws,
+                                  hipStream_t s)
+{
+    const Plan p = plan_of(c, b);
+    const AttnArgs a = {c, b, (const uint16_t *)q, ldq, (const uint8_t *)kp, (const uint8_t *)vp,
+                        scale * 1.4426950408889634f, (uint16_t *)out, ldo, (float *)ws, p.split, p.n_split};
+    if (c.head_dim == 64)
+        return c.act_type == X100_T_F16 ? attn_as<64, X100_T_F16>(a, p, s) : attn_as<64, X100_T_BF16>(a, p, s);
+    return c.act_type == X100_T_F16 ? attn_as<128, X100_T_F16>(a, p, s) : attn_as<128, X100_T_BF16>(a, p, s);
+}

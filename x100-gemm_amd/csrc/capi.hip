@@ -1,8 +1,10 @@
 // C-ABI of libx100hip: argument checking, device state and the host-pointer convenience paths.
-// The kernels live in gemm_i8.hip, gemv_tile.hip, qgemv.hip and moe.hip.
+// The kernels live in gemm_i8.hip, gemv_tile.hip, qgemv.hip, moe.hip, attn.hip, rows.hip, paged.hip and
+// attn_paged.hip.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <condition_variable>
 #include <mutex>
 #include <thread>
@@ -18,7 +20,9 @@
 #include "x100_gemv_tile.h"
 #include "x100_gguf.h"
 #include "x100_moe.h"
+#include "x100_paged.h"
 #include "x100_qgemv.h"
+#include "x100_rows.h"
 #pragma GCC visibility pop
 #include "x100_internal.h"
 
@@ -781,6 +785,207 @@ int x100_decode_layer_hip(const x100_layer_cfg *c, const x100_layer_weights *w, 
     void *ws = nullptr;
     if ((rc = stream_workspace((hipStream_t)stream, x100_decode_workspace_bytes(c), &ws))) return rc;
     return decode_layer(c, w, pos, h, sel, sw, ws, stream);
+}
+
+// ---------------------------------------------------------------------------------------------
+// int8 rows
+// ---------------------------------------------------------------------------------------------
+static int type_bytes(int type)
+{
+    switch (type) {
+    case X100_T_F32: case X100_T_I32: return 4;
+    case X100_T_F16: case X100_T_BF16: return 2;
+    }
+    return 0;
+}
+
+// A row tensor of width d: a known type, aligned to its elements, rows that do not overlap, scales
+// with int32 and only there.
+static bool rows_ok(const x100_rows *r, int d)
+{
+    const int e = r ? type_bytes(r->type) : 0;
+    if (!e || !r->p || (uintptr_t)r->p % e || r->ld < d || r->ld > ((int64_t)1 << 40)) return false;
+    const bool i32 = r->type == X100_T_I32;
+    return i32 == (r->row_scale != nullptr) && i32 == (r->col_scale != nullptr);
+}
+
+static bool i8_out_ok(int n_rows, int d, const int8_t *q, const float *scale)
+{
+    return n_rows >= 0 && n_rows < 1 << 24 && d >= 1 && d <= X100_ROWS_MAX_D && q && scale && !((uintptr_t)scale & 3);
+}
+
+int x100_quant_i8_hip(int n_rows, int d, const x100_rows *x, int8_t *q, float *scale, void *stream)
+{
+    if (!i8_out_ok(n_rows, d, q, scale) || !rows_ok(x, d)) return X100_EINVAL;
+    if (n_rows == 0) return X100_OK;
+    int rc = check_device();
+    if (rc) return rc;
+    hipError_t e = x100_quant_i8_launch(n_rows, d, x, q, scale, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e);
+    return X100_OK;
+}
+
+int x100_add_rmsnorm_i8_hip(int n_rows, int d, const x100_rows *x, const x100_rows *delta, const float *weight,
+                            float eps, void *h, int64_t ldh, int8_t *q, float *scale, void *stream)
+{
+    if (!i8_out_ok(n_rows, d, q, scale) || !rows_ok(x, d) || x->type == X100_T_I32) return X100_EINVAL;
+    if (!weight || ((uintptr_t)weight & 3) || !(eps >= 0.0f) || std::isinf(eps)) return X100_EINVAL;
+    if (delta && (!rows_ok(delta, d) || !h || (uintptr_t)h % type_bytes(x->type) || ldh < d ||
+                  ldh > ((int64_t)1 << 40)))
+        return X100_EINVAL;
+    if (delta && h == x->p && ldh != x->ld) return X100_EINVAL;   // in place: the rows as they lie
+    if (n_rows == 0) return X100_OK;
+    int rc = check_device();
+    if (rc) return rc;
+    hipError_t e = x100_add_rmsnorm_i8_launch(n_rows, d, x, delta, weight, eps, h, ldh, q, scale, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e);
+    return X100_OK;
+}
+
+// ---------------------------------------------------------------------------------------------
+// paged KV cache
+// ---------------------------------------------------------------------------------------------
+static bool kv_cfg_ok(const x100_kv_cfg *c)
+{
+    if (!c || c->n_head < 1 || c->n_head > 1024 || c->n_head_kv < 1 || c->n_head % c->n_head_kv ||
+        c->n_head / c->n_head_kv > 16)
+        return false;
+    if (c->head_dim != 64 && c->head_dim != 128) return false;
+    if (c->page < 16 || c->page > 256 || (c->page & (c->page - 1)) || c->n_pages < 1) return false;
+    if (c->act_type != X100_T_F16 && c->act_type != X100_T_BF16) return false;
+    return c->kv_type == c->act_type || c->kv_type == X100_KV_Q4;
+}
+
+static size_t pool_bytes(const x100_kv_cfg *c)
+{
+    const size_t head = (size_t)c->page * c->head_dim * (c->kv_type == X100_KV_Q4 ? 5 : 16) / 8;
+    return (size_t)c->n_pages * c->n_head_kv * head;
+}
+
+// Bounds of the batch, without its arrays (the workspace's size needs no more).
+static bool kv_bounds_ok(const x100_kv_cfg *c, const x100_kv_batch *b)
+{
+    if (!b || b->n_seq < 0 || b->n_seq > 65535 || b->n_rows < 0 || b->n_rows >= 1 << 24) return false;
+    if (b->max_q < 1 || b->max_q > 1 << 20 || b->max_kv < 1 || b->max_kv > 1 << 26 || b->table_ld < 1) return false;
+    return (int64_t)b->table_ld * c->page >= b->max_kv;
+}
+
+static bool kv_batch_ok(const x100_kv_cfg *c, const x100_kv_batch *b)
+{
+    if (!kv_bounds_ok(c, b)) return false;
+    if (b->n_seq == 0 || b->n_rows == 0) return true;   // nothing to do
+    if (!b->q_start || !b->kv_len || !b->block_table) return false;
+    return !(((uintptr_t)b->q_start | (uintptr_t)b->kv_len | (uintptr_t)b->block_table) & 3);
+}
+
+static bool pools_ok(const void *kp, const void *vp)
+{
+    return kp && vp && kp != vp && !(((uintptr_t)kp | (uintptr_t)vp) & 255);
+}
+
+size_t x100_kv_pool_bytes(const x100_kv_cfg *c) { return kv_cfg_ok(c) ? pool_bytes(c) : 0; }
+
+int x100_rope_table_hip(int head_dim, int n_pos, float base, float *table, void *stream)
+{
+    if ((head_dim != 64 && head_dim != 128) || n_pos < 0 || n_pos > 1 << 25 || !(base > 0.0f) || std::isinf(base) ||
+        !table || ((uintptr_t)table & 15))
+        return X100_EINVAL;
+    if (n_pos == 0) return X100_OK;
+    int rc = check_device();
+    if (rc) return rc;
+    hipError_t e = x100_rope_table_launch(head_dim, n_pos, base, table, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e);
+    return X100_OK;
+}
+
+// q, k or v of the append: as rows_ok, and in 16-byte pieces.
+static bool proj_ok(const x100_rows *r, int width, int type)
+{
+    return rows_ok(r, width) && r->type == type && !((uintptr_t)r->p & 15) && r->ld * type_bytes(type) % 16 == 0;
+}
+
+int x100_kv_append_hip(const x100_kv_cfg *c, const x100_kv_batch *b, const x100_kv_rows *r, void *k_pool, void *v_pool,
+                       void *q_out, void *stream)
+{
+    if (!kv_cfg_ok(c) || !kv_batch_ok(c, b) || !r || !pools_ok(k_pool, v_pool)) return X100_EINVAL;
+    const int wq = c->n_head * c->head_dim, wk = c->n_head_kv * c->head_dim;
+    if (!proj_ok(&r->k, wk, r->k.type) || !proj_ok(&r->v, wk, r->k.type)) return X100_EINVAL;
+    if ((r->q.p != nullptr) != (q_out != nullptr)) return X100_EINVAL;
+    if (q_out && (!proj_ok(&r->q, wq, r->k.type) || ((uintptr_t)q_out & 15))) return X100_EINVAL;
+    if ((r->q_norm || r->k_norm) && (!(r->eps >= 0.0f) || std::isinf(r->eps))) return X100_EINVAL;
+    if (((uintptr_t)r->q_norm | (uintptr_t)r->k_norm) & 3) return X100_EINVAL;
+    if (r->rope && (((uintptr_t)r->rope & 15) || r->rope_len < b->max_kv)) return X100_EINVAL;
+    if (b->n_seq == 0 || b->n_rows == 0) return X100_OK;
+    int rc = check_device();
+    if (rc) return rc;
+    hipError_t e = x100_kv_append_launch(*c, *b, *r, k_pool, v_pool, q_out, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e);
+    return X100_OK;
+}
+
+int x100_kv_read_hip(const x100_kv_cfg *c, const x100_kv_batch *b, const void *k_pool, const void *v_pool, void *k_out,
+                     void *v_out, void *stream)
+{
+    if (!kv_cfg_ok(c) || !kv_batch_ok(c, b) || !pools_ok(k_pool, v_pool) || !k_out || !v_out) return X100_EINVAL;
+    if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) return X100_EINVAL;
+    if (b->n_seq == 0 || b->n_rows == 0) return X100_OK;
+    int rc = check_device();
+    if (rc) return rc;
+    hipError_t e = x100_kv_read_launch(*c, *b, k_pool, v_pool, k_out, v_out, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e);
+    return X100_OK;
+}
+
+size_t x100_attn_paged_workspace_bytes(const x100_kv_cfg *c, const x100_kv_batch *b)
+{
+    if (!kv_cfg_ok(c) || !kv_bounds_ok(c, b) || b->n_seq == 0 || b->n_rows == 0) return 0;
+    return al256(x100_attn_paged_workspace(*c, *b));
+}
+
+static int check_attn_paged(const x100_kv_cfg *c, const x100_kv_batch *b, const void *q, int64_t ldq, const void *kp,
+                            const void *vp, float scale, const void *out, int64_t ldo)
+{
+    if (!kv_cfg_ok(c) || !kv_batch_ok(c, b) || !pools_ok(kp, vp)) return X100_EINVAL;
+    const int64_t width = (int64_t)c->n_head * c->head_dim, most = (int64_t)1 << 40;
+    if (!q || !out || (((uintptr_t)q | (uintptr_t)out) & 15) || ldq < width || ldo < width || ldq > most || ldo > most ||
+        ldq % 8 || ldo % 8)
+        return X100_EINVAL;
+    if (!(scale > 0.0f) || std::isinf(scale)) return X100_EINVAL;
+    return X100_OK;
+}
+
+static int attn_paged(const x100_kv_cfg *c, const x100_kv_batch *b, const void *q, int64_t ldq, const void *kp,
+                      const void *vp, float scale, void *out, int64_t ldo, void *ws, void *stream)
+{
+    hipError_t e = x100_attn_paged_launch(*c, *b, q, ldq, kp, vp, scale, out, ldo, ws, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e);
+    return X100_OK;
+}
+
+int x100_attn_paged_hip_ws(const x100_kv_cfg *c, const x100_kv_batch *b, const void *q, int64_t ldq, const void *k_pool,
+                           const void *v_pool, float scale, void *out, int64_t ldo, void *ws, size_t ws_bytes,
+                           void *stream)
+{
+    int rc = check_attn_paged(c, b, q, ldq, k_pool, v_pool, scale, out, ldo);
+    if (rc) return rc;
+    const size_t need = x100_attn_paged_workspace_bytes(c, b);
+    if (need && (!ws || ((uintptr_t)ws & 255) || ws_bytes < need)) return X100_EINVAL;
+    if (b->n_seq == 0 || b->n_rows == 0) return X100_OK;
+    if ((rc = check_device())) return rc;
+    return attn_paged(c, b, q, ldq, k_pool, v_pool, scale, out, ldo, ws, stream);
+}
+
+int x100_attn_paged_hip(const x100_kv_cfg *c, const x100_kv_batch *b, const void *q, int64_t ldq, const void *k_pool,
+                        const void *v_pool, float scale, void *out, int64_t ldo, void *stream)
+{
+    int rc = check_attn_paged(c, b, q, ldq, k_pool, v_pool, scale, out, ldo);
+    if (rc) return rc;
+    if (b->n_seq == 0 || b->n_rows == 0) return X100_OK;
+    if ((rc = check_device())) return rc;
+    const size_t need = x100_attn_paged_workspace_bytes(c, b);
+    void *ws = nullptr;
+    if (need && (rc = stream_workspace((hipStream_t)stream, need, &ws))) return rc;
+    return attn_paged(c, b, q, ldq, k_pool, v_pool, scale, out, ldo, ws, stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,86 @@
+// The paged KV cache (x100_paged.h) as its kernels see it: the batch, pages and the 4-bit format.
+#pragma once
+#include "rows_load.h"
+#include "x100_paged.h"
+
+struct PagedSeq {
+    int q0, q_len, kv_len;   // first row, rows, cached positions (q_len < 0: the sequence is refused)
+};
+
+// Sequence s of the batch, every entry checked against the host's bounds (x100_paged.h).
+X100_DEV PagedSeq paged_seq(const x100_kv_batch &b, int s)
+{
+    const int q0 = b.q_start[s], q1 = b.q_start[s + 1], kv = b.kv_len[s];
+    const bool ok = q0 >= 0 && q1 >= q0 && q1 <= b.n_rows && q1 - q0 <= b.max_q && kv >= 0 && kv <= b.max_kv;
+    return {q0, ok ? q1 - q0 : -1, kv};
+}
+
+// Page of position p (0 <= p < max_kv) of sequence s, or -1 outside 0 .. n_pages - 1.
+X100_DEV int paged_page(const x100_kv_cfg &c, const x100_kv_batch &b, int s, int p)
+{
+    const int g = b.block_table[(size_t)s * b.table_ld + (p >> __builtin_ctz(c.page))];
+    return g >= 0 && g < c.n_pages ? g : -1;
+}
+
+// The sequence of row r: the first s with q_start[s + 1] > r (n_seq if there is none), by the whole
+// wave, 64 entries per step.
+X100_DEV int paged_find(const x100_kv_batch &b, int r)
+{
+    const int lane = threadIdx.x & 63;
+    int lo = 0, len = b.n_seq;
+    while (len > 0) {
+        const int stride = (len + 63) / 64;              // entries lo + (i + 1) * stride - 1
+        const int i = (lane + 1) * stride - 1;
+        const bool le = i < len && b.q_start[lo + i + 1] <= r;
+        const int n = __popcll(__ballot(le)) * stride;   // entries known to lie at or below r
+        if (stride == 1) return lo + n;
+        lo += n;
+        len = min(stride - 1, len - n);                  // the next entry probed lies above r
+    }
+    return lo;
+}
+
+// Bytes of one head's part of a page, K or V.
+template <int HD, bool Q4> X100_DEV constexpr int page_head_bytes(int page) { return Q4 ? page * HD * 5 / 8 : page * HD * 2; }
+
+// 4-bit codes: number e of 8 at bit 16 (e % 2) + 4 (e / 2) of the word.
+X100_DEV constexpr int q4_shift(int e) { return 16 * (e & 1) + 4 * (e >> 1); }
+
+// d, m of a group from its smallest and largest value (fp16 bits; d = m = NaN where either is not
+// finite) and 1 / d.
+struct Q4Scale {
+    uint16_t d, m;
+    float inv, mf;
+    bool bad;
+};
+X100_DEV Q4Scale q4_scale(float lo, float hi, bool bad)
+{
+    const _Float16 d = (_Float16)((hi - lo) / 15.0f), m = (_Float16)lo;
+    const float df = (float)d, mf = (float)m;
+    bad |= !(fabsf(df) <= 65504.0f) || !(fabsf(mf) <= 65504.0f);
+    Q4Scale s;
+    s.d = bad ? 0x7e00 : __builtin_bit_cast(uint16_t, d);
+    s.m = bad ? 0x7e00 : __builtin_bit_cast(uint16_t, m);
+    s.inv = !bad && df > 0.0f ? 1.0f / df : 0.0f;
+    s.mf = mf;
+    s.bad = bad;
+    return s;
+}
+X100_DEV uint32_t q4_code(const Q4Scale &s, float x)
+{
+    const float n = rintf((x - s.mf) * s.inv);
+    return s.bad ? 0u : (uint32_t)fminf(fmaxf(n, 0.0f), 15.0f);
+}
+
+// The 8 numbers of a word as fp16 codes 0 .. 15, pairs (0,1), (2,3), (4,5), (6,7): a code under the
+// exponent of 1024 reads as 1024 + n (low nibble of a byte) or 1024 + 16 n (high), both exact.
+X100_DEV void q4_unpack(uint32_t w, v2h (&n)[4])
+{
+    const v2h k1024 = {(_Float16)1024.0f, (_Float16)1024.0f};
+    const v2h k16 = {(_Float16)0.0625f, (_Float16)0.0625f}, k64 = {(_Float16)-64.0f, (_Float16)-64.0f};
+    const uint32_t w8 = w >> 8;
+    n[0] = __builtin_bit_cast(v2h, (w & 0x000f000fu) | 0x64006400u) - k1024;
+    n[1] = __builtin_elementwise_fma(__builtin_bit_cast(v2h, (w & 0x00f000f0u) | 0x64006400u), k16, k64);
+    n[2] = __builtin_bit_cast(v2h, (w8 & 0x000f000fu) | 0x64006400u) - k1024;
+    n[3] = __builtin_elementwise_fma(__builtin_bit_cast(v2h, (w8 & 0x00f000f0u) | 0x64006400u), k16, k64);
+}

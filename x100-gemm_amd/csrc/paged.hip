@@ -1,0 +1,362 @@
+// Paged KV cache (x100_paged.h): new rows into the pages (head norms, rotation, 16 or 4 bits), cached
+// rows back out, and the rotation table.
+//
+// Bound by HBM for prompts (a row is read once, its queries, keys and values written once) and by
+// launch and dependent loads (q_start -> kv_len -> block_table) for single tokens.
+#include "paged.h"
+#include "x100_internal.h"
+
+namespace {
+
+// ---- rotation table ------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void k_rope_table(int half, int n_pos, double base, float2 *__restrict__ t)
+{
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (size_t)n_pos * half) return;
+    const int p = (int)(i / half), k = (int)(i % half);
+    double sn, cs;
+    sincos((double)p * pow(base, -(double)k / half), &sn, &cs);
+    t[i] = make_float2((float)cs, (float)sn);
+}
+
+// Exchanges among the 16 lanes of an item: xor 1, 2 within a quad, half-row mirror (the other quad
+// of 8 lanes), rotation by 8 (the other 8 lanes).
+X100_DEV float sum16(float v)
+{
+    v += dpp_f<0xB1>(0.0f, v);
+    v += dpp_f<0x4E>(0.0f, v);
+    v += dpp_f<0x141>(0.0f, v);
+    v += dpp_f<0x128>(0.0f, v);
+    return v;
+}
+// min / max over the lanes of a group of 32 elements: 4 lanes of 8 (head_dim 128), 8 of 4 (64)
+template <int HD> X100_DEV float gmin(float v)
+{
+    v = fminf(v, dpp_f<0xB1>(v, v));
+    v = fminf(v, dpp_f<0x4E>(v, v));
+    if constexpr (HD == 64) v = fminf(v, dpp_f<0x141>(v, v));
+    return v;
+}
+
+struct AppendArgs {
+    x100_kv_cfg c;
+    x100_kv_batch b;
+    x100_kv_rows r;
+    uint8_t *kp, *vp;
+    uint16_t *q_out;
+};
+
+// Block: 8 consecutive rows.  blockIdx.y < n_qk: two of the query and key heads (16 lanes per row and
+// head, 8 or 4 elements each: the pair (i, i + HD/2) of the rotation is 8 lanes away); above: one KV
+// head's values, a thread per element of the head, 8 positions of one page at a time (a 16-byte
+// store of 8 positions, or the word that holds their codes).
+template <int HD, int ST, int AT, bool Q4> __global__ __launch_bounds__(256) void k_append(const AppendArgs a)
+{
+    constexpr int E = HD / 16;
+    const int lane = threadIdx.x & 63, w = wave_id();
+    const int n_h = a.c.n_head, n_kv = a.c.n_head_kv, page = a.c.page;
+    const int n_qk = (n_h + n_kv + 1) / 2;
+    const int row0 = blockIdx.x * 8;
+    if ((int)blockIdx.y < n_qk) {
+        const int head = 2 * blockIdx.y + (w >> 1), rbase = row0 + 4 * (w & 1);
+        if (head >= n_h + n_kv || rbase >= a.b.n_rows) return;
+        const int l = lane & 15, sub = lane >> 4;
+        const int row = min(rbase + sub, a.b.n_rows - 1);
+        const bool is_q = head < n_h;
+        if (is_q && !a.q_out) return;
+        const x100_rows &src = is_q ? a.r.q : a.r.k;
+        const int col = (is_q ? head : head - n_h) * HD + E * l;
+        float v[E];
+        row_elems<ST, E>(src.p, (size_t)row * src.ld + col, v);
+        if constexpr (ST == X100_T_I32) {
+            const float rs = src.row_scale[row];
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] = v[e] * rs * src.col_scale[col + e];
+        }
+        int pos = -1, s = 0;
+        bool mine = false;
+        for (int i = 0; i < 4; i++) {
+            const int r = rbase + i;
+            const int f = r < a.b.n_rows ? paged_find(a.b, r) : a.b.n_seq;
+            if (i == sub && f < a.b.n_seq) {
+                const PagedSeq q = paged_seq(a.b, f);
+                if (q.q_len > 0 && r >= q.q0) {
+                    mine = true;
+                    s = f;
+                    pos = q.kv_len - q.q_len + r - q.q0;
+                }
+            }
+        }
+        const float *nw = is_q ? a.r.q_norm : a.r.k_norm;
+        if (nw) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; e++) ss = __builtin_fmaf(v[e], v[e], ss);
+            const float sc = 1.0f / sqrtf(sum16(ss) / (float)HD + a.r.eps);
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] = v[e] * sc * nw[E * l + e];
+        }
+        if (a.r.rope) {
+            const float2 *t = (const float2 *)a.r.rope + (size_t)max(pos, 0) * (HD / 2) + E * (l & 7);
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const float2 cs = t[e];
+                const float o = dpp_f<0x128>(0.0f, v[e]);   // the pair's other element
+                v[e] = l < 8 ? v[e] * cs.x - o * cs.y : o * cs.y + v[e] * cs.x;
+            }
+        }
+        if (is_q) {
+            if (pos < 0) {   // a row before position 0: zeros
+#pragma unroll
+                for (int e = 0; e < E; e++) v[e] = 0.0f;
+            }
+            if (!mine) return;
+            uint32_t u[E / 2];
+#pragma unroll
+            for (int e = 0; e < E / 2; e++) u[e] = f2act<AT>(v[2 * e]) | f2act<AT>(v[2 * e + 1]) << 16;
+            uint16_t *o = a.q_out + ((size_t)row * n_h + head) * HD + E * l;
+            if constexpr (E == 8) *(v4u *)o = v4u{u[0], u[1], u[2], u[3]};
+            else *(v2u *)o = v2u{u[0], u[1]};
+            return;
+        }
+        const int pg = mine && pos >= 0 ? paged_page(a.c, a.b, s, pos) : -1;
+        const int off = pos & (page - 1), kvh = head - n_h;
+        uint8_t *base = a.kp + ((size_t)max(pg, 0) * n_kv + kvh) * page_head_bytes<HD, Q4>(page);
+        if constexpr (!Q4) {
+            if (pg < 0) return;
+            uint32_t u[E / 2];
+#pragma unroll
+            for (int e = 0; e < E / 2; e++) u[e] = f2act<AT>(v[2 * e]) | f2act<AT>(v[2 * e + 1]) << 16;
+            uint16_t *o = (uint16_t *)base + (size_t)off * HD + E * l;
+            if constexpr (E == 8) *(v4u *)o = v4u{u[0], u[1], u[2], u[3]};
+            else *(v2u *)o = v2u{u[0], u[1]};
+        } else {
+            float lo = v[0], hi = v[0], fin = 1.0f;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                lo = fminf(lo, v[e]);
+                hi = fmaxf(hi, v[e]);
+                if (!(fabsf(v[e]) <= 3.402823466e38f)) fin = 0.0f;
+            }
+            const Q4Scale sc = q4_scale(gmin<HD>(lo), -gmin<HD>(-hi), gmin<HD>(fin) == 0.0f);
+            uint32_t word = 0;
+#pragma unroll
+            for (int e = 0; e < E; e++) word |= q4_code(sc, v[e]) << q4_shift(e);
+            uint32_t *cw = (uint32_t *)base + (size_t)off * (HD / 8);
+            if constexpr (E == 4) {   // two lanes of 4 elements share a word: elements 4 .. 7 sit 8 bits higher
+                if (l & 1) word <<= 8;
+                word |= (uint32_t)dpp_i<0xB1>(0, (int)word);
+            }
+            if (pg < 0) return;
+            if (E == 8) cw[l] = word;
+            else if (!(l & 1)) cw[l >> 1] = word;
+            constexpr int LG = 32 / E;   // lanes of a group
+            if (l % LG == 0)
+                ((uint32_t *)(base + page * HD / 2))[(size_t)off * (HD / 32) + l / LG] = sc.d | (uint32_t)sc.m << 16;
+        }
+        return;
+    }
+    // values
+    const int kvh = blockIdx.y - n_qk;
+    constexpr int WH = HD / 64;                 // waves of a head
+    const int el = (w % WH) * 64 + lane;        // element of the head
+    const x100_rows &src = a.r.v;
+    const int col = kvh * HD + el;
+    for (int i = w / WH; i < 8; i += 4 / WH) {
+        const int row = row0 + i;
+        if (row >= a.b.n_rows) return;
+        const int s = paged_find(a.b, row);
+        if (s >= a.b.n_seq) return;
+        const PagedSeq q = paged_seq(a.b, s);
+        if (q.q_len <= 0 || row < q.q0) continue;
+        const int pos = q.kv_len - q.q_len + row - q.q0;
+        // the row that begins a block of 8 positions, or the sequence's first row, stores the block's rows
+        if (pos < 0 || !(row == q.q0 || pos == 0 || (pos & 7) == 0)) continue;
+        const int n = min(8 - (pos & 7), q.q0 + q.q_len - row);
+        const int pg = paged_page(a.c, a.b, s, pos);
+        if (pg < 0) continue;
+        const int o0 = pos & 7, blk = (pos & (page - 1)) >> 3;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            v[k] = 0.0f;
+            if (k < n) {
+                v[k] = row_elem<ST>(src.p, (size_t)(row + k) * src.ld + col);
+                if constexpr (ST == X100_T_I32) v[k] = v[k] * src.row_scale[row + k] * src.col_scale[col];
+            }
+        }
+        uint8_t *base = a.vp + ((size_t)pg * n_kv + kvh) * page_head_bytes<HD, Q4>(page);
+        if constexpr (!Q4) {
+            uint16_t *o = (uint16_t *)base + ((size_t)blk * HD + el) * 8;
+            if (n == 8) {
+                uint32_t u[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) u[k] = f2act<AT>(v[2 * k]) | f2act<AT>(v[2 * k + 1]) << 16;
+                *(v4u *)o = v4u{u[0], u[1], u[2], u[3]};
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (k < n) o[o0 + k] = (uint16_t)f2act<AT>(v[k]);
+            }
+        } else {
+            uint32_t *cw = (uint32_t *)base + (size_t)blk * HD + el;
+            uint32_t word = n == 8 ? 0u : *cw;
+            uint16_t *sc16 = (uint16_t *)(base + page * HD / 2) + ((size_t)blk * (HD / 32) + el / 32) * 16;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                float lo = v[k], hi = v[k], fin = fabsf(v[k]) <= 3.402823466e38f ? 1.0f : 0.0f;
+                lo = gmin<64>(lo);
+                lo = fminf(lo, dpp_f<0x128>(lo, lo));
+                lo = fminf(lo, xor16_f(lo));
+                hi = -gmin<64>(-hi);
+                hi = fmaxf(hi, dpp_f<0x128>(hi, hi));
+                hi = fmaxf(hi, xor16_f(hi));
+                fin = gmin<64>(fin);
+                fin = fminf(fin, dpp_f<0x128>(fin, fin));
+                fin = fminf(fin, xor16_f(fin));
+                if (k < n) {
+                    const Q4Scale sc = q4_scale(lo, hi, fin == 0.0f);
+                    const int e = o0 + k, sh = 16 * (e & 1) + 4 * (e >> 1);
+                    word = (word & ~(15u << sh)) | q4_code(sc, v[k]) << sh;
+                    if ((lane & 31) == 0) {
+                        sc16[e] = sc.d;
+                        sc16[8 + e] = sc.m;
+                    }
+                }
+            }
+            *cw = word;
+        }
+    }
+}
+
+// ---- cached rows back out ------------------------------------------------------------------------
+struct ReadArgs {
+    x100_kv_cfg c;
+    x100_kv_batch b;
+    const uint8_t *kp, *vp;
+    uint16_t *k_out, *v_out;
+};
+
+// 16 lanes per (row, KV head), HD / 16 elements each.
+template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256) void k_read(const ReadArgs a)
+{
+    constexpr int E = HD / 16;
+    const int lane = threadIdx.x & 63, w = wave_id(), l = lane & 15, sub = lane >> 4;
+    const int kvh = blockIdx.y, n_kv = a.c.n_head_kv, page = a.c.page;
+    const int rbase = blockIdx.x * 16 + 4 * w;
+    if (rbase >= a.b.n_rows) return;
+    int pos = -1, pg = -1;
+    bool mine = false;
+    for (int i = 0; i < 4; i++) {
+        const int r = rbase + i;
+        const int s = r < a.b.n_rows ? paged_find(a.b, r) : a.b.n_seq;
+        if (i == sub && s < a.b.n_seq) {
+            const PagedSeq q = paged_seq(a.b, s);
+            if (q.q_len > 0 && r >= q.q0) {
+                mine = true;
+                pos = q.kv_len - q.q_len + r - q.q0;
+                if (pos >= 0) pg = paged_page(a.c, a.b, s, pos);
+            }
+        }
+    }
+    if (!mine) return;
+    const int row = rbase + sub, off = pos & (page - 1);
+    uint32_t k[E], v[E];   // act_type bits
+#pragma unroll
+    for (int e = 0; e < E; e++) k[e] = v[e] = 0;
+    if (pg >= 0) {
+        const size_t at = ((size_t)pg * n_kv + kvh) * page_head_bytes<HD, Q4>(page);
+        if constexpr (!Q4) {
+            const uint16_t *kr = (const uint16_t *)(a.kp + at) + (size_t)off * HD + E * l;
+            const uint16_t *vr = (const uint16_t *)(a.vp + at) + ((size_t)(off >> 3) * HD + E * l) * 8 + (off & 7);
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                k[e] = kr[e];
+                v[e] = vr[8 * e];
+            }
+        } else {
+            const int g = E * l / 32;
+            const uint32_t kw = ((const uint32_t *)(a.kp + at))[(size_t)off * (HD / 8) + E * l / 8];
+            const uint32_t ks = ((const uint32_t *)(a.kp + at + page * HD / 2))[(size_t)off * (HD / 32) + g];
+            const uint32_t *vw = (const uint32_t *)(a.vp + at) + (size_t)(off >> 3) * HD + E * l;
+            const uint16_t *vs = (const uint16_t *)(a.vp + at + page * HD / 2) + ((size_t)(off >> 3) * (HD / 32) + g) * 16;
+            const _Float16 kd = __builtin_bit_cast(_Float16, (uint16_t)ks), km = __builtin_bit_cast(_Float16, (uint16_t)(ks >> 16));
+            const _Float16 vd = __builtin_bit_cast(_Float16, vs[off & 7]), vm = __builtin_bit_cast(_Float16, vs[8 + (off & 7)]);
+            const int vsh = 16 * (off & 1) + 4 * ((off & 7) >> 1);
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int ke = E == 8 ? e : (l & 1) * 4 + e;
+                const _Float16 nk = (_Float16)(int)((kw >> (16 * (ke & 1) + 4 * (ke >> 1))) & 15);
+                const _Float16 nv = (_Float16)(int)((vw[e] >> vsh) & 15);
+                k[e] = f2act<AT>((float)__builtin_fmaf16(nk, kd, km));
+                v[e] = f2act<AT>((float)__builtin_fmaf16(nv, vd, vm));
+            }
+        }
+    }
+    const size_t o = ((size_t)row * n_kv + kvh) * HD + E * l;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+        *(uint32_t *)(a.k_out + o + e) = k[e] | k[e + 1] << 16;
+        *(uint32_t *)(a.v_out + o + e) = v[e] | v[e + 1] << 16;
+    }
+}
+
+template <int HD, int ST> hipError_t append_as(const AppendArgs &a, hipStream_t s)
+{
+    const dim3 grid((a.b.n_rows + 7) / 8, (a.c.n_head + a.c.n_head_kv + 1) / 2 + a.c.n_head_kv);
+    const bool q4 = a.c.kv_type == X100_KV_Q4;
+    if (a.c.act_type == X100_T_F16) {
+        if (q4) k_append<HD, ST, X100_T_F16, true><<<grid, 256, 0, s>>>(a);
+        else k_append<HD, ST, X100_T_F16, false><<<grid, 256, 0, s>>>(a);
+    } else {
+        if (q4) k_append<HD, ST, X100_T_BF16, true><<<grid, 256, 0, s>>>(a);
+        else k_append<HD, ST, X100_T_BF16, false><<<grid, 256, 0, s>>>(a);
+    }
+    return hipGetLastError();
+}
+template <int HD> hipError_t append_from(const AppendArgs &a, hipStream_t s)
+{
+    switch (a.r.k.type) {
+    case X100_T_F32: return append_as<HD, X100_T_F32>(a, s);
+    case X100_T_F16: return append_as<HD, X100_T_F16>(a, s);
+    case X100_T_BF16: return append_as<HD, X100_T_BF16>(a, s);
+    case X100_T_I32: return append_as<HD, X100_T_I32>(a, s);
+    }
+    return hipErrorInvalidValue;
+}
+template <int HD> hipError_t read_as(const ReadArgs &a, hipStream_t s)
+{
+    const dim3 grid((a.b.n_rows + 15) / 16, a.c.n_head_kv);
+    const bool q4 = a.c.kv_type == X100_KV_Q4;
+    if (a.c.act_type == X100_T_F16) {
+        if (q4) k_read<HD, X100_T_F16, true><<<grid, 256, 0, s>>>(a);
+        else k_read<HD, X100_T_F16, false><<<grid, 256, 0, s>>>(a);
+    } else {
+        if (q4) k_read<HD, X100_T_BF16, true><<<grid, 256, 0, s>>>(a);
+        else k_read<HD, X100_T_BF16, false><<<grid, 256, 0, s>>>(a);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t x100_rope_table_launch(int head_dim, int n_pos, float base, float *table, hipStream_t s)
+{
+    const size_t n = (size_t)n_pos * (head_dim / 2);
+    k_rope_table<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(head_dim / 2, n_pos, (double)base, (float2 *)table);
+    return hipGetLastError();
+}
+
+hipError_t x100_kv_append_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const x100_kv_rows &r, void *kp,
+                                 void *vp, void *q_out, hipStream_t s)
+{
+    const AppendArgs a = {c, b, r, (uint8_t *)kp, (uint8_t *)vp, (uint16_t *)q_out};
+    return c.head_dim == 64 ? append_from<64>(a, s) : append_from<128>(a, s);
+}
+
+hipError_t x100_kv_read_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const void *kp, const void *vp,
+                               void *k_out, void *v_out, hipStream_t s)
+{
+    const ReadArgs a = {c, b, (const uint8_t *)kp, (const uint8_t *)vp, (uint16_t *)k_out, (uint16_t *)v_out};
+    return c.head_dim == 64 ? read_as<64>(a, s) : read_as<128>(a, s);
+}

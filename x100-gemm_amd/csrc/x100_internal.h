@@ -6,6 +6,8 @@
 #include "gemm_plan.h"
 #include "x100_decode.h"
 #include "x100_moe.h"
+#include "x100_paged.h"
+#include "x100_rows.h"
 
 // acc: C += A.B; otherwise the overwrite form C = A.B.
 hipError_t x100_gemm_i8_launch(int M, int N, int K, const int8_t *A, const int8_t *B, int32_t *C,
@@ -57,3 +59,21 @@ size_t x100_attn_workspace_bytes(const x100_layer_cfg *c);
 hipError_t x100_attn_launch(const x100_layer_cfg *c, const x100_layer_weights *w, int pos, float *h,
                             float *ws, float **hn_out, hipStream_t s, float **o_out = nullptr);
 
+
+// int8 rows (rows.hip); arguments as checked by the entry points.
+hipError_t x100_quant_i8_launch(int n_rows, int d, const x100_rows *x, int8_t *q, float *scale, hipStream_t s);
+hipError_t x100_add_rmsnorm_i8_launch(int n_rows, int d, const x100_rows *x, const x100_rows *delta,
+                                      const float *weight, float eps, void *h, int64_t ldh, int8_t *q, float *scale,
+                                      hipStream_t s);
+
+// Paged KV cache (paged.hip) and attention over it (attn_paged.hip).  ws holds
+// x100_attn_paged_workspace(c, b) bytes.
+hipError_t x100_rope_table_launch(int head_dim, int n_pos, float base, float *table, hipStream_t s);
+hipError_t x100_kv_append_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const x100_kv_rows &r, void *kp,
+                                 void *vp, void *q_out, hipStream_t s);
+hipError_t x100_kv_read_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const void *kp, const void *vp,
+                               void *k_out, void *v_out, hipStream_t s);
+size_t x100_attn_paged_workspace(const x100_kv_cfg &c, const x100_kv_batch &b);
+hipError_t x100_attn_paged_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const void *q, int64_t ldq,
+                                  const void *kp, const void *vp, float scale, void *out, int64_t ldo, void *ws,
+                                  hipStream_t s);

@@ -13,6 +13,9 @@ Entry points and what they replace in the reference:
                                                 caller scratch); moe_pack_experts: load-time
                                                 regrouping of the expert tensors (tiled=True)
   gemv_int4_hip / gemv_int8_hip (+ packers)     gemv_nb_int4 / gemv_nb_int8 of bench/q4_gemv.c:67-99
+  x100_kv_append_hip / x100_attn_paged_hip      the attention of qwen_moe.c:284-292 for a batch of
+                                                sequences on a paged cache (x100_paged.h)
+  x100_add_rmsnorm_i8_hip / x100_quant_i8_hip   no counterpart: rows of the int8 GEMM (x100_rows.h)
 """
 import ctypes
 import os
@@ -29,7 +32,7 @@ X100_EIO, X100_EFORMAT, X100_ENOTFOUND, X100_ESCRATCH = -5, -6, -7, -8
 MOE_NOALLOC_MAX_BYTES = 8 << 20
 
 # Every symbol declared in include/x100_gemm.h, x100_gemv_tile.h, x100_qgemv.h, x100_moe.h,
-# x100_gguf.h, x100_decode.h.
+# x100_gguf.h, x100_decode.h, x100_rows.h, x100_paged.h.
 EXPORTS = (
     "gemm_ime_i8", "gemm_hip_i8", "gemm_hip_i8_dev", "gemm_hip_i8_dev_set", "gemm_hip_i8_dev_variant",
     "x100_hip_detect", "x100_hip_caps_print", "x100_hip_strerror",
@@ -44,6 +47,9 @@ EXPORTS = (
     "x100_gguf_block_elems", "x100_gguf_upload", "x100_gguf_pack_rows",
     "x100_attn_decode_hip", "x100_decode_layer_hip", "x100_decode_workspace_bytes",
     "x100_attn_decode_hip_ws", "x100_decode_layer_hip_ws",
+    "x100_quant_i8_hip", "x100_add_rmsnorm_i8_hip",
+    "x100_kv_pool_bytes", "x100_rope_table_hip", "x100_kv_append_hip", "x100_kv_read_hip",
+    "x100_attn_paged_workspace_bytes", "x100_attn_paged_hip", "x100_attn_paged_hip_ws",
 )
 
 GEMM_AUTO, GEMM_TILE256, GEMM_TILE128, GEMM_SKINNY, GEMM_GENERIC, GEMM_TILE256_W4, GEMM_TILE64, GEMM_TILE32 = \
@@ -76,6 +82,34 @@ class LayerWeights(ctypes.Structure):
     """x100_layer_weights (x100_decode.h): device pointers."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("attn_norm", "q_norm", "k_norm", "ffn_norm", "wq", "wk", "wv", "wo",
                                                "router", "wg", "wu", "wd", "k_cache", "v_cache")]
+
+
+# Element types of x100_rows.h (ggml type ids) and the 4-bit cache of x100_paged.h.
+T_F32, T_F16, T_I32, T_BF16, KV_Q4 = 0, 1, 26, 30, 256
+ROWS_MAX_D = 16384
+
+
+class Rows(ctypes.Structure):
+    """x100_rows (x100_rows.h): device rows of one of four types, int32 with row and column scales."""
+    _fields_ = [("type", ctypes.c_int), ("p", ctypes.c_void_p), ("ld", ctypes.c_int64),
+                ("row_scale", ctypes.c_void_p), ("col_scale", ctypes.c_void_p)]
+
+
+class KvCfg(ctypes.Structure):
+    """x100_kv_cfg (x100_paged.h)."""
+    _fields_ = [(n, ctypes.c_int) for n in ("n_head", "n_head_kv", "head_dim", "page", "n_pages", "act_type", "kv_type")]
+
+
+class KvBatch(ctypes.Structure):
+    """x100_kv_batch (x100_paged.h): the arrays are device pointers."""
+    _fields_ = [(n, ctypes.c_int) for n in ("n_seq", "n_rows", "max_q", "max_kv", "table_ld")] + \
+               [(n, ctypes.c_void_p) for n in ("q_start", "kv_len", "block_table")]
+
+
+class KvRows(ctypes.Structure):
+    """x100_kv_rows (x100_paged.h)."""
+    _fields_ = [("q", Rows), ("k", Rows), ("v", Rows), ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p),
+                ("eps", ctypes.c_float), ("rope", ctypes.c_void_p), ("rope_len", ctypes.c_int)]
 
 
 _lib = None
@@ -162,6 +196,20 @@ def lib():
                                            p]
     L.x100_attn_decode_hip_ws.restype = i
     L.x100_decode_layer_hip_ws.restype = i
+    P, f, i64_ = ctypes.POINTER, ctypes.c_float, ctypes.c_int64
+    L.x100_quant_i8_hip.argtypes = [i, i, P(Rows), p, p, p]
+    L.x100_add_rmsnorm_i8_hip.argtypes = [i, i, P(Rows), P(Rows), p, f, p, i64_, p, p, p]
+    L.x100_kv_pool_bytes.argtypes = [P(KvCfg)]
+    L.x100_rope_table_hip.argtypes = [i, i, f, p, p]
+    L.x100_kv_append_hip.argtypes = [P(KvCfg), P(KvBatch), P(KvRows), p, p, p, p]
+    L.x100_kv_read_hip.argtypes = [P(KvCfg), P(KvBatch), p, p, p, p, p]
+    L.x100_attn_paged_workspace_bytes.argtypes = [P(KvCfg), P(KvBatch)]
+    L.x100_attn_paged_hip.argtypes = [P(KvCfg), P(KvBatch), p, i64_, p, p, f, p, i64_, p]
+    L.x100_attn_paged_hip_ws.argtypes = [P(KvCfg), P(KvBatch), p, i64_, p, p, f, p, i64_, p, sz, p]
+    L.x100_kv_pool_bytes.restype = L.x100_attn_paged_workspace_bytes.restype = sz
+    for name in ("x100_quant_i8_hip", "x100_add_rmsnorm_i8_hip", "x100_rope_table_hip", "x100_kv_append_hip",
+                 "x100_kv_read_hip", "x100_attn_paged_hip", "x100_attn_paged_hip_ws"):
+        getattr(L, name).restype = i
     for name in ("gemm_hip_i8", "gemm_hip_i8_dev", "gemm_hip_i8_dev_set", "gemm_hip_i8_dev_variant", "x100_hip_detect",
                  "x100q_pack", "qgemv_hip", "x100q_check_quant_div", "moe_layer_hip", "moe_layer_hip_ws", "moe_layer_hip_noalloc",
                  "moe_pack_experts",
@@ -328,3 +376,50 @@ def decode_layer_ws(cfg, weights, pos, d_h, d_sel, d_sw, d_ws, ws_bytes, stream=
     return _check("x100_decode_layer_hip_ws", lib().x100_decode_layer_hip_ws(ctypes.byref(cfg), ctypes.byref(weights),
                                                                              pos, d_h, d_sel, d_sw, d_ws, ws_bytes,
                                                                              stream))
+
+
+# ---- int8 rows (x100_rows.h) ------------------------------------------------------------------------
+def quant_i8(n_rows, d, rows, d_q, d_scale, stream=None):
+    """int8 codes [n_rows][d] and fp32 scale [n_rows] of rows (Rows)."""
+    return _check("x100_quant_i8_hip", lib().x100_quant_i8_hip(n_rows, d, rows, d_q, d_scale, stream))
+
+
+def add_rmsnorm_i8(n_rows, d, x, delta, d_weight, eps, d_h, ldh, d_q, d_scale, stream=None):
+    """h = x + delta (delta None: h = x, not stored), then RMSNorm(h) as int8 codes and scales."""
+    return _check("x100_add_rmsnorm_i8_hip", lib().x100_add_rmsnorm_i8_hip(n_rows, d, x, delta, d_weight, eps, d_h, ldh,
+                                                                          d_q, d_scale, stream))
+
+
+# ---- paged KV cache (x100_paged.h) ------------------------------------------------------------------
+def kv_pool_bytes(cfg):
+    return lib().x100_kv_pool_bytes(cfg)
+
+
+def rope_table(head_dim, n_pos, base, d_table, stream=None):
+    """(cos, sin) [n_pos][head_dim / 2][2] fp32."""
+    return _check("x100_rope_table_hip", lib().x100_rope_table_hip(head_dim, n_pos, base, d_table, stream))
+
+
+def kv_append(cfg, batch, rows, d_k_pool, d_v_pool, d_q_out, stream=None):
+    """Head norms, rotation, keys and values into the pages, rotated queries out."""
+    return _check("x100_kv_append_hip", lib().x100_kv_append_hip(cfg, batch, rows, d_k_pool, d_v_pool, d_q_out, stream))
+
+
+def kv_read(cfg, batch, d_k_pool, d_v_pool, d_k_out, d_v_out, stream=None):
+    """The cached keys and values at the rows' positions, as rows."""
+    return _check("x100_kv_read_hip", lib().x100_kv_read_hip(cfg, batch, d_k_pool, d_v_pool, d_k_out, d_v_out, stream))
+
+
+def attn_paged_workspace_bytes(cfg, batch):
+    return lib().x100_attn_paged_workspace_bytes(cfg, batch)
+
+
+def attn_paged(cfg, batch, d_q, ldq, d_k_pool, d_v_pool, scale, d_out, ldo, stream=None):
+    """Causal attention of the batch's rows over the paged cache (the library's workspace)."""
+    return _check("x100_attn_paged_hip", lib().x100_attn_paged_hip(cfg, batch, d_q, ldq, d_k_pool, d_v_pool, scale, d_out,
+                                                                  ldo, stream))
+
+
+def attn_paged_ws(cfg, batch, d_q, ldq, d_k_pool, d_v_pool, scale, d_out, ldo, d_ws, ws_bytes, stream=None):
+    return _check("x100_attn_paged_hip_ws", lib().x100_attn_paged_hip_ws(cfg, batch, d_q, ldq, d_k_pool, d_v_pool, scale,
+                                                                        d_out, ldo, d_ws, ws_bytes, stream))
