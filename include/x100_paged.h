@@ -31,7 +31,8 @@
  *            V: codes [page / 8][head_dim] words, then [page / 8][head_dim / 32][2][8] fp16 (d of 8
  *            positions, m of 8).  A K word holds 8 elements of a row, a V word 8 positions of an
  *            element: number e at bit 16 * (e % 2) + 4 * (e / 2).
- *            d = fp16((hi - lo) / 15), m = fp16(lo), n = rint((x - m) * (1 / d)) within 0 .. 15.
+ *            d = fp16((hi - lo) * fp32(1/15)), m = fp16(lo), n = rint((x - m) * (1 / d)) within 0 .. 15,
+ *            in fp32.
  *            Values up to 65504 in size; a group with a larger one, an infinity or a NaN stands for
  *            NaN (d = m = NaN).
  *

@@ -34,7 +34,7 @@ def q4_encode(x):
     g = x.reshape(x.shape[:-1] + (-1, 32))
     with np.errstate(all="ignore"):
         lo, hi = g.min(-1), g.max(-1)
-        d = ((hi - lo) / np.float32(15)).astype(np.float16)
+        d = ((hi - lo) * np.float32(1 / 15)).astype(np.float16)
         m = lo.astype(np.float16)
         bad = ~(np.isfinite(g).all(-1) & np.isfinite(d) & np.isfinite(m))
         inv = np.where(d > 0, np.float32(1) / d.astype(np.float32), np.float32(0))
@@ -176,7 +176,7 @@ def codes_f32(t):
         amax = np.abs(t).max(1)
         fin = np.isfinite(t).all(1)
         some = fin & (amax >= np.float32(2.0 ** -100))
-        inv = np.where(some, np.float32(127) / amax, np.float32(0)).astype(np.float32)
+        inv = np.where(some, np.float32(127) * (np.float32(1) / amax), np.float32(0)).astype(np.float32)
         c = np.rint(t * inv[:, None])
     c = np.where(some[:, None], c, 0).astype(np.int8)
     return c, np.where(some, amax, np.where(fin, np.float32(0), np.float32(np.nan)))

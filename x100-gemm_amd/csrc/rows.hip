@@ -1,6 +1,6 @@
 // int8 rows with one scale per row (x100_rows.h): the residual's addition with RMSNorm, and plain rows.
 //
-// t_i = h_i w_i (or x_i), amax = max |t_i|, code_i = rint(t_i (127 / amax)).  The norm's factor
+// t_i = h_i w_i (or x_i), amax = max |t_i|, code_i = rint(t_i 127 (1 / amax)).  The norm's factor
 // r = 1/sqrt(mean h^2 + eps) multiplies every t_i alike and cancels in the code, so the maximum and the
 // sum of squares come from the same single read of the row, and only the scale depends on the sum.
 // Bound by HBM: every input is read once into registers, every output written once.
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_rows_i8(const RowArgs a
     }
     if (!live) return;
     const bool fin = mx <= 3.402823466e38f, some = fin && mx >= 0x1p-100f;
-    const float inv = some ? 127.0f / mx : 0.0f;
+    const float inv = some ? 127.0f * (1.0f / mx) : 0.0f;
     if (t == 0) {
         float sc = some ? mx : (fin ? 0.0f : __builtin_nanf(""));
         if constexpr (NORM) sc *= 1.0f / sqrtf(ss / (float)d + a.eps);
