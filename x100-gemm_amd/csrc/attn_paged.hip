@@ -11,47 +11,13 @@
 // reason: a lane's operand of V^T is one 16-byte load (16 bits) or one word (4 bits).
 #include <algorithm>
 
-#include "paged.h"
+#include "paged_attn.h"
 #include "x100_internal.h"
 
 namespace {
 
-constexpr float NEG_INF = -__builtin_inff();
-
-struct AttnArgs {
-    x100_kv_cfg c;
-    x100_kv_batch b;
-    const uint16_t *q;
-    int64_t ldq;
-    const uint8_t *kp, *vp;
-    float scale2;        // scale * log2(e): weights are powers of two
-    uint16_t *out;
-    int64_t ldo;
-    float *part;         // [row][head][split][HD + 2]: m, l, then O (not divided by l)
-    int split, n_split;  // positions per split (a multiple of 128), splits
-};
-
-template <int T> struct Mfma16;
-template <> struct Mfma16<X100_T_F16> {
-    static X100_DEV v4f mul(v4u a, v4u b, v4f c)
-    {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
-    }
-};
-template <> struct Mfma16<X100_T_BF16> {
-    static X100_DEV v4f mul(v4u a, v4u b, v4f c)
-    {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
-    }
-};
-
-// The tile's power of two 2^-e that brings a row's largest element (in size) to 1 .. 2: bf16 queries
-// become fp16 that way without loss (elements below 2^-24 of the largest aside), whatever their size.
-X100_DEV int row_exponent(float amax)
-{
-    const int e = (int)(__float_as_uint(amax) >> 23) - 127;
-    return amax > 0.0f && e < 128 ? e : 0;
-}
+constexpr float NEG_INF = X100_NEG_INF;
+using AttnArgs = PagedAttnArgs;
 
 // One block: 16 rows (token, head) of a sequence and KV head, one split of the positions; its 4 waves
 // take tiles of 32 positions in turn and merge at the end.
@@ -67,7 +33,7 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256) void k_attn
     const int G = a.c.n_head / a.c.n_head_kv, page = a.c.page;
     const PagedSeq q = paged_seq(a.b, s);
     const int n_rows = q.q_len * G, i0 = tile * 16;
-    if (i0 >= n_rows) return;
+    if (i0 >= n_rows || n_rows > a.few) return;
     const int pos0 = q.kv_len - q.q_len;                       // position of token 0
     const int vis = pos0 + (min(i0 + 15, n_rows - 1)) / G + 1;  // positions that the tile's last row sees
     const int ns = max(1, (vis + a.split - 1) / a.split);
@@ -308,13 +274,8 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256) void k_attn
             const uint32_t b = ls == 0.0f ? 0u : f2act<AT>(y0 * f) | f2act<AT>(y1 * f) << 16;
             *(uint32_t *)(a.out + (size_t)(q.q0 + tk) * a.ldo + (size_t)hh * HD + el) = b;
         } else {
-            float *p = a.part + (((size_t)(q.q0 + tk) * a.c.n_head + hh) * a.n_split + sp) * (HD + 2);
-            p[2 + el] = y0;
-            p[3 + el] = y1;
-            if (el == 0) {
-                p[0] = mm;
-                p[1] = ls;
-            }
+            *(float2 *)(part_o(a, q.q0 + tk, hh, sp, HD) + el) = make_float2(y0, y1);
+            if (el == 0) *part_ml(a, q.q0 + tk, hh, sp, HD) = make_float2(mm, ls);
         }
     }
 }
@@ -330,21 +291,24 @@ template <int HD, int AT> __global__ __launch_bounds__(256) void k_attn_join(con
     if (q.q_len <= 0 || row < q.q0) return;
     const int G = a.c.n_head / a.c.n_head_kv, n_rows = q.q_len * G;
     const int i = (row - q.q0) * G + head % G;
-    const int vis = q.kv_len - q.q_len + min(i / 16 * 16 + 15, n_rows - 1) / G + 1;
-    const int ns = (vis + a.split - 1) / a.split;
+    const bool few = n_rows <= a.few;
+    const int tr = few ? 16 : PROMPT_ROWS, split = few ? a.split : a.split_p;
+    const int vis = q.kv_len - q.q_len + min(i / tr * tr + tr - 1, n_rows - 1) / G + 1;
+    const int ns = (vis + split - 1) / split;
     if (ns <= 1) return;
-    const float *p = a.part + ((size_t)row * a.c.n_head + head) * a.n_split * (HD + 2);
+    const float *po = part_o(a, row, head, 0, HD);
+    const float2 *ml = part_ml(a, row, head, 0, HD);
     float m = NEG_INF;
-    for (int k = 0; k < ns; k++) m = fmaxf(m, p[(size_t)k * (HD + 2)]);
+    for (int k = 0; k < ns; k++) m = fmaxf(m, ml[k].x);
     const float ms = m == NEG_INF ? 0.0f : m;
     float l = 0.0f, y[HD / 64] = {};
     for (int k = 0; k < ns; k++) {
-        const float *pk = p + (size_t)k * (HD + 2);
-        if (pk[0] == NEG_INF) continue;
-        const float f = __builtin_amdgcn_exp2f(pk[0] - ms);
-        l = __builtin_fmaf(pk[1], f, l);
+        const float2 v = ml[k];
+        if (v.x == NEG_INF) continue;
+        const float f = __builtin_amdgcn_exp2f(v.x - ms);
+        l = __builtin_fmaf(v.y, f, l);
 #pragma unroll
-        for (int e = 0; e < HD / 64; e++) y[e] = __builtin_fmaf(pk[2 + lane * (HD / 64) + e], f, y[e]);
+        for (int e = 0; e < HD / 64; e++) y[e] = __builtin_fmaf(po[(size_t)k * HD + lane * (HD / 64) + e], f, y[e]);
     }
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
     uint16_t *o = a.out + (size_t)row * a.ldo + (size_t)head * HD + lane * (HD / 64);
@@ -352,32 +316,61 @@ template <int HD, int AT> __global__ __launch_bounds__(256) void k_attn_join(con
     for (int e = 0; e < HD / 64; e++) o[e] = l == 0.0f ? 0 : (uint16_t)f2act<AT>(y[e] * f);
 }
 
+// How a call is laid out.  Sequences of up to `few` rows (token, head) go to the tile kernel, longer ones
+// to the prompt kernel; positions are split so that the blocks fill the chip.
 struct Plan {
-    int tiles, split, n_split;
+    int few, tiles, split, n_split;       // tile kernel (tiles 0: not launched)
+    int tiles_p, split_p, n_split_p;      // prompt kernel (tiles_p 0: not launched)
+    int n_part() const { return std::max(n_split, n_split_p); }
 };
 
-// Positions per split: as many splits as give the chip four blocks per CU, of 256 positions or more.
+// Splits of max_kv positions for `want` of them, each of `least` positions or more and a multiple of 128.
+void split_of(int64_t max_kv, int64_t want, int64_t least, int64_t most, int &split, int &n_split)
+{
+    int64_t s = (max_kv + want - 1) / want;
+    s = std::min(most, std::max(least, (s + 127) / 128 * 128));
+    s = std::min<int64_t>(s, (max_kv + 127) / 128 * 128);
+    split = (int)s;
+    n_split = (int)((max_kv + s - 1) / s);
+}
+
 Plan plan_of(const x100_kv_cfg &c, const x100_kv_batch &b)
 {
-    Plan p;
+    Plan p = {};
     const int G = c.n_head / c.n_head_kv;
-    p.tiles = (int)(((int64_t)b.max_q * G + 15) / 16);
-    const int64_t base = std::max<int64_t>(1, std::min<int64_t>((int64_t)p.tiles * b.n_seq, (int64_t)b.n_rows * G)) * c.n_head_kv;
-    const int64_t want = std::max<int64_t>(1, 1024 / base);
-    int64_t split = (b.max_kv + want - 1) / want;
-    split = std::max<int64_t>(256, (split + 127) / 128 * 128);
-    p.split = (int)std::min<int64_t>(split, ((int64_t)b.max_kv + 127) / 128 * 128);
-    p.n_split = (int)(((int64_t)b.max_kv + p.split - 1) / p.split);
+    const int64_t rows = (int64_t)b.max_q * G;   // of the longest sequence
+    p.few = 32;
+    p.split = p.split_p = 128;
+    p.n_split = p.n_split_p = 1;
+    {
+        p.tiles = (int)((std::min<int64_t>(rows, p.few) + 15) / 16);
+        const int64_t base = (int64_t)p.tiles * std::min(b.n_seq, b.n_rows) * c.n_head_kv;
+        split_of(b.max_kv, std::max<int64_t>(1, 1024 / base), 256, (int64_t)1 << 30, p.split, p.n_split);
+    }
+    if (rows > p.few) {
+        p.tiles_p = (int)((rows + PROMPT_ROWS - 1) / PROMPT_ROWS);
+        // tiles that have rows: no more than one per sequence besides the full ones
+        const int64_t full = (int64_t)b.n_rows * G / PROMPT_ROWS + 1;
+        const int64_t base = std::min<int64_t>((int64_t)p.tiles_p * b.n_seq, full + b.n_seq) * c.n_head_kv;
+        split_of(b.max_kv, std::max<int64_t>(1, 512 / base), 512, PROMPT_SPLIT, p.split_p, p.n_split_p);
+    }
     return p;
 }
 
 template <int HD, int AT> hipError_t attn_as(const AttnArgs &a, const Plan &p, hipStream_t s)
 {
-    const dim3 grid((unsigned)(p.tiles * p.n_split), a.c.n_head_kv, a.b.n_seq);
-    if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true><<<grid, 256, 0, s>>>(a);
-    else k_attn_tile<HD, AT, false><<<grid, 256, 0, s>>>(a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.n_split == 1) return e;
+    if (p.tiles) {
+        const dim3 grid((unsigned)(p.tiles * p.n_split), a.c.n_head_kv, a.b.n_seq);
+        if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true><<<grid, 256, 0, s>>>(a);
+        else k_attn_tile<HD, AT, false><<<grid, 256, 0, s>>>(a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (p.tiles_p) {
+        const hipError_t e = x100_attn_prompt_launch(a, p.tiles_p, s);
+        if (e != hipSuccess) return e;
+    }
+    if (p.n_part() == 1) return hipSuccess;
     k_attn_join<HD, AT><<<dim3(a.b.n_rows, (a.c.n_head + 3) / 4), 256, 0, s>>>(a);
     return hipGetLastError();
 }
@@ -387,7 +380,7 @@ template <int HD, int AT> hipError_t attn_as(const AttnArgs &a, const Plan &p, h
 size_t x100_attn_paged_workspace(const x100_kv_cfg &c, const x100_kv_batch &b)
 {
     const Plan p = plan_of(c, b);
-    return p.n_split == 1 ? 0 : (size_t)b.n_rows * c.n_head * p.n_split * (c.head_dim + 2) * sizeof(float);
+    return p.n_part() == 1 ? 0 : (size_t)b.n_rows * c.n_head * p.n_part() * (c.head_dim + 2) * sizeof(float);
 }
 
 hipError_t x100_attn_paged_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const void *q, int64_t ldq,
@@ -395,8 +388,23 @@ hipError_t x100_attn_paged_launch(const x100_kv_cfg &c, const x100_kv_batch &b, 
                                   hipStream_t s)
 {
     const Plan p = plan_of(c, b);
-    const AttnArgs a = {c, b, (const uint16_t *)q, ldq, (const uint8_t *)kp, (const uint8_t *)vp,
-                        scale * 1.4426950408889634f, (uint16_t *)out, ldo, (float *)ws, p.split, p.n_split};
+    AttnArgs a = {};
+    a.c = c;
+    a.b = b;
+    a.q = (const uint16_t *)q;
+    a.ldq = ldq;
+    a.kp = (const uint8_t *)kp;
+    a.vp = (const uint8_t *)vp;
+    a.scale2 = scale * 1.4426950408889634f;
+    a.out = (uint16_t *)out;
+    a.ldo = ldo;
+    a.part = (float *)ws;
+    a.split = p.split;
+    a.n_split = p.n_split;
+    a.few = p.few;
+    a.split_p = p.split_p;
+    a.n_split_p = p.n_split_p;
+    a.n_part = p.n_part();
     if (c.head_dim == 64)
         return c.act_type == X100_T_F16 ? attn_as<64, X100_T_F16>(a, p, s) : attn_as<64, X100_T_BF16>(a, p, s);
     return c.act_type == X100_T_F16 ? attn_as<128, X100_T_F16>(a, p, s) : attn_as<128, X100_T_BF16>(a, p, s);

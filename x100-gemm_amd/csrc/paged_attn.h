@@ -1,0 +1,87 @@
+// What the kernels of attention over the paged cache share (attn_paged.hip, attn_prompt.hip).
+#pragma once
+#include "paged.h"
+
+constexpr float X100_NEG_INF = -__builtin_inff();
+
+struct PagedAttnArgs {
+    x100_kv_cfg c;
+    x100_kv_batch b;
+    const uint16_t *q;
+    int64_t ldq;
+    const uint8_t *kp, *vp;
+    float scale2;        // scale * log2(e): weights are powers of two
+    uint16_t *out;
+    int64_t ldo;
+    float *part;         // split results: O (not divided by l) and (m, l), see part_o
+    int split, n_split;  // positions per split (a multiple of 128), splits
+    int few;             // sequences of up to this many rows (token, head) are the tile kernel's, longer
+                         // ones the prompt kernel's
+    int split_p, n_split_p;   // split, n_split of the prompt kernel
+    int n_part;          // the larger n_split: results per row and head in part
+};
+
+template <int T> struct Mfma16;
+template <> struct Mfma16<X100_T_F16> {
+    static X100_DEV v4f mul(v4u a, v4u b, v4f c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    }
+};
+template <> struct Mfma16<X100_T_BF16> {
+    static X100_DEV v4f mul(v4u a, v4u b, v4f c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+    }
+};
+
+// The tile's power of two 2^-e that brings a row's largest element (in size) to 1 .. 2: bf16 queries
+// become fp16 that way without loss (elements below 2^-24 of the largest aside), whatever their size.
+X100_DEV int row_exponent(float amax)
+{
+    const int e = (int)(__float_as_uint(amax) >> 23) - 127;
+    return amax > 0.0f && e < 128 ? e : 0;
+}
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+
+template <int T> X100_DEV v16f mfma32(v4u a, v4u b, v16f c)
+{
+    if constexpr (T == X100_T_F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+}
+// two fp32 to 16 bits each (nearest even), lo in the low half
+template <int T> X100_DEV uint32_t pack2(float lo, float hi)
+{
+    const v2f v = {lo, hi};
+    if constexpr (T == X100_T_F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, v2h));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, v2b));
+}
+// c + the two 16-bit numbers of w
+template <int T> X100_DEV float add2(uint32_t w, float c)
+{
+    if constexpr (T == X100_T_F16)
+        return __builtin_amdgcn_fdot2(as_h2(w), v2h{(_Float16)1.0f, (_Float16)1.0f}, c, false);
+    else {
+        const uint32_t one = 0x3f803f80u;
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, w), __builtin_bit_cast(v2b, one), c, false);
+    }
+}
+
+// Where the split results of a row and head lie: O [row][head][split][HD], then (m, l) [row][head][split].
+X100_DEV float *part_o(const PagedAttnArgs &a, size_t row, int head, int sp, int hd)
+{
+    return a.part + ((row * a.c.n_head + head) * a.n_part + sp) * hd;
+}
+X100_DEV float2 *part_ml(const PagedAttnArgs &a, size_t row, int head, int sp, int hd)
+{
+    return (float2 *)(a.part + (size_t)a.b.n_rows * a.c.n_head * a.n_part * hd) + (row * a.c.n_head + head) * a.n_part + sp;
+}
+
+constexpr int PROMPT_ROWS = 256;      // rows (token, head) of a block of the prompt kernel
+constexpr int PROMPT_SPLIT = 32768;   // most positions of a split there (its page list is in LDS)
+hipError_t x100_attn_prompt_launch(const PagedAttnArgs &a, int tiles, hipStream_t s);
