@@ -274,54 +274,78 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256) void k_attn
             const uint32_t b = ls == 0.0f ? 0u : f2act<AT>(y0 * f) | f2act<AT>(y1 * f) << 16;
             *(uint32_t *)(a.out + (size_t)(q.q0 + tk) * a.ldo + (size_t)hh * HD + el) = b;
         } else {
-            *(float2 *)(part_o(a, q.q0 + tk, hh, sp, HD) + el) = make_float2(y0, y1);
-            if (el == 0) *part_ml(a, q.q0 + tk, hh, sp, HD) = make_float2(mm, ls);
+            const size_t at = part_few(a, s, kvh, i0 + r) + sp;
+            *(float2 *)(a.o_few + at * HD + el) = make_float2(y0, y1);
+            if (el == 0) a.ml_few[at] = make_float2(mm, ls);
         }
     }
 }
 
-// Merges the splits of rows that have more than one: a wave per (row, head), HD / 64 elements per lane.
-template <int HD, int AT> __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a)
+// Merges the splits of rows that have more than one: a wave per row (token, head), HD / 64 elements per
+// lane.  FEW: the tile kernel's rows, blockIdx.x = sequence, y = KV head and four rows; else the prompt
+// kernel's, x = token row, y = four heads.
+template <int HD, int AT, bool FEW> __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a)
 {
-    const int lane = threadIdx.x & 63, head = blockIdx.y * 4 + wave_id(), row = blockIdx.x;
-    if (head >= a.c.n_head) return;
-    const int s = paged_find(a.b, row);
-    if (s >= a.b.n_seq) return;
-    const PagedSeq q = paged_seq(a.b, s);
-    if (q.q_len <= 0 || row < q.q0) return;
-    const int G = a.c.n_head / a.c.n_head_kv, n_rows = q.q_len * G;
-    const int i = (row - q.q0) * G + head % G;
-    const bool few = n_rows <= a.few;
-    const int tr = few ? 16 : PROMPT_ROWS, split = few ? a.split : a.split_p;
-    const int vis = q.kv_len - q.q_len + min(i / tr * tr + tr - 1, n_rows - 1) / G + 1;
+    constexpr int E = HD / 64;
+    const int lane = threadIdx.x & 63, w = wave_id(), G = a.c.n_head / a.c.n_head_kv;
+    int s, i, kvh;
+    PagedSeq q;
+    if constexpr (FEW) {
+        const int per = (a.few_rows + 3) / 4;
+        s = blockIdx.x;
+        kvh = blockIdx.y / per;
+        i = blockIdx.y % per * 4 + w;
+        q = paged_seq(a.b, s);
+        if (i >= q.q_len * G || q.q_len * G > a.few) return;
+    } else {
+        const int row = blockIdx.x, head = blockIdx.y * 4 + w;
+        if (head >= a.c.n_head) return;
+        s = paged_find(a.b, row);
+        if (s >= a.b.n_seq) return;
+        q = paged_seq(a.b, s);
+        if (q.q_len * G <= a.few || row < q.q0) return;
+        kvh = head / G;
+        i = (row - q.q0) * G + head % G;
+    }
+    const int tr = FEW ? 16 : PROMPT_ROWS, split = FEW ? a.split : a.split_p;
+    const int vis = q.kv_len - q.q_len + min(i / tr * tr + tr - 1, q.q_len * G - 1) / G + 1;
     const int ns = (vis + split - 1) / split;
     if (ns <= 1) return;
-    const float *po = part_o(a, row, head, 0, HD);
-    const float2 *ml = part_ml(a, row, head, 0, HD);
+    const size_t at = FEW ? part_few(a, s, kvh, i) : part_prompt(a, q.q0, kvh, i);
+    const float2 *ml = (FEW ? a.ml_few : a.ml_p) + at;
+    const float *po = (FEW ? a.o_few : a.o_p) + at * HD + lane * E;
     float m = NEG_INF;
     for (int k = 0; k < ns; k++) m = fmaxf(m, ml[k].x);
     const float ms = m == NEG_INF ? 0.0f : m;
-    float l = 0.0f, y[HD / 64] = {};
+    float l = 0.0f, y[E] = {};
     for (int k = 0; k < ns; k++) {
         const float2 v = ml[k];
         if (v.x == NEG_INF) continue;
         const float f = __builtin_amdgcn_exp2f(v.x - ms);
         l = __builtin_fmaf(v.y, f, l);
 #pragma unroll
-        for (int e = 0; e < HD / 64; e++) y[e] = __builtin_fmaf(po[(size_t)k * HD + lane * (HD / 64) + e], f, y[e]);
+        for (int e = 0; e < E; e++) y[e] = __builtin_fmaf(po[(size_t)k * HD + e], f, y[e]);
     }
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t *o = a.out + (size_t)row * a.ldo + (size_t)head * HD + lane * (HD / 64);
+    uint16_t *o = a.out + (size_t)(q.q0 + i / G) * a.ldo + (size_t)(kvh * G + i % G) * HD + lane * E;
 #pragma unroll
-    for (int e = 0; e < HD / 64; e++) o[e] = l == 0.0f ? 0 : (uint16_t)f2act<AT>(y[e] * f);
+    for (int e = 0; e < E; e++) o[e] = l == 0.0f ? 0 : (uint16_t)f2act<AT>(y[e] * f);
 }
 
 // How a call is laid out.  Sequences of up to `few` rows (token, head) go to the tile kernel, longer ones
 // to the prompt kernel; positions are split so that the blocks fill the chip.
 struct Plan {
-    int few, tiles, split, n_split;       // tile kernel (tiles 0: not launched)
-    int tiles_p, split_p, n_split_p;      // prompt kernel (tiles_p 0: not launched)
-    int n_part() const { return std::max(n_split, n_split_p); }
+    int few, few_rows, tiles, split, n_split;   // tile kernel
+    int tiles_p, split_p, n_split_p;            // prompt kernel (tiles_p 0: not launched)
+    // split results that the kernels keep
+    size_t results_few(const x100_kv_cfg &c, const x100_kv_batch &b) const
+    {
+        return n_split == 1 ? 0 : (size_t)b.n_seq * c.n_head_kv * few_rows * n_split;
+    }
+    size_t results_prompt(const x100_kv_cfg &c, const x100_kv_batch &b) const
+    {
+        return n_split_p == 1 ? 0 : (size_t)b.n_rows * c.n_head * n_split_p;
+    }
 };
 
 // Splits of max_kv positions for `want` of them, each of `least` positions or more and a multiple of 128.
@@ -342,17 +366,16 @@ Plan plan_of(const x100_kv_cfg &c, const x100_kv_batch &b)
     p.few = 32;
     p.split = p.split_p = 128;
     p.n_split = p.n_split_p = 1;
-    {
-        p.tiles = (int)((std::min<int64_t>(rows, p.few) + 15) / 16);
-        const int64_t base = (int64_t)p.tiles * std::min(b.n_seq, b.n_rows) * c.n_head_kv;
-        split_of(b.max_kv, std::max<int64_t>(1, 1024 / base), 256, (int64_t)1 << 30, p.split, p.n_split);
-    }
+    p.few_rows = (int)std::min<int64_t>(rows, p.few);
+    p.tiles = (p.few_rows + 15) / 16;
+    const int64_t base = (int64_t)p.tiles * std::min(b.n_seq, b.n_rows) * c.n_head_kv;
+    split_of(b.max_kv, std::max<int64_t>(1, 1024 / base), 256, (int64_t)1 << 30, p.split, p.n_split);
     if (rows > p.few) {
         p.tiles_p = (int)((rows + PROMPT_ROWS - 1) / PROMPT_ROWS);
         // tiles that have rows: no more than one per sequence besides the full ones
         const int64_t full = (int64_t)b.n_rows * G / PROMPT_ROWS + 1;
-        const int64_t base = std::min<int64_t>((int64_t)p.tiles_p * b.n_seq, full + b.n_seq) * c.n_head_kv;
-        split_of(b.max_kv, std::max<int64_t>(1, 512 / base), 512, PROMPT_SPLIT, p.split_p, p.n_split_p);
+        const int64_t base_p = std::min<int64_t>((int64_t)p.tiles_p * b.n_seq, full + b.n_seq) * c.n_head_kv;
+        split_of(b.max_kv, std::max<int64_t>(1, 512 / base_p), 512, PROMPT_SPLIT, p.split_p, p.n_split_p);
     }
     return p;
 }
@@ -365,14 +388,19 @@ template <int HD, int AT> hipError_t attn_as(const AttnArgs &a, const Plan &p, h
         else k_attn_tile<HD, AT, false><<<grid, 256, 0, s>>>(a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
+        if (p.n_split > 1) {
+            k_attn_join<HD, AT, true><<<dim3(a.b.n_seq, a.c.n_head_kv * ((a.few_rows + 3) / 4)), 256, 0, s>>>(a);
+            const hipError_t e2 = hipGetLastError();
+            if (e2 != hipSuccess) return e2;
+        }
     }
     if (p.tiles_p) {
         const hipError_t e = x100_attn_prompt_launch(a, p.tiles_p, s);
         if (e != hipSuccess) return e;
+        if (p.n_split_p > 1) k_attn_join<HD, AT, false><<<dim3(a.b.n_rows, (a.c.n_head + 3) / 4), 256, 0, s>>>(a);
+        return hipGetLastError();
     }
-    if (p.n_part() == 1) return hipSuccess;
-    k_attn_join<HD, AT><<<dim3(a.b.n_rows, (a.c.n_head + 3) / 4), 256, 0, s>>>(a);
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 }  // namespace
@@ -380,7 +408,7 @@ template <int HD, int AT> hipError_t attn_as(const AttnArgs &a, const Plan &p, h
 size_t x100_attn_paged_workspace(const x100_kv_cfg &c, const x100_kv_batch &b)
 {
     const Plan p = plan_of(c, b);
-    return p.n_part() == 1 ? 0 : (size_t)b.n_rows * c.n_head * p.n_part() * (c.head_dim + 2) * sizeof(float);
+    return (p.results_few(c, b) + p.results_prompt(c, b)) * (c.head_dim + 2) * sizeof(float);
 }
 
 hipError_t x100_attn_paged_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const void *q, int64_t ldq,
@@ -398,13 +426,17 @@ hipError_t x100_attn_paged_launch(const x100_kv_cfg &c, const x100_kv_batch &b, 
     a.scale2 = scale * 1.4426950408889634f;
     a.out = (uint16_t *)out;
     a.ldo = ldo;
-    a.part = (float *)ws;
+    const size_t n_few = p.results_few(c, b), n_p = p.results_prompt(c, b);
+    a.o_few = (float *)ws;
+    a.o_p = a.o_few + n_few * c.head_dim;
+    a.ml_few = (float2 *)(a.o_p + n_p * c.head_dim);
+    a.ml_p = a.ml_few + n_few;
     a.split = p.split;
     a.n_split = p.n_split;
     a.few = p.few;
+    a.few_rows = p.few_rows;
     a.split_p = p.split_p;
     a.n_split_p = p.n_split_p;
-    a.n_part = p.n_part();
     if (c.head_dim == 64)
         return c.act_type == X100_T_F16 ? attn_as<64, X100_T_F16>(a, p, s) : attn_as<64, X100_T_BF16>(a, p, s);
     return c.act_type == X100_T_F16 ? attn_as<128, X100_T_F16>(a, p, s) : attn_as<128, X100_T_BF16>(a, p, s);

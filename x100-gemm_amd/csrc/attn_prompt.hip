@@ -401,13 +401,14 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256, 1) void k_a
                     *(v2u *)(o + 32 * j + 8 * e) = y;
                 }
         } else {
-            float *o = part_o(a, row, head, sp, HD) + 4 * h;
+            const size_t at = part_prompt(a, q.q0, kvh, i) + sp;
+            float *o = a.o_p + at * HD + 4 * h;
 #pragma unroll
             for (int j = 0; j < NJ; j++)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     *(float4 *)(o + 32 * j + 8 * e) = make_float4(O[b][j][4 * e], O[b][j][4 * e + 1], O[b][j][4 * e + 2], O[b][j][4 * e + 3]);
-            if (h == 0) *part_ml(a, row, head, sp, HD) = make_float2(m[b], l[b]);
+            if (h == 0) a.ml_p[at] = make_float2(m[b], l[b]);
         }
     }
 }

@@ -13,12 +13,13 @@ struct PagedAttnArgs {
     float scale2;        // scale * log2(e): weights are powers of two
     uint16_t *out;
     int64_t ldo;
-    float *part;         // split results: O (not divided by l) and (m, l), see part_o
+    float *o_few, *o_p;      // split results of the tile kernel and of the prompt kernel: O (not divided by l)
+    float2 *ml_few, *ml_p;   // and (m, l); see part_few, part_prompt
     int split, n_split;  // positions per split (a multiple of 128), splits
     int few;             // sequences of up to this many rows (token, head) are the tile kernel's, longer
                          // ones the prompt kernel's
     int split_p, n_split_p;   // split, n_split of the prompt kernel
-    int n_part;          // the larger n_split: results per row and head in part
+    int few_rows;        // most rows of a sequence of the tile kernel
 };
 
 template <int T> struct Mfma16;
@@ -72,14 +73,17 @@ template <int T> X100_DEV float add2(uint32_t w, float c)
     }
 }
 
-// Where the split results of a row and head lie: O [row][head][split][HD], then (m, l) [row][head][split].
-X100_DEV float *part_o(const PagedAttnArgs &a, size_t row, int head, int sp, int hd)
+// Where the split results of row i (token, head) of a sequence and KV head begin: number `at` of the
+// kernel's results, HD floats of O each, then all (m, l).  The tile kernel's: [sequence][KV head][i < few_rows]
+// [split]; the prompt kernel's: [row * G + ...][KV head][split].
+X100_DEV size_t part_few(const PagedAttnArgs &a, int s, int kvh, int i)
 {
-    return a.part + ((row * a.c.n_head + head) * a.n_part + sp) * hd;
+    return (((size_t)s * a.c.n_head_kv + kvh) * a.few_rows + i) * a.n_split;
 }
-X100_DEV float2 *part_ml(const PagedAttnArgs &a, size_t row, int head, int sp, int hd)
+X100_DEV size_t part_prompt(const PagedAttnArgs &a, int q0, int kvh, int i)
 {
-    return (float2 *)(a.part + (size_t)a.b.n_rows * a.c.n_head * a.n_part * hd) + (row * a.c.n_head + head) * a.n_part + sp;
+    const int G = a.c.n_head / a.c.n_head_kv;
+    return (((size_t)q0 * G + i) * a.c.n_head_kv + kvh) * a.n_split_p;
 }
 
 constexpr int PROMPT_ROWS = 256;      // rows (token, head) of a block of the prompt kernel
