@@ -18,31 +18,138 @@ namespace {
 
 constexpr float NEG_INF = X100_NEG_INF;
 using AttnArgs = PagedAttnArgs;
+constexpr int TILE_SPLIT = 8192;   // most positions of a split of the tile kernel (its page list is in LDS)
 
-// One block: 16 rows (token, head) of a sequence and KV head, one split of the positions; its 4 waves
+// Positions of a split of the tile kernel: a sequence's positions in n_split equal parts, so that the blocks
+// of a batch of unequal sequences are as equal as its lengths let them be; 256 or more, whole turns of
+// four waves.
+X100_DEV int few_split(const AttnArgs &a, int kv_len)
+{
+    return max(256, ((kv_len + a.n_split - 1) / a.n_split + 127) & ~127);
+}
+
+// What a lane reads of a tile of 32 positions, as the cache holds it: K rows 8 (c / 4) + 4 h + c % 4 (h = 0,
+// 1), V block 8 g .. 8 g + 7.
+template <int HD, bool Q4> struct TileRegs;
+template <int HD> struct TileRegs<HD, false> {
+    v4u k[2][HD / 32], v[HD / 16];
+    bool ok;             // the page of the V block (and of the scores' positions) is one
+};
+template <int HD> struct TileRegs<HD, true> {
+    uint32_t k[2][HD / 32], ks[2];
+    v4u v[HD / 64], vd[HD / 64], vm[HD / 64];
+    bool ok;
+};
+
+// One block: 16 rows (token, head) of a sequence and KV head, one split of the positions; its NW waves
 // take tiles of 32 positions in turn and merge at the end.
 // Lane (c = lane % 16, g = lane / 16): query row c; of a tile the positions 8 g .. 8 g + 7.
-template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256) void k_attn_tile(const AttnArgs a)
+// The loop is bound by memory as long as loads are always in flight: K and V of the next tile are requested
+// as soon as their registers are free, the pages come from a list in LDS.
+template <int HD, int AT, bool Q4, int NW> __global__ __launch_bounds__(64 * NW, Q4 || HD == 64 ? 4 : 3) void k_attn_tile(const AttnArgs a)
 {
     constexpr int MT = Q4 ? X100_T_F16 : AT;   // type on the matrix cores
     constexpr int KS = HD / 32, NJ = HD / 16;  // steps of K Q^T, element tiles of V^T P^T
-    __shared__ float s_o[4][16][HD + 4];
-    __shared__ float s_m[4][16], s_l[4][16];
+    __shared__ union {
+        int pg[TILE_SPLIT / 16];               // pages of the split, -1 where there is none
+        float o[NW][16][HD + 4];               // at the end
+    } sh;
+    __shared__ float s_m[NW][16], s_l[NW][16];
     const int lane = threadIdx.x & 63, w = wave_id(), c = lane & 15, g = lane >> 4;
     const int sp = blockIdx.x % a.n_split, tile = blockIdx.x / a.n_split, kvh = blockIdx.y, s = blockIdx.z;
-    const int G = a.c.n_head / a.c.n_head_kv, page = a.c.page;
+    const int n_kv = a.c.n_head_kv, G = a.c.n_head / n_kv, page = a.c.page, psh = __builtin_ctz(page);
+    const int i0 = tile * 16;
+    // A short table's pages are read here, beside the lengths; a long one's when the split is known.
+    const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
+    const int n_all = (a.b.max_kv + page - 1) >> psh;
+    const bool all = n_all <= TILE_SPLIT / 16;
+    auto list = [&](int first, int n) {
+        for (int i = threadIdx.x; i < n; i += 64 * NW) {
+            const int pg = tab[first + i];
+            sh.pg[i] = pg >= 0 && pg < a.c.n_pages ? pg : -1;
+        }
+    };
+    if (all) list(0, n_all);
     const PagedSeq q = paged_seq(a.b, s);
-    const int n_rows = q.q_len * G, i0 = tile * 16;
+    const int n_rows = q.q_len * G;
     if (i0 >= n_rows || n_rows > a.few) return;
     const int pos0 = q.kv_len - q.q_len;                       // position of token 0
     const int vis = pos0 + (min(i0 + 15, n_rows - 1)) / G + 1;  // positions that the tile's last row sees
-    const int ns = max(1, (vis + a.split - 1) / a.split);
+    const int per = few_split(a, q.kv_len);
+    const int ns = max(1, (vis + per - 1) / per);
     if (sp >= ns) return;
-    const int t0 = sp * a.split, t1 = min(t0 + a.split, vis);
+    const int t0 = sp * per, t1 = min(t0 + per, vis);
+    const int pg0 = all ? 0 : t0 >> psh;                       // first page of the list
+    const int n_pg = t1 > t0 ? ((t1 - 1) >> psh) - (t0 >> psh) + 1 : 0;
+    if (!all) list(pg0, n_pg);
 
     const int i = min(i0 + c, n_rows - 1), tok = i / G, head = kvh * G + i % G;
     const int pos = pos0 + tok;
     const int pos_lo = pos0 + i0 / G;                          // the tile's first row's
+    const size_t head_bytes = page_head_bytes<HD, Q4>(page);
+    // positions up to here are seen by every row, on pages that are
+    __syncthreads();
+    bool none = false;
+    for (int i = lane; i < n_pg; i += 64) none |= sh.pg[(t0 >> psh) - pg0 + i] < 0;
+    const int whole = __any(none) ? t0 : min(t1, pos_lo + 1);
+
+    // K, and V, of tile t into registers
+    TileRegs<HD, Q4> R;
+    const uint8_t *kp = a.kp + (size_t)kvh * head_bytes, *vp = a.vp + (size_t)kvh * head_bytes;
+    auto load_k = [&](int t) __attribute__((always_inline)) {
+        const int kb = t + 8 * (c >> 2);
+        const int pg = kb < t1 ? sh.pg[(kb >> psh) - pg0] : -1;
+        const uint8_t *kpage = kp + (size_t)max(pg, 0) * n_kv * head_bytes;
+        const int koff = (kb & (page - 1)) + (c & 3);
+        if constexpr (!Q4) {
+            const uint16_t *kr = (const uint16_t *)kpage + koff * HD + 8 * g;
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int j = 0; j < KS; j++) R.k[h][j] = *(const v4u *)(kr + 4 * h * HD + 32 * j);
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint32_t *kr = (const uint32_t *)kpage + (koff + 4 * h) * (HD / 8) + g * KS;
+                if constexpr (KS == 4) {
+                    const v4u x = __builtin_nontemporal_load((const v4u *)kr);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) R.k[h][j] = x[j];
+                } else {
+                    const v2u x = *(const v2u *)kr;
+                    R.k[h][0] = x[0];
+                    R.k[h][1] = x[1];
+                }
+                R.ks[h] = ((const uint32_t *)(kpage + page * HD / 2))[(koff + 4 * h) * (HD / 32) + g * HD / 128];
+            }
+        }
+    };
+    auto load_v = [&](int t) __attribute__((always_inline)) {
+        const int vb = t + 8 * g;
+        const int pg = vb < t1 ? sh.pg[(vb >> psh) - pg0] : -1;
+        R.ok = pg >= 0;
+        const uint8_t *vpage = vp + (size_t)max(pg, 0) * n_kv * head_bytes;
+        const int vblk = (vb & (page - 1)) >> 3;
+        if constexpr (!Q4) {
+            const uint16_t *vr = (const uint16_t *)vpage + vblk * (HD * 8) + 8 * c;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) R.v[j] = *(const v4u *)(vr + 128 * j);
+        } else {
+            const uint32_t *vr = (const uint32_t *)vpage + vblk * HD + 4 * c;
+            const uint8_t *vs = vpage + page * HD / 2 + (vblk * (HD / 32) + (c >> 3)) * 32;
+#pragma unroll
+            for (int u = 0; u < HD / 64; u++) {   // elements 64 u + 4 c .. + 3, of group 2 u + c / 8
+                R.v[u] = __builtin_nontemporal_load((const v4u *)(vr + 64 * u));
+                R.vd[u] = *(const v4u *)(vs + 64 * u);
+                R.vm[u] = *(const v4u *)(vs + 64 * u + 16);
+            }
+        }
+    };
+    const int tw = t0 + 32 * w;
+    if (tw < t1) {
+        load_k(tw);
+        load_v(tw);
+    }
 
     v4u qf[KS];
     float sc2 = a.scale2;
@@ -64,11 +171,9 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256) void k_attn
 #pragma unroll
             for (int j = 0; j < KS; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const v2h h = {(_Float16)ldexpf(bf2f(qf[j][e] & 0xffffu), -ex),
-                                   (_Float16)ldexpf(__uint_as_float(qf[j][e] & 0xffff0000u), -ex)};
-                    qf[j][e] = __builtin_bit_cast(uint32_t, h);
-                }
+                for (int e = 0; e < 4; e++)
+                    qf[j][e] = pack2<X100_T_F16>(ldexpf(bf2f(qf[j][e] & 0xffffu), -ex),
+                                                 ldexpf(__uint_as_float(qf[j][e] & 0xffff0000u), -ex));
         }
     }
 
@@ -76,55 +181,39 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256) void k_attn
 #pragma unroll
     for (int j = 0; j < NJ; j++) o[j] = v4f{0, 0, 0, 0};
     float m = NEG_INF, msub = 0.0f, l = 0.0f;
-    const size_t head_bytes = page_head_bytes<HD, Q4>(page);
-    const int psh = __builtin_ctz(page);
-    const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
 
-    for (int t = t0 + 32 * w; t < t1; t += 128) {
-        // pages of the two 8-position blocks this lane reads: K rows 8 (c / 4) .., V block 8 g
-        const int kb = t + 8 * (c >> 2), vb = t + 8 * g;
-        const int kpg = kb < t1 ? tab[kb >> psh] : -1, vpg = vb < t1 ? tab[vb >> psh] : -1;
-        const bool kok = kpg >= 0 && kpg < a.c.n_pages, vok = vpg >= 0 && vpg < a.c.n_pages;
-        const uint8_t *kpage = a.kp + ((size_t)(kok ? kpg : 0) * a.c.n_head_kv + kvh) * head_bytes;
-        const uint8_t *vpage = a.vp + ((size_t)(vok ? vpg : 0) * a.c.n_head_kv + kvh) * head_bytes;
-        const int koff = (kb & (page - 1)) + (c & 3), vblk = (vb & (page - 1)) >> 3;
-
-        // S^T: tile row r of half h is position 8 (r / 4) + 4 h + r % 4, so that lane (c, g) receives
-        // positions 8 g + 4 h .. + 3 of row c
-        v4f sc[2] = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}};
+    // S^T: tile row r of half h is position 8 (r / 4) + 4 h + r % 4, so that lane (c, g) receives
+    // positions 8 g + 4 h .. + 3 of row c
+    v4f sc[2];
+    auto scores = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
+            v4f y = {0, 0, 0, 0};
             if constexpr (!Q4) {
-                const uint16_t *kr = (const uint16_t *)kpage + (size_t)(koff + 4 * h) * HD;
 #pragma unroll
-                for (int j = 0; j < KS; j++) sc[h] = Mfma16<MT>::mul(*(const v4u *)(kr + 32 * j + 8 * g), qf[j], sc[h]);
+                for (int j = 0; j < KS; j++) y = Mfma16<MT>::mul(R.k[h][j], qf[j], y);
             } else {
-                const uint32_t *kr = (const uint32_t *)kpage + (size_t)(koff + 4 * h) * (HD / 8) + g * KS;
-                const uint32_t ds = ((const uint32_t *)(kpage + page * HD / 2))[(size_t)(koff + 4 * h) * (HD / 32) + g * HD / 128];
-                const _Float16 d1 = __builtin_bit_cast(_Float16, (uint16_t)ds), m1 = __builtin_bit_cast(_Float16, (uint16_t)(ds >> 16));
-                const v2h d2 = {d1, d1}, m2 = {m1, m1};
+                const v2h d2 = as_h2((R.ks[h] & 0xffffu) * 0x10001u), m2 = as_h2((R.ks[h] >> 16) * 0x10001u);
 #pragma unroll
                 for (int j = 0; j < KS; j++) {
                     v2h n[4];
-                    q4_unpack(kr[j], n);
+                    q4_unpack(R.k[h][j], n);
                     v4u k;
 #pragma unroll
                     for (int e = 0; e < 4; e++) k[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n[e], d2, m2));
-                    sc[h] = Mfma16<MT>::mul(k, qf[j], sc[h]);
+                    y = Mfma16<MT>::mul(k, qf[j], y);
                 }
             }
+            sc[h] = y;
         }
-        // weights
-        float x[8];
-        float mx = NEG_INF;
-        const bool whole = t + 31 <= pos_lo && __all(vok);
+    };
+    // The weights p.  The maximum may stay up to 8 (a factor of 256) behind: every sum is relative to it.
+    v4u p;
+    auto weights = [&]() __attribute__((always_inline)) {
+        float mx = fmaxf(sc[0][0], sc[1][0]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            x[e] = sc[e >> 2][e & 3] * sc2;
-            if (!whole && !(vok && vb + e <= pos)) x[e] = NEG_INF;
-            mx = fmaxf(mx, x[e]);
-        }
-        // The maximum may stay up to 8 (a factor of 256) behind: every sum is relative to it
+        for (int e = 1; e < 4; e++) mx = fmaxf(fmaxf(mx, sc[0][e]), sc[1][e]);
+        mx *= sc2;
         if (__any(mx > m + 8.0f)) {
             mx = fmaxf(mx, xor16_f(mx));
             mx = fmaxf(mx, xor32_f(mx));
@@ -136,137 +225,144 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256) void k_attn
 #pragma unroll
             for (int j = 0; j < NJ; j++) o[j] *= f;
         }
-        v4u p;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const float p0 = __builtin_amdgcn_exp2f(x[2 * e] - msub), p1 = __builtin_amdgcn_exp2f(x[2 * e + 1] - msub);
-            l += p0 + p1;
-            p[e] = f2act<MT>(p0) | f2act<MT>(p1) << 16;
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e >> 1][2 * (e & 1)], sc2, -msub));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e >> 1][2 * (e & 1) + 1], sc2, -msub));
+            p[e] = pack2<MT>(p0, p1);
+            l = add2<MT>(p[e], l);
         }
+    };
+
+    int t = tw;
+    for (; t + 32 <= whole; t += 32 * NW) {
+        const int tn = t + 32 * NW;
+        scores();
+        if (tn < t1) load_k(tn);
+        weights();
+        // O^T += V^T P^T
+        if constexpr (!Q4) {
+#pragma unroll
+            for (int j = 0; j < NJ; j++) o[j] = Mfma16<MT>::mul(R.v[j], p, o[j]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < HD / 64; u++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) o[4 * u + k] = Mfma16<MT>::mul(q4_v(R.v[u][k], R.vd[u], R.vm[u]), p, o[4 * u + k]);
+        }
+        if (tn < t1) load_v(tn);
+    }
+    // Tiles that not every row sees whole, one element tile of V per turn, the accumulators and operands
+    // moving up (unrolled, this would cost the loop above its registers).
+    for (; t < t1; t += 32 * NW) {
+        const int vb = t + 8 * g;
+        scores();
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (!(R.ok && vb + e <= pos)) sc[e >> 2][e & 3] = NEG_INF;
+        weights();
         // positions that no row of the sequence has, and those of a page that is none: V as zeros
         uint32_t keep[4];
-        {
-            const int n = vok ? q.kv_len - vb : 0;
+        const int n = R.ok ? q.kv_len - vb : 0;
 #pragma unroll
-            for (int e = 0; e < 4; e++) keep[e] = n >= 2 * e + 2 ? ~0u : (n == 2 * e + 1 ? 0xffffu : 0u);
-        }
-        // O^T += V^T P^T
-        v4u vf[NJ];
-        if constexpr (!Q4) {
-            const uint16_t *vr = (const uint16_t *)vpage + (size_t)vblk * HD * 8;
+        for (int e = 0; e < 4; e++) keep[e] = n >= 2 * e + 2 ? ~0u : (n == 2 * e + 1 ? 0xffffu : 0u);
+#pragma unroll 1
+        for (int turn = 0; turn < NJ; turn++) {
+            v4u vf;
+            if constexpr (!Q4) {
+                vf = R.v[0];
 #pragma unroll
-            for (int j = 0; j < NJ; j++) vf[j] = *(const v4u *)(vr + (16 * j + c) * 8);
-        } else {
-            const uint32_t *vr = (const uint32_t *)vpage + (size_t)vblk * HD;
-            const uint8_t *vs = vpage + page * HD / 2 + (size_t)vblk * (HD / 32) * 32;
+                for (int j = 0; j + 1 < NJ; j++) R.v[j] = R.v[j + 1];
+            } else {
+                vf = q4_v(R.v[0][0], R.vd[0], R.vm[0]);
 #pragma unroll
-            for (int u = 0; u < HD / 64; u++) {   // elements 64 u + 4 c .. + 3, of group 2 u + c / 8
-                const v4u wd = *(const v4u *)(vr + 64 * u + 4 * c);
-                v4u d = *(const v4u *)(vs + (2 * u + (c >> 3)) * 32), mm = *(const v4u *)(vs + (2 * u + (c >> 3)) * 32 + 16);
+                for (int j = 0; j + 1 < NJ; j++) R.v[j >> 2][j & 3] = R.v[(j + 1) >> 2][(j + 1) & 3];
+                if (turn == 3) {
+                    R.vd[0] = R.vd[HD / 64 - 1];
+                    R.vm[0] = R.vm[HD / 64 - 1];
+                }
+            }
+            // An element that is not finite, in a position that only some of the tile's rows see, must
+            // not meet the others' zero weights: such elements are taken out, and added as infinities
+            // (both signs: a NaN) to the rows that see them.
+            constexpr uint32_t EXP = MT == X100_T_F16 ? 0x7c00u : 0x7f80u, ONE = MT == X100_T_F16 ? 0x3c00u : 0x3f80u;
+            bool odd = false;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t y = vf[e] & keep[e];
+                vf[e] = y;
+                odd |= (y & EXP) == EXP || (y & (EXP << 16)) == EXP << 16;
+            }
+            if (__any(odd)) {
+                v4u up = {0, 0, 0, 0}, dn = {0, 0, 0, 0}, see = {0, 0, 0, 0};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    d[e] &= keep[e];
-                    mm[e] &= keep[e];
-                }
+                    uint32_t y = vf[e], uu = 0, dd = 0;
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    v2h n[4];
-                    q4_unpack(wd[k], n);
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        vf[4 * u + k][e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n[e], as_h2(d[e]), as_h2(mm[e])));
-                }
-            }
-        }
-        if constexpr (!Q4)
-            if (!whole)
-#pragma unroll
-                for (int j = 0; j < NJ; j++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) vf[j][e] &= keep[e];
-        // An element that is not finite, in a position that only some of the tile's rows see, must not
-        // meet the others' zero weights: such elements are taken out, and added as infinities (both
-        // signs: a NaN) to the rows that see them.
-        bool odd = false;
-        if (!whole) {
-            constexpr uint32_t EXP = MT == X100_T_F16 ? 0x7c00u : 0x7f80u;
-            uint32_t any = 0;
-#pragma unroll
-            for (int j = 0; j < NJ; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    any |= (uint32_t)((vf[j][e] & EXP) == EXP) | (uint32_t)((vf[j][e] & (EXP << 16)) == EXP << 16);
-            odd = __any(any);
-            if (odd) {
-                constexpr uint32_t ONE = MT == X100_T_F16 ? 0x3c00u : 0x3f80u;
-                v4u see;
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    see[e] = (vok && vb + 2 * e <= pos ? ONE : 0u) | (vok && vb + 2 * e + 1 <= pos ? ONE << 16 : 0u);
-#pragma unroll
-                for (int j = 0; j < NJ; j++) {
-                    v4u up, dn;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        uint32_t u = 0, dd = 0, fine = vf[j][e];
-#pragma unroll
-                        for (int b = 0; b < 32; b += 16) {
-                            const uint32_t v = vf[j][e] >> b & 0xffffu, ex = v & EXP;
-                            if (ex == EXP) {
-                                const bool nan = (v & 0x7fffu) != EXP;
-                                if (nan || !(v & 0x8000u)) u |= ONE << b;
-                                if (nan || (v & 0x8000u)) dd |= ONE << b;
-                                fine &= ~(0xffffu << b);
-                            }
+                    for (int b = 0; b < 32; b += 16) {
+                        const uint32_t z = y >> b & 0xffffu;
+                        if ((z & EXP) == EXP) {
+                            const bool nan = (z & 0x7fffu) != EXP;
+                            if (nan || !(z & 0x8000u)) uu |= ONE << b;
+                            if (nan || (z & 0x8000u)) dd |= ONE << b;
+                            y &= ~(0xffffu << b);
                         }
-                        up[e] = u;
-                        dn[e] = dd;
-                        vf[j][e] = fine;
                     }
-                    const v4f z = {0, 0, 0, 0};
-                    const v4f nu = Mfma16<MT>::mul(up, see, z), nd = Mfma16<MT>::mul(dn, see, z);
+                    vf[e] = y;
+                    up[e] = uu;
+                    dn[e] = dd;
+                    see[e] = (R.ok && vb + 2 * e <= pos ? ONE : 0u) | (R.ok && vb + 2 * e + 1 <= pos ? ONE << 16 : 0u);
+                }
+                const v4f z4 = {0, 0, 0, 0};
+                const v4f nu = Mfma16<MT>::mul(up, see, z4), nd = Mfma16<MT>::mul(dn, see, z4);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if (nu[e] > 0.0f) o[j][e] += __builtin_inff();
-                        if (nd[e] > 0.0f) o[j][e] -= __builtin_inff();
-                    }
+                for (int e = 0; e < 4; e++) {
+                    if (nu[e] > 0.0f) o[0][e] += __builtin_inff();
+                    if (nd[e] > 0.0f) o[0][e] -= __builtin_inff();
                 }
             }
-        }
+            const v4f first = Mfma16<MT>::mul(vf, p, o[0]);
 #pragma unroll
-        for (int j = 0; j < NJ; j++) o[j] = Mfma16<MT>::mul(vf[j], p, o[j]);
+            for (int j = 0; j + 1 < NJ; j++) o[j] = o[j + 1];
+            o[NJ - 1] = first;
+        }
+        if (t + 32 * NW < t1) {
+            load_k(t + 32 * NW);
+            load_v(t + 32 * NW);
+        }
     }
 
-    // the 4 lane groups hold parts of l; then the 4 waves' m, l, O are merged
+    // the 4 lane groups hold parts of l; then the waves' m, l, O are merged
     l += xor16_f(l);
     l += xor32_f(l);
     if (g == 0) {
         s_m[w][c] = m;
         s_l[w][c] = l;
     }
+    __syncthreads();   // the page list is done with
 #pragma unroll
     for (int j = 0; j < NJ; j++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const int el = Q4 ? 4 * (4 * g + e) + (j & 3) + 64 * (j >> 2) : 16 * j + 4 * g + e;
-            s_o[w][c][el] = o[j][e];
+            sh.o[w][c][el] = o[j][e];
         }
     __syncthreads();
-    for (int u = threadIdx.x; u < 16 * (HD / 2); u += 256) {
+    for (int u = threadIdx.x; u < 16 * (HD / 2); u += 64 * NW) {
         const int r = u / (HD / 2), el = u % (HD / 2) * 2;
         if (i0 + r >= n_rows) continue;
         float mm = NEG_INF;
 #pragma unroll
-        for (int k = 0; k < 4; k++) mm = fmaxf(mm, s_m[k][r]);
+        for (int k = 0; k < NW; k++) mm = fmaxf(mm, s_m[k][r]);
         const float ms = mm == NEG_INF ? 0.0f : mm;
         float ls = 0.0f, y0 = 0.0f, y1 = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < NW; k++) {
             const float f = __builtin_amdgcn_exp2f(s_m[k][r] - ms);
             if (s_m[k][r] == NEG_INF) continue;
             ls = __builtin_fmaf(s_l[k][r], f, ls);
-            y0 = __builtin_fmaf(s_o[k][r][el], f, y0);
-            y1 = __builtin_fmaf(s_o[k][r][el + 1], f, y1);
+            y0 = __builtin_fmaf(sh.o[k][r][el], f, y0);
+            y1 = __builtin_fmaf(sh.o[k][r][el + 1], f, y1);
         }
         const int tk = (i0 + r) / G, hh = kvh * G + (i0 + r) % G;
         if (ns == 1) {
@@ -307,24 +403,38 @@ template <int HD, int AT, bool FEW> __global__ __launch_bounds__(256) void k_att
         kvh = head / G;
         i = (row - q.q0) * G + head % G;
     }
-    const int tr = FEW ? 16 : PROMPT_ROWS, split = FEW ? a.split : a.split_p;
+    const int tr = FEW ? 16 : PROMPT_ROWS, split = FEW ? few_split(a, q.kv_len) : a.split_p;
     const int vis = q.kv_len - q.q_len + min(i / tr * tr + tr - 1, q.q_len * G - 1) / G + 1;
     const int ns = (vis + split - 1) / split;
     if (ns <= 1) return;
     const size_t at = FEW ? part_few(a, s, kvh, i) : part_prompt(a, q.q0, kvh, i);
     const float2 *ml = (FEW ? a.ml_few : a.ml_p) + at;
     const float *po = (FEW ? a.o_few : a.o_p) + at * HD + lane * E;
+    // (m, l) by lane, up to 64 splits at a time; the splits' O eight at a time
     float m = NEG_INF;
-    for (int k = 0; k < ns; k++) m = fmaxf(m, ml[k].x);
+    for (int k = lane; k < ns; k += 64) m = fmaxf(m, ml[k].x);
+    m = wave_max_u(m);
     const float ms = m == NEG_INF ? 0.0f : m;
     float l = 0.0f, y[E] = {};
-    for (int k = 0; k < ns; k++) {
-        const float2 v = ml[k];
-        if (v.x == NEG_INF) continue;
-        const float f = __builtin_amdgcn_exp2f(v.x - ms);
-        l = __builtin_fmaf(v.y, f, l);
+    for (int k0 = 0; k0 < ns; k0 += 64) {
+        const float2 v = k0 + lane < ns ? ml[k0 + lane] : make_float2(NEG_INF, 0.0f);
+        const float fl = __builtin_amdgcn_exp2f(v.x - ms);   // 0 where a split has no position
+        l += wave_sum_uf(v.x == NEG_INF ? 0.0f : v.y * fl);
+        const int n = min(64, ns - k0);
+        for (int k = 0; k < n; k += 8) {
+            float b[8][E];
 #pragma unroll
-        for (int e = 0; e < E; e++) y[e] = __builtin_fmaf(po[(size_t)k * HD + e], f, y[e]);
+            for (int u = 0; u < 8; u++)
+#pragma unroll
+                for (int e = 0; e < E; e++) b[u][e] = po[(size_t)(k0 + min(k + u, n - 1)) * HD + e];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(fl), k + u));
+                if (k + u < n && f != 0.0f)   // a split without positions has no O
+#pragma unroll
+                    for (int e = 0; e < E; e++) y[e] = __builtin_fmaf(b[u][e], f, y[e]);
+            }
+        }
     }
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
     uint16_t *o = a.out + (size_t)(q.q0 + i / G) * a.ldo + (size_t)(kvh * G + i % G) * HD + lane * E;
@@ -369,7 +479,12 @@ Plan plan_of(const x100_kv_cfg &c, const x100_kv_batch &b)
     p.few_rows = (int)std::min<int64_t>(rows, p.few);
     p.tiles = (p.few_rows + 15) / 16;
     const int64_t base = (int64_t)p.tiles * std::min(b.n_seq, b.n_rows) * c.n_head_kv;
-    split_of(b.max_kv, std::max<int64_t>(1, 1024 / base), 256, (int64_t)1 << 30, p.split, p.n_split);
+    // A block per CU where rows of 16 bits are read (256 blocks of four waves keep HBM busy: 64 sequences of up
+    // to 4096 positions, us with 256 / 512 / 1024 blocks wanted: 70.6 / 78.6 / 77.2), three where 4-bit codes have
+    // to be unpacked (16 of up to 60001: 115.8 / 113.9 / 101.8, 768: 98.4).  Up to 512 positions one block is
+    // faster than two and their join (9.6 / 12.6 us).
+    const int64_t blocks = c.kv_type == X100_KV_Q4 ? 768 : 256;
+    split_of(b.max_kv, b.max_kv <= 512 ? 1 : std::max<int64_t>(1, blocks / base), 256, TILE_SPLIT, p.split, p.n_split);
     if (rows > p.few) {
         p.tiles_p = (int)((rows + PROMPT_ROWS - 1) / PROMPT_ROWS);
         // tiles that have rows: no more than one per sequence besides the full ones
@@ -384,8 +499,8 @@ template <int HD, int AT> hipError_t attn_as(const AttnArgs &a, const Plan &p, h
 {
     if (p.tiles) {
         const dim3 grid((unsigned)(p.tiles * p.n_split), a.c.n_head_kv, a.b.n_seq);
-        if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true><<<grid, 256, 0, s>>>(a);
-        else k_attn_tile<HD, AT, false><<<grid, 256, 0, s>>>(a);
+        if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true, 4><<<grid, 256, 0, s>>>(a);
+        else k_attn_tile<HD, AT, false, 4><<<grid, 256, 0, s>>>(a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
         if (p.n_split > 1) {

@@ -73,14 +73,27 @@ X100_DEV uint32_t q4_code(const Q4Scale &s, float x)
 }
 
 // The 8 numbers of a word as fp16 codes 0 .. 15, pairs (0,1), (2,3), (4,5), (6,7): a code under the
-// exponent of 1024 reads as 1024 + n (low nibble of a byte) or 1024 + 16 n (high), both exact.
+// exponent of 1024 reads as 1024 + n (low nibble of a byte) or 1024 + 16 n (high), both exact.  The
+// exponent is kept in a vector register: with it v_and_or_b32 takes a mask and it in one instruction.
 X100_DEV void q4_unpack(uint32_t w, v2h (&n)[4])
 {
+    uint32_t ex;
+    asm("v_mov_b32 %0, 0x64006400" : "=v"(ex));
     const v2h k1024 = {(_Float16)1024.0f, (_Float16)1024.0f};
     const v2h k16 = {(_Float16)0.0625f, (_Float16)0.0625f}, k64 = {(_Float16)-64.0f, (_Float16)-64.0f};
     const uint32_t w8 = w >> 8;
-    n[0] = __builtin_bit_cast(v2h, (w & 0x000f000fu) | 0x64006400u) - k1024;
-    n[1] = __builtin_elementwise_fma(__builtin_bit_cast(v2h, (w & 0x00f000f0u) | 0x64006400u), k16, k64);
-    n[2] = __builtin_bit_cast(v2h, (w8 & 0x000f000fu) | 0x64006400u) - k1024;
-    n[3] = __builtin_elementwise_fma(__builtin_bit_cast(v2h, (w8 & 0x00f000f0u) | 0x64006400u), k16, k64);
+    n[0] = as_h2((w & 0x000f000fu) | ex) - k1024;
+    n[1] = __builtin_elementwise_fma(as_h2((w & 0x00f000f0u) | ex), k16, k64);
+    n[2] = as_h2((w8 & 0x000f000fu) | ex) - k1024;
+    n[3] = __builtin_elementwise_fma(as_h2((w8 & 0x00f000f0u) | ex), k16, k64);
+}
+// A V word's 8 positions as fp16 values, d and m of the 8 positions.
+X100_DEV v4u q4_v(uint32_t w, v4u d, v4u m)
+{
+    v2h n[4];
+    q4_unpack(w, n);
+    v4u r;
+#pragma unroll
+    for (int e = 0; e < 4; e++) r[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n[e], as_h2(d[e]), as_h2(m[e])));
+    return r;
 }
