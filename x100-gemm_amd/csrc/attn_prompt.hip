@@ -9,8 +9,8 @@
 // does not depend on the other's:
 //   first half    weights of block 0, tile i        beside scores of block 1, tile i, and its products of tile i - 1
 //   second half   weights of block 1, tile i        beside scores of block 0, tile i + 1, and its products of tile i
-// The operands of K and V are read from LDS once per tile, in the second half, and kept for both blocks.  K and
-// V tiles come by asynchronous copies from the cache into rings of four tiles in LDS (4-bit pages: through
+// The operands of K and V are read from LDS once per tile, in the first half (as soon as the last ones have been
+// used), and kept for both blocks.  K and V tiles come by asynchronous copies from the cache into rings of four tiles in LDS (4-bit pages: through
 // registers, where they become fp16), read by all four waves.
 //
 // The running maximum m may lag far behind (LAG), so that O and l are rescaled seldom.
@@ -190,7 +190,7 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256, 1) void k_a
             }
         }
     };
-    // Second half of step i: K(i + 1) and V(i) are in LDS for every wave, the slots of K(i) and V(i - 1) free.
+    // Step i: K(i + 1) and V(i) are in LDS for every wave, the slots of K(i) and V(i - 1) free.
     auto next_tiles = [&](int i) __attribute__((always_inline)) {
         if constexpr (!Q4) {
             asm volatile("s_waitcnt vmcnt(%0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::"n"(2 * ND) : "memory");
@@ -278,6 +278,20 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256, 1) void k_a
                 l[b] = add2<MT>(p, l[b]);
             }
     };
+    // The half's weights are made in it (the compiler would move them to where they are used).
+    auto here = [&](int b) __attribute__((always_inline)) {
+        asm volatile("" ::"v"(P[b][0]), "v"(P[b][1]), "v"(l[b]), "v"(mx[b ^ 1]));
+    };
+    // Order of a half: after each matrix instruction the vector instructions that fit beside it; in the
+    // first half the next operands' reads.
+    auto interleave = [&]<bool FIRST>() __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 0; g < KS + 2 * NJ; g++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x402, 4, 0);
+            if (FIRST && g >= KS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+    };
     // Validity of the tile's two groups of 16 positions (their pages).
     auto ok16 = [&](int i, int k) {
         const int t = t0 + 32 * i + 16 * k;
@@ -344,25 +358,29 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256, 1) void k_a
         scores(0);
         maximum(0);
         for (int i = 0; i < n; i++) {
-            if (i >= nw) mask(i, 0);
-            rescale(0);
-            scores(1);
-            weights(0);
-            products(1);
-            maximum(1);
-
             next_tiles(i);
             if (i >= nw) {
                 clean(i);
-                mask(i, 1);
+                mask(i, 0);
             }
-            rescale(1);
+            rescale(0);
+            scores(1);
+            weights(0);
             read_k(i + 1);
+            products(1);
             read_v(i);
+            maximum(1);
+            interleave.template operator()<true>();
+            here(0);
+
+            if (i >= nw) mask(i, 1);
+            rescale(1);
             scores(0);
             weights(1);
             products(0);
             maximum(0);
+            interleave.template operator()<false>();
+            here(1);
         }
         products(1);
         if constexpr (!Q4) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // every copy into this block's LDS
