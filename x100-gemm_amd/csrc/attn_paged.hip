@@ -20,14 +20,6 @@ constexpr float NEG_INF = X100_NEG_INF;
 using AttnArgs = PagedAttnArgs;
 constexpr int TILE_SPLIT = 8192;   // most positions of a split of the tile kernel (its page list is in LDS)
 
-// Positions of a split of the tile kernel: a sequence's positions in n_split equal parts, so that the blocks
-// of a batch of unequal sequences are as equal as its lengths let them be; 256 or more, whole turns of
-// four waves.
-X100_DEV int few_split(const AttnArgs &a, int kv_len)
-{
-    return max(256, ((kv_len + a.n_split - 1) / a.n_split + 127) & ~127);
-}
-
 // What a lane reads of a tile of 32 positions, as the cache holds it: K rows 8 (c / 4) + 4 h + c % 4 (h = 0,
 // 1), V block 8 g .. 8 g + 7.
 template <int HD, bool Q4> struct TileRegs;
@@ -72,10 +64,10 @@ template <int HD, int AT, bool Q4, int NW> __global__ __launch_bounds__(64 * NW,
     if (all) list(0, n_all);
     const PagedSeq q = paged_seq(a.b, s);
     const int n_rows = q.q_len * G;
-    if (i0 >= n_rows || n_rows > a.few) return;
+    if (i0 >= n_rows) return;
     const int pos0 = q.kv_len - q.q_len;                       // position of token 0
     const int vis = pos0 + (min(i0 + 15, n_rows - 1)) / G + 1;  // positions that the tile's last row sees
-    const int per = few_split(a, q.kv_len);
+    const int per = split_of_seq(a, q.kv_len);
     const int ns = max(1, (vis + per - 1) / per);
     if (sp >= ns) return;
     const int t0 = sp * per, t1 = min(t0 + per, vis);
@@ -370,160 +362,134 @@ template <int HD, int AT, bool Q4, int NW> __global__ __launch_bounds__(64 * NW,
             const uint32_t b = ls == 0.0f ? 0u : f2act<AT>(y0 * f) | f2act<AT>(y1 * f) << 16;
             *(uint32_t *)(a.out + (size_t)(q.q0 + tk) * a.ldo + (size_t)hh * HD + el) = b;
         } else {
-            const size_t at = part_few(a, s, kvh, i0 + r) + sp;
-            *(float2 *)(a.o_few + at * HD + el) = make_float2(y0, y1);
-            if (el == 0) a.ml_few[at] = make_float2(mm, ls);
+            const size_t at = part_at(a, q.q0, kvh, i0 + r) + sp;
+            *(float2 *)(a.part_o + at * HD + el) = make_float2(y0, y1);
+            if (el == 0) a.part_ml[at] = make_float2(mm, ls);
         }
     }
 }
 
-// Merges the splits of rows that have more than one: a wave per row (token, head), HD / 64 elements per
-// lane.  FEW: the tile kernel's rows, blockIdx.x = sequence, y = KV head and four rows; else the prompt
-// kernel's, x = token row, y = four heads.
-template <int HD, int AT, bool FEW> __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a)
+// Merges the splits of rows that have more than one: HD / 4 lanes per (row, head), 4 elements each; x = token
+// row, y = the heads of a block.
+template <int HD, int AT> __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a)
 {
-    constexpr int E = HD / 64;
-    const int lane = threadIdx.x & 63, w = wave_id(), G = a.c.n_head / a.c.n_head_kv;
-    int s, i, kvh;
-    PagedSeq q;
-    if constexpr (FEW) {
-        const int per = (a.few_rows + 3) / 4;
-        s = blockIdx.x;
-        kvh = blockIdx.y / per;
-        i = blockIdx.y % per * 4 + w;
-        q = paged_seq(a.b, s);
-        if (i >= q.q_len * G || q.q_len * G > a.few) return;
-    } else {
-        const int row = blockIdx.x, head = blockIdx.y * 4 + w;
-        if (head >= a.c.n_head) return;
-        s = paged_find(a.b, row);
-        if (s >= a.b.n_seq) return;
-        q = paged_seq(a.b, s);
-        if (q.q_len * G <= a.few || row < q.q0) return;
-        kvh = head / G;
-        i = (row - q.q0) * G + head % G;
-    }
-    const int tr = FEW ? 16 : PROMPT_ROWS, split = FEW ? few_split(a, q.kv_len) : a.split_p;
+    constexpr int L = HD / 4;
+    const int G = a.c.n_head / a.c.n_head_kv, row = blockIdx.x;
+    const int head = blockIdx.y * (256 / L) + threadIdx.x / L, l4 = threadIdx.x % L;
+    const int s = paged_find(a.b, row);
+    if (s >= a.b.n_seq) return;
+    const PagedSeq q = paged_seq(a.b, s);
+    if (q.q_len <= 0 || row < q.q0) return;
+    const int hd = min(head, a.c.n_head - 1), kvh = hd / G, i = (row - q.q0) * G + hd % G;
+    const int tr = a.tile_rows, per = split_of_seq(a, q.kv_len);
     const int vis = q.kv_len - q.q_len + min(i / tr * tr + tr - 1, q.q_len * G - 1) / G + 1;
-    const int ns = (vis + split - 1) / split;
-    if (ns <= 1) return;
-    const size_t at = FEW ? part_few(a, s, kvh, i) : part_prompt(a, q.q0, kvh, i);
-    const float2 *ml = (FEW ? a.ml_few : a.ml_p) + at;
-    const float *po = (FEW ? a.o_few : a.o_p) + at * HD + lane * E;
-    // (m, l) by lane, up to 64 splits at a time; the splits' O eight at a time
+    const int ns = (vis + per - 1) / per;
+    const size_t at = part_at(a, q.q0, kvh, i);
+    const float2 *ml = a.part_ml + at;
+    const float4 *po = (const float4 *)(a.part_o + at * HD) + l4;
     float m = NEG_INF;
-    for (int k = lane; k < ns; k += 64) m = fmaxf(m, ml[k].x);
-    m = wave_max_u(m);
+    for (int k = l4; k < ns; k += L) m = fmaxf(m, ml[k].x);
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, L));
+    if (ns <= 1 || head >= a.c.n_head) return;
     const float ms = m == NEG_INF ? 0.0f : m;
-    float l = 0.0f, y[E] = {};
-    for (int k0 = 0; k0 < ns; k0 += 64) {
-        const float2 v = k0 + lane < ns ? ml[k0 + lane] : make_float2(NEG_INF, 0.0f);
-        const float fl = __builtin_amdgcn_exp2f(v.x - ms);   // 0 where a split has no position
-        l += wave_sum_uf(v.x == NEG_INF ? 0.0f : v.y * fl);
-        const int n = min(64, ns - k0);
-        for (int k = 0; k < n; k += 8) {
-            float b[8][E];
+    float l = 0.0f;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k = 0; k < ns; k += 8) {   // eight at a time on their way
+        float2 v[8];
+        float4 b[8];
 #pragma unroll
-            for (int u = 0; u < 8; u++)
+        for (int u = 0; u < 8; u++) {
+            v[u] = ml[min(k + u, ns - 1)];
+            b[u] = po[(size_t)min(k + u, ns - 1) * L];
+        }
 #pragma unroll
-                for (int e = 0; e < E; e++) b[u][e] = po[(size_t)(k0 + min(k + u, n - 1)) * HD + e];
-#pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(fl), k + u));
-                if (k + u < n && f != 0.0f)   // a split without positions has no O
-#pragma unroll
-                    for (int e = 0; e < E; e++) y[e] = __builtin_fmaf(b[u][e], f, y[e]);
-            }
+        for (int u = 0; u < 8; u++) {
+            if (k + u >= ns || v[u].x == NEG_INF) continue;   // a split without positions has no O
+            const float f = __builtin_amdgcn_exp2f(v[u].x - ms);
+            l = __builtin_fmaf(v[u].y, f, l);
+            y.x = __builtin_fmaf(b[u].x, f, y.x);
+            y.y = __builtin_fmaf(b[u].y, f, y.y);
+            y.z = __builtin_fmaf(b[u].z, f, y.z);
+            y.w = __builtin_fmaf(b[u].w, f, y.w);
         }
     }
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t *o = a.out + (size_t)(q.q0 + i / G) * a.ldo + (size_t)(kvh * G + i % G) * HD + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; e++) o[e] = l == 0.0f ? 0 : (uint16_t)f2act<AT>(y[e] * f);
+    v2u o = {0, 0};
+    if (l != 0.0f) o = v2u{pack2<AT>(y.x * f, y.y * f), pack2<AT>(y.z * f, y.w * f)};
+    *(v2u *)(a.out + (size_t)row * a.ldo + (size_t)head * HD + 4 * l4) = o;
 }
 
-// How a call is laid out.  Sequences of up to `few` rows (token, head) go to the tile kernel, longer ones
-// to the prompt kernel; positions are split so that the blocks fill the chip.
+// How a call is laid out: the tile kernel where no sequence has more than FEW rows (token, head), else the
+// prompt kernel; the positions in splits, so that the blocks fill the chip.
+constexpr int FEW = 32;
 struct Plan {
-    int few, few_rows, tiles, split, n_split;   // tile kernel
-    int tiles_p, split_p, n_split_p;            // prompt kernel (tiles_p 0: not launched)
-    // split results that the kernels keep
-    size_t results_few(const x100_kv_cfg &c, const x100_kv_batch &b) const
+    bool prompt;
+    int tiles, n_split, least;
+    size_t results(const x100_kv_cfg &c, const x100_kv_batch &b) const
     {
-        return n_split == 1 ? 0 : (size_t)b.n_seq * c.n_head_kv * few_rows * n_split;
-    }
-    size_t results_prompt(const x100_kv_cfg &c, const x100_kv_batch &b) const
-    {
-        return n_split_p == 1 ? 0 : (size_t)b.n_rows * c.n_head * n_split_p;
+        return n_split == 1 ? 0 : (size_t)b.n_rows * c.n_head * n_split;
     }
 };
-
-// Splits of max_kv positions for `want` of them, each of `least` positions or more and a multiple of 128.
-void split_of(int64_t max_kv, int64_t want, int64_t least, int64_t most, int &split, int &n_split)
-{
-    int64_t s = (max_kv + want - 1) / want;
-    s = std::min(most, std::max(least, (s + 127) / 128 * 128));
-    s = std::min<int64_t>(s, (max_kv + 127) / 128 * 128);
-    split = (int)s;
-    n_split = (int)((max_kv + s - 1) / s);
-}
 
 Plan plan_of(const x100_kv_cfg &c, const x100_kv_batch &b)
 {
     Plan p = {};
     const int G = c.n_head / c.n_head_kv;
-    const int64_t rows = (int64_t)b.max_q * G;   // of the longest sequence
-    p.few = 32;
-    p.split = p.split_p = 128;
-    p.n_split = p.n_split_p = 1;
-    p.few_rows = (int)std::min<int64_t>(rows, p.few);
-    p.tiles = (p.few_rows + 15) / 16;
-    const int64_t base = (int64_t)p.tiles * std::min(b.n_seq, b.n_rows) * c.n_head_kv;
-    // A block per CU where rows of 16 bits are read (256 blocks of four waves keep HBM busy: 64 sequences of up
-    // to 4096 positions, us with 256 / 512 / 1024 blocks wanted: 70.6 / 78.6 / 77.2), three where 4-bit codes have
-    // to be unpacked (16 of up to 60001: 115.8 / 113.9 / 101.8, 768: 98.4).  Up to 512 positions one block is
-    // faster than two and their join (9.6 / 12.6 us).
-    const int64_t blocks = c.kv_type == X100_KV_Q4 ? 768 : 256;
-    split_of(b.max_kv, b.max_kv <= 512 ? 1 : std::max<int64_t>(1, blocks / base), 256, TILE_SPLIT, p.split, p.n_split);
-    if (rows > p.few) {
-        p.tiles_p = (int)((rows + PROMPT_ROWS - 1) / PROMPT_ROWS);
-        // tiles that have rows: no more than one per sequence besides the full ones
-        const int64_t full = (int64_t)b.n_rows * G / PROMPT_ROWS + 1;
-        const int64_t base_p = std::min<int64_t>((int64_t)p.tiles_p * b.n_seq, full + b.n_seq) * c.n_head_kv;
-        split_of(b.max_kv, std::max<int64_t>(1, 512 / base_p), 512, PROMPT_SPLIT, p.split_p, p.n_split_p);
+    const int64_t rows = (int64_t)b.max_q * G, kv = b.max_kv;   // of the longest sequence
+    p.prompt = rows > FEW;
+    if (!p.prompt) {
+        // A block per CU where rows of 16 bits are read (256 blocks of four waves keep HBM busy: 64 sequences of
+        // up to 4096 positions, us with 256 / 512 / 1024 blocks wanted: 70.6 / 78.6 / 77.2), three where 4-bit
+        // codes have to be unpacked (16 of up to 60001: 115.8 / 113.9 / 101.8, 768: 98.4).  Up to 512 positions
+        // one block is faster than two and their join (9.6 / 12.6 us).
+        p.least = 256;
+        p.tiles = (int)((rows + 15) / 16);
+        const int64_t base = (int64_t)p.tiles * std::min(b.n_seq, b.n_rows) * c.n_head_kv;
+        const int64_t want = kv <= 512 ? 1 : std::max<int64_t>(1, (c.kv_type == X100_KV_Q4 ? 768 : 256) / base);
+        p.n_split = (int)std::max(std::min(want, (kv + 255) / 256), (kv + TILE_SPLIT - 1) / TILE_SPLIT);
+        return p;
+    }
+    // One block per CU at a time, so rounds of 256 blocks: the number of splits with the least sum over the
+    // rounds of a block's positions and its own start and end (as long as 512 positions), the join besides.
+    p.least = 512;
+    p.tiles = (int)((rows + PROMPT_ROWS - 1) / PROMPT_ROWS);
+    const int64_t full = (int64_t)b.n_rows * G / PROMPT_ROWS + b.n_seq;   // tiles that have rows
+    const int64_t base = std::min<int64_t>((int64_t)p.tiles * b.n_seq, full) * c.n_head_kv;
+    int64_t best = 0;
+    for (int64_t n = std::max<int64_t>(1, (kv + PROMPT_SPLIT - 1) / PROMPT_SPLIT), n0 = n; n == n0 || (n <= 16 && n * 512 < kv + 512); n++) {
+        const int64_t cost = (base * n + 255) / 256 * (kv / n + 512) + (n > 1 ? 512 : 0);
+        if (n == n0 || cost < best) {
+            best = cost;
+            p.n_split = (int)n;
+        }
     }
     return p;
 }
 
 template <int HD, int AT> hipError_t attn_as(const AttnArgs &a, const Plan &p, hipStream_t s)
 {
-    if (p.tiles) {
+    if (p.prompt) {
+        const hipError_t e = x100_attn_prompt_launch(a, p.tiles, s);
+        if (e != hipSuccess) return e;
+    } else {
         const dim3 grid((unsigned)(p.tiles * p.n_split), a.c.n_head_kv, a.b.n_seq);
         if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true, 4><<<grid, 256, 0, s>>>(a);
         else k_attn_tile<HD, AT, false, 4><<<grid, 256, 0, s>>>(a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        if (p.n_split > 1) {
-            k_attn_join<HD, AT, true><<<dim3(a.b.n_seq, a.c.n_head_kv * ((a.few_rows + 3) / 4)), 256, 0, s>>>(a);
-            const hipError_t e2 = hipGetLastError();
-            if (e2 != hipSuccess) return e2;
-        }
     }
-    if (p.tiles_p) {
-        const hipError_t e = x100_attn_prompt_launch(a, p.tiles_p, s);
-        if (e != hipSuccess) return e;
-        if (p.n_split_p > 1) k_attn_join<HD, AT, false><<<dim3(a.b.n_rows, (a.c.n_head + 3) / 4), 256, 0, s>>>(a);
-        return hipGetLastError();
-    }
-    return hipSuccess;
+    if (p.n_split == 1) return hipSuccess;
+    constexpr int heads = 256 / (HD / 4);
+    k_attn_join<HD, AT><<<dim3(a.b.n_rows, (a.c.n_head + heads - 1) / heads), 256, 0, s>>>(a);
+    return hipGetLastError();
 }
 
 }  // namespace
 
 size_t x100_attn_paged_workspace(const x100_kv_cfg &c, const x100_kv_batch &b)
 {
-    const Plan p = plan_of(c, b);
-    return (p.results_few(c, b) + p.results_prompt(c, b)) * (c.head_dim + 2) * sizeof(float);
+    return plan_of(c, b).results(c, b) * (c.head_dim + 2) * sizeof(float);
 }
 
 hipError_t x100_attn_paged_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const void *q, int64_t ldq,
@@ -541,17 +507,11 @@ hipError_t x100_attn_paged_launch(const x100_kv_cfg &c, const x100_kv_batch &b, 
     a.scale2 = scale * 1.4426950408889634f;
     a.out = (uint16_t *)out;
     a.ldo = ldo;
-    const size_t n_few = p.results_few(c, b), n_p = p.results_prompt(c, b);
-    a.o_few = (float *)ws;
-    a.o_p = a.o_few + n_few * c.head_dim;
-    a.ml_few = (float2 *)(a.o_p + n_p * c.head_dim);
-    a.ml_p = a.ml_few + n_few;
-    a.split = p.split;
+    a.part_o = (float *)ws;
+    a.part_ml = (float2 *)(a.part_o + p.results(c, b) * c.head_dim);
     a.n_split = p.n_split;
-    a.few = p.few;
-    a.few_rows = p.few_rows;
-    a.split_p = p.split_p;
-    a.n_split_p = p.n_split_p;
+    a.least = p.least;
+    a.tile_rows = p.prompt ? PROMPT_ROWS : 16;
     if (c.head_dim == 64)
         return c.act_type == X100_T_F16 ? attn_as<64, X100_T_F16>(a, p, s) : attn_as<64, X100_T_BF16>(a, p, s);
     return c.act_type == X100_T_F16 ? attn_as<128, X100_T_F16>(a, p, s) : attn_as<128, X100_T_BF16>(a, p, s);

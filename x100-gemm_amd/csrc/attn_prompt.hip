@@ -41,16 +41,16 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
     __shared__ int s_inf[2][HD], s_odd;
     const int lane = threadIdx.x & 63, w = wave_id(), c = lane & 31, h = lane >> 5;
     const int n_kv = a.c.n_head_kv, G = a.c.n_head / n_kv, page = a.c.page, psh = __builtin_ctz(page);
-    const int kvh = blockIdx.x % n_kv, u = blockIdx.x / n_kv, sp = u % a.n_split_p;
-    const int tile = gridDim.x / (n_kv * a.n_split_p) - 1 - u / a.n_split_p, s = blockIdx.y;   // longest first
+    const int kvh = blockIdx.x % n_kv, u = blockIdx.x / n_kv, sp = u % a.n_split;
+    const int tile = gridDim.x / (n_kv * a.n_split) - 1 - u / a.n_split, s = blockIdx.y;   // longest first
     const PagedSeq q = paged_seq(a.b, s);
     const int n_rows = q.q_len * G, i0 = tile * PROMPT_ROWS;
-    if (i0 >= n_rows || n_rows <= a.few) return;
+    if (i0 >= n_rows) return;
     const int pos0 = q.kv_len - q.q_len;
     const int vis = pos0 + min(i0 + PROMPT_ROWS - 1, n_rows - 1) / G + 1;
-    const int ns = max(1, (vis + a.split_p - 1) / a.split_p);
+    const int per = split_of_seq(a, q.kv_len), ns = max(1, (vis + per - 1) / per);
     if (sp >= ns) return;
-    const int t0 = sp * a.split_p, t1 = min(t0 + a.split_p, vis);
+    const int t0 = sp * per, t1 = min(t0 + per, vis);
     const int n = max(0, (t1 - t0 + 31) >> 5);   // tiles
 
     // pages of the split; one that is none sends every tile through the masked step
@@ -451,20 +451,20 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
                 *(v2u *)(o + 32 * j + 8 * e) = y;
             }
     } else {
-        const size_t to = part_prompt(a, q.q0, kvh, i) + sp;
-        float *o = a.o_p + to * HD + 4 * h;
+        const size_t to = part_at(a, q.q0, kvh, i) + sp;
+        float *o = a.part_o + to * HD + 4 * h;
 #pragma unroll
         for (int j = 0; j < NJ; j++)
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 *(float4 *)(o + 32 * j + 8 * e) = make_float4(O[j][4 * e], O[j][4 * e + 1], O[j][4 * e + 2], O[j][4 * e + 3]);
-        if (h == 0) a.ml_p[to] = make_float2(m, l);
+        if (h == 0) a.part_ml[to] = make_float2(m, l);
     }
 }
 
 template <int HD, int AT> hipError_t prompt_as(const PagedAttnArgs &a, int tiles, hipStream_t s)
 {
-    const dim3 grid((unsigned)(tiles * a.n_split_p * a.c.n_head_kv), a.b.n_seq);
+    const dim3 grid((unsigned)(tiles * a.n_split * a.c.n_head_kv), a.b.n_seq);
     if (a.c.kv_type == X100_KV_Q4) k_attn_prompt<HD, AT, true><<<grid, 512, 0, s>>>(a);
     else k_attn_prompt<HD, AT, false><<<grid, 512, 0, s>>>(a);
     return hipGetLastError();

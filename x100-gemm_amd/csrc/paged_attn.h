@@ -13,13 +13,10 @@ struct PagedAttnArgs {
     float scale2;        // scale * log2(e): weights are powers of two
     uint16_t *out;
     int64_t ldo;
-    float *o_few, *o_p;      // split results of the tile kernel and of the prompt kernel: O (not divided by l)
-    float2 *ml_few, *ml_p;   // and (m, l); see part_few, part_prompt
-    int split, n_split;  // positions per split (a multiple of 128), splits
-    int few;             // sequences of up to this many rows (token, head) are the tile kernel's, longer
-                         // ones the prompt kernel's
-    int split_p, n_split_p;   // split, n_split of the prompt kernel
-    int few_rows;        // most rows of a sequence of the tile kernel
+    float *part_o;       // split results, n_split per row and head (part_at): O, HD floats each, not divided by l,
+    float2 *part_ml;     // and (m, l)
+    int n_split, least;  // splits of the longest sequence, fewest positions of one
+    int tile_rows;       // rows of a block's tile
 };
 
 template <int T> struct Mfma16;
@@ -73,17 +70,17 @@ template <int T> X100_DEV float add2(uint32_t w, float c)
     }
 }
 
-// Where the split results of row i (token, head) of a sequence and KV head begin: number `at` of the
-// kernel's results, HD floats of O each, then all (m, l).  The tile kernel's: [sequence][KV head][i < few_rows]
-// [split]; the prompt kernel's: [row * G + ...][KV head][split].
-X100_DEV size_t part_few(const PagedAttnArgs &a, int s, int kvh, int i)
-{
-    return (((size_t)s * a.c.n_head_kv + kvh) * a.few_rows + i) * a.n_split;
-}
-X100_DEV size_t part_prompt(const PagedAttnArgs &a, int q0, int kvh, int i)
+// Number of row i's (token, head) first split result; q0: the sequence's first row.
+X100_DEV size_t part_at(const PagedAttnArgs &a, int q0, int kvh, int i)
 {
     const int G = a.c.n_head / a.c.n_head_kv;
-    return (((size_t)q0 * G + i) * a.c.n_head_kv + kvh) * a.n_split_p;
+    return (((size_t)q0 * G + i) * a.c.n_head_kv + kvh) * a.n_split;
+}
+// Positions of a split: a sequence's positions in n_split equal parts, so that the blocks of a batch of
+// unequal sequences are as equal as its lengths let them be; a multiple of 128, a.least or more.
+X100_DEV int split_of_seq(const PagedAttnArgs &a, int kv_len)
+{
+    return max(a.least, ((kv_len + a.n_split - 1) / a.n_split + 127) & ~127);
 }
 
 constexpr int PROMPT_ROWS = 256;      // rows (token, head) of a block of the prompt kernel
