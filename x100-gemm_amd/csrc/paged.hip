@@ -3,6 +3,8 @@
 //
 // Bound by HBM for prompts (a row is read once, its queries, keys and values written once) and by
 // launch and dependent loads (q_start -> kv_len -> block_table) for single tokens.
+#include <algorithm>
+
 #include "paged.h"
 #include "x100_internal.h"
 
@@ -38,54 +40,84 @@ template <int HD> X100_DEV float gmin(float v)
     return v;
 }
 
+// Where row r of a wave's four (lane / 16) lies: the sequence s, the position (pos < 0: before the first),
+// mine: the row is one of a sequence that is not refused.
+struct RowPlace {
+    int s, pos;
+    bool mine;
+};
+X100_DEV RowPlace row_place(const x100_kv_batch &b, int rbase, int sub)
+{
+    RowPlace p = {0, -1, false};
+    const int f0 = paged_find(b, rbase);
+    if (f0 < b.n_seq) {   // mostly all four rows are one sequence's
+        const PagedSeq q = paged_seq(b, f0);
+        if (q.q_len > 0 && rbase >= q.q0 && rbase + 3 < q.q0 + q.q_len) return {f0, q.kv_len - q.q_len + rbase + sub - q.q0, true};
+    }
+    for (int i = 0; i < 4; i++) {
+        const int r = rbase + i;
+        const int f = r < b.n_rows ? paged_find(b, r) : b.n_seq;
+        if (i == sub && f < b.n_seq) {
+            const PagedSeq q = paged_seq(b, f);
+            if (q.q_len > 0 && r >= q.q0) p = {f, q.kv_len - q.q_len + r - q.q0, true};
+        }
+    }
+    return p;
+}
+
 struct AppendArgs {
     x100_kv_cfg c;
     x100_kv_batch b;
     x100_kv_rows r;
     uint8_t *kp, *vp;
     uint16_t *q_out;
+    int heads;     // query and key heads of a wave, one after the other
+    int xq, nq;    // blocks of one group of heads (16 rows each), of all query and key heads; behind them: values
+    int xv;        // blocks of one KV head's values
+    int vrows;     // rows of a value block's unit: 1, or 8
 };
 
-// Block: 8 consecutive rows.  blockIdx.y < n_qk: two of the query and key heads (16 lanes per row and
-// head, 8 or 4 elements each: the pair (i, i + HD/2) of the rotation is 8 lanes away); above: one KV
-// head's values, a thread per element of the head, 8 positions of one page at a time (a 16-byte
-// store of 8 positions, or the word that holds their codes).
-template <int HD, int ST, int AT, bool Q4> __global__ __launch_bounds__(256) void k_append(const AppendArgs a)
+// Queries and keys: a wave has four consecutive rows, 16 lanes each with 8 or 4 elements of a head (the
+// pair (i, i + HD/2) of the rotation is 8 lanes away), and takes `heads` heads one after the other, the next
+// one's elements on their way; a row's place and rotation are looked up once.
+template <int HD, int ST, int AT, bool Q4> X100_DEV void append_qk(const AppendArgs &a)
 {
     constexpr int E = HD / 16;
-    const int lane = threadIdx.x & 63, w = wave_id();
+    const int lane = threadIdx.x & 63, w = wave_id(), l = lane & 15, sub = lane >> 4;
     const int n_h = a.c.n_head, n_kv = a.c.n_head_kv, page = a.c.page;
-    const int n_qk = (n_h + n_kv + 1) / 2;
-    const int row0 = blockIdx.x * 8;
-    if ((int)blockIdx.y < n_qk) {
-        const int head = 2 * blockIdx.y + (w >> 1), rbase = row0 + 4 * (w & 1);
-        if (head >= n_h + n_kv || rbase >= a.b.n_rows) return;
-        const int l = lane & 15, sub = lane >> 4;
-        const int row = min(rbase + sub, a.b.n_rows - 1);
+    const int rbase = blockIdx.x % a.xq * 16 + 4 * w;
+    int head = blockIdx.x / a.xq * a.heads;
+    const int end = min(head + a.heads, n_h + n_kv);
+    if (!a.q_out) head = max(head, n_h);   // keys only
+    if (head >= end || rbase >= a.b.n_rows) return;
+    const int row = min(rbase + sub, a.b.n_rows - 1);
+    float raw[E];
+    auto fetch = [&](int hd) __attribute__((always_inline)) {
+        const x100_rows &src = hd < n_h ? a.r.q : a.r.k;
+        row_elems<ST, E>(src.p, (size_t)row * src.ld + (hd < n_h ? hd : hd - n_h) * HD + E * l, raw);
+    };
+    fetch(head);
+    const RowPlace at = row_place(a.b, rbase, sub);
+    float2 cs[E];
+    if (a.r.rope) {
+        const float2 *t = (const float2 *)a.r.rope + (size_t)max(at.pos, 0) * (HD / 2) + E * (l & 7);
+#pragma unroll
+        for (int e = 0; e < E; e++) cs[e] = t[e];
+    }
+    const int pg = at.mine && at.pos >= 0 ? paged_page(a.c, a.b, at.s, at.pos) : -1;
+    const int off = at.pos & (page - 1);
+    for (; head < end; head++) {
         const bool is_q = head < n_h;
-        if (is_q && !a.q_out) return;
         const x100_rows &src = is_q ? a.r.q : a.r.k;
-        const int col = (is_q ? head : head - n_h) * HD + E * l;
         float v[E];
-        row_elems<ST, E>(src.p, (size_t)row * src.ld + col, v);
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = raw[e];
+        if (head + 1 < end) fetch(head + 1);
         if constexpr (ST == X100_T_I32) {
             const float rs = src.row_scale[row];
+            const float *cl = src.col_scale + (is_q ? head : head - n_h) * HD + E * l;
 #pragma unroll
-            for (int e = 0; e < E; e++) v[e] = v[e] * rs * src.col_scale[col + e];
-        }
-        int pos = -1, s = 0;
-        bool mine = false;
-        for (int i = 0; i < 4; i++) {
-            const int r = rbase + i;
-            const int f = r < a.b.n_rows ? paged_find(a.b, r) : a.b.n_seq;
-            if (i == sub && f < a.b.n_seq) {
-                const PagedSeq q = paged_seq(a.b, f);
-                if (q.q_len > 0 && r >= q.q0) {
-                    mine = true;
-                    s = f;
-                    pos = q.kv_len - q.q_len + r - q.q0;
-                }
-            }
+            for (int e = 0; e < E; e++) v[e] = v[e] * rs * cl[e];
         }
         const float *nw = is_q ? a.r.q_norm : a.r.k_norm;
         if (nw) {
@@ -97,39 +129,37 @@ template <int HD, int ST, int AT, bool Q4> __global__ __launch_bounds__(256) voi
             for (int e = 0; e < E; e++) v[e] = v[e] * sc * nw[E * l + e];
         }
         if (a.r.rope) {
-            const float2 *t = (const float2 *)a.r.rope + (size_t)max(pos, 0) * (HD / 2) + E * (l & 7);
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                const float2 cs = t[e];
                 const float o = dpp_f<0x128>(0.0f, v[e]);   // the pair's other element
-                v[e] = l < 8 ? v[e] * cs.x - o * cs.y : o * cs.y + v[e] * cs.x;
+                v[e] = l < 8 ? v[e] * cs[e].x - o * cs[e].y : o * cs[e].y + v[e] * cs[e].x;
             }
         }
         if (is_q) {
-            if (pos < 0) {   // a row before position 0: zeros
+            if (at.pos < 0) {   // a row before position 0: zeros
 #pragma unroll
                 for (int e = 0; e < E; e++) v[e] = 0.0f;
             }
-            if (!mine) return;
-            uint32_t u[E / 2];
+            if (at.mine) {
+                uint32_t u[E / 2];
 #pragma unroll
-            for (int e = 0; e < E / 2; e++) u[e] = f2act<AT>(v[2 * e]) | f2act<AT>(v[2 * e + 1]) << 16;
-            uint16_t *o = a.q_out + ((size_t)row * n_h + head) * HD + E * l;
-            if constexpr (E == 8) *(v4u *)o = v4u{u[0], u[1], u[2], u[3]};
-            else *(v2u *)o = v2u{u[0], u[1]};
-            return;
+                for (int e = 0; e < E / 2; e++) u[e] = f2act<AT>(v[2 * e]) | f2act<AT>(v[2 * e + 1]) << 16;
+                uint16_t *o = a.q_out + ((size_t)row * n_h + head) * HD + E * l;
+                if constexpr (E == 8) *(v4u *)o = v4u{u[0], u[1], u[2], u[3]};
+                else *(v2u *)o = v2u{u[0], u[1]};
+            }
+            continue;
         }
-        const int pg = mine && pos >= 0 ? paged_page(a.c, a.b, s, pos) : -1;
-        const int off = pos & (page - 1), kvh = head - n_h;
-        uint8_t *base = a.kp + ((size_t)max(pg, 0) * n_kv + kvh) * page_head_bytes<HD, Q4>(page);
+        uint8_t *base = a.kp + ((size_t)max(pg, 0) * n_kv + head - n_h) * page_head_bytes<HD, Q4>(page);
         if constexpr (!Q4) {
-            if (pg < 0) return;
-            uint32_t u[E / 2];
+            if (pg >= 0) {
+                uint32_t u[E / 2];
 #pragma unroll
-            for (int e = 0; e < E / 2; e++) u[e] = f2act<AT>(v[2 * e]) | f2act<AT>(v[2 * e + 1]) << 16;
-            uint16_t *o = (uint16_t *)base + (size_t)off * HD + E * l;
-            if constexpr (E == 8) *(v4u *)o = v4u{u[0], u[1], u[2], u[3]};
-            else *(v2u *)o = v2u{u[0], u[1]};
+                for (int e = 0; e < E / 2; e++) u[e] = f2act<AT>(v[2 * e]) | f2act<AT>(v[2 * e + 1]) << 16;
+                uint16_t *o = (uint16_t *)base + (size_t)off * HD + E * l;
+                if constexpr (E == 8) *(v4u *)o = v4u{u[0], u[1], u[2], u[3]};
+                else *(v2u *)o = v2u{u[0], u[1]};
+            }
         } else {
             float lo = v[0], hi = v[0], fin = 1.0f;
 #pragma unroll
@@ -147,74 +177,90 @@ template <int HD, int ST, int AT, bool Q4> __global__ __launch_bounds__(256) voi
                 if (l & 1) word <<= 8;
                 word |= (uint32_t)dpp_i<0xB1>(0, (int)word);
             }
-            if (pg < 0) return;
-            if (E == 8) cw[l] = word;
-            else if (!(l & 1)) cw[l >> 1] = word;
-            constexpr int LG = 32 / E;   // lanes of a group
-            if (l % LG == 0)
-                ((uint32_t *)(base + page * HD / 2))[(size_t)off * (HD / 32) + l / LG] = sc.d | (uint32_t)sc.m << 16;
+            if (pg >= 0) {
+                if (E == 8) cw[l] = word;
+                else if (!(l & 1)) cw[l >> 1] = word;
+                constexpr int LG = 32 / E;   // lanes of a group
+                if (l % LG == 0)
+                    ((uint32_t *)(base + page * HD / 2))[(size_t)off * (HD / 32) + l / LG] = sc.d | (uint32_t)sc.m << 16;
+            }
         }
-        return;
     }
-    // values
-    const int kvh = blockIdx.y - n_qk;
-    constexpr int WH = HD / 64;                 // waves of a head
-    const int el = (w % WH) * 64 + lane;        // element of the head
+}
+
+// Values: HD / 64 waves per unit of `vrows` rows, a thread per element of the head.  The rows of one sequence in
+// one block of 8 positions are stored together (a 16-byte store of 8 positions, or the word that holds their
+// codes), by the unit that holds the first of them.
+template <int HD, int ST, int AT, bool Q4> X100_DEV void append_v(const AppendArgs &a)
+{
+    constexpr int WH = HD / 64;
+    const int lane = threadIdx.x & 63, w = wave_id(), n_kv = a.c.n_head_kv, page = a.c.page;
+    const int bv = blockIdx.x - a.nq, kvh = bv / a.xv, el = (w % WH) * 64 + lane;
     const x100_rows &src = a.r.v;
     const int col = kvh * HD + el;
-    for (int i = w / WH; i < 8; i += 4 / WH) {
-        const int row = row0 + i;
-        if (row >= a.b.n_rows) return;
+    const int first = (bv % a.xv * (4 / WH) + w / WH) * a.vrows, last = min(first + a.vrows, a.b.n_rows);
+    int row = first;
+    while (row < last) {
         const int s = paged_find(a.b, row);
         if (s >= a.b.n_seq) return;
         const PagedSeq q = paged_seq(a.b, s);
-        if (q.q_len <= 0 || row < q.q0) continue;
-        const int pos = q.kv_len - q.q_len + row - q.q0;
-        // the row that begins a block of 8 positions, or the sequence's first row, stores the block's rows
-        if (pos < 0 || !(row == q.q0 || pos == 0 || (pos & 7) == 0)) continue;
-        const int n = min(8 - (pos & 7), q.q0 + q.q_len - row);
-        const int pg = paged_page(a.c, a.b, s, pos);
-        if (pg < 0) continue;
-        const int o0 = pos & 7, blk = (pos & (page - 1)) >> 3;
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            v[k] = 0.0f;
-            if (k < n) {
-                v[k] = row_elem<ST>(src.p, (size_t)(row + k) * src.ld + col);
-                if constexpr (ST == X100_T_I32) v[k] = v[k] * src.row_scale[row + k] * src.col_scale[col];
-            }
+        if (q.q_len <= 0 || row < q.q0) {
+            row++;
+            continue;
         }
-        uint8_t *base = a.vp + ((size_t)pg * n_kv + kvh) * page_head_bytes<HD, Q4>(page);
-        if constexpr (!Q4) {
-            uint16_t *o = (uint16_t *)base + ((size_t)blk * HD + el) * 8;
-            if (n == 8) {
-                uint32_t u[4];
+        const int shift = q.kv_len - q.q_len - q.q0;   // position - row
+        // this sequence's blocks that begin in the unit: at its first row, and at every position 8 k
+        for (const int stop = min(last, q.q0 + q.q_len); row < stop;) {
+            const int pos = row + shift;
+            if (pos < 0) {
+                row = min(stop, -shift);
+                continue;
+            }
+            if (!(row == q.q0 || (pos & 7) == 0)) {
+                row = min(stop, row + 8 - (pos & 7));
+                continue;
+            }
+            const int o0 = pos & 7, n = min(8 - o0, q.q0 + q.q_len - row);
+            const int pg = paged_page(a.c, a.b, s, pos), blk = (pos & (page - 1)) >> 3;
+            float v[8];
 #pragma unroll
-                for (int k = 0; k < 4; k++) u[k] = f2act<AT>(v[2 * k]) | f2act<AT>(v[2 * k + 1]) << 16;
-                *(v4u *)o = v4u{u[0], u[1], u[2], u[3]};
-            } else {
+            for (int k = 0; k < 8; k++) v[k] = k < n ? row_elem<ST>(src.p, (size_t)(row + k) * src.ld + col) : 0.0f;
+            if constexpr (ST == X100_T_I32) {
+                const float cl = src.col_scale[col];
 #pragma unroll
                 for (int k = 0; k < 8; k++)
-                    if (k < n) o[o0 + k] = (uint16_t)f2act<AT>(v[k]);
+                    if (k < n) v[k] = v[k] * src.row_scale[row + k] * cl;
             }
-        } else {
-            uint32_t *cw = (uint32_t *)base + (size_t)blk * HD + el;
-            uint32_t word = n == 8 ? 0u : *cw;
-            uint16_t *sc16 = (uint16_t *)(base + page * HD / 2) + ((size_t)blk * (HD / 32) + el / 32) * 16;
+            row += n;
+            if (pg < 0) continue;
+            uint8_t *base = a.vp + ((size_t)pg * n_kv + kvh) * page_head_bytes<HD, Q4>(page);
+            if constexpr (!Q4) {
+                uint16_t *o = (uint16_t *)base + ((size_t)blk * HD + el) * 8;
+                if (n == 8) {
+                    uint32_t u[4];
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                float lo = v[k], hi = v[k], fin = fabsf(v[k]) <= 3.402823466e38f ? 1.0f : 0.0f;
-                lo = gmin<64>(lo);
-                lo = fminf(lo, dpp_f<0x128>(lo, lo));
-                lo = fminf(lo, xor16_f(lo));
-                hi = -gmin<64>(-hi);
-                hi = fmaxf(hi, dpp_f<0x128>(hi, hi));
-                hi = fmaxf(hi, xor16_f(hi));
-                fin = gmin<64>(fin);
-                fin = fminf(fin, dpp_f<0x128>(fin, fin));
-                fin = fminf(fin, xor16_f(fin));
-                if (k < n) {
+                    for (int k = 0; k < 4; k++) u[k] = f2act<AT>(v[2 * k]) | f2act<AT>(v[2 * k + 1]) << 16;
+                    *(v4u *)o = v4u{u[0], u[1], u[2], u[3]};
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        if (k < n) o[o0 + k] = (uint16_t)f2act<AT>(v[k]);
+                }
+            } else {
+                uint32_t *cw = (uint32_t *)base + (size_t)blk * HD + el;
+                uint32_t word = n == 8 ? 0u : *cw;
+                uint16_t *sc16 = (uint16_t *)(base + page * HD / 2) + ((size_t)blk * (HD / 32) + el / 32) * 16;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    if (k >= n) break;
+                    float lo = gmin<64>(v[k]), hi = -gmin<64>(-v[k]);
+                    float fin = gmin<64>(fabsf(v[k]) <= 3.402823466e38f ? 1.0f : 0.0f);
+                    lo = fminf(lo, dpp_f<0x128>(lo, lo));
+                    hi = fmaxf(hi, dpp_f<0x128>(hi, hi));
+                    fin = fminf(fin, dpp_f<0x128>(fin, fin));
+                    lo = fminf(lo, xor16_f(lo));
+                    hi = fmaxf(hi, xor16_f(hi));
+                    fin = fminf(fin, xor16_f(fin));
                     const Q4Scale sc = q4_scale(lo, hi, fin == 0.0f);
                     const int e = o0 + k, sh = 16 * (e & 1) + 4 * (e >> 1);
                     word = (word & ~(15u << sh)) | q4_code(sc, v[k]) << sh;
@@ -223,10 +269,16 @@ template <int HD, int ST, int AT, bool Q4> __global__ __launch_bounds__(256) voi
                         sc16[8 + e] = sc.m;
                     }
                 }
+                *cw = word;
             }
-            *cw = word;
         }
     }
+}
+
+template <int HD, int ST, int AT, bool Q4> __global__ __launch_bounds__(256) void k_append(const AppendArgs a)
+{
+    if ((int)blockIdx.x < a.nq) append_qk<HD, ST, AT, Q4>(a);
+    else append_v<HD, ST, AT, Q4>(a);
 }
 
 // ---- cached rows back out ------------------------------------------------------------------------
@@ -245,21 +297,9 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256) void k_read
     const int kvh = blockIdx.y, n_kv = a.c.n_head_kv, page = a.c.page;
     const int rbase = blockIdx.x * 16 + 4 * w;
     if (rbase >= a.b.n_rows) return;
-    int pos = -1, pg = -1;
-    bool mine = false;
-    for (int i = 0; i < 4; i++) {
-        const int r = rbase + i;
-        const int s = r < a.b.n_rows ? paged_find(a.b, r) : a.b.n_seq;
-        if (i == sub && s < a.b.n_seq) {
-            const PagedSeq q = paged_seq(a.b, s);
-            if (q.q_len > 0 && r >= q.q0) {
-                mine = true;
-                pos = q.kv_len - q.q_len + r - q.q0;
-                if (pos >= 0) pg = paged_page(a.c, a.b, s, pos);
-            }
-        }
-    }
-    if (!mine) return;
+    const RowPlace place = row_place(a.b, rbase, sub);
+    if (!place.mine) return;
+    const int pos = place.pos, pg = pos >= 0 ? paged_page(a.c, a.b, place.s, pos) : -1;
     const int row = rbase + sub, off = pos & (page - 1);
     uint32_t k[E], v[E];   // act_type bits
 #pragma unroll
@@ -301,9 +341,19 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256) void k_read
     }
 }
 
-template <int HD, int ST> hipError_t append_as(const AppendArgs &a, hipStream_t s)
+template <int HD, int ST> hipError_t append_as(AppendArgs a, hipStream_t s)
 {
-    const dim3 grid((a.b.n_rows + 7) / 8, (a.c.n_head + a.c.n_head_kv + 1) / 2 + a.c.n_head_kv);
+    // Heads per wave: as many as leave 8192 waves (32 per CU), so that few rows are spread over the chip and many
+    // look their places up once for several heads (12000 rows of 36 heads, int32 to 4 bits: one head 98 us).
+    // Values: a unit of 8 rows holds whole blocks of prompts; single tokens get a unit each.
+    const int n_rows = a.b.n_rows, all = a.c.n_head + a.c.n_head_kv, quads = (n_rows + 3) / 4;
+    a.heads = std::max(1, (int)std::min<int64_t>(all, (int64_t)quads * all / 8192));
+    a.xq = (n_rows + 15) / 16;
+    a.nq = a.xq * ((all + a.heads - 1) / a.heads);
+    a.vrows = (int64_t)n_rows * a.c.n_head_kv <= 2048 ? 1 : 8;
+    const int per = 4 / (HD / 64) * a.vrows;   // rows of a value block
+    a.xv = (n_rows + per - 1) / per;
+    const unsigned grid = (unsigned)a.nq + (unsigned)a.xv * a.c.n_head_kv;
     const bool q4 = a.c.kv_type == X100_KV_Q4;
     if (a.c.act_type == X100_T_F16) {
         if (q4) k_append<HD, ST, X100_T_F16, true><<<grid, 256, 0, s>>>(a);
@@ -350,7 +400,7 @@ hipError_t x100_rope_table_launch(int head_dim, int n_pos, float base, float *ta
 hipError_t x100_kv_append_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const x100_kv_rows &r, void *kp,
                                  void *vp, void *q_out, hipStream_t s)
 {
-    const AppendArgs a = {c, b, r, (uint8_t *)kp, (uint8_t *)vp, (uint16_t *)q_out};
+    const AppendArgs a = {c, b, r, (uint8_t *)kp, (uint8_t *)vp, (uint16_t *)q_out, 0, 0, 0, 0, 0};
     return c.head_dim == 64 ? append_from<64>(a, s) : append_from<128>(a, s);
 }
 
