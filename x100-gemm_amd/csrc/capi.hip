@@ -919,6 +919,7 @@ int x100_kv_append_hip(const x100_kv_cfg *c, const x100_kv_batch *b, const x100_
     int rc = check_device();
     if (rc) return rc;
     hipError_t e = x100_kv_append_launch(*c, *b, *r, k_pool, v_pool, q_out, (hipStream_t)stream);
+    if (e == hipErrorInvalidValue) return X100_EINVAL;
     if (e != hipSuccess) return hip_fail(e);
     return X100_OK;
 }

@@ -343,17 +343,20 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256) void k_read
 
 template <int HD, int ST> hipError_t append_as(AppendArgs a, hipStream_t s)
 {
-    // Heads per wave: as many as leave 8192 waves (32 per CU), so that few rows are spread over the chip and many
-    // look their places up once for several heads (12000 rows of 36 heads, int32 to 4 bits: one head 98 us).
+    // Heads per wave: as many as leave 4096 waves (16 per CU), so that few rows are spread over the chip and many
+    // look their places up once for several heads (8000 rows of 36 heads, int32 to 4 bits and read back, us: one
+    // head per wave 109; 32768 / 16384 / 8192 / 4096 waves 80.6 / 69.4 / 67.6 / 62.2).
     // Values: a unit of 8 rows holds whole blocks of prompts; single tokens get a unit each.
     const int n_rows = a.b.n_rows, all = a.c.n_head + a.c.n_head_kv, quads = (n_rows + 3) / 4;
-    a.heads = std::max(1, (int)std::min<int64_t>(all, (int64_t)quads * all / 8192));
+    a.heads = std::max(1, (int)std::min<int64_t>(all, (int64_t)quads * all / 4096));
     a.xq = (n_rows + 15) / 16;
     a.nq = a.xq * ((all + a.heads - 1) / a.heads);
     a.vrows = (int64_t)n_rows * a.c.n_head_kv <= 2048 ? 1 : 8;
     const int per = 4 / (HD / 64) * a.vrows;   // rows of a value block
     a.xv = (n_rows + per - 1) / per;
-    const unsigned grid = (unsigned)a.nq + (unsigned)a.xv * a.c.n_head_kv;
+    const int64_t blocks = (int64_t)a.nq + (int64_t)a.xv * a.c.n_head_kv;
+    if (blocks >= 1 << 24) return hipErrorInvalidValue;   // past one launch
+    const unsigned grid = (unsigned)blocks;
     const bool q4 = a.c.kv_type == X100_KV_Q4;
     if (a.c.act_type == X100_T_F16) {
         if (q4) k_append<HD, ST, X100_T_F16, true><<<grid, 256, 0, s>>>(a);
