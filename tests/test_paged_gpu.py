@@ -104,9 +104,10 @@ def compare(got, want, tol):
     inf = np.isinf(want)
     assert np.array_equal(got[inf], want[inf])
     fin = np.isfinite(want)
-    off = np.abs(got - want)[fin] - tol[fin]
+    dist = np.abs(got[fin] - want[fin])
+    off = dist - tol[fin]
     assert (off <= 0).all(), "off by %.3g, %.3g allowed (%d of %d outside)" % (
-        np.abs(got - want)[fin][off.argmax()], tol[fin][off.argmax()], (off > 0).sum(), off.size)
+        dist[off.argmax()], tol[fin][off.argmax()], (off > 0).sum(), off.size)
 
 
 KINDS = [(ref.F16, ref.F16), (ref.BF16, ref.BF16), (ref.F16, ref.Q4), (ref.BF16, ref.Q4)]
@@ -309,6 +310,114 @@ def test_cache_past_32_bit_offsets(dev):
     # weights and result rounded to fp16 (2^-11 each), scores in fp32
     tol = (2.0 ** -11 * 1.05 + 1e-4) * (z @ v.abs()).transpose(0, 1).reshape(L, 1024) + 2.0 ** -11 * want.abs() + 1e-7
     assert ((out.double() - want).abs() <= tol).all()
+
+
+@kinds
+@pytest.mark.parametrize("hd,page,L", [(64, 16, 9000), (128, 16, 8500), (64, 256, 8449)])
+def test_long_tables(dev, act, kv, hd, page, L):
+    """Caches whose page list does not fit a block's as a whole, and pages larger than a split's step."""
+    Setup(24, 2, 1, hd, page, act, kv, [1, 1], [L, 77]).check()
+    s = Setup(25, 4, 1, hd, page, act, kv, [1, 2], [L, 300])
+    s.table[0, 3] = -1          # a page that is none, far from the end
+    s.upload()
+    s.check()
+
+
+@kinds
+@pytest.mark.parametrize("n_head,n_kv,hd", [(2, 2, 128), (3, 1, 64), (16, 1, 128), (7, 1, 128), (2, 1, 64)])
+def test_prompts_of_many_tiles(dev, act, kv, n_head, n_kv, hd):
+    """Prompts over several blocks of rows and many tiles of positions, with a decode row among them, against
+    64-bit products on the GPU."""
+    q, L = [300, 1, 33, 700], [300, 1500, 1700, 777]
+    s = Setup(26, n_head, n_kv, hd, 32, act, kv, q, L)
+    dq, qv = s.queries(gain=1.5)
+    out = s.attend(dq, n_head * hd, hd ** -0.5).double().view(s.n_rows, n_head, hd)
+    K, V = (torch.from_numpy(np.nan_to_num(t)).cuda() for t in s.c.decode(s.kb, s.vb))
+    Q = torch.from_numpy(qv).cuda()
+    u = ref.HALF_STEP[act] + ref.HALF_STEP[ref.F16 if kv == ref.Q4 else act]
+    for i in range(len(q)):
+        pg = torch.from_numpy(s.table[i][:-(-L[i] // 32)]).cuda()
+        k, v = (t[pg].transpose(0, 1).reshape(n_kv, -1, hd)[:, :L[i]] for t in (K, V))
+        r0, n = int(s.q_start[i]), q[i]
+        hidden = torch.arange(L[i], device=dev)[None] > torch.arange(L[i] - n, L[i], device=dev)[:, None]
+        for h in range(n_head):
+            kk, vv = k[h * n_kv // n_head].contiguous(), v[h * n_kv // n_head].contiguous()
+            z = (Q[r0:r0 + n, h] @ kk.T.contiguous() * hd ** -0.5).masked_fill(hidden, float("-inf")).softmax(-1)
+            want, size = z @ vv, z @ vv.abs()
+            # the weights' and the result's 16-bit rounding; the scores in fp32
+            assert ((out[r0:r0 + n, h] - want).abs() <= (1.01 * u + 1e-4) * size + 1e-6).all(), (i, h)
+
+
+@kinds
+def test_two_calls_at_once(dev, act, kv):
+    """Calls on two streams at the same time, each with its own workspace (and through the library's)."""
+    sets = [Setup(27 + i, 8, 2, 128, 64, act, kv, [1, q], [3000, 500]) for i, q in enumerate((1, 60))]
+    dqs = [s.queries()[0] for s in sets]
+    alone = [s.attend(d, 1024, 0.1) for s, d in zip(sets, dqs)]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for ws in (True, False):
+        outs, keep = [], []
+        torch.cuda.synchronize()
+        for s, d, st in zip(sets, dqs, streams):
+            out = torch.zeros_like(alone[len(outs)])
+            n = x.attn_paged_workspace_bytes(s.cfg, s.batch)
+            w = torch.empty(max(n, 256), dtype=torch.uint8, device=dev)
+            torch.cuda.synchronize()
+            for _ in range(20):
+                args = (s.cfg, s.batch, d.data_ptr(), 1024, s.dk.data_ptr(), s.dv.data_ptr(), 0.1, out.data_ptr(), 1024)
+                if ws:
+                    x.attn_paged_ws(*args, w.data_ptr(), n, st.cuda_stream)
+                else:
+                    x.attn_paged(*args, st.cuda_stream)
+            outs.append(out)
+            keep.append(w)
+        torch.cuda.synchronize()
+        for a, b in zip(alone, outs):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+@kinds
+def test_a_decode_step_in_a_graph(dev, act, kv):
+    """Append, attention and read-back captured once and replayed as the sequences grow, with eager calls
+    between the replays."""
+    n_seq, page, max_kv = 3, 16, 80
+    c = x.KvCfg(4, 2, 64, page, 20, act, kv)
+    pools = [[torch.zeros(x.kv_pool_bytes(c), dtype=torch.uint8, device=dev) for _ in range(2)] for _ in range(2)]
+    g = np.random.default_rng(5)
+    tab = dev_i32(g.permutation(20)[:15].reshape(3, 5))
+    qs, kl = dev_i32([0, 1, 2, 3]), dev_i32([1, 1, 1])
+    b = x.KvBatch(n_seq, n_seq, 1, max_kv, 5, qs.data_ptr(), kl.data_ptr(), tab.data_ptr())
+    rows, vals, keep = projections(g, n_seq, 4, 2, 64, ref.F32)
+    rope = torch.empty(max_kv * 64, device=dev)
+    x.rope_table(64, max_kv, 1e4, rope.data_ptr(), stream())
+    r = x.KvRows(*rows, None, None, 0.0, rope.data_ptr(), max_kv)
+    bufs = [[torch.zeros(n_seq, w, dtype=TT[act], device=dev) for w in (256, 256, 128, 128)] for _ in range(2)]
+    ws = torch.empty(max(256, x.attn_paged_workspace_bytes(c, b)), dtype=torch.uint8, device=dev)
+
+    def step(i):
+        (q, o, k, v), (kp, vp) = bufs[i], pools[i]
+        x.kv_append(c, b, r, kp.data_ptr(), vp.data_ptr(), q.data_ptr(), stream())
+        x.attn_paged_ws(c, b, q.data_ptr(), 256, kp.data_ptr(), vp.data_ptr(), 0.125, o.data_ptr(), 256, ws.data_ptr(),
+                        ws.numel(), stream())
+        x.kv_read(c, b, kp.data_ptr(), vp.data_ptr(), k.data_ptr(), v.data_ptr(), stream())
+
+    step(0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(0)
+    for p in pools:
+        for t in p:
+            t.zero_()
+    for n in range(1, 40):
+        kl.copy_(dev_i32([n, 2 * n, n // 2]))
+        keep[-1].normal_()          # the step's projections
+        graph.replay()
+        torch.cuda.synchronize()
+        step(1)
+        torch.cuda.synchronize()
+        for s, t in zip(bufs[0] + pools[0], bufs[1] + pools[1]):
+            assert torch.equal(s.view(torch.uint8), t.view(torch.uint8)), n
 
 
 # ---- append and read --------------------------------------------------------------------------------

@@ -18,7 +18,7 @@ namespace {
 
 constexpr float NEG_INF = X100_NEG_INF;
 using AttnArgs = PagedAttnArgs;
-constexpr int TILE_SPLIT = 8192;   // most positions of a split of the tile kernel (its page list is in LDS)
+constexpr int TILE_PAGES = 512;   // most pages of a split of the tile kernel (their list is in LDS)
 
 // What a lane reads of a tile of 32 positions, as the cache holds it: K rows 8 (c / 4) + 4 h + c % 4 (h = 0,
 // 1), V block 8 g .. 8 g + 7.
@@ -43,7 +43,7 @@ template <int HD, int AT, bool Q4, int NW> __global__ __launch_bounds__(64 * NW,
     constexpr int MT = Q4 ? X100_T_F16 : AT;   // type on the matrix cores
     constexpr int KS = HD / 32, NJ = HD / 16;  // steps of K Q^T, element tiles of V^T P^T
     __shared__ union {
-        int pg[TILE_SPLIT / 16];               // pages of the split, -1 where there is none
+        int pg[TILE_PAGES];                     // pages of the split, -1 where there is none
         float o[NW][16][HD + 4];               // at the end
     } sh;
     __shared__ float s_m[NW][16], s_l[NW][16];
@@ -54,7 +54,7 @@ template <int HD, int AT, bool Q4, int NW> __global__ __launch_bounds__(64 * NW,
     // A short table's pages are read here, beside the lengths; a long one's when the split is known.
     const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
     const int n_all = (a.b.max_kv + page - 1) >> psh;
-    const bool all = n_all <= TILE_SPLIT / 16;
+    const bool all = n_all <= TILE_PAGES;
     auto list = [&](int first, int n) {
         for (int i = threadIdx.x; i < n; i += 64 * NW) {
             const int pg = tab[first + i];
@@ -443,11 +443,12 @@ Plan plan_of(const x100_kv_cfg &c, const x100_kv_batch &b)
         // up to 4096 positions, us with 256 / 512 / 1024 blocks wanted: 70.6 / 78.6 / 77.2), three where 4-bit
         // codes have to be unpacked (16 of up to 60001: 115.8 / 113.9 / 101.8, 768: 98.4).  Up to 512 positions
         // one block is faster than two and their join (9.6 / 12.6 us).
+        const int64_t most = (int64_t)TILE_PAGES * c.page;
         p.least = 256;
         p.tiles = (int)((rows + 15) / 16);
         const int64_t base = (int64_t)p.tiles * std::min(b.n_seq, b.n_rows) * c.n_head_kv;
         const int64_t want = kv <= 512 ? 1 : std::max<int64_t>(1, (c.kv_type == X100_KV_Q4 ? 768 : 256) / base);
-        p.n_split = (int)std::max(std::min(want, (kv + 255) / 256), (kv + TILE_SPLIT - 1) / TILE_SPLIT);
+        p.n_split = (int)std::max(std::min(want, (kv + 255) / 256), (kv + most - 1) / most);
         return p;
     }
     // One block per CU at a time, so rounds of 256 blocks: the number of splits with the least sum over the
@@ -457,7 +458,8 @@ Plan plan_of(const x100_kv_cfg &c, const x100_kv_batch &b)
     const int64_t full = (int64_t)b.n_rows * G / PROMPT_ROWS + b.n_seq;   // tiles that have rows
     const int64_t base = std::min<int64_t>((int64_t)p.tiles * b.n_seq, full) * c.n_head_kv;
     int64_t best = 0;
-    for (int64_t n = std::max<int64_t>(1, (kv + PROMPT_SPLIT - 1) / PROMPT_SPLIT), n0 = n; n == n0 || (n <= 16 && n * 512 < kv + 512); n++) {
+    const int64_t most = (int64_t)PROMPT_PAGES * c.page;
+    for (int64_t n = (kv + most - 1) / most, n0 = n; n == n0 || (n <= 16 && n * 512 < kv + 512); n++) {
         const int64_t cost = (base * n + 255) / 256 * (kv / n + 512) + (n > 1 ? 512 : 0);
         if (n == n0 || cost < best) {
             best = cost;
@@ -473,7 +475,9 @@ template <int HD, int AT> hipError_t attn_as(const AttnArgs &a, const Plan &p, h
         const hipError_t e = x100_attn_prompt_launch(a, p.tiles, s);
         if (e != hipSuccess) return e;
     } else {
-        const dim3 grid((unsigned)(p.tiles * p.n_split), a.c.n_head_kv, a.b.n_seq);
+        const int64_t blocks = (int64_t)p.tiles * p.n_split;
+        if (blocks >= 1 << 24) return hipErrorInvalidValue;   // past one launch
+        const dim3 grid((unsigned)blocks, a.c.n_head_kv, a.b.n_seq);
         if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true, 4><<<grid, 256, 0, s>>>(a);
         else k_attn_tile<HD, AT, false, 4><<<grid, 256, 0, s>>>(a);
         const hipError_t e = hipGetLastError();

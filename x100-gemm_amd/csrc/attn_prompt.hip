@@ -37,7 +37,7 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
     constexpr int KB = 32 * HD * 2;       // bytes of a K (or V) tile of 32 positions
     constexpr int ND = 2 * KB / 8192;     // copies of 1 KiB per wave and pair of tiles
     __shared__ __attribute__((aligned(1024))) uint8_t s_k[3][2 * KB], s_v[3][2 * KB];   // pairs of tiles
-    __shared__ int s_pg[PROMPT_SPLIT / 16];
+    __shared__ int s_pg[PROMPT_PAGES];
     __shared__ int s_inf[2][HD], s_odd;
     const int lane = threadIdx.x & 63, w = wave_id(), c = lane & 31, h = lane >> 5;
     const int n_kv = a.c.n_head_kv, G = a.c.n_head / n_kv, page = a.c.page, psh = __builtin_ctz(page);
@@ -55,7 +55,7 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
 
     // pages of the split; one that is none sends every tile through the masked step
     const int *tab = a.b.block_table + (size_t)s * a.b.table_ld + (t0 >> psh);
-    const int n_pg = n > 0 ? ((t1 - 1) >> psh) - (t0 >> psh) + 1 : 0;
+    const int pg0 = t0 >> psh, n_pg = n > 0 ? ((t1 - 1) >> psh) - pg0 + 1 : 0;
     bool bad = false;
     for (int i = threadIdx.x; i < n_pg; i += NT) {
         const int g = tab[i];
@@ -110,7 +110,7 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
     const int np = (n + 1) >> 1;   // pairs
     auto page_at = [&](int pp) {   // entry of the page list for the wave's positions of pair pp
         const int t = t0 + 64 * pp + 8 * w;
-        return s_pg[((t < t1 ? t : t0) >> psh) - (t0 >> psh)];
+        return s_pg[((t < t1 ? t : t0) >> psh) - pg0];
     };
     auto place = [&](int pp, int pg) -> size_t {
         const int t = t0 + 64 * pp + 8 * w;
@@ -135,7 +135,7 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
     v4u rv_d, rv_m;
     const int x4 = threadIdx.x;
     auto base4 = [&](const uint8_t *pool, int pp, int &off) {
-        const int pg = max(s_pg[((pp < t1 ? pp : t0) >> psh) - (t0 >> psh)], 0);
+        const int pg = max(s_pg[((pp < t1 ? pp : t0) >> psh) - pg0], 0);
         off = pp & (page - 1);
         return pool + ((size_t)pg * n_kv + kvh) * head_bytes;
     };
@@ -276,7 +276,7 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
     // Validity of the tile's two groups of 16 positions (their pages).
     auto ok16 = [&](int i, int k) {
         const int t = t0 + 32 * i + 16 * k;
-        return t < t1 && s_pg[(t >> psh) - (t0 >> psh)] >= 0;
+        return t < t1 && s_pg[(t >> psh) - pg0] >= 0;
     };
     auto mask = [&](int i, v16f &X) __attribute__((always_inline)) {
 #pragma unroll
@@ -464,7 +464,9 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
 
 template <int HD, int AT> hipError_t prompt_as(const PagedAttnArgs &a, int tiles, hipStream_t s)
 {
-    const dim3 grid((unsigned)(tiles * a.n_split * a.c.n_head_kv), a.b.n_seq);
+    const int64_t blocks = (int64_t)tiles * a.n_split * a.c.n_head_kv;
+    if (blocks >= 1 << 23) return hipErrorInvalidValue;   // past one launch
+    const dim3 grid((unsigned)blocks, a.b.n_seq);
     if (a.c.kv_type == X100_KV_Q4) k_attn_prompt<HD, AT, true><<<grid, 512, 0, s>>>(a);
     else k_attn_prompt<HD, AT, false><<<grid, 512, 0, s>>>(a);
     return hipGetLastError();

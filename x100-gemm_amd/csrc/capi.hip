@@ -959,6 +959,7 @@ static int attn_paged(const x100_kv_cfg *c, const x100_kv_batch *b, const void *
                       const void *vp, float scale, void *out, int64_t ldo, void *ws, void *stream)
 {
     hipError_t e = x100_attn_paged_launch(*c, *b, q, ldq, kp, vp, scale, out, ldo, ws, (hipStream_t)stream);
+    if (e == hipErrorInvalidValue) return X100_EINVAL;
     if (e != hipSuccess) return hip_fail(e);
     return X100_OK;
 }

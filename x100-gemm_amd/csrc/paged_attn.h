@@ -84,5 +84,5 @@ X100_DEV int split_of_seq(const PagedAttnArgs &a, int kv_len)
 }
 
 constexpr int PROMPT_ROWS = 256;      // rows (token, head) of a block of the prompt kernel
-constexpr int PROMPT_SPLIT = 32768;   // most positions of a split there (its page list is in LDS)
+constexpr int PROMPT_PAGES = 8192;    // most pages of a split there (their list is in LDS)
 hipError_t x100_attn_prompt_launch(const PagedAttnArgs &a, int tiles, hipStream_t s);
