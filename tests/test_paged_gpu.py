@@ -349,6 +349,26 @@ def test_prompts_of_many_tiles(dev, act, kv, n_head, n_kv, hd):
 
 
 @kinds
+@pytest.mark.parametrize("n_head,n_kv,q,L", [
+    (8, 1, [1, 300, 1, 4, 5, 1, 1, 1, 1], [3000, 700, 1, 900, 2000, 17, 0, 256, 4000]),    # 8 .. 40 rows beside a prompt
+    (2, 2, [32, 33, 1, 16, 17, 500, 1, 1, 1, 1, 1, 1, 1, 1, 1], [50, 2000, 1500, 16, 900, 500] + [9] * 9),
+    (4, 2, [0, 0, 257, 0, 1, 0, 0, 0], [0, 5, 1300, 9, 1300, 1, 1, 1]),                   # sequences without rows
+    (16, 1, [2, 70, 1, 3] + [1] * 6, [2500] * 10),
+])
+def test_prompts_beside_single_tokens(dev, act, kv, n_head, n_kv, q, L):
+    """Batches in which sequences of few rows and of many take different kernels, each with its splits."""
+    for hd, page in ((64, 16), (128, 64)):
+        Setup(28, n_head, n_kv, hd, page, act, kv, q, L).check()
+
+
+@kinds
+def test_rows_of_a_wider_bound(dev, act, kv):
+    """The launch sized for more rows and positions than a sequence has (as a captured one is)."""
+    for q, L in (([1, 2, 1], [700, 40, 2000]), ([60, 1, 5], [900, 1, 2000]), ([130, 100, 90], [130, 400, 1000])):
+        Setup(29, 4, 2, 64, 16, act, kv, q, L, max_q=2000, max_kv=5000).check()
+
+
+@kinds
 def test_two_calls_at_once(dev, act, kv):
     """Calls on two streams at the same time, each with its own workspace (and through the library's)."""
     sets = [Setup(27 + i, 8, 2, 128, 64, act, kv, [1, q], [3000, 500]) for i, q in enumerate((1, 60))]

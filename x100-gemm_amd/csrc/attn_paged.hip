@@ -18,6 +18,7 @@ namespace {
 
 constexpr float NEG_INF = X100_NEG_INF;
 using AttnArgs = PagedAttnArgs;
+constexpr int TILE_ROWS = 16;     // rows (token, head) of a block of the tile kernel
 constexpr int TILE_PAGES = 512;   // most pages of a split of the tile kernel (their list is in LDS)
 
 // What a lane reads of a tile of 32 positions, as the cache holds it: K rows 8 (c / 4) + 4 h + c % 4 (h = 0,
@@ -48,7 +49,8 @@ template <int HD, int AT, bool Q4, int NW> __global__ __launch_bounds__(64 * NW,
     } sh;
     __shared__ float s_m[NW][16], s_l[NW][16];
     const int lane = threadIdx.x & 63, w = wave_id(), c = lane & 15, g = lane >> 4;
-    const int sp = blockIdx.x % a.n_split, tile = blockIdx.x / a.n_split, kvh = blockIdx.y, s = blockIdx.z;
+    // tiles last: a sequence's second one is mostly empty, and every other block empty would idle half of the XCDs
+    const int sp = blockIdx.x % a.tile.n, kvh = blockIdx.x / a.tile.n, s = blockIdx.y, tile = blockIdx.z;
     const int n_kv = a.c.n_head_kv, G = a.c.n_head / n_kv, page = a.c.page, psh = __builtin_ctz(page);
     const int i0 = tile * 16;
     // A short table's pages are read here, beside the lengths; a long one's when the split is known.
@@ -64,10 +66,10 @@ template <int HD, int AT, bool Q4, int NW> __global__ __launch_bounds__(64 * NW,
     if (all) list(0, n_all);
     const PagedSeq q = paged_seq(a.b, s);
     const int n_rows = q.q_len * G;
-    if (i0 >= n_rows) return;
+    if (i0 >= n_rows || n_rows > a.few) return;
     const int pos0 = q.kv_len - q.q_len;                       // position of token 0
     const int vis = pos0 + (min(i0 + 15, n_rows - 1)) / G + 1;  // positions that the tile's last row sees
-    const int per = split_of_seq(a, q.kv_len);
+    const int per = a.tile.positions(q.kv_len);
     const int ns = max(1, (vis + per - 1) / per);
     if (sp >= ns) return;
     const int t0 = sp * per, t1 = min(t0 + per, vis);
@@ -362,36 +364,40 @@ template <int HD, int AT, bool Q4, int NW> __global__ __launch_bounds__(64 * NW,
             const uint32_t b = ls == 0.0f ? 0u : f2act<AT>(y0 * f) | f2act<AT>(y1 * f) << 16;
             *(uint32_t *)(a.out + (size_t)(q.q0 + tk) * a.ldo + (size_t)hh * HD + el) = b;
         } else {
-            const size_t at = part_at(a, q.q0, kvh, i0 + r) + sp;
+            const size_t at = tile_part(a, s, kvh, i0 + r) + sp;
             *(float2 *)(a.part_o + at * HD + el) = make_float2(y0, y1);
             if (el == 0) a.part_ml[at] = make_float2(mm, ls);
         }
     }
 }
 
-// Merges the splits of rows that have more than one: HD / 4 lanes per (row, head), 4 elements each; x = token
-// row, y = the heads of a block.
+// Merges the splits of rows that have more than one: HD / 4 lanes per (row, head), 4 elements each; x = row, or
+// (where only the tile kernel has splits) sequence and token, y = the heads of a block.
 template <int HD, int AT> __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a)
 {
     constexpr int L = HD / 4;
-    const int G = a.c.n_head / a.c.n_head_kv, row = blockIdx.x;
+    const int G = a.c.n_head / a.c.n_head_kv;
     const int head = blockIdx.y * (256 / L) + threadIdx.x / L, l4 = threadIdx.x % L;
-    const int s = paged_find(a.b, row);
+    const bool rows = a.prompt.n > 1;
+    const int tokens = a.tile_rows / G;
+    const int s = rows ? paged_find(a.b, blockIdx.x) : blockIdx.x / tokens;
     if (s >= a.b.n_seq) return;
     const PagedSeq q = paged_seq(a.b, s);
-    if (q.q_len <= 0 || row < q.q0) return;
+    const int row = rows ? blockIdx.x : q.q0 + blockIdx.x % tokens;
+    if (row < q.q0 || row - q.q0 >= q.q_len || (!rows && q.q_len * G > a.few)) return;
     const int hd = min(head, a.c.n_head - 1), kvh = hd / G, i = (row - q.q0) * G + hd % G;
-    const int tr = a.tile_rows, per = split_of_seq(a, q.kv_len);
+    const bool few = q.q_len * G <= a.few;
+    const int tr = few ? TILE_ROWS : PROMPT_ROWS, per = (few ? a.tile : a.prompt).positions(q.kv_len);
     const int vis = q.kv_len - q.q_len + min(i / tr * tr + tr - 1, q.q_len * G - 1) / G + 1;
     const int ns = (vis + per - 1) / per;
-    const size_t at = part_at(a, q.q0, kvh, i);
+    if (ns <= 1 || head >= a.c.n_head) return;   // the lanes of a head together
+    const size_t at = few ? tile_part(a, s, kvh, i) : prompt_part(a, q.q0, kvh, i);
     const float2 *ml = a.part_ml + at;
     const float4 *po = (const float4 *)(a.part_o + at * HD) + l4;
     float m = NEG_INF;
     for (int k = l4; k < ns; k += L) m = fmaxf(m, ml[k].x);
 #pragma unroll
     for (int d = 1; d < L; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, L));
-    if (ns <= 1 || head >= a.c.n_head) return;
     const float ms = m == NEG_INF ? 0.0f : m;
     float l = 0.0f;
     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -420,16 +426,13 @@ template <int HD, int AT> __global__ __launch_bounds__(256) void k_attn_join(con
     *(v2u *)(a.out + (size_t)row * a.ldo + (size_t)head * HD + 4 * l4) = o;
 }
 
-// How a call is laid out: the tile kernel where no sequence has more than FEW rows (token, head), else the
+// How a call is laid out: sequences of up to FEW rows (token, head) go to the tile kernel, longer ones to the
 // prompt kernel; the positions in splits, so that the blocks fill the chip.
 constexpr int FEW = 32;
 struct Plan {
-    bool prompt;
-    int tiles, n_split, least;
-    size_t results(const x100_kv_cfg &c, const x100_kv_batch &b) const
-    {
-        return n_split == 1 ? 0 : (size_t)b.n_rows * c.n_head * n_split;
-    }
+    PagedSplit tile, prompt;   // n == 0: the kernel is not launched
+    size_t tile_parts, prompt_parts;   // split results
+    int few, tile_rows, tiles;         // rows of a sequence and their tiles, tile kernel
 };
 
 Plan plan_of(const x100_kv_cfg &c, const x100_kv_batch &b)
@@ -437,55 +440,65 @@ Plan plan_of(const x100_kv_cfg &c, const x100_kv_batch &b)
     Plan p = {};
     const int G = c.n_head / c.n_head_kv;
     const int64_t rows = (int64_t)b.max_q * G, kv = b.max_kv;   // of the longest sequence
-    p.prompt = rows > FEW;
-    if (!p.prompt) {
+    // Prompts beside single tokens (the sequences but one have less than a quarter of max_q on average) take both
+    // kernels: 63 tokens at 4096 positions and 512 at 4608, 290 / 165 us (each alone 91 and 57).  A batch of prompts takes the prompt
+    // kernel alone, which is right for any rows: the other launch costs 2 us.
+    const bool prompts = rows > FEW;
+    const bool both = prompts && b.n_seq > 1 && ((int64_t)b.n_rows - b.max_q) * 4 <= (int64_t)(b.n_seq - 1) * b.max_q;
+    if (!prompts || both) {
         // A block per CU where rows of 16 bits are read (256 blocks of four waves keep HBM busy: 64 sequences of
         // up to 4096 positions, us with 256 / 512 / 1024 blocks wanted: 70.6 / 78.6 / 77.2), three where 4-bit
         // codes have to be unpacked (16 of up to 60001: 115.8 / 113.9 / 101.8, 768: 98.4).  Up to 512 positions
         // one block is faster than two and their join (9.6 / 12.6 us).
         const int64_t most = (int64_t)TILE_PAGES * c.page;
-        p.least = 256;
-        p.tiles = (int)((rows + 15) / 16);
-        const int64_t base = (int64_t)p.tiles * std::min(b.n_seq, b.n_rows) * c.n_head_kv;
+        p.few = FEW;
+        p.tile_rows = (int)std::min<int64_t>(rows, FEW);
+        p.tiles = (p.tile_rows + TILE_ROWS - 1) / TILE_ROWS;
+        const int64_t base = (int64_t)(both ? 1 : p.tiles) * std::min(b.n_seq, b.n_rows) * c.n_head_kv;
         const int64_t want = kv <= 512 ? 1 : std::max<int64_t>(1, (c.kv_type == X100_KV_Q4 ? 768 : 256) / base);
-        p.n_split = (int)std::max(std::min(want, (kv + 255) / 256), (kv + most - 1) / most);
-        return p;
+        p.tile = {(int)std::max(std::min(want, (kv + 255) / 256), (kv + most - 1) / most), 256};
+        if (p.tile.n > 1) p.tile_parts = (size_t)b.n_seq * p.tile_rows * c.n_head_kv * p.tile.n;
     }
-    // One block per CU at a time, so rounds of 256 blocks: the number of splits with the least sum over the
-    // rounds of a block's positions and its own start and end (as long as 512 positions), the join besides.
-    p.least = 512;
-    p.tiles = (int)((rows + PROMPT_ROWS - 1) / PROMPT_ROWS);
-    const int64_t full = (int64_t)b.n_rows * G / PROMPT_ROWS + b.n_seq;   // tiles that have rows
-    const int64_t base = std::min<int64_t>((int64_t)p.tiles * b.n_seq, full) * c.n_head_kv;
-    int64_t best = 0;
-    const int64_t most = (int64_t)PROMPT_PAGES * c.page;
-    for (int64_t n = (kv + most - 1) / most, n0 = n; n == n0 || (n <= 16 && n * 512 < kv + 512); n++) {
-        const int64_t cost = (base * n + 255) / 256 * (kv / n + 512) + (n > 1 ? 512 : 0);
-        if (n == n0 || cost < best) {
-            best = cost;
-            p.n_split = (int)n;
+    if (prompts) {
+        // One block per CU at a time, so rounds of 256 blocks: the number of splits with the least sum over the
+        // rounds of a block's positions and its own start and end (as long as 512 positions), the join besides.
+        const int64_t tiles = (rows + PROMPT_ROWS - 1) / PROMPT_ROWS;
+        // tiles that have rows (of one sequence, the others single tokens, or of all)
+        const int64_t full = both ? std::max(1, b.n_rows - b.n_seq + 1) * (int64_t)G / PROMPT_ROWS : (int64_t)b.n_rows * G / PROMPT_ROWS + b.n_seq;
+        const int64_t base = std::max<int64_t>(1, std::min(tiles * b.n_seq, full)) * c.n_head_kv;
+        const int64_t most = (int64_t)PROMPT_PAGES * c.page;
+        int64_t best = 0;
+        for (int64_t n = (kv + most - 1) / most, n0 = n; n == n0 || (n <= 16 && n * 512 < kv + 512); n++) {
+            const int64_t cost = (base * n + 255) / 256 * (kv / n + 512) + (n > 1 ? 512 : 0);
+            if (n == n0 || cost < best) {
+                best = cost;
+                p.prompt = {(int)n, 512};
+            }
         }
+        if (p.prompt.n > 1) p.prompt_parts = (size_t)b.n_rows * c.n_head * p.prompt.n;
     }
     return p;
 }
 
 template <int HD, int AT> hipError_t attn_as(const AttnArgs &a, const Plan &p, hipStream_t s)
 {
-    if (p.prompt) {
-        const hipError_t e = x100_attn_prompt_launch(a, p.tiles, s);
+    if (p.prompt.n) {
+        const hipError_t e = x100_attn_prompt_launch(a, s);
         if (e != hipSuccess) return e;
-    } else {
-        const int64_t blocks = (int64_t)p.tiles * p.n_split;
+    }
+    if (p.tile.n) {
+        const int64_t blocks = (int64_t)a.c.n_head_kv * p.tile.n;
         if (blocks >= 1 << 24) return hipErrorInvalidValue;   // past one launch
-        const dim3 grid((unsigned)blocks, a.c.n_head_kv, a.b.n_seq);
+        const dim3 grid((unsigned)blocks, a.b.n_seq, p.tiles);
         if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true, 4><<<grid, 256, 0, s>>>(a);
         else k_attn_tile<HD, AT, false, 4><<<grid, 256, 0, s>>>(a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    if (p.n_split == 1) return hipSuccess;
+    if (p.tile.n <= 1 && p.prompt.n <= 1) return hipSuccess;
     constexpr int heads = 256 / (HD / 4);
-    k_attn_join<HD, AT><<<dim3(a.b.n_rows, (a.c.n_head + heads - 1) / heads), 256, 0, s>>>(a);
+    const unsigned rows = p.prompt.n > 1 ? a.b.n_rows : (unsigned)a.b.n_seq * (a.tile_rows / (a.c.n_head / a.c.n_head_kv));
+    k_attn_join<HD, AT><<<dim3(rows, (a.c.n_head + heads - 1) / heads), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -493,7 +506,8 @@ template <int HD, int AT> hipError_t attn_as(const AttnArgs &a, const Plan &p, h
 
 size_t x100_attn_paged_workspace(const x100_kv_cfg &c, const x100_kv_batch &b)
 {
-    return plan_of(c, b).results(c, b) * (c.head_dim + 2) * sizeof(float);
+    const Plan p = plan_of(c, b);
+    return (p.tile_parts + p.prompt_parts) * (c.head_dim + 2) * sizeof(float);
 }
 
 hipError_t x100_attn_paged_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const void *q, int64_t ldq,
@@ -512,10 +526,12 @@ hipError_t x100_attn_paged_launch(const x100_kv_cfg &c, const x100_kv_batch &b, 
     a.out = (uint16_t *)out;
     a.ldo = ldo;
     a.part_o = (float *)ws;
-    a.part_ml = (float2 *)(a.part_o + p.results(c, b) * c.head_dim);
-    a.n_split = p.n_split;
-    a.least = p.least;
-    a.tile_rows = p.prompt ? PROMPT_ROWS : 16;
+    a.part_ml = (float2 *)(a.part_o + (p.prompt_parts + p.tile_parts) * c.head_dim);
+    a.few = p.few;
+    a.tile = p.tile;
+    a.prompt = p.prompt;
+    a.tile_at = p.prompt_parts;
+    a.tile_rows = p.tile_rows;
     if (c.head_dim == 64)
         return c.act_type == X100_T_F16 ? attn_as<64, X100_T_F16>(a, p, s) : attn_as<64, X100_T_BF16>(a, p, s);
     return c.act_type == X100_T_F16 ? attn_as<128, X100_T_F16>(a, p, s) : attn_as<128, X100_T_BF16>(a, p, s);

@@ -41,14 +41,21 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
     __shared__ int s_inf[2][HD], s_odd;
     const int lane = threadIdx.x & 63, w = wave_id(), c = lane & 31, h = lane >> 5;
     const int n_kv = a.c.n_head_kv, G = a.c.n_head / n_kv, page = a.c.page, psh = __builtin_ctz(page);
-    const int kvh = blockIdx.x % n_kv, u = blockIdx.x / n_kv, sp = u % a.n_split;
-    const int tile = gridDim.x / (n_kv * a.n_split) - 1 - u / a.n_split, s = blockIdx.y;   // longest first
+    const int ns_max = a.prompt.n, kvh = blockIdx.x % n_kv, u = blockIdx.x / n_kv, sp = u % ns_max;
+    // Item (sequence, tile of rows): sequence s has the items from q_start[s] G / 256 + s on, which leaves room for
+    // its tiles whatever the rows before it, and at most one item per sequence without rows.  (A grid of the
+    // longest sequence's tiles for every sequence: 64 of 16 rows under a bound of 4096, 200 / 35 us.)
+    const int item = u / ns_max;
+    auto first = [&](int s) { return (int64_t)a.b.q_start[s] * G / PROMPT_ROWS + s; };
+    const int s = a.b.n_seq == 1 ? 0 : paged_search(a.b.n_seq, [&](int s) { return first(s) <= item; });
+    if (s >= a.b.n_seq) return;
     const PagedSeq q = paged_seq(a.b, s);
-    const int n_rows = q.q_len * G, i0 = tile * PROMPT_ROWS;
-    if (i0 >= n_rows) return;
-    const int pos0 = q.kv_len - q.q_len;
+    const int n_rows = q.q_len * G, tiles = (n_rows + PROMPT_ROWS - 1) / PROMPT_ROWS;
+    const int64_t place = item - first(s);
+    if (n_rows <= a.few || place < 0 || place >= tiles) return;
+    const int i0 = (tiles - 1 - (int)place) * PROMPT_ROWS, pos0 = q.kv_len - q.q_len;   // the longest first
     const int vis = pos0 + min(i0 + PROMPT_ROWS - 1, n_rows - 1) / G + 1;
-    const int per = split_of_seq(a, q.kv_len), ns = max(1, (vis + per - 1) / per);
+    const int per = a.prompt.positions(q.kv_len), ns = max(1, (vis + per - 1) / per);
     if (sp >= ns) return;
     const int t0 = sp * per, t1 = min(t0 + per, vis);
     const int n = max(0, (t1 - t0 + 31) >> 5);   // tiles
@@ -112,7 +119,7 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
         const int t = t0 + 64 * pp + 8 * w;
         return s_pg[((t < t1 ? t : t0) >> psh) - pg0];
     };
-    auto place = [&](int pp, int pg) -> size_t {
+    auto bytes_at = [&](int pp, int pg) -> size_t {
         const int t = t0 + 64 * pp + 8 * w;
         return (size_t)(max(__builtin_amdgcn_readfirstlane(pg), 0) * n_kv + kvh) * head_bytes + (t & (page - 1)) * (HD * 2);
     };
@@ -324,8 +331,8 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
         size_t at = 0;   // where the wave's positions of the next V pair are
         int pg = 0;      // page of the next K pair
         if constexpr (!Q4) {
-            const size_t a0 = place(0, page_at(0));
-            at = place(min(1, np - 1), page_at(min(1, np - 1)));
+            const size_t a0 = bytes_at(0, page_at(0));
+            at = bytes_at(min(1, np - 1), page_at(min(1, np - 1)));
 #pragma unroll
             for (int d = 0; d < ND; d++) {
                 load_k(a0, 0, d);
@@ -371,7 +378,7 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
             if constexpr (!Q4) {
                 asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 const size_t av = at;
-                at = place(min(pp + 2, np - 1), pg);
+                at = bytes_at(min(pp + 2, np - 1), pg);
                 step(2 * pp, S, T, v0, s_v[r2] + KB, k1, [&](int g) {
                     if (g % 2 == 1 && g / 2 < ND) load_v(av, r1, g / 2);
                     if (g % 2 == 1 && g / 2 >= ND && g / 2 < 2 * ND) load_k(at, r2, g / 2 - ND);
@@ -402,7 +409,7 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
                 asm volatile("s_waitcnt vmcnt(0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
                 for (int d = 0; d < ND; d++) load_v(at, r1, d);
-                at = place(min(pp + 2, np - 1), pg);
+                at = bytes_at(min(pp + 2, np - 1), pg);
 #pragma unroll
                 for (int d = 0; d < ND; d++) load_k(at, r2, d);
                 pg = page_at(min(pp + 3, np - 1));
@@ -451,7 +458,7 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
                 *(v2u *)(o + 32 * j + 8 * e) = y;
             }
     } else {
-        const size_t to = part_at(a, q.q0, kvh, i) + sp;
+        const size_t to = prompt_part(a, q.q0, kvh, i) + sp;
         float *o = a.part_o + to * HD + 4 * h;
 #pragma unroll
         for (int j = 0; j < NJ; j++)
@@ -462,21 +469,20 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
     }
 }
 
-template <int HD, int AT> hipError_t prompt_as(const PagedAttnArgs &a, int tiles, hipStream_t s)
+template <int HD, int AT> hipError_t prompt_as(const PagedAttnArgs &a, hipStream_t s)
 {
-    const int64_t blocks = (int64_t)tiles * a.n_split * a.c.n_head_kv;
+    const int64_t items = (int64_t)a.b.n_rows * (a.c.n_head / a.c.n_head_kv) / PROMPT_ROWS + a.b.n_seq;
+    const int64_t blocks = items * a.prompt.n * a.c.n_head_kv;
     if (blocks >= 1 << 23) return hipErrorInvalidValue;   // past one launch
-    const dim3 grid((unsigned)blocks, a.b.n_seq);
-    if (a.c.kv_type == X100_KV_Q4) k_attn_prompt<HD, AT, true><<<grid, 512, 0, s>>>(a);
-    else k_attn_prompt<HD, AT, false><<<grid, 512, 0, s>>>(a);
+    if (a.c.kv_type == X100_KV_Q4) k_attn_prompt<HD, AT, true><<<(unsigned)blocks, 512, 0, s>>>(a);
+    else k_attn_prompt<HD, AT, false><<<(unsigned)blocks, 512, 0, s>>>(a);
     return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t x100_attn_prompt_launch(const PagedAttnArgs &a, int tiles, hipStream_t s)
+hipError_t x100_attn_prompt_launch(const PagedAttnArgs &a, hipStream_t s)
 {
-    if (a.c.head_dim == 64)
-        return a.c.act_type == X100_T_F16 ? prompt_as<64, X100_T_F16>(a, tiles, s) : prompt_as<64, X100_T_BF16>(a, tiles, s);
-    return a.c.act_type == X100_T_F16 ? prompt_as<128, X100_T_F16>(a, tiles, s) : prompt_as<128, X100_T_BF16>(a, tiles, s);
+    if (a.c.head_dim == 64) return a.c.act_type == X100_T_F16 ? prompt_as<64, X100_T_F16>(a, s) : prompt_as<64, X100_T_BF16>(a, s);
+    return a.c.act_type == X100_T_F16 ? prompt_as<128, X100_T_F16>(a, s) : prompt_as<128, X100_T_BF16>(a, s);
 }

@@ -22,22 +22,27 @@ X100_DEV int paged_page(const x100_kv_cfg &c, const x100_kv_batch &b, int s, int
     return g >= 0 && g < c.n_pages ? g : -1;
 }
 
-// The sequence of row r: the first s with q_start[s + 1] > r (n_seq if there is none), by the whole
-// wave, 64 entries per step.
-X100_DEV int paged_find(const x100_kv_batch &b, int r)
+// The first s of 0 .. n - 1 for which below(s + 1) does not hold (n if there is none; below holds up to some
+// place and not behind it), by the whole wave, 64 entries per step.
+template <class F> X100_DEV int paged_search(int n_seq, F &&below)
 {
     const int lane = threadIdx.x & 63;
-    int lo = 0, len = b.n_seq;
+    int lo = 0, len = n_seq;
     while (len > 0) {
         const int stride = (len + 63) / 64;              // entries lo + (i + 1) * stride - 1
         const int i = (lane + 1) * stride - 1;
-        const bool le = i < len && b.q_start[lo + i + 1] <= r;
-        const int n = __popcll(__ballot(le)) * stride;   // entries known to lie at or below r
+        const bool le = i < len && below(lo + i + 1);
+        const int n = __popcll(__ballot(le)) * stride;   // entries known to lie below
         if (stride == 1) return lo + n;
         lo += n;
-        len = min(stride - 1, len - n);                  // the next entry probed lies above r
+        len = min(stride - 1, len - n);                  // the next entry probed does not
     }
     return lo;
+}
+// The sequence of row r: the first s with q_start[s + 1] > r (n_seq if there is none).
+X100_DEV int paged_find(const x100_kv_batch &b, int r)
+{
+    return paged_search(b.n_seq, [&](int s) { return b.q_start[s] <= r; });
 }
 
 // Bytes of one head's part of a page, K or V.

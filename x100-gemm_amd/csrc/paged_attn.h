@@ -4,6 +4,13 @@
 
 constexpr float X100_NEG_INF = -__builtin_inff();
 
+// How a kernel splits the positions: a sequence's in n equal parts, so that the blocks of a batch of unequal
+// sequences are as equal as its lengths let them be; a multiple of 128, `least` or more.
+struct PagedSplit {
+    int n, least;
+    X100_DEV int positions(int kv_len) const { return max(least, ((kv_len + n - 1) / n + 127) & ~127); }
+};
+
 struct PagedAttnArgs {
     x100_kv_cfg c;
     x100_kv_batch b;
@@ -13,10 +20,12 @@ struct PagedAttnArgs {
     float scale2;        // scale * log2(e): weights are powers of two
     uint16_t *out;
     int64_t ldo;
-    float *part_o;       // split results, n_split per row and head (part_at): O, HD floats each, not divided by l,
+    float *part_o;       // split results: O, HD floats each, not divided by l,
     float2 *part_ml;     // and (m, l)
-    int n_split, least;  // splits of the longest sequence, fewest positions of one
-    int tile_rows;       // rows of a block's tile
+    int few;             // sequences of up to this many rows (token, head) are the tile kernel's, the rest the prompt kernel's
+    PagedSplit tile, prompt;
+    size_t tile_at;      // the tile kernel's first split result
+    int tile_rows;       // rows of a sequence there
 };
 
 template <int T> struct Mfma16;
@@ -70,19 +79,18 @@ template <int T> X100_DEV float add2(uint32_t w, float c)
     }
 }
 
-// Number of row i's (token, head) first split result; q0: the sequence's first row.
-X100_DEV size_t part_at(const PagedAttnArgs &a, int q0, int kvh, int i)
+// Number of row i's (token, head) first split result: by rows of the batch (q0: the sequence's first), and by
+// sequences.
+X100_DEV size_t prompt_part(const PagedAttnArgs &a, int q0, int kvh, int i)
 {
     const int G = a.c.n_head / a.c.n_head_kv;
-    return (((size_t)q0 * G + i) * a.c.n_head_kv + kvh) * a.n_split;
+    return (((size_t)q0 * G + i) * a.c.n_head_kv + kvh) * a.prompt.n;
 }
-// Positions of a split: a sequence's positions in n_split equal parts, so that the blocks of a batch of
-// unequal sequences are as equal as its lengths let them be; a multiple of 128, a.least or more.
-X100_DEV int split_of_seq(const PagedAttnArgs &a, int kv_len)
+X100_DEV size_t tile_part(const PagedAttnArgs &a, int s, int kvh, int i)
 {
-    return max(a.least, ((kv_len + a.n_split - 1) / a.n_split + 127) & ~127);
+    return a.tile_at + (((size_t)s * a.tile_rows + i) * a.c.n_head_kv + kvh) * a.tile.n;
 }
 
 constexpr int PROMPT_ROWS = 256;      // rows (token, head) of a block of the prompt kernel
 constexpr int PROMPT_PAGES = 8192;    // most pages of a split there (their list is in LDS)
-hipError_t x100_attn_prompt_launch(const PagedAttnArgs &a, int tiles, hipStream_t s);
+hipError_t x100_attn_prompt_launch(const PagedAttnArgs &a, hipStream_t s);
