@@ -449,14 +449,15 @@ Plan plan_of(const x100_kv_cfg &c, const x100_kv_batch &b)
         // A block per CU where rows of 16 bits are read (256 blocks of four waves keep HBM busy: 64 sequences of
         // up to 4096 positions, us with 256 / 512 / 1024 blocks wanted: 70.6 / 78.6 / 77.2), three where 4-bit
         // codes have to be unpacked (16 of up to 60001: 115.8 / 113.9 / 101.8, 768: 98.4).  Up to 512 positions
-        // one block is faster than two and their join (9.6 / 12.6 us).
+        // one block is faster than two and their join (9.6 / 12.6 us); behind that 128 positions, a tile per wave, are
+        // the least (one sequence of 1024: 10.7 us at 256, 9.8 at 128).
         const int64_t most = (int64_t)TILE_PAGES * c.page;
         p.few = FEW;
         p.tile_rows = (int)std::min<int64_t>(rows, FEW);
         p.tiles = (p.tile_rows + TILE_ROWS - 1) / TILE_ROWS;
         const int64_t base = (int64_t)(both ? 1 : p.tiles) * std::min(b.n_seq, b.n_rows) * c.n_head_kv;
         const int64_t want = kv <= 512 ? 1 : std::max<int64_t>(1, (c.kv_type == X100_KV_Q4 ? 768 : 256) / base);
-        p.tile = {(int)std::max(std::min(want, (kv + 255) / 256), (kv + most - 1) / most), 256};
+        p.tile = {(int)std::max(std::min(want, (kv + 127) / 128), (kv + most - 1) / most), 128};
         if (p.tile.n > 1) p.tile_parts = (size_t)b.n_seq * p.tile_rows * c.n_head_kv * p.tile.n;
     }
     if (prompts) {
