@@ -9,8 +9,8 @@
  * int8 weights with a scale per column, row_scale is A's scale array and col_scale the weights'.
  *
  * Codes: t = the row's values, amax = max |t|, code = rint(t * f) with f = 127 * (1 / amax) in fp32
- * (two roundings; ties to even), scale = amax / 127.  A row of zeros (or amax < 2^-100) has codes 0 and scale 0; a row that holds an
- * infinity or a NaN has codes 0 and scale NaN.  In add_rmsnorm_i8 t = h * weight and the norm's
+ * (two roundings; ties to even), scale = amax / 127.  A row of zeros (or amax < 2^-100) has codes 0 and
+ * scale 0; a row that holds an infinity or a NaN has codes 0 and scale NaN.  In add_rmsnorm_i8 t = h * weight and the norm's
  * factor goes into the scale alone (it cancels in the code), so that the codes do not depend on the
  * order in which a sum was taken: they are the same for every layout, alignment and launch.
  *

@@ -368,6 +368,23 @@ def test_rows_of_a_wider_bound(dev, act, kv):
         Setup(29, 4, 2, 64, 16, act, kv, q, L, max_q=2000, max_kv=5000).check()
 
 
+def test_batches_past_one_launch(dev):
+    """Refused by their bounds alone, before anything is enqueued (the arrays are never read)."""
+    some = torch.zeros(4096, dtype=torch.int32, device=dev)
+    pools = [torch.zeros(256, dtype=torch.uint8, device=dev) for _ in range(2)]
+    p = some.data_ptr()
+    c = x.KvCfg(1024, 1024, 64, 16, 1, ref.F16, ref.F16)
+    b = x.KvBatch(65535, (1 << 24) - 1, 1000, 16, 1, p, p, p)
+    with pytest.raises(x.X100Error):
+        x.attn_paged(c, b, p, 65536, pools[0].data_ptr(), pools[1].data_ptr(), 1.0, p, 65536, stream())
+    assert x.attn_paged_workspace_bytes(c, b) == 0
+    rows = [x.Rows(ref.F16, p, 65536, None, None) for _ in range(3)]
+    with pytest.raises(x.X100Error):
+        x.kv_append(c, b, x.KvRows(*rows, None, None, 0.0, None, 0), pools[0].data_ptr(), pools[1].data_ptr(), p, stream())
+    torch.cuda.synchronize()
+    assert not some.any()
+
+
 @kinds
 def test_two_calls_at_once(dev, act, kv):
     """Calls on two streams at the same time, each with its own workspace (and through the library's)."""

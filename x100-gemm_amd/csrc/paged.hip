@@ -1,8 +1,9 @@
 // Paged KV cache (x100_paged.h): new rows into the pages (head norms, rotation, 16 or 4 bits), cached
 // rows back out, and the rotation table.
 //
-// Bound by HBM for prompts (a row is read once, its queries, keys and values written once) and by
-// launch and dependent loads (q_start -> kv_len -> block_table) for single tokens.
+// Bound by HBM for prompts (a row is read once, its queries, keys and values written once): 6400 rows of 40 heads
+// of 128, int32 to f16 and 4 bits, 47 us, 4.0 TB/s (a copy of 2 GiB: 5.0).  For single tokens bound by the launch and
+// dependent loads (q_start -> kv_len -> block_table): 64 rows 5.4 us.
 #include <algorithm>
 
 #include "paged.h"
@@ -91,10 +92,17 @@ template <int HD, int ST, int AT, bool Q4> X100_DEV void append_qk(const AppendA
     if (!a.q_out) head = max(head, n_h);   // keys only
     if (head >= end || rbase >= a.b.n_rows) return;
     const int row = min(rbase + sub, a.b.n_rows - 1);
-    float raw[E];
+    // What a head needs goes out one head ahead, without a branch around it: behind a branch, or with the column scales
+    // loaded at their use, the wait for them was one for the next head's elements (62 us, so 57).
+    RowBits<ST, E> raw;
+    float cl[E];   // column scales
     auto fetch = [&](int hd) __attribute__((always_inline)) {
         const x100_rows &src = hd < n_h ? a.r.q : a.r.k;
-        row_elems<ST, E>(src.p, (size_t)row * src.ld + (hd < n_h ? hd : hd - n_h) * HD + E * l, raw);
+        const int col = (hd < n_h ? hd : hd - n_h) * HD + E * l;
+        if constexpr (ST == X100_T_I32)
+#pragma unroll
+            for (int e = 0; e < E; e++) cl[e] = src.col_scale[col + e];
+        raw.load(src.p, (size_t)row * src.ld + col);
     };
     fetch(head);
     const RowPlace at = row_place(a.b, rbase, sub);
@@ -102,54 +110,65 @@ template <int HD, int ST, int AT, bool Q4> X100_DEV void append_qk(const AppendA
     if (a.r.rope) {
         const float2 *t = (const float2 *)a.r.rope + (size_t)max(at.pos, 0) * (HD / 2) + E * (l & 7);
 #pragma unroll
-        for (int e = 0; e < E; e++) cs[e] = t[e];
+        for (int e = 0; e < E; e++) {
+            cs[e] = t[e];
+            if (l < 8) cs[e].y = -cs[e].y;
+        }
     }
     const int pg = at.mine && at.pos >= 0 ? paged_page(a.c, a.b, at.s, at.pos) : -1;
     const int off = at.pos & (page - 1);
-    for (; head < end; head++) {
-        const bool is_q = head < n_h;
-        const x100_rows &src = is_q ? a.r.q : a.r.k;
-        float v[E];
+    // norm weights and the row's scale, of queries or keys
+    float nw[E], rs = 1.0f;
+    auto weights = [&](const x100_rows &src, const float *w) __attribute__((always_inline)) {
+        if constexpr (ST == X100_T_I32) rs = src.row_scale[row];
+        if (w)
 #pragma unroll
-        for (int e = 0; e < E; e++) v[e] = raw[e];
-        if (head + 1 < end) fetch(head + 1);
-        if constexpr (ST == X100_T_I32) {
-            const float rs = src.row_scale[row];
-            const float *cl = src.col_scale + (is_q ? head : head - n_h) * HD + E * l;
+            for (int e = 0; e < E; e++) nw[e] = w[E * l + e];
+    };
+    // the head's values, normalised and rotated; the next head's on their way
+    auto values = [&](float (&v)[E], bool norm) __attribute__((always_inline)) {
+        raw.values(v);
+        if constexpr (ST == X100_T_I32)
 #pragma unroll
             for (int e = 0; e < E; e++) v[e] = v[e] * rs * cl[e];
-        }
-        const float *nw = is_q ? a.r.q_norm : a.r.k_norm;
-        if (nw) {
+        fetch(min(head + 1, end - 1));
+        if (norm) {
             float ss = 0.0f;
 #pragma unroll
             for (int e = 0; e < E; e++) ss = __builtin_fmaf(v[e], v[e], ss);
             const float sc = 1.0f / sqrtf(sum16(ss) / (float)HD + a.r.eps);
 #pragma unroll
-            for (int e = 0; e < E; e++) v[e] = v[e] * sc * nw[E * l + e];
+            for (int e = 0; e < E; e++) v[e] = v[e] * sc * nw[e];
         }
         if (a.r.rope) {
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 const float o = dpp_f<0x128>(0.0f, v[e]);   // the pair's other element
-                v[e] = l < 8 ? v[e] * cs[e].x - o * cs[e].y : o * cs[e].y + v[e] * cs[e].x;
+                v[e] = v[e] * cs[e].x + o * cs[e].y;
             }
         }
-        if (is_q) {
-            if (at.pos < 0) {   // a row before position 0: zeros
+    };
+    if (head < min(end, n_h)) weights(a.r.q, a.r.q_norm);
+    for (; head < min(end, n_h); head++) {
+        float v[E];
+        values(v, a.r.q_norm);
+        if (at.pos < 0) {   // a row before position 0: zeros
 #pragma unroll
-                for (int e = 0; e < E; e++) v[e] = 0.0f;
-            }
-            if (at.mine) {
-                uint32_t u[E / 2];
-#pragma unroll
-                for (int e = 0; e < E / 2; e++) u[e] = f2act<AT>(v[2 * e]) | f2act<AT>(v[2 * e + 1]) << 16;
-                uint16_t *o = a.q_out + ((size_t)row * n_h + head) * HD + E * l;
-                if constexpr (E == 8) *(v4u *)o = v4u{u[0], u[1], u[2], u[3]};
-                else *(v2u *)o = v2u{u[0], u[1]};
-            }
-            continue;
+            for (int e = 0; e < E; e++) v[e] = 0.0f;
         }
+        if (at.mine) {
+            uint32_t u[E / 2];
+#pragma unroll
+            for (int e = 0; e < E / 2; e++) u[e] = f2act<AT>(v[2 * e]) | f2act<AT>(v[2 * e + 1]) << 16;
+            uint16_t *o = a.q_out + ((size_t)row * n_h + head) * HD + E * l;
+            if constexpr (E == 8) *(v4u *)o = v4u{u[0], u[1], u[2], u[3]};
+            else *(v2u *)o = v2u{u[0], u[1]};
+        }
+    }
+    if (head < end) weights(a.r.k, a.r.k_norm);
+    for (; head < end; head++) {
+        float v[E];
+        values(v, a.r.k_norm);
         uint8_t *base = a.kp + ((size_t)max(pg, 0) * n_kv + head - n_h) * page_head_bytes<HD, Q4>(page);
         if constexpr (!Q4) {
             if (pg >= 0) {
@@ -224,12 +243,11 @@ template <int HD, int ST, int AT, bool Q4> X100_DEV void append_v(const AppendAr
             const int pg = paged_page(a.c, a.b, s, pos), blk = (pos & (page - 1)) >> 3;
             float v[8];
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = k < n ? row_elem<ST>(src.p, (size_t)(row + k) * src.ld + col) : 0.0f;
+            for (int k = 0; k < 8; k++) v[k] = row_elem<ST>(src.p, (size_t)(row + min(k, n - 1)) * src.ld + col);
             if constexpr (ST == X100_T_I32) {
                 const float cl = src.col_scale[col];
 #pragma unroll
-                for (int k = 0; k < 8; k++)
-                    if (k < n) v[k] = v[k] * src.row_scale[row + k] * cl;
+                for (int k = 0; k < 8; k++) v[k] = v[k] * src.row_scale[row + min(k, n - 1)] * cl;
             }
             row += n;
             if (pg < 0) continue;
@@ -344,8 +362,8 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256) void k_read
 template <int HD, int ST> hipError_t append_as(AppendArgs a, hipStream_t s)
 {
     // Heads per wave: as many as leave 4096 waves (16 per CU), so that few rows are spread over the chip and many
-    // look their places up once for several heads (8000 rows of 36 heads, int32 to 4 bits and read back, us: one
-    // head per wave 109; 32768 / 16384 / 8192 / 4096 waves 80.6 / 69.4 / 67.6 / 62.2).
+    // look their places up once for several heads (6400 rows of 36 heads, int32 to 4 bits and read back, us: 16384 /
+    // 8192 / 4096 / 2048 waves 61.4 / 57.8 / 56.6 / 58.0).
     // Values: a unit of 8 rows holds whole blocks of prompts; single tokens get a unit each.
     const int n_rows = a.b.n_rows, all = a.c.n_head + a.c.n_head_kv, quads = (n_rows + 3) / 4;
     a.heads = std::max(1, (int)std::min<int64_t>(all, (int64_t)quads * all / 4096));

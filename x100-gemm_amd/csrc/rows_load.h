@@ -31,31 +31,43 @@ template <int T> X100_DEV float row_elem(const void *p, size_t i)
     if constexpr (T == X100_T_I32) return (float)((const int32_t *)p)[i];
     return act2f<T>(((const uint16_t *)p)[i]);
 }
-// N consecutive elements (4 or 8) from an address aligned to min(16, N * element) bytes.
-template <int T, int N> X100_DEV void row_elems(const void *p, size_t i, float (&v)[N])
-{
-    if constexpr (row_elem_bytes<T>() == 4) {
-#pragma unroll
-        for (int k = 0; k < N / 4; k++) {
-            const v4u u = *(const v4u *)((const uint32_t *)p + i + 4 * k);
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[4 * k + e] = T == X100_T_F32 ? __uint_as_float(u[e]) : (float)(int)u[e];
-        }
-    } else {
-        uint32_t u[N / 2];
-        if constexpr (N == 8) {
-            const v4u w = *(const v4u *)((const uint16_t *)p + i);
-#pragma unroll
-            for (int e = 0; e < 4; e++) u[e] = w[e];
+// N consecutive elements (4 or 8) from an address aligned to min(16, N * element) bytes: as they are stored (a load
+// that can stay on its way), and as floats.
+template <int T, int N> struct RowBits {
+    static constexpr int W = N * row_elem_bytes<T>() / 4;
+    uint32_t w[W];
+    X100_DEV void load(const void *p, size_t i)
+    {
+        const uint8_t *at = (const uint8_t *)p + i * row_elem_bytes<T>();
+        if constexpr (W == 2) {
+            const v2u u = *(const v2u *)at;
+            w[0] = u[0];
+            w[1] = u[1];
         } else {
-            const v2u w = *(const v2u *)((const uint16_t *)p + i);
-            u[0] = w[0];
-            u[1] = w[1];
-        }
 #pragma unroll
-        for (int e = 0; e < N / 2; e++) {
-            v[2 * e] = act2f<T>(u[e] & 0xffffu);
-            v[2 * e + 1] = T == X100_T_F16 ? h2f((uint16_t)(u[e] >> 16)) : __uint_as_float(u[e] & 0xffff0000u);
+            for (int k = 0; k < W / 4; k++) {
+                const v4u u = *(const v4u *)(at + 16 * k);
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[4 * k + e] = u[e];
+            }
         }
     }
+    X100_DEV void values(float (&v)[N]) const
+    {
+#pragma unroll
+        for (int e = 0; e < W; e++) {
+            if constexpr (T == X100_T_F32) v[e] = __uint_as_float(w[e]);
+            else if constexpr (T == X100_T_I32) v[e] = (float)(int)w[e];
+            else {
+                v[2 * e] = act2f<T>(w[e] & 0xffffu);
+                v[2 * e + 1] = T == X100_T_F16 ? h2f((uint16_t)(w[e] >> 16)) : __uint_as_float(w[e] & 0xffff0000u);
+            }
+        }
+    }
+};
+template <int T, int N> X100_DEV void row_elems(const void *p, size_t i, float (&v)[N])
+{
+    RowBits<T, N> b;
+    b.load(p, i);
+    b.values(v);
 }
