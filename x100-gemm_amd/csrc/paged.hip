@@ -41,6 +41,35 @@ template <int HD> X100_DEV float gmin(float v)
     return v;
 }
 
+// 1 / sqrt(x): the hardware's estimate and one Newton step, within its range (at the others the formula).
+X100_DEV float inv_root(float x)
+{
+    if (!(x >= 0x1p-96f && x <= 0x1p96f)) return 1.0f / sqrtf(x);
+    const float r = __builtin_amdgcn_rsqf(x);
+    return __builtin_fmaf(0.5f * r, __builtin_fmaf(-x * r, r, 1.0f), r);
+}
+// Smallest (SGN = 1; -1: minus the largest) of 8 positions each over the 32 lanes of a group: halves of the positions
+// are exchanged for halves of the lanes twice, so that lane c % 4 ends with positions c % 4 and 4 + c % 4.
+template <int SGN> X100_DEV void gmin8(const float (&v)[8], float (&m)[2])
+{
+    const bool b0 = threadIdx.x & 1, b1 = threadIdx.x & 2;
+    float a[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float x = SGN * v[2 * j], y = SGN * v[2 * j + 1];
+        a[j] = fminf(b0 ? y : x, dpp_f<0xB1>(0.0f, b0 ? x : y));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        float r = fminf(b1 ? a[2 * i + 1] : a[2 * i], dpp_f<0x4E>(0.0f, b1 ? a[2 * i] : a[2 * i + 1]));
+        r = fminf(r, dpp_f<0x124>(0.0f, r));
+        r = fminf(r, dpp_f<0x128>(0.0f, r));
+        m[i] = fminf(r, xor16_f(r));
+    }
+}
+// lane C of each four
+template <int C> X100_DEV float quad(float v) { return dpp_f<0x55 * C>(0.0f, v); }
+
 // Where row r of a wave's four (lane / 16) lies: the sequence s, the position (pos < 0: before the first),
 // mine: the row is one of a sequence that is not refused.
 struct RowPlace {
@@ -117,13 +146,17 @@ template <int HD, int ST, int AT, bool Q4> X100_DEV void append_qk(const AppendA
     }
     const int pg = at.mine && at.pos >= 0 ? paged_page(a.c, a.b, at.s, at.pos) : -1;
     const int off = at.pos & (page - 1);
-    // norm weights and the row's scale, of queries or keys
-    float nw[E], rs = 1.0f;
+    // The row's scale; and of queries or keys what an element and its pair's other one are multiplied by: norm weight
+    // and rotation.
+    float rs = 1.0f, wa[E], wb[E];
     auto weights = [&](const x100_rows &src, const float *w) __attribute__((always_inline)) {
         if constexpr (ST == X100_T_I32) rs = src.row_scale[row];
-        if (w)
 #pragma unroll
-            for (int e = 0; e < E; e++) nw[e] = w[E * l + e];
+        for (int e = 0; e < E; e++) {
+            const float x = w ? w[E * l + e] : 1.0f;
+            wa[e] = a.r.rope ? x * cs[e].x : x;
+            wb[e] = a.r.rope ? dpp_f<0x128>(0.0f, x) * cs[e].y : 0.0f;
+        }
     };
     // the head's values, normalised and rotated; the next head's on their way
     auto values = [&](float (&v)[E], bool norm) __attribute__((always_inline)) {
@@ -132,20 +165,24 @@ template <int HD, int ST, int AT, bool Q4> X100_DEV void append_qk(const AppendA
 #pragma unroll
             for (int e = 0; e < E; e++) v[e] = v[e] * rs * cl[e];
         fetch(min(head + 1, end - 1));
-        if (norm) {
-            float ss = 0.0f;
+        float ss = 0.0f;
+        if (norm)
 #pragma unroll
             for (int e = 0; e < E; e++) ss = __builtin_fmaf(v[e], v[e], ss);
-            const float sc = 1.0f / sqrtf(sum16(ss) / (float)HD + a.r.eps);
-#pragma unroll
-            for (int e = 0; e < E; e++) v[e] = v[e] * sc * nw[e];
-        }
         if (a.r.rope) {
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 const float o = dpp_f<0x128>(0.0f, v[e]);   // the pair's other element
-                v[e] = v[e] * cs[e].x + o * cs[e].y;
+                v[e] = __builtin_fmaf(v[e], wa[e], o * wb[e]);
             }
+        } else if (norm) {
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] *= wa[e];
+        }
+        if (norm) {
+            const float sc = inv_root(sum16(ss) / (float)HD + a.r.eps);
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] *= sc;
         }
     };
     if (head < min(end, n_h)) weights(a.r.q, a.r.q_norm);
@@ -266,8 +303,43 @@ template <int HD, int ST, int AT, bool Q4> X100_DEV void append_v(const AppendAr
                 }
             } else {
                 uint32_t *cw = (uint32_t *)base + (size_t)blk * HD + el;
-                uint32_t word = n == 8 ? 0u : *cw;
                 uint16_t *sc16 = (uint16_t *)(base + page * HD / 2) + ((size_t)blk * (HD / 32) + el / 32) * 16;
+                float z = 0.0f;   // NaN where a value is not finite
+#pragma unroll
+                for (int k = 0; k < 8; k++) z = __builtin_fmaf(v[k], 0.0f, z);
+                if (n == 8 && !__any(z != 0.0f)) {
+                    // A whole block: each scale is worked out by one lane of four (position by position, below, 1100
+                    // instructions instead of 230).
+                    float lo[2], hi[2];
+                    gmin8<1>(v, lo);
+                    gmin8<-1>(v, hi);
+                    Q4Scale sc[2];
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        sc[i] = q4_scale(lo[i], -hi[i], false);
+                        if ((lane & 28) == 0) {
+                            sc16[4 * i + (lane & 3)] = sc[i].d;
+                            sc16[8 + 4 * i + (lane & 3)] = sc[i].m;
+                        }
+                        if (sc[i].bad) sc[i].mf = 0.0f;   // codes 0
+                    }
+                    uint32_t word = 0;
+                    auto code = [&](int e, float mf, float inv) __attribute__((always_inline)) {
+                        const float n = __builtin_amdgcn_fmed3f(rintf((v[e] - mf) * inv), 0.0f, 15.0f);
+                        word |= (uint32_t)n << q4_shift(e);
+                    };
+                    code(0, quad<0>(sc[0].mf), quad<0>(sc[0].inv));
+                    code(1, quad<1>(sc[0].mf), quad<1>(sc[0].inv));
+                    code(2, quad<2>(sc[0].mf), quad<2>(sc[0].inv));
+                    code(3, quad<3>(sc[0].mf), quad<3>(sc[0].inv));
+                    code(4, quad<0>(sc[1].mf), quad<0>(sc[1].inv));
+                    code(5, quad<1>(sc[1].mf), quad<1>(sc[1].inv));
+                    code(6, quad<2>(sc[1].mf), quad<2>(sc[1].inv));
+                    code(7, quad<3>(sc[1].mf), quad<3>(sc[1].inv));
+                    *cw = word;
+                    continue;
+                }
+                uint32_t word = n == 8 ? 0u : *cw;
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
                     if (k >= n) break;
