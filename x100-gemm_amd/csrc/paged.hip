@@ -79,18 +79,21 @@ struct RowPlace {
 X100_DEV RowPlace row_place(const x100_kv_batch &b, int rbase, int sub)
 {
     RowPlace p = {0, -1, false};
-    const int f0 = paged_find(b, rbase);
-    if (f0 < b.n_seq) {   // mostly all four rows are one sequence's
-        const PagedSeq q = paged_seq(b, f0);
-        if (q.q_len > 0 && rbase >= q.q0 && rbase + 3 < q.q0 + q.q_len) return {f0, q.kv_len - q.q_len + rbase + sub - q.q0, true};
+    const int r = rbase + sub, f0 = paged_find(b, rbase), l = threadIdx.x & 15;
+    if (f0 >= b.n_seq) return p;
+    // mostly the row is one of the next 16 sequences' (a search for each of four single tokens of 512: 14.8 us, so
+    // 11.5)
+    const bool le = f0 + l < b.n_seq && b.q_start[f0 + l + 1] <= r;
+    const int n = __popc((uint32_t)(__ballot(le) >> (16 * sub)) & 0xffffu);
+    int f = f0 + n;
+    for (uint64_t far = __ballot(n == 16); far;) {
+        const int i = __builtin_ctzll(far) >> 4, g = paged_find(b, rbase + i);
+        if (i == sub) f = g;
+        far &= ~(0xffffull << (16 * i));
     }
-    for (int i = 0; i < 4; i++) {
-        const int r = rbase + i;
-        const int f = r < b.n_rows ? paged_find(b, r) : b.n_seq;
-        if (i == sub && f < b.n_seq) {
-            const PagedSeq q = paged_seq(b, f);
-            if (q.q_len > 0 && r >= q.q0) p = {f, q.kv_len - q.q_len + r - q.q0, true};
-        }
+    if (r < b.n_rows && f < b.n_seq) {
+        const PagedSeq q = paged_seq(b, f);
+        if (q.q_len > 0 && r >= q.q0) p = {f, q.kv_len - q.q_len + r - q.q0, true};
     }
     return p;
 }
@@ -104,7 +107,7 @@ struct AppendArgs {
     int heads;     // query and key heads of a wave, one after the other
     int xq, nq;    // blocks of one group of heads (16 rows each), of all query and key heads; behind them: values
     int xv;        // blocks of one KV head's values
-    int vrows;     // rows of a value block's unit: 1, or 8
+    int vrows;     // rows of a value block's unit: 2, or 8
 };
 
 // Queries and keys: a wave has four consecutive rows, 16 lanes each with 8 or 4 elements of a head (the
@@ -433,15 +436,19 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256) void k_read
 
 template <int HD, int ST> hipError_t append_as(AppendArgs a, hipStream_t s)
 {
-    // Heads per wave: as many as leave 4096 waves (16 per CU), so that few rows are spread over the chip and many
-    // look their places up once for several heads (6400 rows of 36 heads, int32 to 4 bits and read back, us: 16384 /
-    // 8192 / 4096 / 2048 waves 61.4 / 57.8 / 56.6 / 58.0).
-    // Values: a unit of 8 rows holds whole blocks of prompts; single tokens get a unit each.
+    // Heads per wave: as many as leave 2048 waves, so that few rows are spread over the chip and many look their places
+    // up once for several heads, but 12 at most, which leaves more loads on their way (us for 512 tokens / 6400 rows
+    // of 36 heads, int32 to 4 bits and read back: one head 11.5 / -, 4096 waves 11.5 / 56, 2048 9.4 / 58-62, with the
+    // bound 9.4 / 56; a bound of 9 or 18: 62).
+    // Values: a unit of 8 rows holds whole blocks of prompts; of single tokens each row is looked up and stored by
+    // itself, and shorter units do that beside each other (512 tokens 17.6 us in eights, 14.9 in twos, 14.8 alone;
+    // 2048 rows of a prompt 13.0 / 13.2 / 16.2).
     const int n_rows = a.b.n_rows, all = a.c.n_head + a.c.n_head_kv, quads = (n_rows + 3) / 4;
-    a.heads = std::max(1, (int)std::min<int64_t>(all, (int64_t)quads * all / 4096));
+    const int most = std::max(1, (int)std::min<int64_t>(std::min(all, 12), (int64_t)quads * all / 2048)), groups = (all + most - 1) / most;
+    a.heads = (all + groups - 1) / groups;
     a.xq = (n_rows + 15) / 16;
     a.nq = a.xq * ((all + a.heads - 1) / a.heads);
-    a.vrows = (int64_t)n_rows * a.c.n_head_kv <= 2048 ? 1 : 8;
+    a.vrows = n_rows < 4 * (int64_t)a.b.n_seq ? 2 : 8;
     const int per = 4 / (HD / 64) * a.vrows;   // rows of a value block
     a.xv = (n_rows + per - 1) / per;
     const int64_t blocks = (int64_t)a.nq + (int64_t)a.xv * a.c.n_head_kv;
