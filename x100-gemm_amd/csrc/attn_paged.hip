@@ -54,9 +54,12 @@ template <int HD, int AT, bool Q4, int NW> __global__ __launch_bounds__(64 * NW,
     } sh;
     __shared__ float s_m[NW][16], s_l[NW][16];
     const int lane = threadIdx.x & 63, w = wave_id(), c = lane & 15, g = lane >> 4;
-    // tiles last: a sequence's second one is mostly empty, and every other block empty would idle half of the XCDs
-    const int sp = blockIdx.x % a.tile.n, kvh = blockIdx.x / a.tile.n, s = blockIdx.y, tile = blockIdx.z;
-    const int n_kv = a.c.n_head_kv, G = a.c.n_head / n_kv, page = a.c.page, psh = __builtin_ctz(page);
+    // Units (sequence, KV head, split) in runs of a.run, each run with all its tiles (plan_of)
+    const int n_kv = a.c.n_head_kv, unit = blockIdx.x / (a.run * a.tiles) * a.run + blockIdx.x % a.run;
+    const int tile = blockIdx.x / a.run % a.tiles;
+    const int sp = unit % a.tile.n, kvh = unit / a.tile.n % n_kv, s = unit / (a.tile.n * n_kv);
+    if (s >= a.b.n_seq) return;
+    const int G = a.c.n_head / n_kv, page = a.c.page, psh = __builtin_ctz(page);
     const int i0 = tile * 16;
     // A short table's pages are read here, beside the lengths; a long one's when the split is known.
     const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
@@ -377,12 +380,15 @@ template <int HD, int AT, bool Q4, int NW> __global__ __launch_bounds__(64 * NW,
 }
 
 // Merges the splits of rows that have more than one: HD / 4 lanes per (row, head), 4 elements each; x = row, or
-// (where only the tile kernel has splits) sequence and token, y = the heads of a block.
-template <int HD, int AT> __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a)
+// (where only the tile kernel has splits) sequence and token, y = the heads of a block.  WIDE: the whole block takes
+// one head, its lane groups every 256 / (HD / 4)-th split (64 splits: 8 turns of dependent loads become one).
+template <int HD, int AT, bool WIDE> __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a)
 {
-    constexpr int L = HD / 4;
-    const int G = a.c.n_head / a.c.n_head_kv;
-    const int head = blockIdx.y * (256 / L) + threadIdx.x / L, l4 = threadIdx.x % L;
+    constexpr int L = HD / 4, GR = 256 / L;
+    __shared__ float4 s_o[WIDE ? GR : 1][L];
+    __shared__ float s_l[WIDE ? GR : 1];
+    const int G = a.c.n_head / a.c.n_head_kv, gr = threadIdx.x / L, l4 = threadIdx.x % L;
+    const int head = WIDE ? blockIdx.y : blockIdx.y * GR + gr;
     const bool rows = a.prompt.n > 1;
     const int tokens = a.tile_rows / G;
     const int s = rows ? paged_find(a.b, blockIdx.x) : blockIdx.x / tokens;
@@ -406,17 +412,19 @@ template <int HD, int AT> __global__ __launch_bounds__(256) void k_attn_join(con
     const float ms = m == NEG_INF ? 0.0f : m;
     float l = 0.0f;
     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k = 0; k < ns; k += 8) {   // eight at a time on their way
+    constexpr int ST = WIDE ? GR : 1;
+    for (int k0 = WIDE ? gr : 0; k0 < ns; k0 += 8 * ST) {   // eight at a time on their way
         float2 v[8];
         float4 b[8];
 #pragma unroll
         for (int u = 0; u < 8; u++) {
-            v[u] = ml[min(k + u, ns - 1)];
-            b[u] = po[(size_t)min(k + u, ns - 1) * L];
+            const int k = min(k0 + u * ST, ns - 1);
+            v[u] = ml[k];
+            b[u] = po[(size_t)k * L];
         }
 #pragma unroll
         for (int u = 0; u < 8; u++) {
-            if (k + u >= ns || v[u].x == NEG_INF) continue;   // a split without positions has no O
+            if (k0 + u * ST >= ns || v[u].x == NEG_INF) continue;   // a split without positions has no O
             const float f = __builtin_amdgcn_exp2f(v[u].x - ms);
             l = __builtin_fmaf(v[u].y, f, l);
             y.x = __builtin_fmaf(b[u].x, f, y.x);
@@ -425,30 +433,49 @@ template <int HD, int AT> __global__ __launch_bounds__(256) void k_attn_join(con
             y.w = __builtin_fmaf(b[u].w, f, y.w);
         }
     }
+    if constexpr (WIDE) {
+        s_o[gr][l4] = y;
+        if (l4 == 0) s_l[gr] = l;
+        __syncthreads();
+        if (gr != 0) return;
+        for (int k = 1; k < GR; k++) {
+            const float4 z = s_o[k][l4];
+            y.x += z.x;
+            y.y += z.y;
+            y.z += z.z;
+            y.w += z.w;
+            l += s_l[k];
+        }
+    }
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
     v2u o = {0, 0};
     if (l != 0.0f) o = v2u{pack2<AT>(y.x * f, y.y * f), pack2<AT>(y.z * f, y.w * f)};
     *(v2u *)(a.out + (size_t)row * a.ldo + (size_t)head * HD + 4 * l4) = o;
 }
 
-// How a call is laid out: sequences of up to FEW rows (token, head) go to the tile kernel, longer ones to the
+// How a call is laid out: sequences of up to `few` rows (token, head) go to the tile kernel, longer ones to the
 // prompt kernel; the positions in splits, so that the blocks fill the chip.
-constexpr int FEW = 32;
+constexpr int FEW = 32, FEW_Q4 = 64;   // us with 32 / 64: 64 sequences of 64 rows at 2048 positions, 16 bits 45 / 86,
+                                       // 4 bits 62 / 60; of 40 rows 44 / 66 and 60 / 48
+constexpr int WIDE_SPLITS = 8;   // more splits than this are joined by a block per head
+
 struct Plan {
     PagedSplit tile, prompt;   // n == 0: the kernel is not launched
     size_t tile_parts, prompt_parts;   // split results
-    int few, tile_rows, tiles;         // rows of a sequence and their tiles, tile kernel
+    int few, tile_rows, tiles, run;    // rows of a sequence and their tiles, tile kernel; units of a run of blocks
 };
 
 Plan plan_of(const x100_kv_cfg &c, const x100_kv_batch &b)
 {
     Plan p = {};
+    p.run = 8;
     const int G = c.n_head / c.n_head_kv;
     const int64_t rows = (int64_t)b.max_q * G, kv = b.max_kv;   // of the longest sequence
     // Prompts beside single tokens (the sequences but one have less than a quarter of max_q on average) take both
     // kernels: 63 tokens at 4096 positions and 512 at 4608, 290 / 165 us (each alone 91 and 57).  A batch of prompts takes the prompt
     // kernel alone, which is right for any rows: the other launch costs 2 us.
-    const bool prompts = rows > FEW;
+    const int few = c.kv_type == X100_KV_Q4 ? FEW_Q4 : FEW;
+    const bool prompts = rows > few;
     const bool both = prompts && b.n_seq > 1 && ((int64_t)b.n_rows - b.max_q) * 4 <= (int64_t)(b.n_seq - 1) * b.max_q;
     if (!prompts || both) {
         // A block per CU where rows of 16 bits are read (256 blocks of four waves keep HBM busy: 64 sequences of
@@ -457,12 +484,17 @@ Plan plan_of(const x100_kv_cfg &c, const x100_kv_batch &b)
         // one block is faster than two and their join (9.6 / 12.6 us); behind that 128 positions, a tile per wave, are
         // the least (one sequence of 1024: 10.7 us at 256, 9.8 at 128).
         const int64_t most = (int64_t)TILE_PAGES * c.page;
-        p.few = FEW;
-        p.tile_rows = (int)std::min<int64_t>(rows, FEW);
+        p.few = few;
+        p.tile_rows = (int)std::min<int64_t>(rows, few);
         p.tiles = (p.tile_rows + TILE_ROWS - 1) / TILE_ROWS;
         const int64_t base = (int64_t)(both ? 1 : p.tiles) * std::min(b.n_seq, b.n_rows) * c.n_head_kv;
         const int64_t want = kv <= 512 ? 1 : std::max<int64_t>(1, (c.kv_type == X100_KV_Q4 ? 768 : 256) / base);
         p.tile = {(int)std::max(std::min(want, (kv + 127) / 128), (kv + most - 1) / most), 128};
+        // Runs of eight, one per XCD, where most sequences have their last tile: the tiles of a unit share an L2 (64
+        // sequences of 32 rows at 2048 positions, 48 us; all first tiles before all second ones 80).  Else of 256, a
+        // block per CU: empty tiles between others leave CUs without work (63 tokens beside a prompt, every other
+        // block or eight blocks empty, 125 / 91 us).
+        if (both || (int64_t)b.n_rows * G <= (int64_t)b.n_seq * TILE_ROWS * (p.tiles - 1)) p.run = 256;
         if (p.tile.n > 1) p.tile_parts = (size_t)b.n_seq * p.tile_rows * c.n_head_kv * p.tile.n;
     }
     if (prompts) {
@@ -488,21 +520,23 @@ Plan plan_of(const x100_kv_cfg &c, const x100_kv_batch &b)
 
 template <int HD, int AT> hipError_t attn_as(const AttnArgs &a, const Plan &p, hipStream_t s)
 {
+    const int64_t blocks = ((int64_t)a.b.n_seq * a.c.n_head_kv * p.tile.n + a.run - 1) / a.run * a.run * p.tiles;
+    if (blocks >= 1 << 24) return hipErrorInvalidValue;   // past one launch
     if (p.prompt.n) {
         const hipError_t e = x100_attn_prompt_launch(a, s);
         if (e != hipSuccess) return e;
     }
     if (p.tile.n) {
-        const dim3 grid(a.c.n_head_kv * p.tile.n, a.b.n_seq, p.tiles);   // x: 2^23 at most (2^26 positions, 1024 heads)
-        if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true, 4><<<grid, 256, 0, s>>>(a);
-        else k_attn_tile<HD, AT, false, 4><<<grid, 256, 0, s>>>(a);
+        if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true, 4><<<(unsigned)blocks, 256, 0, s>>>(a);
+        else k_attn_tile<HD, AT, false, 4><<<(unsigned)blocks, 256, 0, s>>>(a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     if (p.tile.n <= 1 && p.prompt.n <= 1) return hipSuccess;
     constexpr int heads = 256 / (HD / 4);
     const unsigned rows = p.prompt.n > 1 ? a.b.n_rows : (unsigned)a.b.n_seq * (a.tile_rows / (a.c.n_head / a.c.n_head_kv));
-    k_attn_join<HD, AT><<<dim3(rows, (a.c.n_head + heads - 1) / heads), 256, 0, s>>>(a);
+    if (p.tile.n > WIDE_SPLITS && p.prompt.n <= 1) k_attn_join<HD, AT, true><<<dim3(rows, a.c.n_head), 256, 0, s>>>(a);
+    else k_attn_join<HD, AT, false><<<dim3(rows, (a.c.n_head + heads - 1) / heads), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -536,6 +570,8 @@ hipError_t x100_attn_paged_launch(const x100_kv_cfg &c, const x100_kv_batch &b, 
     a.prompt = p.prompt;
     a.tile_at = p.prompt_parts;
     a.tile_rows = p.tile_rows;
+    a.tiles = p.tiles;
+    a.run = p.run;
     if (c.head_dim == 64)
         return c.act_type == X100_T_F16 ? attn_as<64, X100_T_F16>(a, p, s) : attn_as<64, X100_T_BF16>(a, p, s);
     return c.act_type == X100_T_F16 ? attn_as<128, X100_T_F16>(a, p, s) : attn_as<128, X100_T_BF16>(a, p, s);

@@ -32,6 +32,18 @@ X100_DEV void dma16s(uint32_t voff, const void *sbase, uint32_t lds_base)
     asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(lds_base) : "memory");
 }
 
+// sum over the wave's lanes up to this one
+X100_DEV int prefix_sum(int v)
+{
+    v += dpp_i<0x111>(0, v);
+    v += dpp_i<0x112>(0, v);
+    v += dpp_i<0x114>(0, v);
+    v += dpp_i<0x118>(0, v);
+    v += dpp_i<0x142, 0xa>(0, v);
+    v += dpp_i<0x143, 0xc>(0, v);
+    return v;
+}
+
 // LDS of every wave written and read up to here
 X100_DEV void lds_sync() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -48,18 +60,41 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
     const int lane = threadIdx.x & 63, w = wave_id(), c = lane & 31, h = lane >> 5;
     const int n_kv = a.c.n_head_kv, G = a.c.n_head / n_kv, page = a.c.page, psh = __builtin_ctz(page);
     const int ns_max = a.prompt.n, kvh = blockIdx.x % n_kv, u = blockIdx.x / n_kv, sp = u % ns_max;
-    // Item (sequence, tile of rows): sequence s has the items from q_start[s] G / 256 + s on, which leaves room for
-    // its tiles whatever the rows before it, and at most one item per sequence without rows.  (A grid of the
-    // longest sequence's tiles for every sequence: 64 of 16 rows under a bound of 4096, 200 / 35 us.)
-    const int item = u / ns_max;
+    // Item u / ns_max of the sequences' tiles of rows, counted by each wave, 64 sequences at a time.  (A grid of the
+    // longest sequence's tiles for every sequence: 64 of 16 rows under a bound of 4096, 200 / 24 us; blocks without work
+    // among the others leave a shader engine a block more than it has CUs for: 16 of 32 rows, 80 / 56 us.)
+    const int item = u / ns_max, n_seq = a.b.n_seq;
     auto first = [&](int s) { return (int64_t)a.b.q_start[s] * G / PROMPT_ROWS + s; };
-    const int s = a.b.n_seq == 1 ? 0 : paged_search(a.b.n_seq, [&](int s) { return first(s) <= item; });
-    if (s >= a.b.n_seq) return;
+    int s = 0, place = item;
+    if (n_seq > 512) {
+        // more sequences: s has the items from q_start[s] G / 256 + s on, which leaves room for its tiles whatever the
+        // rows before it
+        s = paged_search(n_seq, [&](int s) { return first(s) <= item; });
+        if (s >= n_seq) return;
+        place = (int)max(min(item - first(s), (int64_t)INT_MAX), (int64_t)-1);
+    } else if (n_seq > 1) {
+        for (int before = 0; s < n_seq; s += 64) {
+            int mine = 0;
+            if (s + lane < n_seq) {
+                const int rows = paged_seq(a.b, s + lane).q_len * G;
+                if (rows > a.few) mine = (rows + PROMPT_ROWS - 1) / PROMPT_ROWS;
+            }
+            const int incl = before + prefix_sum(mine);   // tiles up to this lane's sequence
+            const uint64_t over = __ballot(incl > item);
+            if (over) {
+                const int k = __builtin_ctzll(over);
+                place = item - __builtin_amdgcn_readlane(incl - mine, k);
+                s += k;
+                break;
+            }
+            before = __builtin_amdgcn_readlane(incl, 63);
+        }
+        if (s >= n_seq) return;
+    }
     const PagedSeq q = paged_seq(a.b, s);
     const int n_rows = q.q_len * G, tiles = (n_rows + PROMPT_ROWS - 1) / PROMPT_ROWS;
-    const int64_t place = item - first(s);
     if (n_rows <= a.few || place < 0 || place >= tiles) return;
-    const int i0 = (tiles - 1 - (int)place) * PROMPT_ROWS, pos0 = q.kv_len - q.q_len;   // the longest first
+    const int i0 = (tiles - 1 - place) * PROMPT_ROWS, pos0 = q.kv_len - q.q_len;   // the longest first
     const int vis = pos0 + min(i0 + PROMPT_ROWS - 1, n_rows - 1) / G + 1;
     const int per = a.prompt.positions(q.kv_len), ns = max(1, (vis + per - 1) / per);
     if (sp >= ns) return;

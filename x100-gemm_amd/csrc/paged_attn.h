@@ -25,7 +25,8 @@ struct PagedAttnArgs {
     int few;             // sequences of up to this many rows (token, head) are the tile kernel's, the rest the prompt kernel's
     PagedSplit tile, prompt;
     size_t tile_at;      // the tile kernel's first split result
-    int tile_rows;       // rows of a sequence there
+    int tile_rows, tiles;   // rows of a sequence there, and their tiles
+    int run;             // units of a run of blocks there
 };
 
 template <int T> struct Mfma16;
