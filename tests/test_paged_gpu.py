@@ -362,6 +362,27 @@ def test_prompts_beside_single_tokens(dev, act, kv, n_head, n_kv, q, L):
 
 
 @kinds
+@pytest.mark.parametrize("n_seq", [65, 130, 512, 513, 700])
+def test_prompts_of_many_sequences(dev, act, kv, n_seq):
+    """More sequences than a wave counts at a time, and than are counted at all."""
+    g = np.random.default_rng(n_seq)
+    q = [int(n) for n in g.integers(33, 40, n_seq)]     # every one long
+    Setup(30, 2, 1, 64, 16, act, kv, q, [n + int(e) for n, e in zip(q, g.integers(0, 30, n_seq))]).check()
+    q = [1] * n_seq                                     # a few long among single tokens
+    q[0], q[n_seq // 2], q[-1] = 40, 300, 150
+    Setup(31, 2, 1, 64, 16, act, kv, q, [n + int(e) for n, e in zip(q, g.integers(0, 30, n_seq))]).check()
+
+
+@kinds
+@pytest.mark.parametrize("n_head,q", [(2, 16), (8, 4), (8, 8), (16, 3), (16, 1)])
+def test_tiles_of_few_rows(dev, act, kv, n_head, q):
+    """Two to four tiles of rows per sequence, whole and ragged, with few splits and many."""
+    for n_seq, L in ((1, 5000), (3, 1100), (40, 70)):
+        Setup(32, n_head, 1, 64, 16, act, kv, [q] * n_seq, [L - 7 * i % 50 for i in range(n_seq)]).check()
+        Setup(33, n_head, 1, 64, 16, act, kv, [q] + [1] * (n_seq - 1), [L - i for i in range(n_seq)]).check()
+
+
+@kinds
 def test_rows_of_a_wider_bound(dev, act, kv):
     """The launch sized for more rows and positions than a sequence has (as a captured one is)."""
     for q, L in (([1, 2, 1], [700, 40, 2000]), ([60, 1, 5], [900, 1, 2000]), ([130, 100, 90], [130, 400, 1000])):
