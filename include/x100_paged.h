@@ -39,8 +39,9 @@
  * All pointers are device pointers unless they are the argument structures; every call is
  * asynchronous on stream and capturable.  All arguments that the host can see are checked before
  * anything is enqueued.  X100_EINVAL also for a batch that no launch can hold, with G query heads per KV
- * head: (n_rows * G / 256 + n_seq) * n_head_kv times the splits of the positions (one with many rows) of
- * 2^23 and more in the attention of prompts, n_rows * n_head_kv of about 2^28 in the append.
+ * head: (n_rows * G / 256 + n_seq) * n_head_kv * splits of 2^23 and more in the attention of prompts,
+ * n_seq * n_head_kv * splits of about 2^22 in that of single tokens (splits: of the positions, 1 where
+ * there are many sequences), n_rows * n_head_kv of about 2^28 in the append.  Outputs overlap no input.
  */
 #ifndef X100_HIP_PAGED_H
 #define X100_HIP_PAGED_H

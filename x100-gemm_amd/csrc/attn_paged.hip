@@ -43,7 +43,7 @@ template <int HD> struct TileRegs<HD, true> {
 // The loop is bound by memory as long as loads are always in flight: K and V of the next tile are requested
 // as soon as their registers are free, the pages come from a list in LDS.  63 sequences of 4096 positions, 32 heads on 4 of
 // 128, bf16: 91 us, 5.8 TB/s (a read of 2 GiB: 6.1); 16 of up to 60001 in 4 bits: 94 us, 4.8 TB/s, where unpacking
-// takes half of the issue slots.  One of 1024: 7 us, the chain of loads lengths -> pages -> K -> V.
+// takes half of the issue slots.  One of 1024: 6.5 us, the chain of loads lengths -> pages -> K -> V.
 template <int HD, int AT, bool Q4, int NW> __global__ __launch_bounds__(64 * NW, Q4 || HD == 64 ? 4 : 3) void k_attn_tile(const AttnArgs a)
 {
     constexpr int MT = Q4 ? X100_T_F16 : AT;   // type on the matrix cores
