@@ -472,8 +472,8 @@ Plan plan_of(const x100_kv_cfg &c, const x100_kv_batch &b)
     const int G = c.n_head / c.n_head_kv;
     const int64_t rows = (int64_t)b.max_q * G, kv = b.max_kv;   // of the longest sequence
     // Prompts beside single tokens (the sequences but one have less than a quarter of max_q on average) take both
-    // kernels: 63 tokens at 4096 positions and 512 at 4608, 290 / 165 us (each alone 91 and 57).  A batch of prompts takes the prompt
-    // kernel alone, which is right for any rows: the other launch costs 2 us.
+    // kernels: 63 tokens at 4096 positions and 512 at 4608, 290 / 165 us (each alone 91 and 57).  A batch of prompts
+    // takes the prompt kernel alone, which is right for any rows: the other launch costs 2 us.
     const int few = c.kv_type == X100_KV_Q4 ? FEW_Q4 : FEW;
     const bool prompts = rows > few;
     const bool both = prompts && b.n_seq > 1 && ((int64_t)b.n_rows - b.max_q) * 4 <= (int64_t)(b.n_seq - 1) * b.max_q;

@@ -101,23 +101,7 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
     const int t0 = sp * per, t1 = min(t0 + per, vis);
     const int n = max(0, (t1 - t0 + 31) >> 5);   // tiles
 
-    // pages of the split; one that is none sends every tile through the masked step
-    const int *tab = a.b.block_table + (size_t)s * a.b.table_ld + (t0 >> psh);
-    const int pg0 = t0 >> psh, n_pg = n > 0 ? ((t1 - 1) >> psh) - pg0 + 1 : 0;
-    bool bad = false;
-    for (int i = threadIdx.x; i < n_pg; i += NT) {
-        const int g = tab[i];
-        const bool ok = g >= 0 && g < a.c.n_pages;
-        s_pg[i] = ok ? g : -1;
-        bad |= !ok;
-    }
-    bad = __syncthreads_or(bad);
-    // Tiles that every row of the block sees whole; that the wave's rows see whole; that they see at all.
     const int iw = i0 + 32 * w;
-    const int nw = bad ? 0 : max(0, min(n, (pos0 + i0 / G + 1 - t0) >> 5));
-    const int ww = bad ? 0 : max(0, min(n, (pos0 + min(iw, n_rows - 1) / G + 1 - t0) >> 5));
-    const int wn = iw >= n_rows ? 0 : max(0, min(n, (pos0 + min(iw + 31, n_rows - 1) / G + 1 - t0 + 31) >> 5));
-
     // query row iw + c
     int pos;
     float sc2 = a.scale2;
@@ -146,6 +130,22 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
                                                  ldexpf(__uint_as_float(qf[j][e] & 0xffff0000u), -ex));
         }
     }
+
+    // pages of the split; one that is none sends every tile through the masked step
+    const int *tab = a.b.block_table + (size_t)s * a.b.table_ld + (t0 >> psh);
+    const int pg0 = t0 >> psh, n_pg = n > 0 ? ((t1 - 1) >> psh) - pg0 + 1 : 0;
+    bool bad = false;
+    for (int i = threadIdx.x; i < n_pg; i += NT) {
+        const int g = tab[i];
+        const bool ok = g >= 0 && g < a.c.n_pages;
+        s_pg[i] = ok ? g : -1;
+        bad |= !ok;
+    }
+    bad = __syncthreads_or(bad);
+    // Tiles that every row of the block sees whole; that the wave's rows see whole; that they see at all.
+    const int nw = bad ? 0 : max(0, min(n, (pos0 + i0 / G + 1 - t0) >> 5));
+    const int ww = bad ? 0 : max(0, min(n, (pos0 + min(iw, n_rows - 1) / G + 1 - t0) >> 5));
+    const int wn = iw >= n_rows ? 0 : max(0, min(n, (pos0 + min(iw + 31, n_rows - 1) / G + 1 - t0 + 31) >> 5));
 
     // ---- pairs of tiles into LDS -------------------------------------------------------------------
     // K: [64 positions][HD], the 16-byte pieces of a row exchanged by an XOR with the position, so that
@@ -488,15 +488,23 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
     const size_t row = q.q0 + tok;
     if (ns == 1) {
         const float r = l == 0.0f ? 0.0f : 1.0f / l;
-        uint16_t *o = a.out + row * a.ldo + (size_t)head * HD + 4 * h;
+        uint16_t *o = a.out + row * a.ldo + (size_t)head * HD + 8 * h;
+        // Lanes c and c + 32 have halves of 8 elements each; of two such pieces each lane stores one (16 bytes).
 #pragma unroll
         for (int j = 0; j < NJ; j++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                v2u y = {0, 0};
-                if (l != 0.0f)
-                    y = v2u{pack2<AT>(O[j][4 * e] * r, O[j][4 * e + 1] * r), pack2<AT>(O[j][4 * e + 2] * r, O[j][4 * e + 3] * r)};
-                *(v2u *)(o + 32 * j + 8 * e) = y;
+            for (int e = 0; e < 16; e += 8) {
+                v4u y;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const uint32_t p0 = pack2<AT>(O[j][e + 2 * k] * r, O[j][e + 2 * k + 1] * r);
+                    const uint32_t p1 = pack2<AT>(O[j][e + 4 + 2 * k] * r, O[j][e + 5 + 2 * k] * r);
+                    const auto sw = __builtin_amdgcn_permlane32_swap(p0, p1, false, false);
+                    y[k] = sw[0];
+                    y[2 + k] = sw[1];
+                }
+                if (l == 0.0f) y = v4u{0, 0, 0, 0};
+                *(v4u *)(o + 32 * j + 2 * e) = y;
             }
     } else {
         const size_t to = prompt_part(a, q.q0, kvh, i) + sp;
