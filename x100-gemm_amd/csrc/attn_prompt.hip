@@ -481,15 +481,30 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
     }
 
     // ---- results -----------------------------------------------------------------------------------
+    // Through LDS, so that a store instruction writes whole rows: a lane holds 4 elements here and there (stored from
+    // the registers, 1 x 4096 rows of bf16: pieces of 8 bytes 141 us, of 16 136; on another card 16 132.4, so 131.4, and
+    // split results, 512 rows behind 8192, 81.4, so 79.3).  Each wave has 32 rows of 2 HD bytes, a row's 16-byte pieces
+    // exchanged by an XOR with its number.
+    constexpr int NP = HD / 8;
     l += xor32_f(l);
-    const int i = iw + c;
-    if (i >= n_rows) return;
-    const int tok = i / G, head = kvh * G + i % G;
-    const size_t row = q.q0 + tok;
+    lds_sync();   // the last tiles are read
+    uint8_t *st = (w < 4 ? s_k[0] : s_v[0]) + (w & 3) * KB;
+    auto at = [&](int r, int p) __attribute__((always_inline)) { return (v4u *)(st + r * (2 * HD) + ((p ^ (r & (NP - 1))) * 16)); };
+    const uint32_t inv_g = (1u << 31) / G + 1;   // i / G = i inv_g / 2^31 for i < 2^27
+    // row and piece of the lane in the t-th store; the row's number among the sequence's, token and head
+    auto rows = [&](auto &&store) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // other lanes' pieces
+#pragma unroll
+        for (int t = 0; t < NP / 2; t++) {
+            const int r = (64 * t + lane) / NP, p = lane % NP, i = iw + r;
+            const int tok = __umulhi(2 * i, inv_g);
+            if (i < n_rows) store(*at(r, p), i, tok, kvh * G + i - tok * G, p);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    };
     if (ns == 1) {
         const float r = l == 0.0f ? 0.0f : 1.0f / l;
-        uint16_t *o = a.out + row * a.ldo + (size_t)head * HD + 8 * h;
-        // Lanes c and c + 32 have halves of 8 elements each; of two such pieces each lane stores one (16 bytes).
+        // Lanes c and c + 32 have halves of 8 elements each; of two such pieces each lane takes one.
 #pragma unroll
         for (int j = 0; j < NJ; j++)
 #pragma unroll
@@ -504,17 +519,27 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
                     y[2 + k] = sw[1];
                 }
                 if (l == 0.0f) y = v4u{0, 0, 0, 0};
-                *(v4u *)(o + 32 * j + 2 * e) = y;
+                *at(c, 4 * j + e / 4 + h) = y;
             }
+        rows([&](v4u y, int, int tok, int head, int p) __attribute__((always_inline)) {
+            *(v4u *)(a.out + (size_t)(q.q0 + tok) * a.ldo + (size_t)head * HD + 8 * p) = y;
+        });
     } else {
-        const size_t to = prompt_part(a, q.q0, kvh, i) + sp;
-        float *o = a.part_o + to * HD + 4 * h;
 #pragma unroll
-        for (int j = 0; j < NJ; j++)
+        for (int half = 0; half < 2; half++) {   // of the elements
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                *(float4 *)(o + 32 * j + 8 * e) = make_float4(O[j][4 * e], O[j][4 * e + 1], O[j][4 * e + 2], O[j][4 * e + 3]);
-        if (h == 0) a.part_ml[to] = make_float2(m, l);
+            for (int j = 0; j < NJ / 2; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const v16f &o = O[half * (NJ / 2) + j];
+                    *at(c, 8 * j + 2 * e + h) = v4u{__float_as_uint(o[4 * e]), __float_as_uint(o[4 * e + 1]),
+                                                    __float_as_uint(o[4 * e + 2]), __float_as_uint(o[4 * e + 3])};
+                }
+            rows([&](v4u y, int i, int, int, int p) __attribute__((always_inline)) {
+                *(v4u *)(a.part_o + (prompt_part(a, q.q0, kvh, i) + sp) * HD + half * (HD / 2) + 4 * p) = y;
+            });
+        }
+        if (h == 0 && iw + c < n_rows) a.part_ml[prompt_part(a, q.q0, kvh, iw + c) + sp] = make_float2(m, l);
     }
 }
 
