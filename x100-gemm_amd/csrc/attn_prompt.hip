@@ -14,11 +14,11 @@
 // The running maximum m is taken from the first tile and then only followed where a weight would leave
 // its 16 bits: the weights' sum, which is needed anyway, says so, and the tile's weights are made again.
 //
-// 4 x 4000 rows of 32 heads on 4 of 128, bf16: 515 us, 1020 TFLOP/s counted over the visible half (an 8192^3 product
+// 4 x 4000 rows of 32 heads on 4 of 128, bf16: 485 us, 1080 TFLOP/s counted over the visible half (an 8192^3 product
 // of the library: 1216); in a step of 32 positions the matrix instructions take 512 cycles of a wave, the weights'
 // vector instructions 380.  Heads of 64 have half the former for the same weights and are bound by the latter: 4096
-// rows of 32 heads 740 TFLOP/s; twelve waves of 168 registers instead of eight 450.  4 bits: unpacking once per
-// block costs 13% more (2 x 4096 rows 249 / 280 us).
+// rows of 32 heads 750 TFLOP/s; twelve waves of 168 registers instead of eight 450.  4 bits: unpacking once per
+// block costs 14% more (2 x 4096 rows 248 / 283 us).
 #include "paged_attn.h"
 #include "x100_internal.h"
 
