@@ -604,6 +604,13 @@ def test_append(dev, act, kv, st, hd):
 
 
 @kinds
+@pytest.mark.parametrize("st", [ref.F32, ref.I32], ids=["f32", "i32"])
+def test_append_many_groups(dev, act, kv, st):
+    """Enough values for a scale or a number that is rounded once too often, or not from fp32, to show."""
+    append_case(40, 8, 8, 128, 64, act, kv, st, [3000], [3000], False, False)
+
+
+@kinds
 def test_append_odd_batches(dev, act, kv):
     # empty sequences, rows before position 0, rows behind the last sequence
     append_case(5, 4, 2, 128, 16, act, kv, ref.F32, [0, 3, 5, 0, 12, 1, 0], [10, 3, 2, 0, 7, 0, 5], True, True, tail=5)

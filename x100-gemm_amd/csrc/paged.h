@@ -60,7 +60,7 @@ struct Q4Scale {
 };
 X100_DEV Q4Scale q4_scale(float lo, float hi, bool bad)
 {
-    const _Float16 d = (_Float16)((hi - lo) * (1.0f / 15.0f)), m = (_Float16)lo;
+    const _Float16 d = f2h_rne((hi - lo) * (1.0f / 15.0f)), m = f2h_rne(lo);
     const float df = (float)d, mf = (float)m;
     bad |= !(fabsf(df) <= 65504.0f) || !(fabsf(mf) <= 65504.0f);
     Q4Scale s;

@@ -41,13 +41,6 @@ template <int HD> X100_DEV float gmin(float v)
     return v;
 }
 
-// 1 / sqrt(x): the hardware's estimate and one Newton step, within its range (at the others the formula).
-X100_DEV float inv_root(float x)
-{
-    if (!(x >= 0x1p-96f && x <= 0x1p96f)) return 1.0f / sqrtf(x);
-    const float r = __builtin_amdgcn_rsqf(x);
-    return __builtin_fmaf(0.5f * r, __builtin_fmaf(-x * r, r, 1.0f), r);
-}
 // Smallest (SGN = 1; -1: minus the largest) of 8 positions each over the 32 lanes of a group: halves of the positions
 // are exchanged for halves of the lanes twice, so that lane c % 4 ends with positions c % 4 and 4 + c % 4.
 template <int SGN> X100_DEV void gmin8(const float (&v)[8], float (&m)[2])
@@ -149,17 +142,13 @@ template <int HD, int ST, int AT, bool Q4> X100_DEV void append_qk(const AppendA
     }
     const int pg = at.mine && at.pos >= 0 ? paged_page(a.c, a.b, at.s, at.pos) : -1;
     const int off = at.pos & (page - 1);
-    // The row's scale; and of queries or keys what an element and its pair's other one are multiplied by: norm weight
-    // and rotation.
-    float rs = 1.0f, wa[E], wb[E];
+    // norm weights and the row's scale, of queries or keys
+    float nw[E], rs = 1.0f;
     auto weights = [&](const x100_rows &src, const float *w) __attribute__((always_inline)) {
         if constexpr (ST == X100_T_I32) rs = src.row_scale[row];
+        if (w)
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            const float x = w ? w[E * l + e] : 1.0f;
-            wa[e] = a.r.rope ? x * cs[e].x : x;
-            wb[e] = a.r.rope ? dpp_f<0x128>(0.0f, x) * cs[e].y : 0.0f;
-        }
+            for (int e = 0; e < E; e++) nw[e] = w[E * l + e];
     };
     // the head's values, normalised and rotated; the next head's on their way
     auto values = [&](float (&v)[E], bool norm) __attribute__((always_inline)) {
@@ -168,24 +157,27 @@ template <int HD, int ST, int AT, bool Q4> X100_DEV void append_qk(const AppendA
 #pragma unroll
             for (int e = 0; e < E; e++) v[e] = v[e] * rs * cl[e];
         fetch(min(head + 1, end - 1));
-        float ss = 0.0f;
-        if (norm)
+        // The formula's own products and sums, each rounded: a 4-bit code of a key that lies between two steps is then the
+        // one that other fp32 code gets, but for the order of the sum of squares (here in pairs).  Weights and rotation
+        // multiplied beforehand, a fused sum and an estimated root were no faster and turned ten times as many codes.
+        if (norm) {
+            float sq[E];
 #pragma unroll
-            for (int e = 0; e < E; e++) ss = __builtin_fmaf(v[e], v[e], ss);
+            for (int e = 0; e < E; e++) sq[e] = v[e] * v[e];
+#pragma unroll
+            for (int d = 1; d < E; d *= 2)
+#pragma unroll
+                for (int e = 0; e < E; e += 2 * d) sq[e] += sq[e + d];
+            const float sc = 1.0f / sqrtf(sum16(sq[0]) / (float)HD + a.r.eps);
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] = v[e] * sc * nw[e];
+        }
         if (a.r.rope) {
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 const float o = dpp_f<0x128>(0.0f, v[e]);   // the pair's other element
-                v[e] = __builtin_fmaf(v[e], wa[e], o * wb[e]);
+                v[e] = v[e] * cs[e].x + o * cs[e].y;
             }
-        } else if (norm) {
-#pragma unroll
-            for (int e = 0; e < E; e++) v[e] *= wa[e];
-        }
-        if (norm) {
-            const float sc = inv_root(sum16(ss) / (float)HD + a.r.eps);
-#pragma unroll
-            for (int e = 0; e < E; e++) v[e] *= sc;
         }
     };
     if (head < min(end, n_h)) weights(a.r.q, a.r.q_norm);

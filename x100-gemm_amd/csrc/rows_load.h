@@ -11,10 +11,17 @@ typedef unsigned int v2u __attribute__((ext_vector_type(2)));
 // by value: __builtin_bit_cast of a vector's element reads element 0
 X100_DEV v2h as_h2(uint32_t u) { return __builtin_bit_cast(v2h, u); }
 X100_DEV float bf2f(uint32_t b) { return __uint_as_float(b << 16); }
+// fp32 -> fp16, nearest even, of the fp32 number: with a product or a sum in front the compiler would take an
+// instruction that rounds once, from more than fp32 (a group of 4-bit codes in 30000 got another scale).
+X100_DEV _Float16 f2h_rne(float f)
+{
+    asm("" : "+v"(f));
+    return (_Float16)f;
+}
 // fp32 -> 16 bits, nearest even (NaN stays NaN)
 template <int T> X100_DEV uint32_t f2act(float f)
 {
-    if constexpr (T == X100_T_F16) return __builtin_bit_cast(uint16_t, (_Float16)f);
+    if constexpr (T == X100_T_F16) return __builtin_bit_cast(uint16_t, f2h_rne(f));
     return __builtin_bit_cast(uint16_t, (__bf16)f);
 }
 template <int T> X100_DEV float act2f(uint32_t b)
