@@ -96,8 +96,8 @@ size_t x100_kv_pool_bytes(const x100_kv_cfg *cfg);
 int x100_rope_table_hip(int head_dim, int n_pos, float base, float *table, void *stream);
 
 /* Head norms and rotation of q and k, rotated queries to q_out [n_rows][n_head * head_dim] (act_type),
- * keys and values into the pools at the rows' positions.  fp32 throughout, one rounding at the store
- * (and the codes' for 4 bits). */
+ * keys and values into the pools at the rows' positions.  fp32 throughout (squares of the head norms
+ * added by fours, then as a tree over neighbours), one rounding at the store (and the codes' for 4 bits). */
 int x100_kv_append_hip(const x100_kv_cfg *cfg, const x100_kv_batch *batch, const x100_kv_rows *rows, void *k_pool,
                        void *v_pool, void *q_out, void *stream);
 

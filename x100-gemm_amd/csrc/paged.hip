@@ -2,7 +2,7 @@
 // rows back out, and the rotation table.
 //
 // Bound by HBM for prompts (a row is read once, its queries, keys and values written once): 6400 rows of 40 heads
-// of 128, int32 to f16 and 4 bits, 47 us, 4.0 TB/s (a copy of 2 GiB: 5.0).  For single tokens bound by the launch and
+// of 128, int32 to f16 and 4 bits, 44 us, 4.2 TB/s (a copy of 2 GiB: 5.0).  For single tokens bound by the launch and
 // dependent loads (q_start -> kv_len -> block_table): 64 rows 4.9 us.
 #include <algorithm>
 
@@ -157,17 +157,17 @@ template <int HD, int ST, int AT, bool Q4> X100_DEV void append_qk(const AppendA
 #pragma unroll
             for (int e = 0; e < E; e++) v[e] = v[e] * rs * cl[e];
         fetch(min(head + 1, end - 1));
-        // The formula's own products and sums, each rounded: a 4-bit code of a key that lies between two steps is then the
-        // one that other fp32 code gets, but for the order of the sum of squares (here in pairs).  Weights and rotation
-        // multiplied beforehand, a fused sum and an estimated root were no faster and turned ten times as many codes.
+        // The formula's own products and sums, each rounded, the squares added by fours and then as a tree over
+        // neighbours: a 4-bit code of a key that lies between two steps is then the one that a tensor library's fp32
+        // gets.  Weights and rotation multiplied beforehand, a fused sum and an estimated root were no faster and turned
+        // some codes of 10^5 groups.
         if (norm) {
             float sq[E];
 #pragma unroll
             for (int e = 0; e < E; e++) sq[e] = v[e] * v[e];
 #pragma unroll
-            for (int d = 1; d < E; d *= 2)
-#pragma unroll
-                for (int e = 0; e < E; e += 2 * d) sq[e] += sq[e + d];
+            for (int e = 0; e < E; e += 4) sq[e] = ((sq[e] + sq[e + 1]) + sq[e + 2]) + sq[e + 3];
+            if constexpr (E == 8) sq[0] += sq[4];
             const float sc = 1.0f / sqrtf(sum16(sq[0]) / (float)HD + a.r.eps);
 #pragma unroll
             for (int e = 0; e < E; e++) v[e] = v[e] * sc * nw[e];
