@@ -15,8 +15,9 @@
  *   - Rows before position 0 (q_len > kv_len): not appended, read as zeros, attention output zeros.
  *   - A sequence whose entries break the bounds (q_start decreasing or outside 0 .. n_rows, more than
  *     max_q rows, kv_len < 0 or > max_kv) and rows at or behind q_start[n_seq]: nothing of them is
- *     read, and their outputs are left as they were.  (Where q_start decreases, rows of the sequences
- *     beside the break may be left as well.)
+ *     stored, and their outputs are left as they were.  Where q_start decreases, accepted sequences may
+ *     name the same rows: such a row, and any row behind the break, is taken for one of the sequences
+ *     that name it, in parts for one and another, or left.
  *   - A page number outside 0 .. n_pages - 1: nothing is stored there, its positions are not attended
  *     to, and they read as zeros.
  *   - Sequences may share pages that are only read; a page that gets new rows belongs to one sequence

@@ -1,18 +1,13 @@
 // The paged KV cache (x100_paged.h) as its kernels see it: the batch, pages and the 4-bit format.
 #pragma once
+#include "paged_rows.h"
 #include "rows_load.h"
 #include "x100_paged.h"
-
-struct PagedSeq {
-    int q0, q_len, kv_len;   // first row, rows, cached positions (q_len < 0: the sequence is refused)
-};
 
 // Sequence s of the batch, every entry checked against the host's bounds (x100_paged.h).
 X100_DEV PagedSeq paged_seq(const x100_kv_batch &b, int s)
 {
-    const int q0 = b.q_start[s], q1 = b.q_start[s + 1], kv = b.kv_len[s];
-    const bool ok = q0 >= 0 && q1 >= q0 && q1 <= b.n_rows && q1 - q0 <= b.max_q && kv >= 0 && kv <= b.max_kv;
-    return {q0, ok ? q1 - q0 : -1, kv};
+    return paged_checked(b.q_start[s], b.q_start[s + 1], b.kv_len[s], b.n_rows, b.max_q, b.max_kv);
 }
 
 // Page of position p (0 <= p < max_kv) of sequence s, or -1 outside 0 .. n_pages - 1.
@@ -27,19 +22,12 @@ X100_DEV int paged_page(const x100_kv_cfg &c, const x100_kv_batch &b, int s, int
 template <class F> X100_DEV int paged_search(int n_seq, F &&below)
 {
     const int lane = threadIdx.x & 63;
-    int lo = 0, len = n_seq;
-    while (len > 0) {
-        const int stride = (len + 63) / 64;              // entries lo + (i + 1) * stride - 1
+    return paged_steps(n_seq, [&](int lo, int len, int stride) __attribute__((always_inline)) {
         const int i = (lane + 1) * stride - 1;
-        const bool le = i < len && below(lo + i + 1);
-        const int n = __popcll(__ballot(le)) * stride;   // entries known to lie below
-        if (stride == 1) return lo + n;
-        lo += n;
-        len = min(stride - 1, len - n);                  // the next entry probed does not
-    }
-    return lo;
+        return __popcll(__ballot(i < len && below(lo + i + 1)));
+    });
 }
-// The sequence of row r: the first s with q_start[s + 1] > r (n_seq if there is none).
+// The sequence of row r: the first s with q_start[s + 1] > r (n_seq if there is none; any, where q_start decreases).
 X100_DEV int paged_find(const x100_kv_batch &b, int r)
 {
     return paged_search(b.n_seq, [&](int s) { return b.q_start[s] <= r; });

@@ -86,7 +86,7 @@ X100_DEV RowPlace row_place(const x100_kv_batch &b, int rbase, int sub)
     }
     if (r < b.n_rows && f < b.n_seq) {
         const PagedSeq q = paged_seq(b, f);
-        if (q.q_len > 0 && r >= q.q0) p = {f, q.kv_len - q.q_len + r - q.q0, true};
+        if (q.holds(r)) p = {f, q.position(r), true};
     }
     return p;
 }
@@ -250,29 +250,11 @@ template <int HD, int ST, int AT, bool Q4> X100_DEV void append_v(const AppendAr
     const x100_rows &src = a.r.v;
     const int col = kvh * HD + el;
     const int first = (bv % a.xv * (4 / WH) + w / WH) * a.vrows, last = min(first + a.vrows, a.b.n_rows);
-    int row = first;
-    while (row < last) {
-        const int s = paged_find(a.b, row);
-        if (s >= a.b.n_seq) return;
-        const PagedSeq q = paged_seq(a.b, s);
-        if (q.q_len <= 0 || row < q.q0) {
-            row++;
-            continue;
-        }
-        const int shift = q.kv_len - q.q_len - q.q0;   // position - row
-        // this sequence's blocks that begin in the unit: at its first row, and at every position 8 k
-        for (const int stop = min(last, q.q0 + q.q_len); row < stop;) {
-            const int pos = row + shift;
-            if (pos < 0) {
-                row = min(stop, -shift);
-                continue;
-            }
-            if (!(row == q.q0 || (pos & 7) == 0)) {
-                row = min(stop, row + 8 - (pos & 7));
-                continue;
-            }
-            const int o0 = pos & 7, n = min(8 - o0, q.q0 + q.q_len - row);
-            const int pg = paged_page(a.c, a.b, s, pos), blk = (pos & (page - 1)) >> 3;
+    paged_blocks(
+        first, last, a.b.n_seq, [&](int row) __attribute__((always_inline)) { return paged_find(a.b, row); },
+        [&](int s) __attribute__((always_inline)) { return paged_seq(a.b, s); },
+        [&](int s, int row, int pos, int n) __attribute__((always_inline)) {
+            const int o0 = pos & 7, pg = paged_page(a.c, a.b, s, pos), blk = (pos & (page - 1)) >> 3;
             float v[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) v[k] = row_elem<ST>(src.p, (size_t)(row + min(k, n - 1)) * src.ld + col);
@@ -281,8 +263,7 @@ template <int HD, int ST, int AT, bool Q4> X100_DEV void append_v(const AppendAr
 #pragma unroll
                 for (int k = 0; k < 8; k++) v[k] = v[k] * src.row_scale[row + min(k, n - 1)] * cl;
             }
-            row += n;
-            if (pg < 0) continue;
+            if (pg < 0) return;
             uint8_t *base = a.vp + ((size_t)pg * n_kv + kvh) * page_head_bytes<HD, Q4>(page);
             if constexpr (!Q4) {
                 uint16_t *o = (uint16_t *)base + ((size_t)blk * HD + el) * 8;
@@ -332,7 +313,7 @@ template <int HD, int ST, int AT, bool Q4> X100_DEV void append_v(const AppendAr
                     code(6, quad<2>(sc[1].mf), quad<2>(sc[1].inv));
                     code(7, quad<3>(sc[1].mf), quad<3>(sc[1].inv));
                     *cw = word;
-                    continue;
+                    return;
                 }
                 uint32_t word = n == 8 ? 0u : *cw;
 #pragma unroll
@@ -356,8 +337,7 @@ template <int HD, int ST, int AT, bool Q4> X100_DEV void append_v(const AppendAr
                 }
                 *cw = word;
             }
-        }
-    }
+        });
 }
 
 template <int HD, int ST, int AT, bool Q4> __global__ __launch_bounds__(256) void k_append(const AppendArgs a)
