@@ -112,8 +112,8 @@ int x100_kv_read_hip(const x100_kv_cfg *cfg, const x100_kv_batch *batch, const v
  * q: row r at element r * ldq, out: at r * ldo, heads contiguous, act_type; scale > 0.  Query head h
  * reads KV head h / (n_head / n_head_kv).  Scores, softmax and sums in fp32; the weights are rounded
  * to 16 bits (act_type, or fp16 for 4-bit pages) for the product with V.  A row that attends to
- * nothing (no position, no valid page, or every score -inf) gives zeros.  Infinities and NaN in
- * positions that a row does not attend to do not reach it.
+ * nothing (no position, no valid page, or every score -inf) gives zeros; one with a score that is NaN
+ * gives NaN.  Infinities and NaN in positions that a row does not attend to do not reach it.
  * Scratch: x100_attn_paged_workspace_bytes(cfg, batch) bytes (0: none needed, ws may be NULL; it
  * depends on n_rows, n_seq, max_q and max_kv only), 256-byte aligned, any contents, for the _ws form;
  * overlapping calls need distinct buffers.  The plain form uses the library's workspace of the

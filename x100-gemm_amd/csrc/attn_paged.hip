@@ -360,8 +360,9 @@ template <int HD, int AT, bool Q4, int NW> __global__ __launch_bounds__(64 * NW,
         float ls = 0.0f, y0 = 0.0f, y1 = 0.0f;
 #pragma unroll
         for (int k = 0; k < NW; k++) {
+            // a wave without weights has no O; one whose every score is NaN has no maximum either, but a NaN as l
             const float f = __builtin_amdgcn_exp2f(s_m[k][r] - ms);
-            if (s_m[k][r] == NEG_INF) continue;
+            if (s_l[k][r] == 0.0f) continue;
             ls = __builtin_fmaf(s_l[k][r], f, ls);
             y0 = __builtin_fmaf(sh.o[k][r][el], f, y0);
             y1 = __builtin_fmaf(sh.o[k][r][el + 1], f, y1);
@@ -424,7 +425,7 @@ template <int HD, int AT, bool WIDE> __global__ __launch_bounds__(256) void k_at
         }
 #pragma unroll
         for (int u = 0; u < 8; u++) {
-            if (k0 + u * ST >= ns || v[u].x == NEG_INF) continue;   // a split without positions has no O
+            if (k0 + u * ST >= ns || v[u].y == 0.0f) continue;   // a split without weights has no O
             const float f = __builtin_amdgcn_exp2f(v[u].x - ms);
             l = __builtin_fmaf(v[u].y, f, l);
             y.x = __builtin_fmaf(b[u].x, f, y.x);
