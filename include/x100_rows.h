@@ -10,10 +10,10 @@
  *
  * Codes: t = the row's values, amax = max |t|, code = rint(t * f) with f = 127 * (1 / amax) in fp32
  * (two roundings; ties to even), scale = amax / 127.  A row of zeros (or amax < 2^-100) has codes 0 and
- * scale 0; a row that holds an infinity or a NaN has codes 0 and scale NaN.  In add_rmsnorm_i8
- * t = h * weight and the norm's
- * factor goes into the scale alone (it cancels in the code), so that the codes do not depend on the
- * order in which a sum was taken: they are the same for every layout, alignment and launch.
+ * scale 0; a row with a t that is an infinity or a NaN has codes 0 and scale NaN.  In add_rmsnorm_i8
+ * t = h * weight and the norm's factor goes into the scale alone (it cancels in the code), so that the
+ * codes do not depend on the order in which a sum was taken: they are the same for every layout,
+ * alignment and launch.
  *
  * All pointers are device pointers; asynchronous on stream (a hipStream_t as void *, NULL = the
  * default stream); no workspace; capturable.  Every argument is checked before anything is
@@ -54,7 +54,8 @@ int x100_quant_i8_hip(int n_rows, int d, const x100_rows *x, int8_t *q, float *s
  * x->ld updates in place; no other output overlaps an input); then RMSNorm of the stored h with weight[d] and eps, as codes and scales:
  *   r = 1 / sqrt(mean(h^2) + eps),  t = h * weight,  scale = max|t| * r / 127.
  * x: F32, F16 or BF16; delta: any of the four types, or NULL for no addition (h is then not written
- * and may be NULL).  Values up to 1e18 (their squares are summed in fp32); eps >= 0. */
+ * and may be NULL).  Squares are summed in fp64, so h of any size; eps >= 0, and a row of zeros has
+ * scale 0 for eps = 0 too. */
 int x100_add_rmsnorm_i8_hip(int n_rows, int d, const x100_rows *x, const x100_rows *delta, const float *weight,
                             float eps, void *h, int64_t ldh, int8_t *q, float *scale, void *stream);
 

@@ -11,6 +11,30 @@
 
 namespace {
 
+template <int CTRL, int ROWM = 0xf> X100_DEV double dpp_d(double v)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = dpp_i<CTRL, ROWM>(0, (int)(uint32_t)u), hi = dpp_i<CTRL, ROWM>(0, (int)(uint32_t)(u >> 32));
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// sum over the wave, in its last lane
+X100_DEV double wave_sum_last(double v)
+{
+    v += dpp_d<0x111>(v);
+    v += dpp_d<0x112>(v);
+    v += dpp_d<0x114>(v);
+    v += dpp_d<0x118>(v);
+    v += dpp_d<0x142, 0xa>(v);
+    v += dpp_d<0x143, 0xc>(v);
+    return v;
+}
+// mx / (127 sqrt(m)) for m > 0, in fp32: m is brought to 1 .. 4 first, the root's power of two goes into the result
+X100_DEV float norm_scale(float mx, double m)
+{
+    const int e = ((int)(__builtin_bit_cast(uint64_t, m) >> 52) - 1023) & ~1;
+    return ldexpf(mx * (1.0f / sqrtf((float)ldexp(m, -e))) / 127.0f, -e / 2);
+}
+
 struct RowArgs {
     int n_rows, d;
     x100_rows x, delta;
@@ -29,12 +53,16 @@ template <int NT, int CH, bool VEC, int XT, int DT, bool NORM>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_rows_i8(const RowArgs a)
 {
     constexpr int BT = NT < 256 ? 256 : NT, RPB = BT / NT, NW = NT / 64;
-    __shared__ float s_red[BT / 64][2];
+    __shared__ float s_mx[BT / 64];
+    __shared__ double s_ss[BT / 64];
     const int t = threadIdx.x % NT, row = blockIdx.x * RPB + threadIdx.x / NT, w = threadIdx.x >> 6;
     const bool live = row < a.n_rows;
     const int d = a.d;
     float v[CH][8];
-    float ss = 0.0f, mx = 0.0f;
+    // Squares are summed in fp64, where those of every fp32 number are normal: in fp32 they left its range at 1e18 and
+    // below 1e-22 (a row of 1e-24 got the scale inf for eps = 0).
+    double ss = 0.0;
+    float mx = 0.0f;
     bool bad = false;
     if (live) {
         const float drs = DT == X100_T_I32 ? a.delta.row_scale[row] : 1.0f;
@@ -93,7 +121,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_rows_i8(const RowArgs a
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 if constexpr (NORM) {
-                    ss = __builtin_fmaf(v[c][e], v[c][e], ss);
+                    ss = __builtin_fma((double)v[c][e], (double)v[c][e], ss);
                     if (VEC || e0 + e < d) v[c][e] *= a.weight[e0 + e];
                 }
                 mx = fmaxf(mx, fabsf(v[c][e]));
@@ -104,28 +132,28 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_rows_i8(const RowArgs a
     // over the row's threads; a value that is not finite makes mx an infinity
     if (bad) mx = __builtin_inff();
     mx = wave_max_u(mx);
-    if constexpr (NORM) ss = wave_sum_uf(ss);
+    if constexpr (NORM) ss = wave_sum_last(ss);
     if constexpr (NW > 1) {
-        if ((threadIdx.x & 63) == 0) {
-            s_red[w][0] = mx;
-            s_red[w][1] = ss;
+        if ((threadIdx.x & 63) == 63) {
+            s_mx[w] = mx;
+            s_ss[w] = ss;
         }
         __syncthreads();
-        mx = s_red[w / NW * NW][0];
-        ss = s_red[w / NW * NW][1];
+        mx = s_mx[w / NW * NW];
+        ss = s_ss[w / NW * NW];
 #pragma unroll
         for (int i = 1; i < NW; i++) {
-            mx = fmaxf(mx, s_red[w / NW * NW + i][0]);
-            ss += s_red[w / NW * NW + i][1];
+            mx = fmaxf(mx, s_mx[w / NW * NW + i]);
+            ss += s_ss[w / NW * NW + i];
         }
     }
     if (!live) return;
     const bool fin = mx <= 3.402823466e38f, some = fin && mx >= 0x1p-100f;
     const float inv = some ? 127.0f * (1.0f / mx) : 0.0f;
-    if (t == 0) {
-        float sc = some ? mx : (fin ? 0.0f : __builtin_nanf(""));
-        if constexpr (NORM) sc *= 1.0f / sqrtf(ss / (float)d + a.eps);
-        a.scale[row] = sc / 127.0f;
+    if (t == NT - 1) {   // NT = 64: the lane that has the sum
+        float sc = fin ? 0.0f : __builtin_nanf("");
+        if (some) sc = NORM ? norm_scale(mx, ss / d + (double)a.eps) : mx / 127.0f;
+        a.scale[row] = sc;
     }
 #pragma unroll
     for (int c = 0; c < CH; c++) {
