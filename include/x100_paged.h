@@ -33,9 +33,9 @@
  *            positions, m of 8).  A K word holds 8 elements of a row, a V word 8 positions of an
  *            element: number e at bit 16 * (e % 2) + 4 * (e / 2).
  *            d = fp16((hi - lo) * fp32(1/15)), m = fp16(lo), n = rint((x - m) * (1 / d)) within 0 .. 15,
- *            in fp32.
- *            Values up to 65504 in size; a group with a larger one, an infinity or a NaN stands for
- *            NaN (d = m = NaN).
+ *            in fp32; d is the fp16 below that where m + 15 d would round past 65504.
+ *            Values up to 65504 in size, whose codes stand for finite numbers; a group with a larger one,
+ *            an infinity or a NaN stands for NaN (d = m = NaN).
  *
  * All pointers are device pointers unless they are the argument structures; every call is
  * asynchronous on stream and capturable.  All arguments that the host can see are checked before

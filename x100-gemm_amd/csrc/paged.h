@@ -39,8 +39,9 @@ template <int HD, bool Q4> X100_DEV constexpr int page_head_bytes(int page) { re
 // 4-bit codes: number e of 8 at bit 16 (e % 2) + 4 (e / 2) of the word.
 X100_DEV constexpr int q4_shift(int e) { return 16 * (e & 1) + 4 * (e >> 1); }
 
-// d, m of a group from its smallest and largest value (fp16 bits; d = m = NaN where either is not
-// finite) and 1 / d.
+// d, m of a group from its smallest and largest value (fp16 bits; d = m = NaN where bad, or where either is past
+// fp16's range) and 1 / d.  d is mostly rounded to nearest; where that would take the largest code's value past fp16's
+// range (0 .. 65504: d = 4368, 15 d = 65520), the fp16 below it, 15 of whose steps end at the largest value or below.
 struct Q4Scale {
     uint16_t d, m;
     float inv, mf;
@@ -48,9 +49,12 @@ struct Q4Scale {
 };
 X100_DEV Q4Scale q4_scale(float lo, float hi, bool bad)
 {
-    const _Float16 d = f2h_rne((hi - lo) * (1.0f / 15.0f)), m = f2h_rne(lo);
+    bad |= !(lo >= -65504.0f) || !(hi <= 65504.0f);
+    const _Float16 m = f2h_rne(lo);
+    _Float16 d = f2h_rne((hi - lo) * (1.0f / 15.0f));
+    if (__builtin_fmaf16((_Float16)15.0f, d, m) > (_Float16)65504.0f)
+        d = __builtin_bit_cast(_Float16, (uint16_t)(__builtin_bit_cast(uint16_t, d) - 1));
     const float df = (float)d, mf = (float)m;
-    bad |= !(fabsf(df) <= 65504.0f) || !(fabsf(mf) <= 65504.0f);
     Q4Scale s;
     s.d = bad ? 0x7e00 : __builtin_bit_cast(uint16_t, d);
     s.m = bad ? 0x7e00 : __builtin_bit_cast(uint16_t, m);
