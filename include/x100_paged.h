@@ -111,9 +111,10 @@ int x100_kv_read_hip(const x100_kv_cfg *cfg, const x100_kv_batch *batch, const v
 /* out[row][head] = sum_p softmax_p(scale * q[row][head] . K_p) V_p over the positions p <= the row's own;
  * q: row r at element r * ldq, out: at r * ldo, heads contiguous, act_type; scale > 0.  Query head h
  * reads KV head h / (n_head / n_head_kv).  Scores, softmax and sums in fp32; the weights are rounded
- * to 16 bits (act_type, or fp16 for 4-bit pages) for the product with V.  A row that attends to
- * nothing (no position, no valid page, or every score -inf) gives zeros; one with a score that is NaN
- * gives NaN.  Infinities and NaN in positions that a row does not attend to do not reach it.
+ * to 16 bits (act_type, or fp16 for 4-bit pages) for the product with V, and in fp16 a weight below
+ * 2^-29 of the largest is zero.  A row that attends to nothing (no position, no valid page, or every
+ * score -inf) gives zeros; one with a score that is NaN gives NaN.  Infinities and NaN in positions
+ * that a row does not attend to do not reach it.
  * Scratch: x100_attn_paged_workspace_bytes(cfg, batch) bytes (0: none needed, ws may be NULL; it
  * depends on n_rows, n_seq, max_q and max_kv only), 256-byte aligned, any contents, for the _ws form;
  * overlapping calls need distinct buffers.  The plain form uses the library's workspace of the

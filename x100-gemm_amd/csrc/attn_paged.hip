@@ -209,13 +209,13 @@ template <int HD, int AT, bool Q4, int NW> __global__ __launch_bounds__(64 * NW,
             sc[h] = y;
         }
     };
-    // The weights p.  The maximum may stay up to 8 (a factor of 256) behind: every sum is relative to it.
+    // The weights p, relative to m (tile_lift), which may stay up to 8 (a factor of 256) behind.
     v4u p;
     auto weights = [&]() __attribute__((always_inline)) {
         float mx = fmaxf(sc[0][0], sc[1][0]);
 #pragma unroll
         for (int e = 1; e < 4; e++) mx = fmaxf(fmaxf(mx, sc[0][e]), sc[1][e]);
-        mx *= sc2;
+        mx = __builtin_fmaf(mx, sc2, -tile_lift<MT>());
         if (__any(mx > m + 8.0f)) {
             mx = fmaxf(mx, xor16_f(mx));
             mx = fmaxf(mx, xor32_f(mx));
