@@ -47,14 +47,15 @@ typedef struct {
 } x100_rows;
 
 /* q[n_rows][d] (contiguous) and scale[n_rows] from the rows x (any of the four types).
- * 1 <= d <= X100_ROWS_MAX_D, x->ld >= d, n_rows >= 0. */
+ * 1 <= d <= X100_ROWS_MAX_D, x->ld >= d, 0 <= n_rows < 2^24 (2^22 for d > 4096). */
 int x100_quant_i8_hip(int n_rows, int d, const x100_rows *x, int8_t *q, float *scale, void *stream);
 
 /* h = x + delta, rounded to x's type and stored (h: row r at element r * ldh; h == x->p with ldh ==
- * x->ld updates in place; no other output overlaps an input); then RMSNorm of the stored h with weight[d] and eps, as codes and scales:
+ * x->ld updates in place; no other output overlaps an input); then RMSNorm of the stored h with
+ * weight[d] and eps, as codes and scales:
  *   r = 1 / sqrt(mean(h^2) + eps),  t = h * weight,  scale = max|t| * r / 127.
  * x: F32, F16 or BF16; delta: any of the four types, or NULL for no addition (h is then not written
- * and may be NULL).  Squares are summed in fp64, so h of any size; eps >= 0, and a row of zeros has
+ * and may be NULL); n_rows and d as in quant_i8.  Squares are summed in fp64, so h of any size; eps >= 0, and a row of zeros has
  * scale 0 for eps = 0 too. */
 int x100_add_rmsnorm_i8_hip(int n_rows, int d, const x100_rows *x, const x100_rows *delta, const float *weight,
                             float eps, void *h, int64_t ldh, int8_t *q, float *scale, void *stream);

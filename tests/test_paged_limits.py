@@ -1,0 +1,20 @@
+"""Refusals at the limits that x100_rows.h / x100_paged.h state (no GPU: an argument error returns before the device
+is looked at; what is within them gets as far as the device)."""
+import pytest
+import torch
+
+import x100hip as x
+from test_paged_args import A, batch, cfg, refused, rows
+
+
+def test_rows_past_one_launch():
+    for n, d, fine in [(1 << 22, 4097, False), (1 << 22, 16384, False), ((1 << 24) - 1, 8192, False), (1 << 24, 1, False),
+                       (1 << 24, 4096, False)]:
+        refused(x.quant_i8, n, d, rows(ld=1 << 20), A, A)
+        refused(x.add_rmsnorm_i8, n, d, rows(ld=1 << 20), None, A, 1e-6, None, 0, A, A)
+    if torch.cuda.is_available():
+        return
+    for n, d in [((1 << 22) - 1, 16384), ((1 << 24) - 1, 4096)]:    # accepted: no device here
+        with pytest.raises(x.X100Error) as e:
+            x.quant_i8(n, d, rows(ld=1 << 20), A, A)
+        assert e.value.code == x.X100_ENODEV

@@ -809,9 +809,10 @@ static bool rows_ok(const x100_rows *r, int d)
     return i32 == (r->row_scale != nullptr) && i32 == (r->col_scale != nullptr);
 }
 
+// A launch has up to 256 threads per row, 1024 for d > 4096, and less than 2^32 in all.
 static bool i8_out_ok(int n_rows, int d, const int8_t *q, const float *scale)
 {
-    return n_rows >= 0 && n_rows < 1 << 24 && d >= 1 && d <= X100_ROWS_MAX_D && q && scale && !((uintptr_t)scale & 3);
+    return n_rows >= 0 && n_rows < (d > 4096 ? 1 << 22 : 1 << 24) && d >= 1 && d <= X100_ROWS_MAX_D && q && scale && !((uintptr_t)scale & 3);
 }
 
 int x100_quant_i8_hip(int n_rows, int d, const x100_rows *x, int8_t *q, float *scale, void *stream)
