@@ -18,3 +18,10 @@ def test_rows_past_one_launch():
         with pytest.raises(x.X100Error) as e:
             x.quant_i8(n, d, rows(ld=1 << 20), A, A)
         assert e.value.code == x.X100_ENODEV
+
+
+def test_scales_that_are_not_aligned():
+    for r in (rows(t=x.T_I32, rs=A + 2, cs=A), rows(t=x.T_I32, rs=A, cs=A + 1)):
+        refused(x.quant_i8, 1, 64, r, A, A)
+        refused(x.add_rmsnorm_i8, 1, 64, rows(), r, A, 1e-6, 2 * A, 64, A, A)
+        refused(x.kv_append, cfg(), batch(), x.KvRows(r, r, r), A, 2 * A, A)

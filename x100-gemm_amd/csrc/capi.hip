@@ -800,11 +800,12 @@ static int type_bytes(int type)
 }
 
 // A row tensor of width d: a known type, aligned to its elements, rows that do not overlap, scales
-// with int32 and only there.
+// (aligned fp32) with int32 and only there.
 static bool rows_ok(const x100_rows *r, int d)
 {
     const int e = r ? type_bytes(r->type) : 0;
     if (!e || !r->p || (uintptr_t)r->p % e || r->ld < d || r->ld > ((int64_t)1 << 40)) return false;
+    if (((uintptr_t)r->row_scale | (uintptr_t)r->col_scale) & 3) return false;
     const bool i32 = r->type == X100_T_I32;
     return i32 == (r->row_scale != nullptr) && i32 == (r->col_scale != nullptr);
 }
