@@ -59,7 +59,7 @@ extern "C" {
 #define X100_KV_Q4 256   /* kv_type: 4-bit codes (above); not a ggml type */
 
 typedef struct {
-    int n_head, n_head_kv;   /* query heads, KV heads: 1 to 16 query heads per KV head            */
+    int n_head, n_head_kv;   /* query heads (<= 1024), KV heads: 1 to 16 query heads per KV head  */
     int head_dim;            /* 64 or 128                                                         */
     int page;                /* positions of a page: 16, 32, 64, 128 or 256                       */
     int n_pages;             /* pages in each pool                                                */
@@ -68,8 +68,8 @@ typedef struct {
 } x100_kv_cfg;
 
 typedef struct {
-    int n_seq, n_rows;       /* sequences (<= 65535), rows of the row arrays                      */
-    int max_q, max_kv;       /* bounds of q_len and kv_len, >= 1                                  */
+    int n_seq, n_rows;       /* sequences (<= 65535), rows of the row arrays (< 2^24)             */
+    int max_q, max_kv;       /* bounds of q_len (1 .. 2^20) and kv_len (1 .. 2^26)                */
     int table_ld;            /* entries of a block_table row, table_ld * page >= max_kv           */
     const int *q_start;      /* [n_seq + 1]                                                       */
     const int *kv_len;       /* [n_seq]                                                           */
@@ -93,7 +93,7 @@ typedef struct {
 size_t x100_kv_pool_bytes(const x100_kv_cfg *cfg);
 
 /* table[p][i] = (cos, sin)(p * base^(-2 i / head_dim)) for p < n_pos, angles in fp64: the rotation
- * of the reference (table qwen_moe_hp.c:799-804).  Once per model. */
+ * of the reference (table qwen_moe_hp.c:799-804).  n_pos <= 2^25.  Once per model. */
 int x100_rope_table_hip(int head_dim, int n_pos, float base, float *table, void *stream);
 
 /* Head norms and rotation of q and k, rotated queries to q_out [n_rows][n_head * head_dim] (act_type),
@@ -109,12 +109,13 @@ int x100_kv_read_hip(const x100_kv_cfg *cfg, const x100_kv_batch *batch, const v
                      void *k_out, void *v_out, void *stream);
 
 /* out[row][head] = sum_p softmax_p(scale * q[row][head] . K_p) V_p over the positions p <= the row's own;
- * q: row r at element r * ldq, out: at r * ldo, heads contiguous, act_type; scale > 0.  Query head h
- * reads KV head h / (n_head / n_head_kv).  Scores, softmax and sums in fp32; the weights are rounded
- * to 16 bits (act_type, or fp16 for 4-bit pages) for the product with V, and in fp16 a weight below
- * 2^-29 of the largest is zero.  A row that attends to nothing (no position, no valid page, or every
- * score -inf) gives zeros; one with a score that is NaN gives NaN.  Infinities and NaN in positions
- * that a row does not attend to do not reach it.
+ * q: row r at element r * ldq, out: at r * ldo, heads contiguous, act_type; 0 < scale <= 1e38.  Query head h
+ * reads KV head h / (n_head / n_head_kv).  Scores, softmax and sums in fp32, the weights divided by
+ * their sum at the end (so bf16 V up to 2^100 in size); for the product with V they are rounded to 16
+ * bits (act_type, or fp16 for 4-bit pages), and in fp16 a weight below 2^-29 of the largest is zero.
+ * A row that attends to nothing (no position, no valid page, or every score -inf) gives zeros; one
+ * with a score that is NaN gives NaN.  Infinities and NaN in positions that a row does not attend to
+ * do not reach it.
  * Scratch: x100_attn_paged_workspace_bytes(cfg, batch) bytes (0: none needed, ws may be NULL; it
  * depends on n_rows, n_seq, max_q and max_kv only), 256-byte aligned, any contents, for the _ws form;
  * overlapping calls need distinct buffers.  The plain form uses the library's workspace of the

@@ -25,3 +25,9 @@ def test_scales_that_are_not_aligned():
         refused(x.quant_i8, 1, 64, r, A, A)
         refused(x.add_rmsnorm_i8, 1, 64, rows(), r, A, 1e-6, 2 * A, 64, A, A)
         refused(x.kv_append, cfg(), batch(), x.KvRows(r, r, r), A, 2 * A, A)
+
+
+def test_a_scale_that_overflows():
+    for scale in (1.1e38, 3.4e38):
+        refused(x.attn_paged_ws, cfg(), batch(), A, 1024, A, 2 * A, scale, A, 1024, A, 1 << 30)
+        refused(x.attn_paged, cfg(), batch(), A, 1024, A, 2 * A, scale, A, 1024)

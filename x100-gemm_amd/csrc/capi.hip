@@ -953,7 +953,7 @@ static int check_attn_paged(const x100_kv_cfg *c, const x100_kv_batch *b, const 
     if (!q || !out || (((uintptr_t)q | (uintptr_t)out) & 15) || ldq < width || ldo < width || ldq > most || ldo > most ||
         ldq % 8 || ldo % 8)
         return X100_EINVAL;
-    if (!(scale > 0.0f) || std::isinf(scale)) return X100_EINVAL;
+    if (!(scale > 0.0f) || scale > 1e38f) return X100_EINVAL;   // times log2(e) it stays finite
     return X100_OK;
 }
 
