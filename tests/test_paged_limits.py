@@ -31,3 +31,15 @@ def test_a_scale_that_overflows():
     for scale in (1.1e38, 3.4e38):
         refused(x.attn_paged_ws, cfg(), batch(), A, 1024, A, 2 * A, scale, A, 1024, A, 1 << 30)
         refused(x.attn_paged, cfg(), batch(), A, 1024, A, 2 * A, scale, A, 1024)
+
+
+def test_batches_past_one_launch_ask_for_no_workspace():
+    """Refused before the library's workspace is looked for (here it would have been tebibytes)."""
+    many = dict(n_seq=65535, n_rows=(1 << 24) - 1, max_kv=1 << 26, table_ld=1 << 22)
+    for c, b in [(cfg(n_head=16, n_head_kv=16, page=16), batch(max_q=1, **many)),       # single tokens in many splits
+                 (cfg(n_head=16, n_head_kv=16, page=16), batch(max_q=1 << 20, **many)),  # prompts
+                 (cfg(n_head=1024, n_head_kv=1024), batch(n_seq=65535, n_rows=(1 << 24) - 1, max_q=1000, max_kv=16))]:
+        w = c.n_head * c.head_dim
+        assert x.attn_paged_workspace_bytes(c, b) == 0
+        refused(x.attn_paged, c, b, A, w, A, 2 * A, 0.1, A, w)
+        refused(x.attn_paged_ws, c, b, A, w, A, 2 * A, 0.1, A, w, A, 1 << 60)

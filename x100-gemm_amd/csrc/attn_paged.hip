@@ -519,17 +519,21 @@ Plan plan_of(const x100_kv_cfg &c, const x100_kv_batch &b)
     return p;
 }
 
+int64_t tile_blocks(const Plan &p, const x100_kv_cfg &c, const x100_kv_batch &b)
+{
+    return ((int64_t)b.n_seq * c.n_head_kv * p.tile.n + p.run - 1) / p.run * p.run * p.tiles;
+}
+
 template <int HD, int AT> hipError_t attn_as(const AttnArgs &a, const Plan &p, hipStream_t s)
 {
-    const int64_t blocks = ((int64_t)a.b.n_seq * a.c.n_head_kv * p.tile.n + a.run - 1) / a.run * a.run * p.tiles;
-    if (blocks >= 1 << 24) return hipErrorInvalidValue;   // past one launch
     if (p.prompt.n) {
         const hipError_t e = x100_attn_prompt_launch(a, s);
         if (e != hipSuccess) return e;
     }
     if (p.tile.n) {
-        if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true, 4><<<(unsigned)blocks, 256, 0, s>>>(a);
-        else k_attn_tile<HD, AT, false, 4><<<(unsigned)blocks, 256, 0, s>>>(a);
+        const unsigned blocks = (unsigned)tile_blocks(p, a.c, a.b);
+        if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true, 4><<<blocks, 256, 0, s>>>(a);
+        else k_attn_tile<HD, AT, false, 4><<<blocks, 256, 0, s>>>(a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
@@ -543,10 +547,12 @@ template <int HD, int AT> hipError_t attn_as(const AttnArgs &a, const Plan &p, h
 
 }  // namespace
 
-size_t x100_attn_paged_workspace(const x100_kv_cfg &c, const x100_kv_batch &b)
+bool x100_attn_paged_workspace(const x100_kv_cfg &c, const x100_kv_batch &b, size_t *bytes)
 {
     const Plan p = plan_of(c, b);
-    return (p.tile_parts + p.prompt_parts) * (c.head_dim + 2) * sizeof(float);
+    if (tile_blocks(p, c, b) >= 1 << 24 || x100_attn_prompt_blocks(c, b, p.prompt.n) >= 1 << 23) return false;
+    *bytes = (p.tile_parts + p.prompt_parts) * (c.head_dim + 2) * sizeof(float);
+    return true;
 }
 
 hipError_t x100_attn_paged_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const void *q, int64_t ldq,

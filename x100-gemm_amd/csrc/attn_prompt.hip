@@ -549,15 +549,18 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(512, 2) void k_a
 
 template <int HD, int AT> hipError_t prompt_as(const PagedAttnArgs &a, hipStream_t s)
 {
-    const int64_t items = (int64_t)a.b.n_rows * (a.c.n_head / a.c.n_head_kv) / PROMPT_ROWS + a.b.n_seq;
-    const int64_t blocks = items * a.prompt.n * a.c.n_head_kv;
-    if (blocks >= 1 << 23) return hipErrorInvalidValue;   // past one launch
-    if (a.c.kv_type == X100_KV_Q4) k_attn_prompt<HD, AT, true><<<(unsigned)blocks, 512, 0, s>>>(a);
-    else k_attn_prompt<HD, AT, false><<<(unsigned)blocks, 512, 0, s>>>(a);
+    const unsigned blocks = (unsigned)x100_attn_prompt_blocks(a.c, a.b, a.prompt.n);
+    if (a.c.kv_type == X100_KV_Q4) k_attn_prompt<HD, AT, true><<<blocks, 512, 0, s>>>(a);
+    else k_attn_prompt<HD, AT, false><<<blocks, 512, 0, s>>>(a);
     return hipGetLastError();
 }
 
 }  // namespace
+
+int64_t x100_attn_prompt_blocks(const x100_kv_cfg &c, const x100_kv_batch &b, int splits)
+{
+    return ((int64_t)b.n_rows * (c.n_head / c.n_head_kv) / PROMPT_ROWS + b.n_seq) * splits * c.n_head_kv;
+}
 
 hipError_t x100_attn_prompt_launch(const PagedAttnArgs &a, hipStream_t s)
 {

@@ -939,14 +939,24 @@ int x100_kv_read_hip(const x100_kv_cfg *c, const x100_kv_batch *b, const void *k
     return X100_OK;
 }
 
+// Bytes of the workspace; false for a batch that no launch holds.
+static bool attn_paged_need(const x100_kv_cfg *c, const x100_kv_batch *b, size_t *need)
+{
+    *need = 0;
+    if (b->n_seq == 0 || b->n_rows == 0) return true;
+    if (!x100_attn_paged_workspace(*c, *b, need)) return false;
+    *need = al256(*need);
+    return true;
+}
+
 size_t x100_attn_paged_workspace_bytes(const x100_kv_cfg *c, const x100_kv_batch *b)
 {
-    if (!kv_cfg_ok(c) || !kv_bounds_ok(c, b) || b->n_seq == 0 || b->n_rows == 0) return 0;
-    return al256(x100_attn_paged_workspace(*c, *b));
+    size_t need = 0;
+    return kv_cfg_ok(c) && kv_bounds_ok(c, b) && attn_paged_need(c, b, &need) ? need : 0;
 }
 
 static int check_attn_paged(const x100_kv_cfg *c, const x100_kv_batch *b, const void *q, int64_t ldq, const void *kp,
-                            const void *vp, float scale, const void *out, int64_t ldo)
+                            const void *vp, float scale, const void *out, int64_t ldo, size_t *need)
 {
     if (!kv_cfg_ok(c) || !kv_batch_ok(c, b) || !pools_ok(kp, vp)) return X100_EINVAL;
     const int64_t width = (int64_t)c->n_head * c->head_dim, most = (int64_t)1 << 40;
@@ -954,14 +964,13 @@ static int check_attn_paged(const x100_kv_cfg *c, const x100_kv_batch *b, const 
         ldq % 8 || ldo % 8)
         return X100_EINVAL;
     if (!(scale > 0.0f) || scale > 1e38f) return X100_EINVAL;   // times log2(e) it stays finite
-    return X100_OK;
+    return attn_paged_need(c, b, need) ? X100_OK : X100_EINVAL;
 }
 
 static int attn_paged(const x100_kv_cfg *c, const x100_kv_batch *b, const void *q, int64_t ldq, const void *kp,
                       const void *vp, float scale, void *out, int64_t ldo, void *ws, void *stream)
 {
     hipError_t e = x100_attn_paged_launch(*c, *b, q, ldq, kp, vp, scale, out, ldo, ws, (hipStream_t)stream);
-    if (e == hipErrorInvalidValue) return X100_EINVAL;
     if (e != hipSuccess) return hip_fail(e);
     return X100_OK;
 }
@@ -970,9 +979,9 @@ int x100_attn_paged_hip_ws(const x100_kv_cfg *c, const x100_kv_batch *b, const v
                            const void *v_pool, float scale, void *out, int64_t ldo, void *ws, size_t ws_bytes,
                            void *stream)
 {
-    int rc = check_attn_paged(c, b, q, ldq, k_pool, v_pool, scale, out, ldo);
+    size_t need = 0;
+    int rc = check_attn_paged(c, b, q, ldq, k_pool, v_pool, scale, out, ldo, &need);
     if (rc) return rc;
-    const size_t need = x100_attn_paged_workspace_bytes(c, b);
     if (need && (!ws || ((uintptr_t)ws & 255) || ws_bytes < need)) return X100_EINVAL;
     if (b->n_seq == 0 || b->n_rows == 0) return X100_OK;
     if ((rc = check_device())) return rc;
@@ -982,11 +991,11 @@ int x100_attn_paged_hip_ws(const x100_kv_cfg *c, const x100_kv_batch *b, const v
 int x100_attn_paged_hip(const x100_kv_cfg *c, const x100_kv_batch *b, const void *q, int64_t ldq, const void *k_pool,
                         const void *v_pool, float scale, void *out, int64_t ldo, void *stream)
 {
-    int rc = check_attn_paged(c, b, q, ldq, k_pool, v_pool, scale, out, ldo);
+    size_t need = 0;
+    int rc = check_attn_paged(c, b, q, ldq, k_pool, v_pool, scale, out, ldo, &need);
     if (rc) return rc;
     if (b->n_seq == 0 || b->n_rows == 0) return X100_OK;
     if ((rc = check_device())) return rc;
-    const size_t need = x100_attn_paged_workspace_bytes(c, b);
     void *ws = nullptr;
     if (need && (rc = stream_workspace((hipStream_t)stream, need, &ws))) return rc;
     return attn_paged(c, b, q, ldq, k_pool, v_pool, scale, out, ldo, ws, stream);

@@ -102,4 +102,5 @@ X100_DEV size_t tile_part(const PagedAttnArgs &a, int s, int kvh, int i)
 
 constexpr int PROMPT_ROWS = 256;      // rows (token, head) of a block of the prompt kernel
 constexpr int PROMPT_PAGES = 8192;    // most pages of a split there (their list is in LDS)
+int64_t x100_attn_prompt_blocks(const x100_kv_cfg &c, const x100_kv_batch &b, int splits);
 hipError_t x100_attn_prompt_launch(const PagedAttnArgs &a, hipStream_t s);

@@ -66,14 +66,14 @@ hipError_t x100_add_rmsnorm_i8_launch(int n_rows, int d, const x100_rows *x, con
                                       const float *weight, float eps, void *h, int64_t ldh, int8_t *q, float *scale,
                                       hipStream_t s);
 
-// Paged KV cache (paged.hip) and attention over it (attn_paged.hip).  ws holds
-// x100_attn_paged_workspace(c, b) bytes.
+// Paged KV cache (paged.hip) and attention over it (attn_paged.hip).  ws holds the bytes that
+// x100_attn_paged_workspace gives; a batch that it refuses is not launched.
 hipError_t x100_rope_table_launch(int head_dim, int n_pos, float base, float *table, hipStream_t s);
 hipError_t x100_kv_append_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const x100_kv_rows &r, void *kp,
                                  void *vp, void *q_out, hipStream_t s);
 hipError_t x100_kv_read_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const void *kp, const void *vp,
                                void *k_out, void *v_out, hipStream_t s);
-size_t x100_attn_paged_workspace(const x100_kv_cfg &c, const x100_kv_batch &b);
+bool x100_attn_paged_workspace(const x100_kv_cfg &c, const x100_kv_batch &b, size_t *bytes);   // false: past one launch
 hipError_t x100_attn_paged_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const void *q, int64_t ldq,
                                   const void *kp, const void *vp, float scale, void *out, int64_t ldo, void *ws,
                                   hipStream_t s);
