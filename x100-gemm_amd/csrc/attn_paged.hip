@@ -10,6 +10,11 @@
 // registers they were made in.  The cache keeps V in blocks of 8 positions per element for the same
 // reason: a lane's operand of V^T is one 16-byte load (16 bits) or one word (4 bits).
 //
+// The weights are rounded to 16 bits for the second product, which takes no more; their sum is of the rounded ones, so
+// that they still sum to one.  Against 64 bits the results' distance (2-norm, relative) grows from the result's own
+// rounding, 0.0016 in bf16 and 0.00021 in f16, to 0.0018-0.0021 and 0.00028.  A second product with what the rounding left
+// would cost single tokens nothing, but make a NaN of every infinity in V whose weight 16 bits hold exactly.
+//
 // Here: k_attn_tile for sequences of few rows (bound by the cache's bytes), k_attn_join, which merges split
 // results, and a call's layout.  attn_prompt.hip has the kernel of many rows (bound by the matrix cores).
 #include <algorithm>
@@ -37,16 +42,17 @@ template <int HD> struct TileRegs<HD, true> {
     bool ok;
 };
 
-// One block: 16 rows (token, head) of a sequence and KV head, one split of the positions; its NW waves
+// One block: 16 rows (token, head) of a sequence and KV head, one split of the positions; its four waves
 // take tiles of 32 positions in turn and merge at the end.
 // Lane (c = lane % 16, g = lane / 16): query row c; of a tile the positions 8 g .. 8 g + 7.
 // The loop is bound by memory as long as loads are always in flight: K and V of the next tile are requested
 // as soon as their registers are free, the pages come from a list in LDS.  63 sequences of 4096 positions, 32 heads on 4 of
 // 128, bf16: 91 us, 5.8 TB/s (a read of 2 GiB: 6.1); 16 of up to 60001 in 4 bits: 94 us, 4.8 TB/s, where unpacking
 // takes half of the issue slots.  One of 1024: 6.5 us, the chain of loads lengths -> pages -> K -> V.
-template <int HD, int AT, bool Q4, int NW> __global__ __launch_bounds__(64 * NW, Q4 || HD == 64 ? 4 : 3) void k_attn_tile(const AttnArgs a)
+template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256, Q4 || HD == 64 ? 4 : 3) void k_attn_tile(const AttnArgs a)
 {
     constexpr int MT = Q4 ? X100_T_F16 : AT;   // type on the matrix cores
+    constexpr int NW = 4;                      // waves
     constexpr int KS = HD / 32, NJ = HD / 16;  // steps of K Q^T, element tiles of V^T P^T
     __shared__ union {
         int pg[TILE_PAGES];                     // pages of the split, -1 where there is none
@@ -532,8 +538,8 @@ template <int HD, int AT> hipError_t attn_as(const AttnArgs &a, const Plan &p, h
     }
     if (p.tile.n) {
         const unsigned blocks = (unsigned)tile_blocks(p, a.c, a.b);
-        if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true, 4><<<blocks, 256, 0, s>>>(a);
-        else k_attn_tile<HD, AT, false, 4><<<blocks, 256, 0, s>>>(a);
+        if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true><<<blocks, 256, 0, s>>>(a);
+        else k_attn_tile<HD, AT, false><<<blocks, 256, 0, s>>>(a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

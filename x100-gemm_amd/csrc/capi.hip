@@ -1,6 +1,6 @@
 // C-ABI of libx100hip: argument checking, device state and the host-pointer convenience paths.
-// The kernels live in gemm_i8.hip, gemv_tile.hip, qgemv.hip, moe.hip, attn.hip, rows.hip, paged.hip and
-// attn_paged.hip.
+// The kernels live in gemm_i8.hip, gemv_tile.hip, qgemv.hip, moe.hip, attn.hip, rows.hip, paged.hip,
+// attn_paged.hip and attn_prompt.hip.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -51,8 +51,9 @@ template <> struct Mfma16<X100_T_BF16> {
     }
 };
 
-// The tile's power of two 2^-e that brings a row's largest element (in size) to 1 .. 2: bf16 queries
-// become fp16 that way without loss (elements below 2^-24 of the largest aside), whatever their size.
+// The row's power of two 2^-e that brings its largest element (in size) to 1 .. 2: bf16 queries become fp16 that way
+// whatever their size.  Exact for elements down to 2^-17 of the largest; below, fp16's numbers are multiples of 2^-24,
+// so that an element is off by 2^-25 of the largest at most, far less than a rounding of the largest to bf16.
 X100_DEV int row_exponent(float amax)
 {
     const int e = (int)(__float_as_uint(amax) >> 23) - 127;

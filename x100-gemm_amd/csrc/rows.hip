@@ -4,8 +4,8 @@
 // r = 1/sqrt(mean h^2 + eps) multiplies every t_i alike and cancels in the code, so the maximum and the
 // sum of squares come from the same single read of the row, and only the scale depends on the sum.
 // Bound by HBM: every input is read once into registers, every output written once.  16381 rows of 2048, bf16 with
-// an int32 delta: 62 us, 4.9 TB/s; 16384 rows of 4096, f16 without the norm: 39 us, 5.2 TB/s (a copy of 2 GiB: 5.0).
-// 64 rows: 3.6 us, a launch and two trips to memory.
+// an int32 delta: 59 us, 5.1 TB/s; 16384 rows of 4096, f16 without the norm: 39 us, 5.2 TB/s (a copy of 2 GiB: 5.0).
+// 64 rows: 3.7 us, a launch and two trips to memory.
 #include "rows_load.h"
 #include "x100_internal.h"
 
