@@ -16,8 +16,8 @@
  *   - A sequence whose entries break the bounds (q_start decreasing or outside 0 .. n_rows, more than
  *     max_q rows, kv_len < 0 or > max_kv) and rows at or behind q_start[n_seq]: nothing of them is
  *     stored, and their outputs are left as they were.  Where q_start decreases, accepted sequences may
- *     name the same rows: such a row, and any row behind the break, is taken for one of the sequences
- *     that name it, in parts for one and another, or left.
+ *     name the same rows: outputs of such rows, and of rows behind the break, may be of one of them, mixed
+ *     or left, and positions of accepted sequences may keep what they held; nothing else is touched.
  *   - A page number outside 0 .. n_pages - 1: nothing is stored there, its positions are not attended
  *     to, and they read as zeros.
  *   - Sequences may share pages that are only read; a page that gets new rows belongs to one sequence
@@ -98,7 +98,8 @@ int x100_rope_table_hip(int head_dim, int n_pos, float base, float *table, void 
 
 /* Head norms and rotation of q and k, rotated queries to q_out [n_rows][n_head * head_dim] (act_type),
  * keys and values into the pools at the rows' positions.  fp32 throughout (squares of the head norms
- * added by fours, then as a tree over neighbours), one rounding at the store (and the codes' for 4 bits). */
+ * added by fours, then as a tree over neighbours: heads with norms up to 1e18 in size; with eps = 0 a
+ * head of zeros gives 0 / 0, a NaN), one rounding at the store (and the codes' for 4 bits). */
 int x100_kv_append_hip(const x100_kv_cfg *cfg, const x100_kv_batch *batch, const x100_kv_rows *rows, void *k_pool,
                        void *v_pool, void *q_out, void *stream);
 

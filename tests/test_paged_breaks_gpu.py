@@ -120,3 +120,59 @@ def test_attention(dev, act, kv, q_start, n_rows, kv_len):
     assert left[~named].all()
     if all(a <= b for a, b in zip(q_start, q_start[1:])):
         assert not left[named].any()
+
+
+def broken(seed, n_seq, most, wrong):
+    """Lengths of 0 .. most rows, then `wrong` entries anywhere within the rows."""
+    g = np.random.default_rng(seed)
+    q = np.concatenate([[0], np.cumsum(g.integers(0, most + 1, n_seq))])
+    n_rows = int(q[-1]) + 1
+    q[g.integers(0, n_seq + 1, wrong)] = g.integers(0, n_rows + 1, wrong)
+    return [int(v) for v in q], n_rows, [int(v) for v in g.integers(0, 33, n_seq)]
+
+
+MANY = [broken(s, n, m, w) for s, n, m, w in ((1, 600, 3, 1), (2, 600, 2, 5), (3, 520, 3, 40), (4, 30, 40, 3), (5, 70, 20, 6))]
+
+
+@kinds
+@pytest.mark.parametrize("case", range(len(MANY)))
+def test_many_sequences(dev, act, kv, case):
+    """More sequences than the prompt kernel counts, and prompts without the kernel of few rows beside them."""
+    test_append_and_read_back(dev, act, kv, *MANY[case])
+    test_attention(dev, act, kv, *MANY[case])
+
+
+@kinds
+def test_a_graph_replayed_over_broken_arrays(dev, act, kv):
+    """The arrays break between replays and are put right again: sound replays give what they gave."""
+    s = setup([0, 40, 41, 60], 60, [32, 7, 32], act, kv)
+    rows, vals, keep = projections(s.g, 60, 4, 2, 64, ref.F32)
+    outs = [torch.zeros((60, w), dtype=TT[act], device=dev) for w in (256, 256, 128, 128)]
+    n = x.attn_paged_workspace_bytes(s.cfg, s.batch)
+    ws = torch.empty(max(n, 256), dtype=torch.uint8, device=dev)
+
+    def call():
+        q, o, k, v = (t.data_ptr() for t in outs)
+        x.kv_append(s.cfg, s.batch, x.KvRows(*rows), s.dk.data_ptr(), s.dv.data_ptr(), q, stream())
+        x.attn_paged_ws(s.cfg, s.batch, q, 256, s.dk.data_ptr(), s.dv.data_ptr(), 0.125, o, 256, ws.data_ptr(), n, stream())
+        x.kv_read(s.cfg, s.batch, s.dk.data_ptr(), s.dv.data_ptr(), k, v, stream())
+
+    call()
+    torch.cuda.synchronize()
+    want, pools = [t.clone() for t in outs], [s.dk.clone(), s.dv.clone()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    sound = s.d_qs.clone()
+    for bad in ([0, 40, 3, 60], [50, 10, 45, 60], [0, 70, 3, 8], [-5, 40, 1 << 30, 60]):
+        s.d_qs.copy_(torch.tensor(bad, dtype=torch.int32))
+        graph.replay()
+        s.d_qs.copy_(sound)
+        s.dk.copy_(pools[0])     # rows stored for accepted sequences, over their cached positions
+        s.dv.copy_(pools[1])
+        for t in outs:
+            t.fill_(-7)
+        graph.replay()
+        torch.cuda.synchronize()
+        for t, w in zip(outs, want):
+            assert torch.equal(t.view(torch.int16), w.view(torch.int16))
