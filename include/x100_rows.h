@@ -55,8 +55,8 @@ int x100_quant_i8_hip(int n_rows, int d, const x100_rows *x, int8_t *q, float *s
  * weight[d] and eps, as codes and scales:
  *   r = 1 / sqrt(mean(h^2) + eps),  t = h * weight,  scale = max|t| * r / 127.
  * x: F32, F16 or BF16; delta: any of the four types, or NULL for no addition (h is then not written
- * and may be NULL); n_rows and d as in quant_i8.  Squares are summed in fp64, so h of any size; eps >= 0, and a row of zeros has
- * scale 0 for eps = 0 too. */
+ * and may be NULL); n_rows and d as in quant_i8.  Squares are summed in fp64, so h of any size;
+ * eps >= 0, and a row of zeros has scale 0 for eps = 0 too. */
 int x100_add_rmsnorm_i8_hip(int n_rows, int d, const x100_rows *x, const x100_rows *delta, const float *weight,
                             float eps, void *h, int64_t ldh, int8_t *q, float *scale, void *stream);
 
