@@ -1,0 +1,67 @@
+/*
+ * x100_fp8.h -- 8-bit floating point with a scale per block of 128 (libx100hip, gfx950): rows to codes, the
+ * residual's addition with RMSNorm to codes, and the matrix product of such rows with such weights.
+ *
+ * No counterpart in the reference (its products are integer, x100_gemm.h).  Codes are e4m3 as in OCP's 8-bit formats
+ * (bias 7, largest value 448, 0x7f and 0xff NaN, no infinities).
+ *
+ *   rows     code (r, k) at byte r * ld + k, scale of (row r, block b of 128 elements) at b * ld_scale + r
+ *            (block-major: a tile's scales of one block are consecutive);
+ *   weights  code (n, k) at byte n * ld + k, one scale for 128 rows by 128 elements, (n / 128, b) at
+ *            (n / 128) * ld_scale + b, as checkpoints of this form have them.
+ * The last blocks of a row and of the rows may be short.
+ *
+ * All pointers are device pointers; asynchronous on stream (a hipStream_t as void *, NULL = the default
+ * stream); no workspace; capturable.  Every argument is checked before anything is enqueued.  Outputs overlap no
+ * input (but h, below).
+ */
+#ifndef X100_HIP_FP8_H
+#define X100_HIP_FP8_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include "x100_rows.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+typedef struct {
+    void *p;             /* codes                */
+    int64_t ld;          /* bytes of a row       */
+    float *scale;
+    int64_t ld_scale;
+} x100_fp8;
+
+/* Rows x (any of the four types of x100_rows.h) to codes and scales.  Per block: amax = max |x|,
+ * code = e4m3(x * f) to nearest (ties to even) with f = 448 * (1 / amax) in fp32, scale = amax / 448.  A block of zeros (or
+ * amax < 2^-100) has codes 0 and scale 0; one that holds an infinity or a NaN has codes 0 and scale NaN.
+ * Columns d .. 16 * ceil(d / 16) - 1 get code 0, so that the rows are an operand of x100_gemm_fp8_hip with
+ * K = 16 * ceil(d / 16).
+ * 1 <= d <= X100_ROWS_MAX_D, x->ld >= d, q->ld >= 16 * ceil(d / 16), q->ld_scale >= n_rows,
+ * 0 <= n_rows < 2^24 (2^22 for d > 4096). */
+int x100_quant_fp8_hip(int n_rows, int d, const x100_rows *x, const x100_fp8 *q, void *stream);
+
+/* h = x + delta, rounded to x's type and stored (h: row r at element r * ldh; h == x->p with ldh == x->ld updates in
+ * place), then RMSNorm of the stored h with weight [d] and eps, as codes and scales:
+ *   r = 1 / sqrt(mean(h^2) + eps), t = h * weight, code = e4m3(t * 448 (1 / amax)), scale = amax * r / 448
+ * with amax = max |t| of the block: the norm's factor goes into the scales alone.  Blocks as in quant_fp8; where h
+ * holds an infinity or a NaN, every scale of the row is NaN.
+ * x: F32, F16 or BF16; delta: any of the four types, or NULL for no addition (h is then not written and may be NULL);
+ * limits as in quant_fp8.  Squares are summed in fp64, so h of any size; eps >= 0. */
+int x100_add_rmsnorm_fp8_hip(int n_rows, int d, const x100_rows *x, const x100_rows *delta, const float *weight,
+                             float eps, void *h, int64_t ldh, const x100_fp8 *q, void *stream);
+
+/* C[m][n] = sum over blocks b of a_scale(m, b) * w_scale(n, b) * sum_{k in b} A[m][k] W[n][k]
+ * A: M rows, W: N weight rows, both of K elements; C: c_type (X100_T_F32, F16 or BF16), element m * ldc + n.
+ * Products and sums in fp32, one rounding at the store.  A NaN code or scale gives NaN where it is used.
+ * M, N >= 0; K >= 16, K % 16 == 0; a->p and w->p 16-byte aligned, a->ld and w->ld multiples of 16 and >= K;
+ * a->ld_scale >= M, w->ld_scale >= ceil(K / 128), ldc >= N; K and both ld <= 2^24; M * N / 256 < 2^31. */
+int x100_gemm_fp8_hip(int M, int N, int K, const x100_fp8 *a, const x100_fp8 *w, int c_type, void *c, int64_t ldc,
+                      void *stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

@@ -26,12 +26,6 @@ namespace {
 
 constexpr float NEG_INF = X100_NEG_INF;
 
-// 16 bytes per lane from sbase + voff to lds_base + 16 * lane; not counted by the compiler.
-X100_DEV void dma16s(uint32_t voff, const void *sbase, uint32_t lds_base)
-{
-    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(lds_base) : "memory");
-}
-
 // sum over the wave's lanes up to this one
 X100_DEV int prefix_sum(int v)
 {

@@ -1,5 +1,5 @@
 // C-ABI of libx100hip: argument checking, device state and the host-pointer convenience paths.
-// The kernels live in gemm_i8.hip, gemv_tile.hip, qgemv.hip, moe.hip, attn.hip, rows.hip, paged.hip,
+// The kernels live in gemm_i8.hip, gemm_fp8.hip, gemv_tile.hip, qgemv.hip, moe.hip, attn.hip, rows.hip, paged.hip,
 // attn_paged.hip and attn_prompt.hip.
 #include <hip/hip_runtime.h>
 
@@ -16,6 +16,7 @@
 // Only the extern "C" entry points are exported (the library is built with -fvisibility=hidden).
 #pragma GCC visibility push(default)
 #include "x100_decode.h"
+#include "x100_fp8.h"
 #include "x100_gemm.h"
 #include "x100_gemv_tile.h"
 #include "x100_gguf.h"
@@ -827,20 +828,82 @@ int x100_quant_i8_hip(int n_rows, int d, const x100_rows *x, int8_t *q, float *s
     return X100_OK;
 }
 
+// x, delta, weight, eps and h of the two forms with a norm.
+static bool norm_ok(int d, const x100_rows *x, const x100_rows *delta, const float *weight, float eps, const void *h, int64_t ldh)
+{
+    if (!rows_ok(x, d) || x->type == X100_T_I32) return false;
+    if (!weight || ((uintptr_t)weight & 3) || !(eps >= 0.0f) || std::isinf(eps)) return false;
+    if (delta && (!rows_ok(delta, d) || !h || (uintptr_t)h % type_bytes(x->type) || ldh < d ||
+                  ldh > ((int64_t)1 << 40)))
+        return false;
+    return !(delta && h == x->p && ldh != x->ld);   // in place: the rows as they lie
+}
+
 int x100_add_rmsnorm_i8_hip(int n_rows, int d, const x100_rows *x, const x100_rows *delta, const float *weight,
                             float eps, void *h, int64_t ldh, int8_t *q, float *scale, void *stream)
 {
-    if (!i8_out_ok(n_rows, d, q, scale) || !rows_ok(x, d) || x->type == X100_T_I32) return X100_EINVAL;
-    if (!weight || ((uintptr_t)weight & 3) || !(eps >= 0.0f) || std::isinf(eps)) return X100_EINVAL;
-    if (delta && (!rows_ok(delta, d) || !h || (uintptr_t)h % type_bytes(x->type) || ldh < d ||
-                  ldh > ((int64_t)1 << 40)))
-        return X100_EINVAL;
-    if (delta && h == x->p && ldh != x->ld) return X100_EINVAL;   // in place: the rows as they lie
+    if (!i8_out_ok(n_rows, d, q, scale) || !norm_ok(d, x, delta, weight, eps, h, ldh)) return X100_EINVAL;
     if (n_rows == 0) return X100_OK;
     int rc = check_device();
     if (rc) return rc;
     hipError_t e = x100_add_rmsnorm_i8_launch(n_rows, d, x, delta, weight, eps, h, ldh, q, scale, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(e);
+    return X100_OK;
+}
+
+// ---------------------------------------------------------------------------------------------
+// 8-bit floating point
+// ---------------------------------------------------------------------------------------------
+static const int64_t FP8_MAX_LD = (int64_t)1 << 40;
+
+static bool fp8_out_ok(int n_rows, int d, const x100_fp8 *q)
+{
+    if (!q || !i8_out_ok(n_rows, d, (const int8_t *)q->p, q->scale)) return false;
+    return q->ld >= (d + 15) / 16 * 16 && q->ld <= FP8_MAX_LD && q->ld_scale >= n_rows && q->ld_scale <= FP8_MAX_LD;
+}
+
+int x100_quant_fp8_hip(int n_rows, int d, const x100_rows *x, const x100_fp8 *q, void *stream)
+{
+    if (!fp8_out_ok(n_rows, d, q) || !rows_ok(x, d)) return X100_EINVAL;
+    if (n_rows == 0) return X100_OK;
+    int rc = check_device();
+    if (rc) return rc;
+    hipError_t e = x100_quant_fp8_launch(n_rows, d, x, q, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e);
+    return X100_OK;
+}
+
+int x100_add_rmsnorm_fp8_hip(int n_rows, int d, const x100_rows *x, const x100_rows *delta, const float *weight,
+                             float eps, void *h, int64_t ldh, const x100_fp8 *q, void *stream)
+{
+    if (!fp8_out_ok(n_rows, d, q) || !norm_ok(d, x, delta, weight, eps, h, ldh)) return X100_EINVAL;
+    if (n_rows == 0) return X100_OK;
+    int rc = check_device();
+    if (rc) return rc;
+    hipError_t e = x100_add_rmsnorm_fp8_launch(n_rows, d, x, delta, weight, eps, h, ldh, q, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e);
+    return X100_OK;
+}
+
+// An operand of the product: rows in whole, aligned 16-byte pieces, fp32 scales.
+static bool fp8_operand_ok(const x100_fp8 *x, int K, int64_t least_scales)
+{
+    if (!x || !x->p || ((uintptr_t)x->p & 15) || x->ld < K || x->ld % 16 || x->ld > 1 << 24) return false;
+    return x->scale && !((uintptr_t)x->scale & 3) && x->ld_scale >= least_scales && x->ld_scale <= FP8_MAX_LD;
+}
+
+int x100_gemm_fp8_hip(int M, int N, int K, const x100_fp8 *a, const x100_fp8 *w, int c_type, void *c, int64_t ldc,
+                      void *stream)
+{
+    if (M < 0 || N < 0 || K < 16 || K % 16 || K > 1 << 24 || (int64_t)M * N / 256 >= (int64_t)1 << 31) return X100_EINVAL;
+    if (!fp8_operand_ok(a, K, M) || !fp8_operand_ok(w, K, (K + 127) / 128)) return X100_EINVAL;
+    const int e = c_type == X100_T_I32 ? 0 : type_bytes(c_type);
+    if (!e || !c || (uintptr_t)c % e || ldc < N || ldc > FP8_MAX_LD) return X100_EINVAL;
+    if (M == 0 || N == 0) return X100_OK;
+    int rc = check_device();
+    if (rc) return rc;
+    hipError_t err = x100_gemm_fp8_launch(M, N, K, a, w, c_type, c, ldc, (hipStream_t)stream);
+    if (err != hipSuccess) return hip_fail(err);
     return X100_OK;
 }
 

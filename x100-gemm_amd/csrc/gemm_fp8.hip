@@ -1,0 +1,401 @@
+// C = A W^T in 8-bit floating point (e4m3) with a scale per block of 128 (x100_fp8.h).
+//
+//   C[m][n] = sum_b sa[b][m] sw[n / 128][b] sum_{k in b} A[m][k] W[n][k]
+//
+// The inner sum of a block is one matrix instruction for 16 x 16 outputs (16x16x128), started from zero; its result
+// times the two scales is added to the accumulators in fp32 on the vector unit.  W is the first operand, so that a lane
+// holds one row m of C (one sa per lane and block) and four consecutive columns.
+//
+// Both operands are rows of consecutive k, and a sum over k does not mind its order: lane group g of 4 takes the 16-byte
+// pieces g and g + 4 of the 128, the same in A and W, so that an operand is two plain 16-byte loads.
+// A last block of fewer than 128: A's pieces behind K are zeros, W's repeat the row's last piece (a NaN there makes
+// column n NaN anyway).  Rows behind M or N repeat the last one; their products are not stored.
+#include "rows_load.h"
+#include "x100_internal.h"
+
+namespace {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+
+// What a lane holds of a 16-row operand over 128 k, and the product of two from zero (W first).
+//   EXACT  as fp16 (every e4m3 number is one), four instructions: products and sums in fp32;
+//   else   as they are, one instruction at twice the rate.  It adds the products of 8 neighbouring k in fixed point, and
+//          cuts them below 2^-13 of the largest: with normal data 1.4e-5 of the result (2-norm), with codes of random
+//          exponents 4.8e-5; fp16 8e-8.  A result rounded to 16 bits is off by 2^-12 or 2^-9 itself.
+template <bool EXACT> struct Frag;
+template <> struct Frag<false> {
+    v4i x[2];
+    X100_DEV void set(int h, v4i v) { x[h] = v; }
+    static X100_DEV v4f mul(const Frag &w, const Frag &a)
+    {
+        const v8i wv = __builtin_shufflevector(w.x[0], w.x[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        const v8i av = __builtin_shufflevector(a.x[0], a.x[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, av, v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+    }
+};
+X100_DEV v8h fp8_to_half(int lo, int hi)
+{
+    const v2h a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+    const v2h c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+    return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+template <> struct Frag<true> {
+    v8h x[4];
+    X100_DEV void set(int h, v4i v)
+    {
+        x[2 * h] = fp8_to_half(v[0], v[1]);
+        x[2 * h + 1] = fp8_to_half(v[2], v[3]);
+    }
+    static X100_DEV v4f mul(const Frag &w, const Frag &a)
+    {
+        v4f d = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; i++) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.x[i], a.x[i], d, 0, 0, 0);
+        return d;
+    }
+};
+
+struct Fp8Args {
+    int M, N, K;
+    const uint8_t *a, *w;
+    uint32_t lda, ldw;
+    const float *as, *ws;
+    int64_t ld_as, ld_ws;
+    void *c;
+    int64_t ldc;
+    bool vec;   // four consecutive columns can be stored at once
+};
+
+// Columns n .. n + 3 of row m (m < M).
+template <int CT> X100_DEV void store_c4(const Fp8Args &g, int m, int n, v4f v)
+{
+    const size_t at = (size_t)m * g.ldc + n;
+    if (g.vec && n + 4 <= g.N) {
+        if constexpr (CT == X100_T_F32) *(v4f *)((float *)g.c + at) = v;
+        else *(v2u *)((uint16_t *)g.c + at) = v2u{f2act<CT>(v[0]) | f2act<CT>(v[1]) << 16, f2act<CT>(v[2]) | f2act<CT>(v[3]) << 16};
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (n + e < g.N) {
+            if constexpr (CT == X100_T_F32) ((float *)g.c)[at + e] = v[e];
+            else ((uint16_t *)g.c)[at + e] = (uint16_t)f2act<CT>(v[e]);
+        }
+}
+
+// Few rows: bound by W's bytes.  A wave has 16 columns and 16 FM rows and takes every WK-th block of k; the WK waves of a
+// tile are summed through LDS.  Operands go from memory to registers, U blocks of k at a time.
+template <int FM, int WK, int WN, int U, int CT> __global__ __launch_bounds__(64 * WK *WN) void k_fp8_rows(const Fp8Args g)
+{
+    __shared__ v4f part[WK > 1 ? (WK - 1) * WN * FM * 64 : 1];
+    const int lane = threadIdx.x & 63, w = wave_id(), wk = w % WK, wn = w / WK, r = lane & 15, q = lane >> 4;
+    const int n0 = (blockIdx.x * WN + wn) * 16, m0 = blockIdx.y * 16 * FM;
+    const int nb = (g.K + 127) >> 7, full = g.K >> 7;
+    const uint8_t *wp = g.w + (size_t)min(n0 + r, g.N - 1) * g.ldw + 16 * q;
+    const uint8_t *ap[FM];
+    const float *sa[FM];
+#pragma unroll
+    for (int i = 0; i < FM; i++) {
+        const int m = min(m0 + 16 * i + r, g.M - 1);
+        ap[i] = g.a + (size_t)m * g.lda + 16 * q;
+        sa[i] = g.as + m;
+    }
+    const float *sw = g.ws + (int64_t)(min(n0, g.N - 1) >> 7) * g.ld_ws;
+    v4f acc[FM];
+#pragma unroll
+    for (int i = 0; i < FM; i++) acc[i] = v4f{0, 0, 0, 0};
+
+    v4i wf[U][2], af[U][FM][2];
+    float s[U][FM], t[U];
+    auto load = [&](int u, int b) __attribute__((always_inline)) {
+        wf[u][0] = *(const v4i *)(wp + 128 * (size_t)b);
+        wf[u][1] = *(const v4i *)(wp + 128 * (size_t)b + 64);
+        t[u] = sw[b];
+#pragma unroll
+        for (int i = 0; i < FM; i++) {
+            af[u][i][0] = *(const v4i *)(ap[i] + 128 * (size_t)b);
+            af[u][i][1] = *(const v4i *)(ap[i] + 128 * (size_t)b + 64);
+            s[u][i] = sa[i][b * g.ld_as];
+        }
+    };
+    auto add = [&](int u) __attribute__((always_inline)) {
+        Frag<true> y;
+        y.set(0, wf[u][0]);
+        y.set(1, wf[u][1]);
+#pragma unroll
+        for (int i = 0; i < FM; i++) {
+            Frag<true> x;
+            x.set(0, af[u][i][0]);
+            x.set(1, af[u][i][1]);
+            const v4f d = Frag<true>::mul(y, x);
+            const float f = s[u][i] * t[u];
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[i][e] = __builtin_fmaf(d[e], f, acc[i][e]);
+        }
+    };
+    int b = wk;
+    for (; b + (U - 1) * WK < full; b += U * WK) {
+#pragma unroll
+        for (int u = 0; u < U; u++) load(u, b + u * WK);
+#pragma unroll
+        for (int u = 0; u < U; u++) add(u);
+    }
+    for (; b < full; b += WK) {
+        load(0, b);
+        add(0);
+    }
+    if (b < nb) {   // the short block
+        const int left = g.K - 128 * b;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int k = 16 * q + 64 * h, at = min(k, left - 16) - 16 * q;
+            wf[0][h] = *(const v4i *)(wp + 128 * (size_t)b + at);
+#pragma unroll
+            for (int i = 0; i < FM; i++) {
+                const v4i x = *(const v4i *)(ap[i] + 128 * (size_t)b + at);
+                af[0][i][h] = k < left ? x : v4i{0, 0, 0, 0};
+            }
+        }
+        t[0] = sw[b];
+#pragma unroll
+        for (int i = 0; i < FM; i++) s[0][i] = sa[i][b * g.ld_as];
+        add(0);
+    }
+    if constexpr (WK > 1) {
+        if (wk > 0) {
+#pragma unroll
+            for (int i = 0; i < FM; i++) part[(((wk - 1) * WN + wn) * FM + i) * 64 + lane] = acc[i];
+        }
+        __syncthreads();
+        if (wk > 0) return;
+#pragma unroll
+        for (int k = 0; k < WK - 1; k++)
+#pragma unroll
+            for (int i = 0; i < FM; i++) acc[i] += part[((k * WN + wn) * FM + i) * 64 + lane];
+    }
+#pragma unroll
+    for (int i = 0; i < FM; i++) {
+        const int m = m0 + 16 * i + r, n = n0 + 4 * q;
+        if (m < g.M && n < g.N) store_c4<CT>(g, m, n, acc[i]);
+    }
+}
+
+// Tiles: bound by the matrix cores.  WM x WN waves of 16 FM rows and 16 FN columns each; a stage is one block of k of the
+// tile's rows of A and W and its row scales, copied to LDS by DMA into a ring of NS slots.
+//   * Rows of a slot are 128 bytes; 16-byte piece c of row r lies at c ^ (r / 2 % 8), so that the 16 lanes that read one
+//     piece of 16 rows meet 16 different places of LDS.
+//   * W's operands of a stage stay in registers, A's come one ahead of their use.  A stage ends for a wave before its last
+//     A operand's products: the barrier, and the next stage's first reads, run beside them.
+//   * EXACT costs twice the matrix cores' time, and registers for 16-bit operands.
+X100_DEV int fp8_piece(int r, int c) { return c ^ ((r >> 1) & 7); }
+
+template <int FM, int FN, int WM, int WN, int NS, bool EXACT, int CT>
+__global__ __launch_bounds__(64 * WM *WN) void k_fp8_tile(const Fp8Args g, int tiles_m, int tiles_n)
+{
+    constexpr int NW = WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN;
+    constexpr int OA = BM / 8 / NW, OW = BN / 8 / NW, OPS = OA + OW + 1;   // DMA operations of a wave per stage
+    constexpr int WOFF = BM * 128, SOFF = (BM + BN) * 128, SLOT = SOFF + BM * 4;
+    static_assert(OA * NW * 8 == BM && OW * NW * 8 == BN && BM % 64 == 0 && 128 % (16 * FN) == 0 && NW % 2 == 0, "");
+    __shared__ __attribute__((aligned(256))) uint8_t smem[NS * SLOT];
+    const int lane = threadIdx.x & 63, w = wave_id(), wm = w / WN, wn = w % WN, r = lane & 15, q = lane >> 4;
+    int tm, tn;
+    tile_coords(blockIdx.x, gridDim.x, tiles_m, tiles_n, tm, tn);
+    const int m0 = tm * BM, n0 = tn * BN, nb = (g.K + 127) >> 7;
+    const uint32_t sb = lds_addr(smem);
+
+    // DMA: operation p of a wave has tile rows 8 (NW p + w) .. + 7, lane l row l / 8 of them and place l % 8.
+    const uint8_t *ga = g.a + (size_t)m0 * g.lda, *gw = g.w + (size_t)n0 * g.ldw;
+    uint32_t va[OA], vw[OW];
+#pragma unroll
+    for (int p = 0; p < OA; p++) {
+        const int t = 8 * (NW * p + w) + (lane >> 3);
+        va[p] = (uint32_t)min(t, g.M - 1 - m0) * g.lda + 16 * fp8_piece(t, lane & 7);
+    }
+#pragma unroll
+    for (int p = 0; p < OW; p++) {
+        const int t = 8 * (NW * p + w) + (lane >> 3);
+        vw[p] = (uint32_t)min(t, g.N - 1 - n0) * g.ldw + 16 * fp8_piece(t, lane & 7);
+    }
+    const int seg = w % (BM / 64);   // the wave's 64 row scales
+    const uint32_t vs = 4u * (uint32_t)min(64 * seg + lane, g.M - 1 - m0);
+    const float *gs = g.as + m0;
+    // Operation p of block b.  LAST: the last block, whose pieces behind K are the row's last one again (A's are zeros
+    // when they are read).
+    const int over = max(128 * (nb - 1) + 16 * fp8_piece(8 * w + (lane >> 3), lane & 7) - (g.K - 16), 0);
+    auto dma = [&](int b, uint32_t slot, int p, auto last_c) __attribute__((always_inline)) {
+        constexpr bool LAST = decltype(last_c)::value;   // 8 NW rows are whole turns of the pieces: one `over` for all p
+        if (p < OA)
+            dma16s(LAST ? va[p] - over : va[p], ga + (size_t)b * 128,
+                   __builtin_amdgcn_readfirstlane(sb + slot + 1024u * (uint32_t)(NW * p + w)));
+        else if (p < OA + OW)
+            dma16s(LAST ? vw[p - OA] - over : vw[p - OA], gw + (size_t)b * 128,
+                   __builtin_amdgcn_readfirstlane(sb + slot + WOFF + 1024u * (uint32_t)(NW * (p - OA) + w)));
+        else
+            dma4s(vs, gs + (int64_t)b * g.ld_as, __builtin_amdgcn_readfirstlane(sb + slot + SOFF + 256u * (uint32_t)seg));
+    };
+    // Operand reads.  Piece q + 4 of a row lies at q's place ^ 4.
+    const uint32_t ra = (uint32_t)(wm * FM * 16 + r) * 128 + 16 * fp8_piece(r, q);
+    const uint32_t rw = WOFF + (uint32_t)(wn * FN * 16 + r) * 128 + 16 * fp8_piece(r, q);
+    const uint32_t rs = SOFF + 4 * (uint32_t)(wm * FM * 16 + r);
+    const int left = g.K - 128 * (nb - 1);   // of the last block
+    auto frag_a = [&](Frag<EXACT> &f, uint32_t slot, int i, auto last_c) __attribute__((always_inline)) {
+        v4i x = *(const v4i *)(smem + (slot + ra) + 2048 * i), y = *(const v4i *)(smem + (slot + (ra ^ 64)) + 2048 * i);
+        if constexpr (decltype(last_c)::value) {
+            if (16 * q >= left) x = v4i{0, 0, 0, 0};
+            if (16 * q + 64 >= left) y = v4i{0, 0, 0, 0};
+        }
+        f.set(0, x);
+        f.set(1, y);
+    };
+    auto frag_w = [&](Frag<EXACT> &f, uint32_t slot, int j) __attribute__((always_inline)) {
+        f.set(0, *(const v4i *)(smem + (slot + rw) + 2048 * j));
+        f.set(1, *(const v4i *)(smem + (slot + (rw ^ 64)) + 2048 * j));
+    };
+    auto scale_a = [&](uint32_t slot, int i) __attribute__((always_inline)) { return *(const float *)(smem + (slot + rs) + 64 * i); };
+    const int nblk = min(n0 + wn * FN * 16, g.N - 1) >> 7;   // the wave's columns have one weight scale per block
+    // a constant to the kernel: loaded into scalar registers, beside the LDS reads
+    typedef __attribute__((address_space(4))) const float const_float;
+    const const_float *sw = (const const_float *)(uintptr_t)(g.ws + (int64_t)nblk * g.ld_ws);
+
+    v4f acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] = v4f{0, 0, 0, 0};
+
+    using yes = std::true_type;
+    using no = std::false_type;
+    auto dma_all = [&](int b, uint32_t slot, auto last_c) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < OPS; p++) dma(b, slot, p, last_c);
+    };
+#pragma unroll
+    for (int s = 0; s < NS - 1; s++) {
+        if (s < nb - 1) dma_all(s, s * SLOT, no{});
+        else if (s == nb - 1) dma_all(s, s * SLOT, yes{});
+    }
+    if (nb >= NS - 1) wait_vmcnt<(NS - 2) * OPS>();
+    else wait_vmcnt<0>();
+    lds_barrier();
+
+    Frag<EXACT> W[FN], A[2];
+    float sa[2];
+    uint32_t at = 0, to = (NS - 1) * SLOT;   // slots of this stage, and of the one that is copied
+#pragma unroll
+    for (int j = 0; j < FN; j++) frag_w(W[j], at, j);
+    if (nb > 1) frag_a(A[0], at, 0, no{});
+    else frag_a(A[0], at, 0, yes{});
+    sa[0] = scale_a(at, 0);
+    float t = sw[0];
+    // Block b.  COPY: block b + NS - 1 is copied (2: it is the last one); NEXT: another block follows (2: it is the last
+    // one).  No branch inside: the compiler would move the additions behind it, and the products with them.
+    auto stage = [&](int b, auto copy_c, auto next_c) __attribute__((always_inline)) {
+        constexpr int COPY = decltype(copy_c)::value, NEXT = decltype(next_c)::value;
+        using last = std::bool_constant<NEXT == 0>;
+        const uint32_t nx = at + SLOT == NS * SLOT ? 0 : at + SLOT;
+        float t1 = 0.0f;
+        if constexpr (NEXT > 0) t1 = sw[b + 1];
+        static_for<FM>([&](auto ic) __attribute__((always_inline)) {
+            constexpr int i = decltype(ic)::value, cur = i & 1;
+            if constexpr (COPY > 0) {
+#pragma unroll
+                for (int p = i * OPS / FM; p < (i + 1) * OPS / FM; p++)
+                    dma(b + NS - 1, to, p, std::bool_constant<COPY == 2>{});
+            }
+            if constexpr (i + 1 < FM) {
+                frag_a(A[cur ^ 1], at, i + 1, last{});
+                sa[cur ^ 1] = scale_a(at, i + 1);
+            } else if constexpr (NEXT > 0) {
+                if constexpr (COPY > 0) wait_vmcnt<(NS - 2) * OPS>();
+                else wait_vmcnt<0>();
+                lds_barrier();
+                frag_a(A[cur ^ 1], nx, 0, std::bool_constant<NEXT == 2>{});
+                sa[cur ^ 1] = scale_a(nx, 0);
+            }
+            const float f = sa[cur] * t;
+#pragma unroll
+            for (int j = 0; j < FN; j++) {
+                const v4f d = Frag<EXACT>::mul(W[j], A[cur]);
+                if constexpr (NEXT > 0 && i + 1 == FM) frag_w(W[j], nx, j);
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[i][j][e] = __builtin_fmaf(d[e], f, acc[i][j][e]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        if constexpr (FM & 1) {
+            A[0] = A[1];
+            sa[0] = sa[1];
+        }
+        t = t1;
+        at = nx;
+        to = to + SLOT == NS * SLOT ? 0 : to + SLOT;
+    };
+    using c0 = std::integral_constant<int, 0>;
+    using c1 = std::integral_constant<int, 1>;
+    using c2 = std::integral_constant<int, 2>;
+    int b = 0;
+    for (; b + NS < nb; b++) stage(b, c1{}, c1{});
+    if constexpr (NS == 2) {
+        if (b + 1 < nb) stage(b++, c2{}, c2{});
+    } else {
+        if (b + NS == nb) stage(b++, c2{}, c1{});
+        for (; b + 2 < nb; b++) stage(b, c0{}, c1{});
+        if (b + 1 < nb) stage(b++, c0{}, c2{});
+    }
+    stage(b, c0{}, c0{});
+    // the last additions here, not behind the stores' branches with the products kept until then
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) asm volatile("" : "+v"(acc[i][j]));
+
+#pragma unroll
+    for (int i = 0; i < FM; i++) {
+        const int m = m0 + wm * FM * 16 + 16 * i + r;
+#pragma unroll
+        for (int j = 0; j < FN; j++) {
+            const int n = n0 + wn * FN * 16 + 16 * j + 4 * q;
+            if (m < g.M && n < g.N) store_c4<CT>(g, m, n, acc[i][j]);
+        }
+    }
+}
+
+template <int FM, int FN, int WM, int WN, int NS, bool EXACT, int CT> hipError_t tile(const Fp8Args &g, hipStream_t s)
+{
+    constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN;
+    const int tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN;
+    k_fp8_tile<FM, FN, WM, WN, NS, EXACT, CT><<<tm * tn, 64 * WM * WN, 0, s>>>(g, tm, tn);
+    return hipGetLastError();
+}
+
+template <int CT> hipError_t gemm(const Fp8Args &g, hipStream_t s)
+{
+    constexpr bool EXACT = CT == X100_T_F32;
+    if (g.M <= 64) {
+        const dim3 grid((g.N + 15) / 16, (g.M + 15) / 16);
+        k_fp8_rows<1, 8, 1, 1, CT><<<grid, 512, 0, s>>>(g);
+        return hipGetLastError();
+    }
+    if constexpr (!EXACT) {
+        if (g.M > 512) return tile<8, 4, 2, 4, 2, false, CT>(g, s);
+    }
+    if (g.M > 128) return tile<4, 4, 2, 2, 2, EXACT, CT>(g, s);
+    return tile<2, 2, 2, 2, 4, EXACT, CT>(g, s);
+}
+
+}  // namespace
+
+hipError_t x100_gemm_fp8_launch(int M, int N, int K, const x100_fp8 *a, const x100_fp8 *w, int c_type, void *c,
+                                int64_t ldc, hipStream_t s)
+{
+    Fp8Args g = {M, N, K, (const uint8_t *)a->p, (const uint8_t *)w->p, (uint32_t)a->ld, (uint32_t)w->ld,
+                 a->scale, w->scale, a->ld_scale, w->ld_scale, c, ldc, false};
+    const int e = c_type == X100_T_F32 ? 4 : 2;
+    g.vec = (uintptr_t)c % (4 * e) == 0 && ldc % 4 == 0;
+    switch (c_type) {
+    case X100_T_F32: return gemm<X100_T_F32>(g, s);
+    case X100_T_F16: return gemm<X100_T_F16>(g, s);
+    case X100_T_BF16: return gemm<X100_T_BF16>(g, s);
+    }
+    return hipErrorInvalidValue;
+}

@@ -20,27 +20,6 @@
 
 namespace {
 
-// Tile order: blocks are dealt to the 8 XCDs round-robin, so block b runs on XCD b%8.  Give each
-// XCD a contiguous range of tile ids, and walk tile ids in groups of GROUP_M tile rows so the
-// tiles of one XCD share A row panels and B column panels in its L2.
-// EVEN: only where the ids divide evenly, else block order (k_gemm_mfma: C of few rows is written at a
-// higher rate in that order, 256 x 278640 x 144 107 -> 90 us).
-template <bool EVEN = false>
-X100_DEV void tile_coords(int bid, int nblk, int tiles_m, int tiles_n, int &tm, int &tn)
-{
-    const int x = bid & 7, q = nblk >> 3;
-    int t = x * q + min(x, nblk & 7) + (bid >> 3);
-    if (EVEN && (nblk & 7)) t = bid;
-    constexpr int GROUP_M = 4;
-    int per_group = GROUP_M * tiles_n;
-    int g = t / per_group;
-    int first_m = g * GROUP_M;
-    int gsize = min(tiles_m - first_m, GROUP_M);
-    int r = t - g * per_group;
-    tm = first_m + r % gsize;
-    tn = r / gsize;
-}
-
 // ------------------------------------------------------------------------------------------------
 // k_gemm_mfma: tiles of 64-k stages through registers into two LDS buffers (A in 16-byte chunks, B
 // transposed in registers into dwords of four consecutive k of one column).  Two (128x128) to five blocks
@@ -238,16 +217,6 @@ X100_DEV int big_b_chunk(int k, int c) { return c ^ (2 * (k & 7)); }
 //   chunk c -> granule 8*(r&1) + (c ^ ((r>>1)&7)).
 X100_DEV int big_a2_chunk(int r, int c) { return c ^ ((r >> 1) & 7); }
 
-// Global -> LDS DMA of 16 bytes per lane: a wave-uniform 64-bit base address plus a 32-bit per-lane
-// byte offset.  The LDS destination (wave-uniform) is passed in M0 through the "{m0}" operand, so
-// the compiler knows the register is written.
-X100_DEV void dma16s(uint32_t voff, const void *sbase, uint32_t lds_base)
-{
-    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(lds_base) : "memory");
-}
-
-template <int N> X100_DEV void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
-
 // Wait until at most n of this wave's vector-memory operations are outstanding.
 X100_DEV void wait_vmcnt_le(int n)
 {
@@ -263,8 +232,6 @@ X100_DEV void wait_vmcnt_le(int n)
     else if (n >= 4) wait_vmcnt<4>();
     else wait_vmcnt<0>();
 }
-
-X100_DEV void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // 16-byte global store of a finished C chunk with the system-scope policy bits (sc0 sc1): C is
 // written once and not read back by the kernel, and this form measured 69.5 -> 68.5 us at

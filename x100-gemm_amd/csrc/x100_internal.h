@@ -5,6 +5,7 @@
 
 #include "gemm_plan.h"
 #include "x100_decode.h"
+#include "x100_fp8.h"
 #include "x100_moe.h"
 #include "x100_paged.h"
 #include "x100_rows.h"
@@ -65,6 +66,14 @@ hipError_t x100_quant_i8_launch(int n_rows, int d, const x100_rows *x, int8_t *q
 hipError_t x100_add_rmsnorm_i8_launch(int n_rows, int d, const x100_rows *x, const x100_rows *delta,
                                       const float *weight, float eps, void *h, int64_t ldh, int8_t *q, float *scale,
                                       hipStream_t s);
+
+// 8-bit floating point (x100_fp8.h): rows (rows.hip), and the product (gemm_fp8.hip); arguments as checked.
+hipError_t x100_quant_fp8_launch(int n_rows, int d, const x100_rows *x, const x100_fp8 *q, hipStream_t s);
+hipError_t x100_add_rmsnorm_fp8_launch(int n_rows, int d, const x100_rows *x, const x100_rows *delta,
+                                       const float *weight, float eps, void *h, int64_t ldh, const x100_fp8 *q,
+                                       hipStream_t s);
+hipError_t x100_gemm_fp8_launch(int M, int N, int K, const x100_fp8 *a, const x100_fp8 *w, int c_type, void *c,
+                                int64_t ldc, hipStream_t s);
 
 // Paged KV cache (paged.hip) and attention over it (attn_paged.hip).  ws holds the bytes that
 // x100_attn_paged_workspace gives; a batch that it refuses is not launched.

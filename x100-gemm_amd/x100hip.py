@@ -16,6 +16,8 @@ Entry points and what they replace in the reference:
   x100_kv_append_hip / x100_attn_paged_hip      the attention of qwen_moe.c:284-292 for a batch of
                                                 sequences on a paged cache (x100_paged.h)
   x100_add_rmsnorm_i8_hip / x100_quant_i8_hip   no counterpart: rows of the int8 GEMM (x100_rows.h)
+  x100_gemm_fp8_hip (+ rows to fp8)             no counterpart: e4m3 products with a scale per block of
+                                                128 (x100_fp8.h)
 """
 import ctypes
 import os
@@ -32,7 +34,7 @@ X100_EIO, X100_EFORMAT, X100_ENOTFOUND, X100_ESCRATCH = -5, -6, -7, -8
 MOE_NOALLOC_MAX_BYTES = 8 << 20
 
 # Every symbol declared in include/x100_gemm.h, x100_gemv_tile.h, x100_qgemv.h, x100_moe.h,
-# x100_gguf.h, x100_decode.h, x100_rows.h, x100_paged.h.
+# x100_gguf.h, x100_decode.h, x100_rows.h, x100_paged.h, x100_fp8.h.
 EXPORTS = (
     "gemm_ime_i8", "gemm_hip_i8", "gemm_hip_i8_dev", "gemm_hip_i8_dev_set", "gemm_hip_i8_dev_variant",
     "x100_hip_detect", "x100_hip_caps_print", "x100_hip_strerror",
@@ -50,6 +52,7 @@ EXPORTS = (
     "x100_quant_i8_hip", "x100_add_rmsnorm_i8_hip",
     "x100_kv_pool_bytes", "x100_rope_table_hip", "x100_kv_append_hip", "x100_kv_read_hip",
     "x100_attn_paged_workspace_bytes", "x100_attn_paged_hip", "x100_attn_paged_hip_ws",
+    "x100_quant_fp8_hip", "x100_add_rmsnorm_fp8_hip", "x100_gemm_fp8_hip",
 )
 
 GEMM_AUTO, GEMM_TILE256, GEMM_TILE128, GEMM_SKINNY, GEMM_GENERIC, GEMM_TILE256_W4, GEMM_TILE64, GEMM_TILE32 = \
@@ -93,6 +96,11 @@ class Rows(ctypes.Structure):
     """x100_rows (x100_rows.h): device rows of one of four types, int32 with row and column scales."""
     _fields_ = [("type", ctypes.c_int), ("p", ctypes.c_void_p), ("ld", ctypes.c_int64),
                 ("row_scale", ctypes.c_void_p), ("col_scale", ctypes.c_void_p)]
+
+
+class Fp8(ctypes.Structure):
+    """x100_fp8 (x100_fp8.h): device codes and scales of rows or weights."""
+    _fields_ = [("p", ctypes.c_void_p), ("ld", ctypes.c_int64), ("scale", ctypes.c_void_p), ("ld_scale", ctypes.c_int64)]
 
 
 class KvCfg(ctypes.Structure):
@@ -206,9 +214,13 @@ def lib():
     L.x100_attn_paged_workspace_bytes.argtypes = [P(KvCfg), P(KvBatch)]
     L.x100_attn_paged_hip.argtypes = [P(KvCfg), P(KvBatch), p, i64_, p, p, f, p, i64_, p]
     L.x100_attn_paged_hip_ws.argtypes = [P(KvCfg), P(KvBatch), p, i64_, p, p, f, p, i64_, p, sz, p]
+    L.x100_quant_fp8_hip.argtypes = [i, i, P(Rows), P(Fp8), p]
+    L.x100_add_rmsnorm_fp8_hip.argtypes = [i, i, P(Rows), P(Rows), p, f, p, i64_, P(Fp8), p]
+    L.x100_gemm_fp8_hip.argtypes = [i, i, i, P(Fp8), P(Fp8), i, p, i64_, p]
     L.x100_kv_pool_bytes.restype = L.x100_attn_paged_workspace_bytes.restype = sz
     for name in ("x100_quant_i8_hip", "x100_add_rmsnorm_i8_hip", "x100_rope_table_hip", "x100_kv_append_hip",
-                 "x100_kv_read_hip", "x100_attn_paged_hip", "x100_attn_paged_hip_ws"):
+                 "x100_kv_read_hip", "x100_attn_paged_hip", "x100_attn_paged_hip_ws", "x100_quant_fp8_hip",
+                 "x100_add_rmsnorm_fp8_hip", "x100_gemm_fp8_hip"):
         getattr(L, name).restype = i
     for name in ("gemm_hip_i8", "gemm_hip_i8_dev", "gemm_hip_i8_dev_set", "gemm_hip_i8_dev_variant", "x100_hip_detect",
                  "x100q_pack", "qgemv_hip", "x100q_check_quant_div", "moe_layer_hip", "moe_layer_hip_ws", "moe_layer_hip_noalloc",
@@ -388,6 +400,23 @@ def add_rmsnorm_i8(n_rows, d, x, delta, d_weight, eps, d_h, ldh, d_q, d_scale, s
     """h = x + delta (delta None: h = x, not stored), then RMSNorm(h) as int8 codes and scales."""
     return _check("x100_add_rmsnorm_i8_hip", lib().x100_add_rmsnorm_i8_hip(n_rows, d, x, delta, d_weight, eps, d_h, ldh,
                                                                           d_q, d_scale, stream))
+
+
+# ---- 8-bit floating point (x100_fp8.h) --------------------------------------------------------------
+def quant_fp8(n_rows, d, rows, q, stream=None):
+    """e4m3 codes and a scale per 128 elements (q: Fp8) of rows (Rows)."""
+    return _check("x100_quant_fp8_hip", lib().x100_quant_fp8_hip(n_rows, d, rows, q, stream))
+
+
+def add_rmsnorm_fp8(n_rows, d, x, delta, d_weight, eps, d_h, ldh, q, stream=None):
+    """h = x + delta (delta None: h = x, not stored), then RMSNorm(h) as e4m3 codes and scales (q: Fp8)."""
+    return _check("x100_add_rmsnorm_fp8_hip", lib().x100_add_rmsnorm_fp8_hip(n_rows, d, x, delta, d_weight, eps, d_h, ldh,
+                                                                            q, stream))
+
+
+def gemm_fp8(M, N, K, a, w, c_type, d_c, ldc, stream=None):
+    """C [M][N] (c_type) = rows a (Fp8) times weight rows w (Fp8), a scale per block of 128."""
+    return _check("x100_gemm_fp8_hip", lib().x100_gemm_fp8_hip(M, N, K, a, w, c_type, d_c, ldc, stream))
 
 
 # ---- paged KV cache (x100_paged.h) ------------------------------------------------------------------
