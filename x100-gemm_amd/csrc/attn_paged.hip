@@ -15,8 +15,8 @@
 // rounding, 0.0016 in bf16 and 0.00021 in f16, to 0.0018-0.0021 and 0.00028.  A second product with what the rounding left
 // would cost single tokens nothing, but make a NaN of every infinity in V whose weight 16 bits hold exactly.
 //
-// Here: k_attn_tile for sequences of few rows (bound by the cache's bytes), k_attn_join, which merges split
-// results, and a call's layout.  attn_prompt.hip has the kernel of many rows (bound by the matrix cores).
+// Here: k_attn_tile for sequences of few rows (bound by the cache's bytes) and for rows with lists of blocks
+// (x100_sparse.h), k_attn_join, which merges split results, and a call's layout.  attn_prompt.hip has the kernel of many rows (bound by the matrix cores).
 #include <algorithm>
 
 #include "paged_attn.h"
@@ -49,7 +49,11 @@ template <int HD> struct TileRegs<HD, true> {
 // as soon as their registers are free, the pages come from a list in LDS.  63 sequences of 4096 positions, 32 heads on 4 of
 // 128, bf16: 91 us, 5.8 TB/s (a read of 2 GiB: 6.1); 16 of up to 60001 in 4 bits: 94 us, 4.8 TB/s, where unpacking
 // takes half of the issue slots.  One of 1024: 6.5 us, the chain of loads lengths -> pages -> K -> V.
-template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256, Q4 || HD == 64 ? 4 : 3) void k_attn_tile(const AttnArgs a)
+//
+// SP (x100_sparse.h): a tile is one token's rows, with a list of blocks of its own.  The list's pages in order are a
+// sequence to the rest of the kernel: its positions are counted through them, and only the last block can be the token's
+// own, of which the positions behind it are left out.
+template <int HD, int AT, bool Q4, bool SP> __global__ __launch_bounds__(256, Q4 || HD == 64 ? 4 : 3) void k_attn_tile(const AttnArgs a)
 {
     constexpr int MT = Q4 ? X100_T_F16 : AT;   // type on the matrix cores
     constexpr int NW = 4;                      // waves
@@ -60,40 +64,87 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256, Q4 || HD ==
     } sh;
     __shared__ float s_m[NW][16], s_l[NW][16];
     const int lane = threadIdx.x & 63, w = wave_id(), c = lane & 15, g = lane >> 4;
-    // Units (sequence, KV head, split) in runs of a.run, each run with all its tiles (plan_of)
-    const int n_kv = a.c.n_head_kv, unit = blockIdx.x / (a.run * a.tiles) * a.run + blockIdx.x % a.run;
-    const int tile = blockIdx.x / a.run % a.tiles;
-    const int sp = unit % a.tile.n, kvh = unit / a.tile.n % n_kv, s = unit / (a.tile.n * n_kv);
-    if (s >= a.b.n_seq) return;
-    const int G = a.c.n_head / n_kv, page = a.c.page, psh = __builtin_ctz(page);
-    const int i0 = tile * 16;
-    // A short table's pages are read here, beside the lengths; a long one's when the split is known.
-    const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
-    const int n_all = (a.b.max_kv + page - 1) >> psh;
-    const bool all = n_all <= TILE_PAGES;
-    auto list = [&](int first, int n) {
-        for (int i = threadIdx.x; i < n; i += 64 * NW) {
-            const int pg = tab[first + i];
-            sh.pg[i] = pg >= 0 && pg < a.c.n_pages ? pg : -1;
+    const int n_kv = a.c.n_head_kv, G = a.c.n_head / n_kv, page = a.c.page, psh = __builtin_ctz(page);
+    int sp, kvh, s, i0, row0, kv_len, n_rows, pos0, vis, ns, per, pg0;   // row0: token 0's row, pos0: its position
+    auto valid = [&](int pg) __attribute__((always_inline)) { return pg >= 0 && pg < a.c.n_pages ? pg : -1; };
+    if constexpr (SP) {
+        const int unit = blockIdx.x;
+        kvh = unit % n_kv;
+        sp = unit / n_kv % a.tile.n;
+        row0 = unit / (n_kv * a.tile.n);
+        i0 = 0;
+        n_rows = G;
+        s = paged_find(a.b, row0);
+        if (s >= a.b.n_seq) return;
+        const PagedSeq q = paged_seq(a.b, s);
+        if (!q.holds(row0)) return;
+        const int at = q.position(row0), own = at >> psh;   // below 0: no block
+        const int *list = a.sel + ((size_t)row0 * n_kv + kvh) * a.n_sel;
+        const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
+        // the list's pages, up to the first entry that breaks its order
+        __shared__ int s_cnt[NW], s_own[NW];
+        int end = a.n_sel, own_at = -1;
+        for (int i = threadIdx.x; i < a.n_sel; i += 64 * NW) {
+            const int e = list[i], before = i ? list[i - 1] : -1;
+            const bool ok = e > before && e >= 0 && e <= own;
+            if (!ok) end = min(end, i);
+            if (ok && e == own) own_at = i;
+            sh.pg[i] = ok ? valid(tab[e]) : -1;
         }
-    };
-    if (all) list(0, n_all);
-    const PagedSeq q = paged_seq(a.b, s);
-    const int n_rows = q.q_len * G;
-    if (i0 >= n_rows || n_rows > a.few) return;
-    const int pos0 = q.kv_len - q.q_len;                       // position of token 0
-    const int vis = pos0 + (min(i0 + 15, n_rows - 1)) / G + 1;  // positions that the tile's last row sees
-    const int per = a.tile.positions(q.kv_len);
-    const int ns = max(1, (vis + per - 1) / per);
-    if (sp >= ns) return;
+        end = -wave_max_iu(-end);
+        own_at = wave_max_iu(own_at);
+        if (lane == 0) {
+            s_cnt[w] = end;
+            s_own[w] = own_at;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < NW; k++) end = min(end, s_cnt[k]);
+        vis = end * page;
+#pragma unroll
+        for (int k = 0; k < NW; k++)   // only the last entry can be the own block: an entry is above all before it
+            if (s_own[k] >= 0 && s_own[k] == end - 1) vis = end * page - (page - 1 - (at & (page - 1)));
+        kv_len = vis;
+        pos0 = vis - 1;
+        per = a.tile.positions(a.n_sel << psh);
+        ns = a.tile.n;
+        pg0 = 0;
+    } else {
+        // Units (sequence, KV head, split) in runs of a.run, each run with all its tiles (plan_of)
+        const int unit = blockIdx.x / (a.run * a.tiles) * a.run + blockIdx.x % a.run, tile = blockIdx.x / a.run % a.tiles;
+        sp = unit % a.tile.n;
+        kvh = unit / a.tile.n % n_kv;
+        s = unit / (a.tile.n * n_kv);
+        if (s >= a.b.n_seq) return;
+        i0 = tile * 16;
+        // A short table's pages are read here, beside the lengths; a long one's when the split is known.
+        const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
+        const int n_all = (a.b.max_kv + page - 1) >> psh;
+        const bool all = n_all <= TILE_PAGES;
+        auto list = [&](int first, int n) {
+            for (int i = threadIdx.x; i < n; i += 64 * NW) sh.pg[i] = valid(tab[first + i]);
+        };
+        if (all) list(0, n_all);
+        const PagedSeq q = paged_seq(a.b, s);
+        row0 = q.q0;
+        kv_len = q.kv_len;
+        n_rows = q.q_len * G;
+        if (i0 >= n_rows || n_rows > a.few) return;
+        pos0 = kv_len - q.q_len;
+        vis = pos0 + (min(i0 + 15, n_rows - 1)) / G + 1;   // positions that the tile's last row sees
+        per = a.tile.positions(kv_len);
+        ns = max(1, (vis + per - 1) / per);
+        if (sp >= ns) return;
+        const int t0 = sp * per, t1 = min(t0 + per, vis);
+        pg0 = all ? 0 : t0 >> psh;                         // first page of the list
+        if (!all) list(pg0, t1 > t0 ? ((t1 - 1) >> psh) - (t0 >> psh) + 1 : 0);
+    }
     const int t0 = sp * per, t1 = min(t0 + per, vis);
-    const int pg0 = all ? 0 : t0 >> psh;                       // first page of the list
     const int n_pg = t1 > t0 ? ((t1 - 1) >> psh) - (t0 >> psh) + 1 : 0;
-    if (!all) list(pg0, n_pg);
 
-    const int i = min(i0 + c, n_rows - 1), tok = i / G, head = kvh * G + i % G;
+    const int i = min(i0 + c, n_rows - 1), tok = SP ? 0 : i / G, head = kvh * G + i % G;
     const int pos = pos0 + tok;
-    const int pos_lo = pos0 + i0 / G;                          // the tile's first row's
+    const int pos_lo = pos0 + (SP ? 0 : i0 / G);               // the tile's first row's
     const size_t head_bytes = page_head_bytes<HD, Q4>(page);
     // positions up to here are seen by every row, on pages that are
     __syncthreads();
@@ -162,7 +213,7 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256, Q4 || HD ==
     v4u qf[KS];
     float sc2 = a.scale2;
     {
-        const uint16_t *qr = a.q + (size_t)(q.q0 + tok) * a.ldq + (size_t)head * HD;
+        const uint16_t *qr = a.q + (size_t)(row0 + tok) * a.ldq + (size_t)head * HD;
 #pragma unroll
         for (int j = 0; j < KS; j++) qf[j] = *(const v4u *)(qr + (Q4 ? g * (HD / 4) + 8 * j : 32 * j + 8 * g));
         if constexpr (Q4 && AT == X100_T_BF16) {
@@ -271,7 +322,7 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256, Q4 || HD ==
         weights();
         // positions that no row of the sequence has, and those of a page that is none: V as zeros
         uint32_t keep[4];
-        const int n = R.ok ? q.kv_len - vb : 0;
+        const int n = R.ok ? kv_len - vb : 0;
 #pragma unroll
         for (int e = 0; e < 4; e++) keep[e] = n >= 2 * e + 2 ? ~0u : (n == 2 * e + 1 ? 0xffffu : 0u);
 #pragma unroll 1
@@ -373,13 +424,13 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256, Q4 || HD ==
             y0 = __builtin_fmaf(sh.o[k][r][el], f, y0);
             y1 = __builtin_fmaf(sh.o[k][r][el + 1], f, y1);
         }
-        const int tk = (i0 + r) / G, hh = kvh * G + (i0 + r) % G;
+        const int tk = SP ? 0 : (i0 + r) / G, hh = kvh * G + (i0 + r) % G;
         if (ns == 1) {
             const float f = ls == 0.0f ? 0.0f : 1.0f / ls;
             const uint32_t b = ls == 0.0f ? 0u : f2act<AT>(y0 * f) | f2act<AT>(y1 * f) << 16;
-            *(uint32_t *)(a.out + (size_t)(q.q0 + tk) * a.ldo + (size_t)hh * HD + el) = b;
+            *(uint32_t *)(a.out + (size_t)(row0 + tk) * a.ldo + (size_t)hh * HD + el) = b;
         } else {
-            const size_t at = tile_part(a, s, kvh, i0 + r) + sp;
+            const size_t at = (SP ? sparse_part(a, row0, kvh, r) : tile_part(a, s, kvh, i0 + r)) + sp;
             *(float2 *)(a.part_o + at * HD + el) = make_float2(y0, y1);
             if (el == 0) a.part_ml[at] = make_float2(mm, ls);
         }
@@ -389,27 +440,28 @@ template <int HD, int AT, bool Q4> __global__ __launch_bounds__(256, Q4 || HD ==
 // Merges the splits of rows that have more than one: HD / 4 lanes per (row, head), 4 elements each; x = row, or
 // (where only the tile kernel has splits) sequence and token, y = the heads of a block.  WIDE: the whole block takes
 // one head, its lane groups every 256 / (HD / 4)-th split (64 splits: 8 turns of dependent loads become one).
-template <int HD, int AT, bool WIDE> __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a)
+// SP: rows with lists, whose splits are all there.
+template <int HD, int AT, bool WIDE, bool SP> __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a)
 {
     constexpr int L = HD / 4, GR = 256 / L;
     __shared__ float4 s_o[WIDE ? GR : 1][L];
     __shared__ float s_l[WIDE ? GR : 1];
     const int G = a.c.n_head / a.c.n_head_kv, gr = threadIdx.x / L, l4 = threadIdx.x % L;
     const int head = WIDE ? blockIdx.y : blockIdx.y * GR + gr;
-    const bool rows = a.prompt.n > 1;
+    const bool rows = SP || a.prompt.n > 1;
     const int tokens = a.tile_rows / G;
     const int s = rows ? paged_find(a.b, blockIdx.x) : blockIdx.x / tokens;
     if (s >= a.b.n_seq) return;
     const PagedSeq q = paged_seq(a.b, s);
     const int row = rows ? blockIdx.x : q.q0 + blockIdx.x % tokens;
-    if (row < q.q0 || row - q.q0 >= q.q_len || (!rows && q.q_len * G > a.few)) return;
-    const int hd = min(head, a.c.n_head - 1), kvh = hd / G, i = (row - q.q0) * G + hd % G;
-    const bool few = q.q_len * G <= a.few;
+    if (!q.holds(row) || (!rows && q.q_len * G > a.few)) return;
+    const int hd = min(head, a.c.n_head - 1), kvh = hd / G, i = (SP ? 0 : row - q.q0) * G + hd % G;
+    const bool few = SP || q.q_len * G <= a.few;
     const int tr = few ? TILE_ROWS : PROMPT_ROWS, per = (few ? a.tile : a.prompt).positions(q.kv_len);
     const int vis = q.kv_len - q.q_len + min(i / tr * tr + tr - 1, q.q_len * G - 1) / G + 1;
-    const int ns = (vis + per - 1) / per;
+    const int ns = SP ? a.tile.n : (vis + per - 1) / per;
     if (ns <= 1 || head >= a.c.n_head) return;   // the lanes of a head together
-    const size_t at = few ? tile_part(a, s, kvh, i) : prompt_part(a, q.q0, kvh, i);
+    const size_t at = SP ? sparse_part(a, row, kvh, i) : few ? tile_part(a, s, kvh, i) : prompt_part(a, q.q0, kvh, i);
     const float2 *ml = a.part_ml + at;
     const float4 *po = (const float4 *)(a.part_o + at * HD) + l4;
     float m = NEG_INF;
@@ -538,20 +590,73 @@ template <int HD, int AT> hipError_t attn_as(const AttnArgs &a, const Plan &p, h
     }
     if (p.tile.n) {
         const unsigned blocks = (unsigned)tile_blocks(p, a.c, a.b);
-        if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true><<<blocks, 256, 0, s>>>(a);
-        else k_attn_tile<HD, AT, false><<<blocks, 256, 0, s>>>(a);
+        if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true, false><<<blocks, 256, 0, s>>>(a);
+        else k_attn_tile<HD, AT, false, false><<<blocks, 256, 0, s>>>(a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     if (p.tile.n <= 1 && p.prompt.n <= 1) return hipSuccess;
     constexpr int heads = 256 / (HD / 4);
     const unsigned rows = p.prompt.n > 1 ? a.b.n_rows : (unsigned)a.b.n_seq * (a.tile_rows / (a.c.n_head / a.c.n_head_kv));
-    if (p.tile.n > WIDE_SPLITS && p.prompt.n <= 1) k_attn_join<HD, AT, true><<<dim3(rows, a.c.n_head), 256, 0, s>>>(a);
-    else k_attn_join<HD, AT, false><<<dim3(rows, (a.c.n_head + heads - 1) / heads), 256, 0, s>>>(a);
+    if (p.tile.n > WIDE_SPLITS && p.prompt.n <= 1) k_attn_join<HD, AT, true, false><<<dim3(rows, a.c.n_head), 256, 0, s>>>(a);
+    else k_attn_join<HD, AT, false, false><<<dim3(rows, (a.c.n_head + heads - 1) / heads), 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+// Rows with lists: a block per row, KV head and split of the list, splits as for single tokens (their counts there).
+PagedSplit sparse_split(const x100_kv_cfg &c, const x100_kv_batch &b, int n_sel)
+{
+    const int64_t kv = (int64_t)n_sel * c.page, base = (int64_t)b.n_rows * c.n_head_kv;
+    const int64_t want = kv <= 512 ? 1 : std::max<int64_t>(1, (c.kv_type == X100_KV_Q4 ? 768 : 256) / base);
+    return {(int)std::min(want, (kv + 127) / 128), 128};
+}
+
+template <int HD, int AT> hipError_t sparse_as(const AttnArgs &a, hipStream_t s)
+{
+    const unsigned blocks = (unsigned)((int64_t)a.b.n_rows * a.c.n_head_kv * a.tile.n);
+    if (a.c.kv_type == X100_KV_Q4) k_attn_tile<HD, AT, true, true><<<blocks, 256, 0, s>>>(a);
+    else k_attn_tile<HD, AT, false, true><<<blocks, 256, 0, s>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.tile.n <= 1) return e;
+    constexpr int heads = 256 / (HD / 4);
+    if (a.tile.n > WIDE_SPLITS) k_attn_join<HD, AT, true, true><<<dim3(a.b.n_rows, a.c.n_head), 256, 0, s>>>(a);
+    else k_attn_join<HD, AT, false, true><<<dim3(a.b.n_rows, (a.c.n_head + heads - 1) / heads), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
 }  // namespace
+
+bool x100_attn_sparse_workspace(const x100_kv_cfg &c, const x100_kv_batch &b, int n_sel, size_t *bytes)
+{
+    const PagedSplit p = sparse_split(c, b, n_sel);
+    if ((int64_t)b.n_rows * c.n_head_kv * p.n >= 1 << 24) return false;
+    *bytes = p.n > 1 ? (size_t)b.n_rows * c.n_head * p.n * (c.head_dim + 2) * sizeof(float) : 0;
+    return true;
+}
+
+hipError_t x100_attn_sparse_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const void *q, int64_t ldq,
+                                   const void *kp, const void *vp, float scale, const int *sel, int n_sel, void *out,
+                                   int64_t ldo, void *ws, hipStream_t s)
+{
+    AttnArgs a = {};
+    a.c = c;
+    a.b = b;
+    a.q = (const uint16_t *)q;
+    a.ldq = ldq;
+    a.kp = (const uint8_t *)kp;
+    a.vp = (const uint8_t *)vp;
+    a.scale2 = scale * 1.4426950408889634f;
+    a.out = (uint16_t *)out;
+    a.ldo = ldo;
+    a.tile = sparse_split(c, b, n_sel);
+    a.tile_rows = c.n_head / c.n_head_kv;   // the join's rows of a token
+    a.part_o = (float *)ws;
+    a.part_ml = (float2 *)(a.part_o + (size_t)b.n_rows * c.n_head * a.tile.n * c.head_dim);
+    a.sel = sel;
+    a.n_sel = n_sel;
+    if (c.head_dim == 64) return c.act_type == X100_T_F16 ? sparse_as<64, X100_T_F16>(a, s) : sparse_as<64, X100_T_BF16>(a, s);
+    return c.act_type == X100_T_F16 ? sparse_as<128, X100_T_F16>(a, s) : sparse_as<128, X100_T_BF16>(a, s);
+}
 
 bool x100_attn_paged_workspace(const x100_kv_cfg &c, const x100_kv_batch &b, size_t *bytes)
 {

@@ -1,6 +1,6 @@
 // C-ABI of libx100hip: argument checking, device state and the host-pointer convenience paths.
 // The kernels live in gemm_i8.hip, gemm_fp8.hip, gemv_tile.hip, qgemv.hip, moe.hip, attn.hip, rows.hip, paged.hip,
-// attn_paged.hip and attn_prompt.hip.
+// attn_paged.hip, attn_prompt.hip and sparse.hip.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -24,6 +24,7 @@
 #include "x100_paged.h"
 #include "x100_qgemv.h"
 #include "x100_rows.h"
+#include "x100_sparse.h"
 #pragma GCC visibility pop
 #include "x100_internal.h"
 
@@ -1018,15 +1019,23 @@ size_t x100_attn_paged_workspace_bytes(const x100_kv_cfg *c, const x100_kv_batch
     return kv_cfg_ok(c) && kv_bounds_ok(c, b) && attn_paged_need(c, b, &need) ? need : 0;
 }
 
+// Rows of all query heads, in whole 16-byte pieces.
+static bool heads_ok(const x100_kv_cfg *c, const void *p, int64_t ld)
+{
+    return p && !((uintptr_t)p & 15) && ld >= (int64_t)c->n_head * c->head_dim && ld <= (int64_t)1 << 40 && ld % 8 == 0;
+}
+
+static bool attn_args_ok(const x100_kv_cfg *c, const x100_kv_batch *b, const void *q, int64_t ldq, const void *kp,
+                         const void *vp, float scale, const void *out, int64_t ldo)
+{
+    if (!kv_cfg_ok(c) || !kv_batch_ok(c, b) || !pools_ok(kp, vp) || !heads_ok(c, q, ldq) || !heads_ok(c, out, ldo)) return false;
+    return scale > 0.0f && scale <= 1e38f;   // times log2(e) it stays finite
+}
+
 static int check_attn_paged(const x100_kv_cfg *c, const x100_kv_batch *b, const void *q, int64_t ldq, const void *kp,
                             const void *vp, float scale, const void *out, int64_t ldo, size_t *need)
 {
-    if (!kv_cfg_ok(c) || !kv_batch_ok(c, b) || !pools_ok(kp, vp)) return X100_EINVAL;
-    const int64_t width = (int64_t)c->n_head * c->head_dim, most = (int64_t)1 << 40;
-    if (!q || !out || (((uintptr_t)q | (uintptr_t)out) & 15) || ldq < width || ldo < width || ldq > most || ldo > most ||
-        ldq % 8 || ldo % 8)
-        return X100_EINVAL;
-    if (!(scale > 0.0f) || scale > 1e38f) return X100_EINVAL;   // times log2(e) it stays finite
+    if (!attn_args_ok(c, b, q, ldq, kp, vp, scale, out, ldo)) return X100_EINVAL;
     return attn_paged_need(c, b, need) ? X100_OK : X100_EINVAL;
 }
 
@@ -1062,6 +1071,102 @@ int x100_attn_paged_hip(const x100_kv_cfg *c, const x100_kv_batch *b, const void
     void *ws = nullptr;
     if (need && (rc = stream_workspace((hipStream_t)stream, need, &ws))) return rc;
     return attn_paged(c, b, q, ldq, k_pool, v_pool, scale, out, ldo, ws, stream);
+}
+
+// ---------------------------------------------------------------------------------------------
+// sparse attention
+// ---------------------------------------------------------------------------------------------
+size_t x100_kv_means_bytes(const x100_kv_cfg *c)
+{
+    return kv_cfg_ok(c) ? (size_t)c->n_pages * c->n_head_kv * c->head_dim * 2 : 0;
+}
+
+int x100_kv_means_hip(const x100_kv_cfg *c, const x100_kv_batch *b, const void *k_pool, void *means, void *stream)
+{
+    if (!kv_cfg_ok(c) || !kv_batch_ok(c, b) || !k_pool || ((uintptr_t)k_pool & 255) || !means || ((uintptr_t)means & 15))
+        return X100_EINVAL;
+    if ((int64_t)b->n_rows * c->n_head_kv >= (int64_t)1 << 28) return X100_EINVAL;   // past one launch
+    if (b->n_seq == 0 || b->n_rows == 0) return X100_OK;
+    int rc = check_device();
+    if (rc) return rc;
+    hipError_t e = x100_kv_means_launch(*c, *b, k_pool, means, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e);
+    return X100_OK;
+}
+
+int x100_attn_select_hip(const x100_kv_cfg *c, const x100_kv_batch *b, const x100_kv_sel *pick, const void *q, int64_t ldq,
+                         const void *means, int *sel, void *stream)
+{
+    if (!kv_cfg_ok(c) || !kv_batch_ok(c, b) || !heads_ok(c, q, ldq) || !means || ((uintptr_t)means & 15) || !sel || ((uintptr_t)sel & 3))
+        return X100_EINVAL;
+    if (!pick || pick->n_sel < 1 || pick->n_sel > X100_SPARSE_MAX_SEL || pick->n_first < 0 || pick->n_last < 1 ||
+        pick->n_first > pick->n_sel - pick->n_last)
+        return X100_EINVAL;
+    if ((b->max_kv - 1) / c->page >= X100_SPARSE_MAX_BLOCKS || (int64_t)b->n_rows * c->n_head_kv >= 1 << 24) return X100_EINVAL;
+    if (b->n_seq == 0 || b->n_rows == 0) return X100_OK;
+    int rc = check_device();
+    if (rc) return rc;
+    hipError_t e = x100_attn_select_launch(*c, *b, *pick, q, ldq, means, sel, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e);
+    return X100_OK;
+}
+
+// Bytes of the workspace; false for lists of no length, or a batch that no launch holds.
+static bool attn_sparse_need(const x100_kv_cfg *c, const x100_kv_batch *b, int n_sel, size_t *need)
+{
+    *need = 0;
+    if (n_sel < 1 || n_sel > X100_SPARSE_MAX_SEL) return false;
+    if (b->n_seq == 0 || b->n_rows == 0) return true;
+    if (!x100_attn_sparse_workspace(*c, *b, n_sel, need)) return false;
+    *need = al256(*need);
+    return true;
+}
+
+size_t x100_attn_sparse_workspace_bytes(const x100_kv_cfg *c, const x100_kv_batch *b, int n_sel)
+{
+    size_t need = 0;
+    return kv_cfg_ok(c) && kv_bounds_ok(c, b) && attn_sparse_need(c, b, n_sel, &need) ? need : 0;
+}
+
+static int check_attn_sparse(const x100_kv_cfg *c, const x100_kv_batch *b, const void *q, int64_t ldq, const void *kp,
+                             const void *vp, float scale, const int *sel, int n_sel, const void *out, int64_t ldo, size_t *need)
+{
+    if (!attn_args_ok(c, b, q, ldq, kp, vp, scale, out, ldo) || !sel || ((uintptr_t)sel & 3)) return X100_EINVAL;
+    return attn_sparse_need(c, b, n_sel, need) ? X100_OK : X100_EINVAL;
+}
+
+static int attn_sparse(const x100_kv_cfg *c, const x100_kv_batch *b, const void *q, int64_t ldq, const void *kp,
+                       const void *vp, float scale, const int *sel, int n_sel, void *out, int64_t ldo, void *ws, void *stream)
+{
+    hipError_t e = x100_attn_sparse_launch(*c, *b, q, ldq, kp, vp, scale, sel, n_sel, out, ldo, ws, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e);
+    return X100_OK;
+}
+
+int x100_attn_sparse_hip_ws(const x100_kv_cfg *c, const x100_kv_batch *b, const void *q, int64_t ldq, const void *k_pool,
+                            const void *v_pool, float scale, const int *sel, int n_sel, void *out, int64_t ldo, void *ws,
+                            size_t ws_bytes, void *stream)
+{
+    size_t need = 0;
+    int rc = check_attn_sparse(c, b, q, ldq, k_pool, v_pool, scale, sel, n_sel, out, ldo, &need);
+    if (rc) return rc;
+    if (need && (!ws || ((uintptr_t)ws & 255) || ws_bytes < need)) return X100_EINVAL;
+    if (b->n_seq == 0 || b->n_rows == 0) return X100_OK;
+    if ((rc = check_device())) return rc;
+    return attn_sparse(c, b, q, ldq, k_pool, v_pool, scale, sel, n_sel, out, ldo, ws, stream);
+}
+
+int x100_attn_sparse_hip(const x100_kv_cfg *c, const x100_kv_batch *b, const void *q, int64_t ldq, const void *k_pool,
+                         const void *v_pool, float scale, const int *sel, int n_sel, void *out, int64_t ldo, void *stream)
+{
+    size_t need = 0;
+    int rc = check_attn_sparse(c, b, q, ldq, k_pool, v_pool, scale, sel, n_sel, out, ldo, &need);
+    if (rc) return rc;
+    if (b->n_seq == 0 || b->n_rows == 0) return X100_OK;
+    if ((rc = check_device())) return rc;
+    void *ws = nullptr;
+    if (need && (rc = stream_workspace((hipStream_t)stream, need, &ws))) return rc;
+    return attn_sparse(c, b, q, ldq, k_pool, v_pool, scale, sel, n_sel, out, ldo, ws, stream);
 }
 
 }  // extern "C"

@@ -35,6 +35,8 @@ struct PagedAttnArgs {
     size_t tile_at;      // the tile kernel's first split result
     int tile_rows, tiles;   // rows of a sequence there, and their tiles
     int run;             // units of a run of blocks there
+    const int *sel;      // sparse: lists of blocks [row][KV head][n_sel]
+    int n_sel;
 };
 
 template <int T> struct Mfma16;
@@ -99,6 +101,13 @@ X100_DEV size_t prompt_part(const PagedAttnArgs &a, int q0, int kvh, int i)
 X100_DEV size_t tile_part(const PagedAttnArgs &a, int s, int kvh, int i)
 {
     return a.tile_at + (((size_t)s * a.tile_rows + i) * a.c.n_head_kv + kvh) * a.tile.n;
+}
+
+// The same of a row with a list (sparse): by rows.
+X100_DEV size_t sparse_part(const PagedAttnArgs &a, int row, int kvh, int i)
+{
+    const int G = a.c.n_head / a.c.n_head_kv;
+    return (((size_t)row * G + i) * a.c.n_head_kv + kvh) * a.tile.n;
 }
 
 constexpr int PROMPT_ROWS = 256;      // rows (token, head) of a block of the prompt kernel

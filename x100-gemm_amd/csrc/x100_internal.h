@@ -9,6 +9,7 @@
 #include "x100_moe.h"
 #include "x100_paged.h"
 #include "x100_rows.h"
+#include "x100_sparse.h"
 
 // acc: C += A.B; otherwise the overwrite form C = A.B.
 hipError_t x100_gemm_i8_launch(int M, int N, int K, const int8_t *A, const int8_t *B, int32_t *C,
@@ -86,3 +87,12 @@ bool x100_attn_paged_workspace(const x100_kv_cfg &c, const x100_kv_batch &b, siz
 hipError_t x100_attn_paged_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const void *q, int64_t ldq,
                                   const void *kp, const void *vp, float scale, void *out, int64_t ldo, void *ws,
                                   hipStream_t s);
+
+// Sparse attention: block means and selection (sparse.hip), attention over lists of blocks (attn_paged.hip).
+hipError_t x100_kv_means_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const void *kp, void *means, hipStream_t s);
+hipError_t x100_attn_select_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const x100_kv_sel &pick, const void *q,
+                                   int64_t ldq, const void *means, int *sel, hipStream_t s);
+bool x100_attn_sparse_workspace(const x100_kv_cfg &c, const x100_kv_batch &b, int n_sel, size_t *bytes);   // false: past one launch
+hipError_t x100_attn_sparse_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const void *q, int64_t ldq,
+                                   const void *kp, const void *vp, float scale, const int *sel, int n_sel, void *out,
+                                   int64_t ldo, void *ws, hipStream_t s);

@@ -18,6 +18,8 @@ Entry points and what they replace in the reference:
   x100_add_rmsnorm_i8_hip / x100_quant_i8_hip   no counterpart: rows of the int8 GEMM (x100_rows.h)
   x100_gemm_fp8_hip (+ rows to fp8)             no counterpart: e4m3 products with a scale per block of
                                                 128 (x100_fp8.h)
+  x100_attn_select_hip / x100_attn_sparse_hip   no counterpart: attention over selected blocks of the
+                                                paged cache (x100_sparse.h)
 """
 import ctypes
 import os
@@ -34,7 +36,7 @@ X100_EIO, X100_EFORMAT, X100_ENOTFOUND, X100_ESCRATCH = -5, -6, -7, -8
 MOE_NOALLOC_MAX_BYTES = 8 << 20
 
 # Every symbol declared in include/x100_gemm.h, x100_gemv_tile.h, x100_qgemv.h, x100_moe.h,
-# x100_gguf.h, x100_decode.h, x100_rows.h, x100_paged.h, x100_fp8.h.
+# x100_gguf.h, x100_decode.h, x100_rows.h, x100_paged.h, x100_fp8.h, x100_sparse.h.
 EXPORTS = (
     "gemm_ime_i8", "gemm_hip_i8", "gemm_hip_i8_dev", "gemm_hip_i8_dev_set", "gemm_hip_i8_dev_variant",
     "x100_hip_detect", "x100_hip_caps_print", "x100_hip_strerror",
@@ -53,6 +55,8 @@ EXPORTS = (
     "x100_kv_pool_bytes", "x100_rope_table_hip", "x100_kv_append_hip", "x100_kv_read_hip",
     "x100_attn_paged_workspace_bytes", "x100_attn_paged_hip", "x100_attn_paged_hip_ws",
     "x100_quant_fp8_hip", "x100_add_rmsnorm_fp8_hip", "x100_gemm_fp8_hip",
+    "x100_kv_means_bytes", "x100_kv_means_hip", "x100_attn_select_hip", "x100_attn_sparse_workspace_bytes",
+    "x100_attn_sparse_hip", "x100_attn_sparse_hip_ws",
 )
 
 GEMM_AUTO, GEMM_TILE256, GEMM_TILE128, GEMM_SKINNY, GEMM_GENERIC, GEMM_TILE256_W4, GEMM_TILE64, GEMM_TILE32 = \
@@ -90,6 +94,7 @@ class LayerWeights(ctypes.Structure):
 # Element types of x100_rows.h (ggml type ids) and the 4-bit cache of x100_paged.h.
 T_F32, T_F16, T_I32, T_BF16, KV_Q4 = 0, 1, 26, 30, 256
 ROWS_MAX_D = 16384
+SPARSE_MAX_SEL, SPARSE_MAX_BLOCKS = 512, 16384
 
 
 class Rows(ctypes.Structure):
@@ -112,6 +117,11 @@ class KvBatch(ctypes.Structure):
     """x100_kv_batch (x100_paged.h): the arrays are device pointers."""
     _fields_ = [(n, ctypes.c_int) for n in ("n_seq", "n_rows", "max_q", "max_kv", "table_ld")] + \
                [(n, ctypes.c_void_p) for n in ("q_start", "kv_len", "block_table")]
+
+
+class KvSel(ctypes.Structure):
+    """x100_kv_sel (x100_sparse.h)."""
+    _fields_ = [(n, ctypes.c_int) for n in ("n_sel", "n_first", "n_last")]
 
 
 class KvRows(ctypes.Structure):
@@ -217,10 +227,19 @@ def lib():
     L.x100_quant_fp8_hip.argtypes = [i, i, P(Rows), P(Fp8), p]
     L.x100_add_rmsnorm_fp8_hip.argtypes = [i, i, P(Rows), P(Rows), p, f, p, i64_, P(Fp8), p]
     L.x100_gemm_fp8_hip.argtypes = [i, i, i, P(Fp8), P(Fp8), i, p, i64_, p]
-    L.x100_kv_pool_bytes.restype = L.x100_attn_paged_workspace_bytes.restype = sz
+    L.x100_kv_means_bytes.argtypes = [P(KvCfg)]
+    L.x100_kv_means_hip.argtypes = [P(KvCfg), P(KvBatch), p, p, p]
+    L.x100_attn_select_hip.argtypes = [P(KvCfg), P(KvBatch), P(KvSel), p, i64_, p, p, p]
+    L.x100_attn_sparse_workspace_bytes.argtypes = [P(KvCfg), P(KvBatch), i]
+    L.x100_attn_sparse_hip.argtypes = [P(KvCfg), P(KvBatch), p, i64_, p, p, f, p, i, p, i64_, p]
+    L.x100_attn_sparse_hip_ws.argtypes = [P(KvCfg), P(KvBatch), p, i64_, p, p, f, p, i, p, i64_, p, sz, p]
+    for name in ("x100_kv_pool_bytes", "x100_attn_paged_workspace_bytes", "x100_kv_means_bytes",
+                 "x100_attn_sparse_workspace_bytes"):
+        getattr(L, name).restype = sz
     for name in ("x100_quant_i8_hip", "x100_add_rmsnorm_i8_hip", "x100_rope_table_hip", "x100_kv_append_hip",
                  "x100_kv_read_hip", "x100_attn_paged_hip", "x100_attn_paged_hip_ws", "x100_quant_fp8_hip",
-                 "x100_add_rmsnorm_fp8_hip", "x100_gemm_fp8_hip"):
+                 "x100_add_rmsnorm_fp8_hip", "x100_gemm_fp8_hip", "x100_kv_means_hip", "x100_attn_select_hip",
+                 "x100_attn_sparse_hip", "x100_attn_sparse_hip_ws"):
         getattr(L, name).restype = i
     for name in ("gemm_hip_i8", "gemm_hip_i8_dev", "gemm_hip_i8_dev_set", "gemm_hip_i8_dev_variant", "x100_hip_detect",
                  "x100q_pack", "qgemv_hip", "x100q_check_quant_div", "moe_layer_hip", "moe_layer_hip_ws", "moe_layer_hip_noalloc",
@@ -452,3 +471,33 @@ def attn_paged(cfg, batch, d_q, ldq, d_k_pool, d_v_pool, scale, d_out, ldo, stre
 def attn_paged_ws(cfg, batch, d_q, ldq, d_k_pool, d_v_pool, scale, d_out, ldo, d_ws, ws_bytes, stream=None):
     return _check("x100_attn_paged_hip_ws", lib().x100_attn_paged_hip_ws(cfg, batch, d_q, ldq, d_k_pool, d_v_pool, scale,
                                                                         d_out, ldo, d_ws, ws_bytes, stream))
+
+
+# ---- sparse attention (x100_sparse.h) ---------------------------------------------------------------
+def kv_means_bytes(cfg):
+    return lib().x100_kv_means_bytes(cfg)
+
+
+def kv_means(cfg, batch, d_k_pool, d_means, stream=None):
+    """Mean keys of the pages that the batch's rows complete."""
+    return _check("x100_kv_means_hip", lib().x100_kv_means_hip(cfg, batch, d_k_pool, d_means, stream))
+
+
+def attn_select(cfg, batch, pick, d_q, ldq, d_means, d_sel, stream=None):
+    """The blocks [row][KV head][n_sel] that each row attends to (pick: KvSel)."""
+    return _check("x100_attn_select_hip", lib().x100_attn_select_hip(cfg, batch, pick, d_q, ldq, d_means, d_sel, stream))
+
+
+def attn_sparse_workspace_bytes(cfg, batch, n_sel):
+    return lib().x100_attn_sparse_workspace_bytes(cfg, batch, n_sel)
+
+
+def attn_sparse(cfg, batch, d_q, ldq, d_k_pool, d_v_pool, scale, d_sel, n_sel, d_out, ldo, stream=None):
+    """Attention of the batch's rows over the blocks of their lists (the library's workspace)."""
+    return _check("x100_attn_sparse_hip", lib().x100_attn_sparse_hip(cfg, batch, d_q, ldq, d_k_pool, d_v_pool, scale, d_sel,
+                                                                    n_sel, d_out, ldo, stream))
+
+
+def attn_sparse_ws(cfg, batch, d_q, ldq, d_k_pool, d_v_pool, scale, d_sel, n_sel, d_out, ldo, d_ws, ws_bytes, stream=None):
+    return _check("x100_attn_sparse_hip_ws", lib().x100_attn_sparse_hip_ws(cfg, batch, d_q, ldq, d_k_pool, d_v_pool, scale,
+                                                                          d_sel, n_sel, d_out, ldo, d_ws, ws_bytes, stream))
