@@ -63,7 +63,7 @@ struct Fp8Args {
     int64_t ld_as, ld_ws;
     void *c;
     int64_t ldc;
-    bool vec;   // four consecutive columns can be stored at once
+    bool vec, vec8;   // four, eight consecutive columns can be stored at once
 };
 
 // Columns n .. n + 3 of row m (m < M).
@@ -186,6 +186,10 @@ template <int FM, int WK, int WN, int U, int CT> __global__ __launch_bounds__(64
 //     piece of 16 rows meet 16 different places of LDS.
 //   * W's operands of a stage stay in registers, A's come one ahead of their use.  A stage ends for a wave before its last
 //     A operand's products: the barrier, and the next stage's first reads, run beside them.
+//   * A product is added two products later, so that the matrix cores never wait for the vector unit.
+//   * The copies of a stage are issued at its start: the later ones have least time before the barrier waits for them.
+//   * NS == 2 (K > 128): the block has tiles blockIdx, + grid, ... in one stream of stages: a tile's last stage copies the next
+//     one's first, and its results are stored beside the next one's products.
 //   * EXACT costs twice the matrix cores' time, and registers for 16-bit operands.
 X100_DEV int fp8_piece(int r, int c) { return c ^ ((r >> 1) & 7); }
 
@@ -195,30 +199,40 @@ __global__ __launch_bounds__(64 * WM *WN) void k_fp8_tile(const Fp8Args g, int t
     constexpr int NW = WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN;
     constexpr int OA = BM / 8 / NW, OW = BN / 8 / NW, OPS = OA + OW + 1;   // DMA operations of a wave per stage
     constexpr int WOFF = BM * 128, SOFF = (BM + BN) * 128, SLOT = SOFF + BM * 4;
-    static_assert(OA * NW * 8 == BM && OW * NW * 8 == BN && BM % 64 == 0 && 128 % (16 * FN) == 0 && NW % 2 == 0, "");
+    constexpr int HEAD = FM > 4 ? 3 : 1;   // A operands beside whose products they are issued
+    static_assert(OA * NW * 8 == BM && OW * NW * 8 == BN && BM % 64 == 0 && 128 % (16 * FN) == 0 && NW % 2 == 0 && FN % 2 == 0 &&
+                      FM % 2 == 0, "");
     __shared__ __attribute__((aligned(256))) uint8_t smem[NS * SLOT];
     const int lane = threadIdx.x & 63, w = wave_id(), wm = w / WN, wn = w % WN, r = lane & 15, q = lane >> 4;
-    int tm, tn;
-    tile_coords(blockIdx.x, gridDim.x, tiles_m, tiles_n, tm, tn);
-    const int m0 = tm * BM, n0 = tn * BN, nb = (g.K + 127) >> 7;
+    const int nb = (g.K + 127) >> 7, n_tiles = tiles_m * tiles_n;
     const uint32_t sb = lds_addr(smem);
 
     // DMA: operation p of a wave has tile rows 8 (NW p + w) .. + 7, lane l row l / 8 of them and place l % 8.
-    const uint8_t *ga = g.a + (size_t)m0 * g.lda, *gw = g.w + (size_t)n0 * g.ldw;
-    uint32_t va[OA], vw[OW];
-#pragma unroll
-    for (int p = 0; p < OA; p++) {
-        const int t = 8 * (NW * p + w) + (lane >> 3);
-        va[p] = (uint32_t)min(t, g.M - 1 - m0) * g.lda + 16 * fp8_piece(t, lane & 7);
-    }
-#pragma unroll
-    for (int p = 0; p < OW; p++) {
-        const int t = 8 * (NW * p + w) + (lane >> 3);
-        vw[p] = (uint32_t)min(t, g.N - 1 - n0) * g.ldw + 16 * fp8_piece(t, lane & 7);
-    }
     const int seg = w % (BM / 64);   // the wave's 64 row scales
-    const uint32_t vs = 4u * (uint32_t)min(64 * seg + lane, g.M - 1 - m0);
-    const float *gs = g.as + m0;
+    const uint8_t *ga, *gw;
+    const float *gs;
+    uint32_t va[OA], vw[OW], vs;
+    int m0, n0;
+    auto place = [&](int tile) __attribute__((always_inline)) {
+        int tm, tn;
+        tile_coords(tile, n_tiles, tiles_m, tiles_n, tm, tn);
+        m0 = tm * BM;
+        n0 = tn * BN;
+        ga = g.a + (size_t)m0 * g.lda;
+        gw = g.w + (size_t)n0 * g.ldw;
+        gs = g.as + m0;
+#pragma unroll
+        for (int p = 0; p < OA; p++) {
+            const int t = 8 * (NW * p + w) + (lane >> 3);
+            va[p] = (uint32_t)min(t, g.M - 1 - m0) * g.lda + 16 * fp8_piece(t, lane & 7);
+        }
+#pragma unroll
+        for (int p = 0; p < OW; p++) {
+            const int t = 8 * (NW * p + w) + (lane >> 3);
+            vw[p] = (uint32_t)min(t, g.N - 1 - n0) * g.ldw + 16 * fp8_piece(t, lane & 7);
+        }
+        vs = 4u * (uint32_t)min(64 * seg + lane, g.M - 1 - m0);
+    };
     // Operation p of block b.  LAST: the last block, whose pieces behind K are the row's last one again (A's are zeros
     // when they are read).
     const int over = max(128 * (nb - 1) + 16 * fp8_piece(8 * w + (lane >> 3), lane & 7) - (g.K - 16), 0);
@@ -252,27 +266,39 @@ __global__ __launch_bounds__(64 * WM *WN) void k_fp8_tile(const Fp8Args g, int t
         f.set(1, *(const v4i *)(smem + (slot + (rw ^ 64)) + 2048 * j));
     };
     auto scale_a = [&](uint32_t slot, int i) __attribute__((always_inline)) { return *(const float *)(smem + (slot + rs) + 64 * i); };
-    const int nblk = min(n0 + wn * FN * 16, g.N - 1) >> 7;   // the wave's columns have one weight scale per block
-    // a constant to the kernel: loaded into scalar registers, beside the LDS reads
+    // The wave's columns have one weight scale per block: a constant to the kernel, loaded into scalar registers.
     typedef __attribute__((address_space(4))) const float const_float;
-    const const_float *sw = (const const_float *)(uintptr_t)(g.ws + (int64_t)nblk * g.ld_ws);
+    auto scales_w = [&]() __attribute__((always_inline)) {
+        return (const const_float *)(uintptr_t)(g.ws + (int64_t)(min(n0 + wn * FN * 16, g.N - 1) >> 7) * g.ld_ws);
+    };
 
     v4f acc[FM][FN];
+    auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < FM; i++)
+        for (int i = 0; i < FM; i++)
 #pragma unroll
-        for (int j = 0; j < FN; j++) acc[i][j] = v4f{0, 0, 0, 0};
-
+            for (int j = 0; j < FN; j++) acc[i][j] = v4f{0, 0, 0, 0};
+    };
+    // The additions up to here are done here, not behind the next branch with the products kept until then.
+    auto hold = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < FM; i++)
+#pragma unroll
+            for (int j = 0; j < FN; j++) asm volatile("" : "+v"(acc[i][j]));
+        __builtin_amdgcn_sched_barrier(0);
+    };
     using yes = std::true_type;
     using no = std::false_type;
-    auto dma_all = [&](int b, uint32_t slot, auto last_c) __attribute__((always_inline)) {
-#pragma unroll
-        for (int p = 0; p < OPS; p++) dma(b, slot, p, last_c);
-    };
+    place(blockIdx.x);
 #pragma unroll
     for (int s = 0; s < NS - 1; s++) {
-        if (s < nb - 1) dma_all(s, s * SLOT, no{});
-        else if (s == nb - 1) dma_all(s, s * SLOT, yes{});
+        if (s < nb) {
+#pragma unroll
+            for (int p = 0; p < OPS; p++) {
+                if (s < nb - 1) dma(s, s * SLOT, p, no{});
+                else dma(s, s * SLOT, p, yes{});
+            }
+        }
     }
     if (nb >= NS - 1) wait_vmcnt<(NS - 2) * OPS>();
     else wait_vmcnt<0>();
@@ -286,77 +312,116 @@ __global__ __launch_bounds__(64 * WM *WN) void k_fp8_tile(const Fp8Args g, int t
     if (nb > 1) frag_a(A[0], at, 0, no{});
     else frag_a(A[0], at, 0, yes{});
     sa[0] = scale_a(at, 0);
+    const const_float *sw = scales_w();
     float t = sw[0];
-    // Block b.  COPY: block b + NS - 1 is copied (2: it is the last one); NEXT: another block follows (2: it is the last
-    // one).  No branch inside: the compiler would move the additions behind it, and the products with them.
-    auto stage = [&](int b, auto copy_c, auto next_c) __attribute__((always_inline)) {
+    clear();
+    // A stage.  COPY: block cb is copied (2: it is a tile's last one); NEXT: another stage follows, of weight scale t1 (2: of a
+    // tile's last block); LAST: this is one.  No branch inside: the compiler would move the additions behind it, and the
+    // products with them.
+    auto stage = [&](int cb, const const_float *next_sw, auto copy_c, auto next_c, auto last_c) __attribute__((always_inline)) {
         constexpr int COPY = decltype(copy_c)::value, NEXT = decltype(next_c)::value;
-        using last = std::bool_constant<NEXT == 0>;
         const uint32_t nx = at + SLOT == NS * SLOT ? 0 : at + SLOT;
-        float t1 = 0.0f;
-        if constexpr (NEXT > 0) t1 = sw[b + 1];
-        static_for<FM>([&](auto ic) __attribute__((always_inline)) {
-            constexpr int i = decltype(ic)::value, cur = i & 1;
-            if constexpr (COPY > 0) {
+        float t1 = 0.0f, f[2];
+        v4f d[3];
+        if constexpr (NEXT > 0) t1 = *next_sw;
+        static_for<FM * FN + 2>([&](auto kc) __attribute__((always_inline)) {
+            constexpr int k = decltype(kc)::value, i = k / FN, j = k % FN, cur = i & 1;
+            if constexpr (k < FM * FN && j == 0) {
+                if constexpr (COPY > 0) {
 #pragma unroll
-                for (int p = i * OPS / FM; p < (i + 1) * OPS / FM; p++)
-                    dma(b + NS - 1, to, p, std::bool_constant<COPY == 2>{});
+                    for (int p = i * OPS / HEAD; p < OPS && p < (i + 1) * OPS / HEAD; p++)
+                        dma(cb, to, p, std::bool_constant<COPY == 2>{});
+                }
+                if constexpr (i + 1 < FM) {
+                    frag_a(A[cur ^ 1], at, i + 1, last_c);
+                    sa[cur ^ 1] = scale_a(at, i + 1);
+                } else if constexpr (NEXT > 0) {
+                    if constexpr (COPY > 0) wait_vmcnt<(NS - 2) * OPS>();
+                    else wait_vmcnt<0>();
+                    lds_barrier();
+                    frag_a(A[cur ^ 1], nx, 0, std::bool_constant<NEXT == 2>{});
+                    sa[cur ^ 1] = scale_a(nx, 0);
+                }
+                f[cur] = sa[cur] * t;
             }
-            if constexpr (i + 1 < FM) {
-                frag_a(A[cur ^ 1], at, i + 1, last{});
-                sa[cur ^ 1] = scale_a(at, i + 1);
-            } else if constexpr (NEXT > 0) {
-                if constexpr (COPY > 0) wait_vmcnt<(NS - 2) * OPS>();
-                else wait_vmcnt<0>();
-                lds_barrier();
-                frag_a(A[cur ^ 1], nx, 0, std::bool_constant<NEXT == 2>{});
-                sa[cur ^ 1] = scale_a(nx, 0);
-            }
-            const float f = sa[cur] * t;
-#pragma unroll
-            for (int j = 0; j < FN; j++) {
-                const v4f d = Frag<EXACT>::mul(W[j], A[cur]);
+            if constexpr (k < FM * FN) {
+                d[k % 3] = Frag<EXACT>::mul(W[j], A[cur]);
                 if constexpr (NEXT > 0 && i + 1 == FM) frag_w(W[j], nx, j);
+            }
+            if constexpr (k >= 2) {
+                constexpr int l = k - 2, li = l / FN, lj = l % FN;
 #pragma unroll
-                for (int e = 0; e < 4; e++) acc[i][j][e] = __builtin_fmaf(d[e], f, acc[i][j][e]);
+                for (int e = 0; e < 4; e++) acc[li][lj][e] = __builtin_fmaf(d[l % 3][e], f[li & 1], acc[li][lj][e]);
             }
             __builtin_amdgcn_sched_barrier(0);
         });
-        if constexpr (FM & 1) {
-            A[0] = A[1];
-            sa[0] = sa[1];
-        }
         t = t1;
         at = nx;
         to = to + SLOT == NS * SLOT ? 0 : to + SLOT;
     };
+    // The tile's results from row sm, column sn.  16 bits: a lane has columns 4 q .. + 3 of its row of every product; lane
+    // groups of two neighbouring products exchange theirs, so that a lane has 8 consecutive columns of one.
+    auto store = [&](int sm, int sn) __attribute__((always_inline)) {
+        hold();
+        const int m = sm + wm * FM * 16 + r, n = sn + wn * FN * 16;
+        if (CT != X100_T_F32 && g.vec8 && n + 16 * FN <= g.N) {
+            uint16_t *row = (uint16_t *)g.c + (size_t)m * g.ldc + n + 16 * (q & 1) + 8 * (q >> 1);
+#pragma unroll
+            for (int i = 0; i < FM; i++) {
+#pragma unroll
+                for (int j = 0; j < FN; j += 2) {
+                    const v4f x = acc[i][j], y = acc[i][j + 1];
+                    uint32_t u[4];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        constexpr int T = CT == X100_T_F32 ? X100_T_F16 : CT;
+                        const auto z = __builtin_amdgcn_permlane16_swap(pack2<T>(x[2 * e], x[2 * e + 1]), pack2<T>(y[2 * e], y[2 * e + 1]), false, false);
+                        u[e] = z[0];
+                        u[2 + e] = z[1];
+                    }
+                    if (m + 16 * i < g.M) *(v4u *)(row + 16 * j) = v4u{u[0], u[1], u[2], u[3]};
+                }
+                row += 16 * g.ldc;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < FM; i++)
+#pragma unroll
+            for (int j = 0; j < FN; j++) {
+                if (m + 16 * i < g.M && n + 16 * j + 4 * q < g.N) store_c4<CT>(g, m + 16 * i, n + 16 * j + 4 * q, acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    };
     using c0 = std::integral_constant<int, 0>;
     using c1 = std::integral_constant<int, 1>;
     using c2 = std::integral_constant<int, 2>;
-    int b = 0;
-    for (; b + NS < nb; b++) stage(b, c1{}, c1{});
-    if constexpr (NS == 2) {
-        if (b + 1 < nb) stage(b++, c2{}, c2{});
-    } else {
-        if (b + NS == nb) stage(b++, c2{}, c1{});
-        for (; b + 2 < nb; b++) stage(b, c0{}, c1{});
-        if (b + 1 < nb) stage(b++, c0{}, c2{});
-    }
-    stage(b, c0{}, c0{});
-    // the last additions here, not behind the stores' branches with the products kept until then
-#pragma unroll
-    for (int i = 0; i < FM; i++)
-#pragma unroll
-        for (int j = 0; j < FN; j++) asm volatile("" : "+v"(acc[i][j]));
-
-#pragma unroll
-    for (int i = 0; i < FM; i++) {
-        const int m = m0 + wm * FM * 16 + 16 * i + r;
-#pragma unroll
-        for (int j = 0; j < FN; j++) {
-            const int n = n0 + wn * FN * 16 + 16 * j + 4 * q;
-            if (m < g.M && n < g.N) store_c4<CT>(g, m, n, acc[i][j]);
+    if constexpr (NS == 2) {   // nb > 1
+        for (int tile = blockIdx.x;;) {
+            for (int b = 0; b + 2 < nb; b++) stage(b + 1, sw + b + 1, c1{}, c1{}, no{});
+            stage(nb - 1, sw + nb - 1, c2{}, c2{}, no{});
+            hold();
+            const int sm = m0, sn = n0, next = tile + gridDim.x;
+            place(next < n_tiles ? next : tile);   // this one's first block again: nobody reads it
+            tile = next;
+            sw = scales_w();
+            stage(0, sw, c1{}, c1{}, yes{});
+            store(sm, sn);
+            if (tile >= n_tiles) return;
+            clear();
         }
+    } else {
+        int b = 0;
+        for (; b + NS < nb; b++) stage(b + NS - 1, sw + b + 1, c1{}, c1{}, no{});
+        if (b + NS == nb) {
+            stage(b + NS - 1, sw + b + 1, c2{}, c1{}, no{});
+            b++;
+        }
+        for (; b + 2 < nb; b++) stage(0, sw + b + 1, c0{}, c1{}, no{});
+        if (b + 1 < nb) stage(0, sw + b + 1, c0{}, c2{}, no{});
+        stage(0, sw, c0{}, c0{}, yes{});
+        store(m0, n0);
     }
 }
 
@@ -364,7 +429,9 @@ template <int FM, int FN, int WM, int WN, int NS, bool EXACT, int CT> hipError_t
 {
     constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN;
     const int tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN;
-    k_fp8_tile<FM, FN, WM, WN, NS, EXACT, CT><<<tm * tn, 64 * WM * WN, 0, s>>>(g, tm, tn);
+    // persistent blocks: one per CU (256 on eight XCDs, to which blocks go in turn: a block's tiles stay on its XCD)
+    const int blocks = NS == 2 ? (tm * tn < 256 ? tm * tn : 256) : tm * tn;
+    k_fp8_tile<FM, FN, WM, WN, NS, EXACT, CT><<<blocks, 64 * WM * WN, 0, s>>>(g, tm, tn);
     return hipGetLastError();
 }
 
@@ -377,9 +444,9 @@ template <int CT> hipError_t gemm(const Fp8Args &g, hipStream_t s)
         return hipGetLastError();
     }
     if constexpr (!EXACT) {
-        if (g.M > 512) return tile<8, 4, 2, 4, 2, false, CT>(g, s);
+        if (g.M > 512 && g.K > 128) return tile<8, 4, 2, 4, 2, false, CT>(g, s);
     }
-    if (g.M > 128) return tile<4, 4, 2, 2, 2, EXACT, CT>(g, s);
+    if (g.M > 128) return tile<4, 4, 2, 2, 3, EXACT, CT>(g, s);
     return tile<2, 2, 2, 2, 4, EXACT, CT>(g, s);
 }
 
@@ -389,9 +456,10 @@ hipError_t x100_gemm_fp8_launch(int M, int N, int K, const x100_fp8 *a, const x1
                                 int64_t ldc, hipStream_t s)
 {
     Fp8Args g = {M, N, K, (const uint8_t *)a->p, (const uint8_t *)w->p, (uint32_t)a->ld, (uint32_t)w->ld,
-                 a->scale, w->scale, a->ld_scale, w->ld_scale, c, ldc, false};
+                 a->scale, w->scale, a->ld_scale, w->ld_scale, c, ldc, false, false};
     const int e = c_type == X100_T_F32 ? 4 : 2;
     g.vec = (uintptr_t)c % (4 * e) == 0 && ldc % 4 == 0;
+    g.vec8 = (uintptr_t)c % (8 * e) == 0 && ldc % 8 == 0;
     switch (c_type) {
     case X100_T_F32: return gemm<X100_T_F32>(g, s);
     case X100_T_F16: return gemm<X100_T_F16>(g, s);

@@ -63,8 +63,6 @@ X100_DEV int row_exponent(float amax)
 }
 
 typedef float v16f __attribute__((ext_vector_type(16)));
-typedef float v2f __attribute__((ext_vector_type(2)));
-typedef __bf16 v2b __attribute__((ext_vector_type(2)));
 
 template <int T> X100_DEV v16f mfma32(v4u a, v4u b, v16f c)
 {
@@ -72,13 +70,6 @@ template <int T> X100_DEV v16f mfma32(v4u a, v4u b, v16f c)
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
-}
-// two fp32 to 16 bits each (nearest even), lo in the low half
-template <int T> X100_DEV uint32_t pack2(float lo, float hi)
-{
-    const v2f v = {lo, hi};
-    if constexpr (T == X100_T_F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, v2h));
-    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, v2b));
 }
 // c + the two 16-bit numbers of w
 template <int T> X100_DEV float add2(uint32_t w, float c)

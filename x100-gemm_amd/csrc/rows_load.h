@@ -7,6 +7,8 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef unsigned int v2u __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
 
 // by value: __builtin_bit_cast of a vector's element reads element 0
 X100_DEV v2h as_h2(uint32_t u) { return __builtin_bit_cast(v2h, u); }
@@ -23,6 +25,13 @@ template <int T> X100_DEV uint32_t f2act(float f)
 {
     if constexpr (T == X100_T_F16) return __builtin_bit_cast(uint16_t, f2h_rne(f));
     return __builtin_bit_cast(uint16_t, (__bf16)f);
+}
+// two fp32 to 16 bits each (nearest even), lo in the low half
+template <int T> X100_DEV uint32_t pack2(float lo, float hi)
+{
+    const v2f v = {lo, hi};
+    if constexpr (T == X100_T_F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, v2h));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, v2b));
 }
 template <int T> X100_DEV float act2f(uint32_t b)
 {
