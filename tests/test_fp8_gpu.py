@@ -166,6 +166,10 @@ GEMM = [(1, 1, 16), (1, 16, 128), (1, 5120, 2048), (3, 17, 48), (2, 130, 144), (
         (65, 127, 640), (100, 1000, 1008), (127, 129, 112), (128, 128, 128), (129, 255, 2064), (200, 384, 16), (255, 257, 384),
         (256, 256, 256), (257, 513, 2048), (333, 6144, 2048), (511, 640, 144), (600, 520, 1296), (1024, 1024, 512),
         (1000, 96, 4096), (2050, 70, 320), (40, 4000, 7168)]
+# every kind of tile, with a short last block, rows and columns that end inside a tile, and groups without a last block
+GEMM += [(33, 70, 1808), (18, 33, 656), (64, 4096, 656), (128, 5120, 656), (130, 5100, 400), (17, 64, 400), (300, 5120, 400),
+         (130, 5100, 272), (700, 5120, 400), (900, 5130, 1296), (1500, 5120, 400), (2300, 4400, 112), (2048, 5120, 144),
+         (2047, 5111, 656), (4100, 4300, 272), (5, 8208, 1040), (16, 9000, 144), (4, 8200, 272)]
 
 
 @pytest.mark.parametrize("ct", [ref.F32, ref.F16, ref.BF16])

@@ -83,54 +83,52 @@ template <int CT> X100_DEV void store_c4(const Fp8Args &g, int m, int n, v4f v)
         }
 }
 
-// Few rows: bound by W's bytes.  A wave has 16 columns and 16 FM rows and takes every WK-th block of k; the WK waves of a
-// tile are summed through LDS.  Operands go from memory to registers, U blocks of k at a time.
-template <int FM, int WK, int WN, int U, int CT> __global__ __launch_bounds__(64 * WK *WN) void k_fp8_rows(const Fp8Args g)
+// Few rows (M <= 16): bound by W's bytes.  A wave has 16 FN columns and takes every WK-th block of k; the WK waves of its columns
+// are summed through LDS.  Operands go from memory to registers, U blocks of k at a time, W's as it streams by and A's
+// out of the caches, once for FN of W's.
+template <int FN, int WK, int WN, int U, int CT> __global__ __launch_bounds__(64 * WK *WN) void k_fp8_rows(const Fp8Args g)
 {
-    __shared__ v4f part[WK > 1 ? (WK - 1) * WN * FM * 64 : 1];
+    __shared__ v4f part[WK > 1 ? (WK - 1) * WN * FN * 64 : 1];
     const int lane = threadIdx.x & 63, w = wave_id(), wk = w % WK, wn = w / WK, r = lane & 15, q = lane >> 4;
-    const int n0 = (blockIdx.x * WN + wn) * 16, m0 = blockIdx.y * 16 * FM;
+    const int n0 = (blockIdx.x * WN + wn) * 16 * FN, m = min(r, g.M - 1);
     const int nb = (g.K + 127) >> 7, full = g.K >> 7;
-    const uint8_t *wp = g.w + (size_t)min(n0 + r, g.N - 1) * g.ldw + 16 * q;
-    const uint8_t *ap[FM];
-    const float *sa[FM];
+    const uint8_t *ap = g.a + (size_t)m * g.lda + 16 * q, *wp[FN];
+    const float *sa = g.as + m, *sw[FN];
 #pragma unroll
-    for (int i = 0; i < FM; i++) {
-        const int m = min(m0 + 16 * i + r, g.M - 1);
-        ap[i] = g.a + (size_t)m * g.lda + 16 * q;
-        sa[i] = g.as + m;
+    for (int j = 0; j < FN; j++) {
+        wp[j] = g.w + (size_t)min(n0 + 16 * j + r, g.N - 1) * g.ldw + 16 * q;
+        sw[j] = g.ws + (int64_t)(min(n0 + 16 * j, g.N - 1) >> 7) * g.ld_ws;
     }
-    const float *sw = g.ws + (int64_t)(min(n0, g.N - 1) >> 7) * g.ld_ws;
-    v4f acc[FM];
+    v4f acc[FN];
 #pragma unroll
-    for (int i = 0; i < FM; i++) acc[i] = v4f{0, 0, 0, 0};
+    for (int j = 0; j < FN; j++) acc[j] = v4f{0, 0, 0, 0};
 
-    v4i wf[U][2], af[U][FM][2];
-    float s[U][FM], t[U];
+    v4i wf[U][FN][2], af[U][2];
+    float s[U], t[U][FN];
     auto load = [&](int u, int b) __attribute__((always_inline)) {
-        wf[u][0] = *(const v4i *)(wp + 128 * (size_t)b);
-        wf[u][1] = *(const v4i *)(wp + 128 * (size_t)b + 64);
-        t[u] = sw[b];
 #pragma unroll
-        for (int i = 0; i < FM; i++) {
-            af[u][i][0] = *(const v4i *)(ap[i] + 128 * (size_t)b);
-            af[u][i][1] = *(const v4i *)(ap[i] + 128 * (size_t)b + 64);
-            s[u][i] = sa[i][b * g.ld_as];
+        for (int j = 0; j < FN; j++) {
+            wf[u][j][0] = *(const v4i *)(wp[j] + 128 * (size_t)b);
+            wf[u][j][1] = *(const v4i *)(wp[j] + 128 * (size_t)b + 64);
+            t[u][j] = sw[j][b];
         }
+        af[u][0] = *(const v4i *)(ap + 128 * (size_t)b);
+        af[u][1] = *(const v4i *)(ap + 128 * (size_t)b + 64);
+        s[u] = sa[b * g.ld_as];
     };
     auto add = [&](int u) __attribute__((always_inline)) {
-        Frag<true> y;
-        y.set(0, wf[u][0]);
-        y.set(1, wf[u][1]);
+        Frag<true> x;
+        x.set(0, af[u][0]);
+        x.set(1, af[u][1]);
 #pragma unroll
-        for (int i = 0; i < FM; i++) {
-            Frag<true> x;
-            x.set(0, af[u][i][0]);
-            x.set(1, af[u][i][1]);
+        for (int j = 0; j < FN; j++) {
+            Frag<true> y;
+            y.set(0, wf[u][j][0]);
+            y.set(1, wf[u][j][1]);
             const v4f d = Frag<true>::mul(y, x);
-            const float f = s[u][i] * t[u];
+            const float f = s[u] * t[u][j];
 #pragma unroll
-            for (int e = 0; e < 4; e++) acc[i][e] = __builtin_fmaf(d[e], f, acc[i][e]);
+            for (int e = 0; e < 4; e++) acc[j][e] = __builtin_fmaf(d[e], f, acc[j][e]);
         }
     };
     int b = wk;
@@ -149,34 +147,32 @@ template <int FM, int WK, int WN, int U, int CT> __global__ __launch_bounds__(64
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const int k = 16 * q + 64 * h, at = min(k, left - 16) - 16 * q;
-            wf[0][h] = *(const v4i *)(wp + 128 * (size_t)b + at);
+            const v4i x = *(const v4i *)(ap + 128 * (size_t)b + at);
+            af[0][h] = k < left ? x : v4i{0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < FM; i++) {
-                const v4i x = *(const v4i *)(ap[i] + 128 * (size_t)b + at);
-                af[0][i][h] = k < left ? x : v4i{0, 0, 0, 0};
-            }
+            for (int j = 0; j < FN; j++) wf[0][j][h] = *(const v4i *)(wp[j] + 128 * (size_t)b + at);
         }
-        t[0] = sw[b];
+        s[0] = sa[b * g.ld_as];
 #pragma unroll
-        for (int i = 0; i < FM; i++) s[0][i] = sa[i][b * g.ld_as];
+        for (int j = 0; j < FN; j++) t[0][j] = sw[j][b];
         add(0);
     }
     if constexpr (WK > 1) {
         if (wk > 0) {
 #pragma unroll
-            for (int i = 0; i < FM; i++) part[(((wk - 1) * WN + wn) * FM + i) * 64 + lane] = acc[i];
+            for (int j = 0; j < FN; j++) part[(((wk - 1) * WN + wn) * FN + j) * 64 + lane] = acc[j];
         }
         __syncthreads();
         if (wk > 0) return;
 #pragma unroll
         for (int k = 0; k < WK - 1; k++)
 #pragma unroll
-            for (int i = 0; i < FM; i++) acc[i] += part[((k * WN + wn) * FM + i) * 64 + lane];
+            for (int j = 0; j < FN; j++) acc[j] += part[((k * WN + wn) * FN + j) * 64 + lane];
     }
 #pragma unroll
-    for (int i = 0; i < FM; i++) {
-        const int m = m0 + 16 * i + r, n = n0 + 4 * q;
-        if (m < g.M && n < g.N) store_c4<CT>(g, m, n, acc[i]);
+    for (int j = 0; j < FN; j++) {
+        const int n = n0 + 16 * j + 4 * q;
+        if (r < g.M && n < g.N) store_c4<CT>(g, r, n, acc[j]);
     }
 }
 
@@ -193,19 +189,25 @@ template <int FM, int WK, int WN, int U, int CT> __global__ __launch_bounds__(64
 //   * EXACT costs twice the matrix cores' time, and registers for 16-bit operands.
 X100_DEV int fp8_piece(int r, int c) { return c ^ ((r >> 1) & 7); }
 
-template <int FM, int FN, int WM, int WN, int NS, bool EXACT, int CT>
-__global__ __launch_bounds__(64 * WM *WN) void k_fp8_tile(const Fp8Args g, int tiles_m, int tiles_n)
+//   * WK > 1, few tiles: WK groups of such waves, each with a ring of its own, take the blocks of k in turn, and are summed
+//     through LDS in their order.
+template <int FM, int FN, int WM, int WN, int WK, int NS, bool EXACT, int CT>
+__global__ __launch_bounds__(64 * WM *WN *WK) void k_fp8_tile(const Fp8Args g, int tiles_m, int tiles_n)
 {
     constexpr int NW = WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN;
     constexpr int OA = BM / 8 / NW, OW = BN / 8 / NW, OPS = OA + OW + 1;   // DMA operations of a wave per stage
     constexpr int WOFF = BM * 128, SOFF = (BM + BN) * 128, SLOT = SOFF + BM * 4;
     constexpr int HEAD = FM > 4 ? 3 : 1;   // A operands beside whose products they are issued
     static_assert(OA * NW * 8 == BM && OW * NW * 8 == BN && BM % 64 == 0 && 128 % (16 * FN) == 0 && NW % 2 == 0 && FN % 2 == 0 &&
-                      FM % 2 == 0, "");
-    __shared__ __attribute__((aligned(256))) uint8_t smem[NS * SLOT];
-    const int lane = threadIdx.x & 63, w = wave_id(), wm = w / WN, wn = w % WN, r = lane & 15, q = lane >> 4;
-    const int nb = (g.K + 127) >> 7, n_tiles = tiles_m * tiles_n;
-    const uint32_t sb = lds_addr(smem);
+                      FM % 2 == 0 && (WK == 1 || NS > 2), "");
+    __shared__ __attribute__((aligned(256))) uint8_t smem[WK * NS * SLOT];
+    const int lane = threadIdx.x & 63, wk = wave_id() / NW, w = wave_id() % NW, wm = w / WN, wn = w % WN, r = lane & 15, q = lane >> 4;
+    // blocks of k, the group's stages, and the block of its last one (beyond the end: a group without one multiplies the
+    // last block by zeros)
+    const int n_blocks = (g.K + 127) >> 7, nb = (n_blocks + WK - 1) / WK, last_b = wk + WK * (nb - 1), n_tiles = tiles_m * tiles_n;
+    const bool idle = last_b >= n_blocks;
+    const uint8_t *const ring = smem + wk * NS * SLOT;
+    const uint32_t sb = lds_addr(ring);
 
     // DMA: operation p of a wave has tile rows 8 (NW p + w) .. + 7, lane l row l / 8 of them and place l % 8.
     const int seg = w % (BM / 64);   // the wave's 64 row scales
@@ -233,11 +235,12 @@ __global__ __launch_bounds__(64 * WM *WN) void k_fp8_tile(const Fp8Args g, int t
         }
         vs = 4u * (uint32_t)min(64 * seg + lane, g.M - 1 - m0);
     };
-    // Operation p of block b.  LAST: the last block, whose pieces behind K are the row's last one again (A's are zeros
+    // Operation p of stage s.  LAST: the last one, whose pieces behind K are the row's last one again (A's are zeros
     // when they are read).
-    const int over = max(128 * (nb - 1) + 16 * fp8_piece(8 * w + (lane >> 3), lane & 7) - (g.K - 16), 0);
-    auto dma = [&](int b, uint32_t slot, int p, auto last_c) __attribute__((always_inline)) {
+    const int over = max(128 * min(last_b, n_blocks - 1) + 16 * fp8_piece(8 * w + (lane >> 3), lane & 7) - (g.K - 16), 0);
+    auto dma = [&](int s, uint32_t slot, int p, auto last_c) __attribute__((always_inline)) {
         constexpr bool LAST = decltype(last_c)::value;   // 8 NW rows are whole turns of the pieces: one `over` for all p
+        const int b = LAST && WK > 1 ? min(last_b, n_blocks - 1) : wk + WK * s;
         if (p < OA)
             dma16s(LAST ? va[p] - over : va[p], ga + (size_t)b * 128,
                    __builtin_amdgcn_readfirstlane(sb + slot + 1024u * (uint32_t)(NW * p + w)));
@@ -251,9 +254,9 @@ __global__ __launch_bounds__(64 * WM *WN) void k_fp8_tile(const Fp8Args g, int t
     const uint32_t ra = (uint32_t)(wm * FM * 16 + r) * 128 + 16 * fp8_piece(r, q);
     const uint32_t rw = WOFF + (uint32_t)(wn * FN * 16 + r) * 128 + 16 * fp8_piece(r, q);
     const uint32_t rs = SOFF + 4 * (uint32_t)(wm * FM * 16 + r);
-    const int left = g.K - 128 * (nb - 1);   // of the last block
+    const int left = idle ? 0 : g.K - 128 * last_b;   // of the last block
     auto frag_a = [&](Frag<EXACT> &f, uint32_t slot, int i, auto last_c) __attribute__((always_inline)) {
-        v4i x = *(const v4i *)(smem + (slot + ra) + 2048 * i), y = *(const v4i *)(smem + (slot + (ra ^ 64)) + 2048 * i);
+        v4i x = *(const v4i *)(ring + (slot + ra) + 2048 * i), y = *(const v4i *)(ring + (slot + (ra ^ 64)) + 2048 * i);
         if constexpr (decltype(last_c)::value) {
             if (16 * q >= left) x = v4i{0, 0, 0, 0};
             if (16 * q + 64 >= left) y = v4i{0, 0, 0, 0};
@@ -262,15 +265,16 @@ __global__ __launch_bounds__(64 * WM *WN) void k_fp8_tile(const Fp8Args g, int t
         f.set(1, y);
     };
     auto frag_w = [&](Frag<EXACT> &f, uint32_t slot, int j) __attribute__((always_inline)) {
-        f.set(0, *(const v4i *)(smem + (slot + rw) + 2048 * j));
-        f.set(1, *(const v4i *)(smem + (slot + (rw ^ 64)) + 2048 * j));
+        f.set(0, *(const v4i *)(ring + (slot + rw) + 2048 * j));
+        f.set(1, *(const v4i *)(ring + (slot + (rw ^ 64)) + 2048 * j));
     };
-    auto scale_a = [&](uint32_t slot, int i) __attribute__((always_inline)) { return *(const float *)(smem + (slot + rs) + 64 * i); };
+    auto scale_a = [&](uint32_t slot, int i) __attribute__((always_inline)) { return *(const float *)(ring + (slot + rs) + 64 * i); };
     // The wave's columns have one weight scale per block: a constant to the kernel, loaded into scalar registers.
     typedef __attribute__((address_space(4))) const float const_float;
     auto scales_w = [&]() __attribute__((always_inline)) {
         return (const const_float *)(uintptr_t)(g.ws + (int64_t)(min(n0 + wn * FN * 16, g.N - 1) >> 7) * g.ld_ws);
     };
+    auto block = [&](int s) __attribute__((always_inline)) { return min(wk + WK * s, n_blocks - 1); };
 
     v4f acc[FM][FN];
     auto clear = [&]() __attribute__((always_inline)) {
@@ -313,7 +317,7 @@ __global__ __launch_bounds__(64 * WM *WN) void k_fp8_tile(const Fp8Args g, int t
     else frag_a(A[0], at, 0, yes{});
     sa[0] = scale_a(at, 0);
     const const_float *sw = scales_w();
-    float t = sw[0];
+    float t = sw[block(0)];
     clear();
     // A stage.  COPY: block cb is copied (2: it is a tile's last one); NEXT: another stage follows, of weight scale t1 (2: of a
     // tile's last block); LAST: this is one.  No branch inside: the compiler would move the additions behind it, and the
@@ -343,6 +347,7 @@ __global__ __launch_bounds__(64 * WM *WN) void k_fp8_tile(const Fp8Args g, int t
                     sa[cur ^ 1] = scale_a(nx, 0);
                 }
                 f[cur] = sa[cur] * t;
+                if (WK > 1 && decltype(last_c)::value && idle) f[cur] = 0.0f;
             }
             if constexpr (k < FM * FN) {
                 d[k % 3] = Frag<EXACT>::mul(W[j], A[cur]);
@@ -412,42 +417,105 @@ __global__ __launch_bounds__(64 * WM *WN) void k_fp8_tile(const Fp8Args g, int t
             clear();
         }
     } else {
-        int b = 0;
-        for (; b + NS < nb; b++) stage(b + NS - 1, sw + b + 1, c1{}, c1{}, no{});
-        if (b + NS == nb) {
-            stage(b + NS - 1, sw + b + 1, c2{}, c1{}, no{});
-            b++;
+        int s = 0;
+        for (; s + NS < nb; s++) stage(s + NS - 1, sw + block(s + 1), c1{}, c1{}, no{});
+        if (s + NS == nb) {
+            stage(s + NS - 1, sw + block(s + 1), c2{}, c1{}, no{});
+            s++;
         }
-        for (; b + 2 < nb; b++) stage(0, sw + b + 1, c0{}, c1{}, no{});
-        if (b + 1 < nb) stage(0, sw + b + 1, c0{}, c2{}, no{});
+        for (; s + 2 < nb; s++) stage(0, sw + block(s + 1), c0{}, c1{}, no{});
+        if (s + 1 < nb) stage(0, sw + block(s + 1), c0{}, c2{}, no{});
         stage(0, sw, c0{}, c0{}, yes{});
+        if constexpr (WK > 1) {   // no copy is on its way
+            hold();
+            lds_barrier();
+            v4f *part = (v4f *)smem + (w * FM * FN) * 64 + lane;
+            static_assert((WK - 1) * NW * FM * FN * 1024 <= WK * NS * SLOT, "");
+            if (wk > 0) {
+#pragma unroll
+                for (int i = 0; i < FM; i++)
+#pragma unroll
+                    for (int j = 0; j < FN; j++) part[((wk - 1) * NW * FM * FN + i * FN + j) * 64] = acc[i][j];
+            }
+            lds_barrier();
+            if (wk > 0) return;
+#pragma unroll
+            for (int k = 0; k < WK - 1; k++)
+#pragma unroll
+                for (int i = 0; i < FM; i++)
+#pragma unroll
+                    for (int j = 0; j < FN; j++) acc[i][j] += part[(k * NW * FM * FN + i * FN + j) * 64];
+        }
         store(m0, n0);
     }
 }
 
-template <int FM, int FN, int WM, int WN, int NS, bool EXACT, int CT> hipError_t tile(const Fp8Args &g, hipStream_t s)
+template <int FM, int FN, int WM, int WN, int WK, int NS, bool EXACT, int CT> hipError_t tile(const Fp8Args &g, hipStream_t s)
 {
     constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN;
     const int tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN;
     // persistent blocks: one per CU (256 on eight XCDs, to which blocks go in turn: a block's tiles stay on its XCD)
     const int blocks = NS == 2 ? (tm * tn < 256 ? tm * tn : 256) : tm * tn;
-    k_fp8_tile<FM, FN, WM, WN, NS, EXACT, CT><<<blocks, 64 * WM * WN, 0, s>>>(g, tm, tn);
+    k_fp8_tile<FM, FN, WM, WN, WK, NS, EXACT, CT><<<blocks, 64 * WM * WN * WK, 0, s>>>(g, tm, tn);
     return hipGetLastError();
+}
+
+template <int FN, int WK, int WN, int U, int CT> hipError_t few_rows(const Fp8Args &g, hipStream_t s)
+{
+    k_fp8_rows<FN, WK, WN, U, CT><<<(g.N + 16 * FN * WN - 1) / (16 * FN * WN), 64 * WK * WN, 0, s>>>(g);
+    return hipGetLastError();
+}
+
+// The tiles that there are, and what they cost: us of a round of blocks (one per CU, or `occ`) with s stages, start + s * stage,
+// and, where a CU holds several, of a block's stage in the midst of others.  Fitted to all of them timed at M 17 .. 4096 by
+// N x K of 5120 x 2048, 2048 x 4096, 4096 x 4096 and 4096 x 7168 (bf16; f32 takes 1.6 to 1.8 times as long in all).  us, the others beside the
+// fastest: 64 x 2048 x 4096  64x32 7.1 (64x64 halves 9.0, 64x64 11.0);  128 x 5120 x 2048  64x64 halves 6.6 (64x32 9.5, 64x64 7.4);
+// 512 x 5120 x 2048  64x64 12.5 (128x128 12.4, 64x64 halves 16.8);  1024 x 4096 x 7168  128x128 37 (64x64 49, 128x256 49);
+// 1500 x 5120 x 2048  128x256 20 (128x128 24, 256x256 28);  2048 x 5120 x 2048  256x256 29 (128x128 34, 128x256 35).
+struct TileCost {
+    int bm, bn, wk, occ;
+    float start, stage, shared;
+};
+enum { T64X32, T64X64_HALVES, T64X64, T128X128, T128X256, T256X256, TILES };
+constexpr TileCost TILE_COST[TILES] = {
+    {64, 32, 4, 1, 1.8f, 0.575f, 0.575f}, {64, 64, 2, 1, 1.5f, 0.43f, 0.43f}, {64, 64, 1, 3, 1.2f, 0.29f, 0.215f},
+    {128, 128, 1, 1, 1.7f, 0.6f, 0.6f},   {128, 256, 1, 1, 1.7f, 1.0f, 1.0f}, {256, 256, 1, 1, 2.4f, 1.7f, 1.7f},
+};
+
+int best_tile(const Fp8Args &g, bool exact)
+{
+    int best = T64X64;
+    float least = 0.0f;
+    for (int i = 0; i < TILES; i++) {
+        if (i == T256X256 && (exact || g.K <= 128)) continue;   // its registers; its stream of stages
+        const TileCost &t = TILE_COST[i];
+        const int64_t tiles = (int64_t)((g.M + t.bm - 1) / t.bm) * ((g.N + t.bn - 1) / t.bn);
+        const float per_cu = (float)((tiles + 255) / 256), s = (float)(((g.K + 127) / 128 + t.wk - 1) / t.wk);
+        const float rounds = (float)((tiles + 256 * t.occ - 1) / (256 * t.occ));
+        const float a = rounds * (t.start + s * t.stage), b = t.start + per_cu * s * t.shared, us = a > b ? a : b;
+        if (i == 0 || us < least) {
+            best = i;
+            least = us;
+        }
+    }
+    return best;
 }
 
 template <int CT> hipError_t gemm(const Fp8Args &g, hipStream_t s)
 {
     constexpr bool EXACT = CT == X100_T_F32;
-    if (g.M <= 64) {
-        const dim3 grid((g.N + 15) / 16, (g.M + 15) / 16);
-        k_fp8_rows<1, 8, 1, 1, CT><<<grid, 512, 0, s>>>(g);
-        return hipGetLastError();
+    // Two 16-column tiles of W per wave halve A's reads, where there are waves enough for it (us with one / two: 8 x 151936 x
+    // 2048 62 / 55, 8 x 5120 x 2048 5.2 / 5.0, 16 x 2048 x 4096 5.9 / 7.8) and rows to read (1 x 151936 x 2048: 49 / 55).
+    if (g.M <= 16) return g.M > 4 && g.N >= 8192 ? few_rows<2, 8, 1, 1, CT>(g, s) : few_rows<1, 8, 1, 1, CT>(g, s);
+    switch (best_tile(g, EXACT)) {
+    case T64X32: return tile<2, 2, 2, 1, 4, 3, EXACT, CT>(g, s);
+    case T64X64_HALVES: return tile<2, 2, 2, 2, 2, 4, EXACT, CT>(g, s);
+    case T64X64: return tile<2, 2, 2, 2, 1, 3, EXACT, CT>(g, s);
+    case T128X128: return tile<4, 2, 2, 4, 1, 3, EXACT, CT>(g, s);
+    case T128X256: return tile<4, 4, 2, 4, 1, 3, EXACT, CT>(g, s);
     }
-    if constexpr (!EXACT) {
-        if (g.M > 512 && g.K > 128) return tile<8, 4, 2, 4, 2, false, CT>(g, s);
-    }
-    if (g.M > 128) return tile<4, 4, 2, 2, 3, EXACT, CT>(g, s);
-    return tile<2, 2, 2, 2, 4, EXACT, CT>(g, s);
+    if constexpr (!EXACT) return tile<8, 4, 2, 4, 1, 2, false, CT>(g, s);
+    return hipErrorInvalidValue;
 }
 
 }  // namespace
