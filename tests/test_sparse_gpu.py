@@ -434,3 +434,42 @@ def test_half_layer(dev):
     out = np.zeros((n, nh, hd))
     tol = sp.attend(t.c, K, V, q, rr, t.table, want, 0.125, out)
     compare(host(o).reshape(n, nh, hd), out, tol)
+
+
+def test_select_under_wide_bounds(dev):
+    """Single tokens and prompts under bounds that any of them may reach, as a captured graph has them."""
+    for q_lens, rows_more in (([1, 1, 1], 0), ([1, 20, 7], 0), ([8, 9, 1], 12), ([3, 3, 3, 40, 1, 8], 100)):
+        n = len(q_lens)
+        for max_q in (40, 300):
+            p = Pick(20, 4, 2, 64, 16, ref.BF16, q_lens, [700, 650, 300, 900, 16, 100][:n], tail_rows=rows_more, max_q=max_q, max_kv=2000)
+            p.check(6, 1, 2)
+            p = Pick(21, 4, 2, 64, 16, ref.BF16, q_lens, [700, 650, 300, 900, 16, 100][:n], tail_rows=n * max_q - sum(q_lens),
+                     max_q=max_q, max_kv=1000)
+            p.check(6, 1, 2)
+
+
+def test_select_and_means_of_many_sequences(dev):
+    """More sequences than a wave looks at together, most of them without rows."""
+    q_lens = ([0] * 70 + [1] + [0] * 3 + [2]) * 4 + [1] * 40
+    kv_lens = [16 * (i % 7 + 1) for i in range(len(q_lens))]
+    p = Pick(22, 2, 1, 64, 16, ref.F16, q_lens, kv_lens)
+    p.check(3)
+    t = Setup(23, 2, 1, 64, 16, ref.F16, ref.F16, q_lens, kv_lens)
+    d = torch.zeros(t.c.n_pages, 1, 64, dtype=torch.int16, device=dev)
+    x.kv_means(t.cfg, t.batch, t.dk.data_ptr(), d.data_ptr(), stream())
+    torch.cuda.synchronize()
+    K, _ = t.c.decode(t.kb, t.vb)
+    want = sp.means(t.c, K, rows_of(t), t.table, np.zeros((t.c.n_pages, 1, 64), np.uint16))
+    assert np.array_equal(d.cpu().numpy().view(np.uint16), want)
+
+
+def test_means_of_refused_sequences(dev):
+    """A sequence that breaks its bounds between others: theirs are made, its own and no other page is touched."""
+    t = Setup(24, 2, 1, 64, 16, ref.BF16, ref.BF16, [1, 17, 1, 16, 1], [32, 48, 64, 80, 16], max_q=16, max_kv=80)
+    old = np.full((t.c.n_pages, 1, 64), 0x77, np.uint16)
+    d = torch.from_numpy(old.view(np.int16).copy()).cuda()
+    x.kv_means(t.cfg, t.batch, t.dk.data_ptr(), d.data_ptr(), stream())
+    torch.cuda.synchronize()
+    K, _ = t.c.decode(t.kb, t.vb)
+    want = sp.means(t.c, K, rows_of(t), t.table, old)
+    assert len(rows_of(t)) == 19 and np.array_equal(d.cpu().numpy().view(np.uint16), want)

@@ -21,6 +21,7 @@
 
 #include "paged_attn.h"
 #include "x100_internal.h"
+#include "x100_sparse.h"
 
 namespace {
 
@@ -74,19 +75,29 @@ template <int HD, int AT, bool Q4, bool SP> __global__ __launch_bounds__(256, Q4
         row0 = unit / (n_kv * a.tile.n);
         i0 = 0;
         n_rows = G;
+        const int *list = a.sel + ((size_t)row0 * n_kv + kvh) * a.n_sel;
+        constexpr int LE = X100_SPARSE_MAX_SEL / (64 * NW);   // entries of a thread: on their way beside the search
+        int entry[LE], before[LE];
+#pragma unroll
+        for (int k = 0; k < LE; k++) {
+            const int i = threadIdx.x + 64 * NW * k;
+            entry[k] = i < a.n_sel ? list[i] : -1;
+            before[k] = i < a.n_sel && i ? list[i - 1] : -1;
+        }
         s = paged_find(a.b, row0);
         if (s >= a.b.n_seq) return;
         const PagedSeq q = paged_seq(a.b, s);
         if (!q.holds(row0)) return;
         const int at = q.position(row0), own = at >> psh;   // below 0: no block
-        const int *list = a.sel + ((size_t)row0 * n_kv + kvh) * a.n_sel;
         const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
         // the list's pages, up to the first entry that breaks its order
         __shared__ int s_cnt[NW], s_own[NW];
         int end = a.n_sel, own_at = -1;
-        for (int i = threadIdx.x; i < a.n_sel; i += 64 * NW) {
-            const int e = list[i], before = i ? list[i - 1] : -1;
-            const bool ok = e > before && e >= 0 && e <= own;
+#pragma unroll
+        for (int k = 0; k < LE; k++) {
+            const int i = threadIdx.x + 64 * NW * k, e = entry[k];
+            if (i >= a.n_sel) continue;
+            const bool ok = e > before[k] && e >= 0 && e <= own;
             if (!ok) end = min(end, i);
             if (ok && e == own) own_at = i;
             sh.pg[i] = ok ? valid(tab[e]) : -1;

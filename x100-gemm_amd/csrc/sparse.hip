@@ -9,13 +9,30 @@
 
 namespace {
 
-X100_DEV double xor_d(double v, int m)
+template <int CTRL> X100_DEV double dpp_d(double v)
 {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    uint32_t lo = (uint32_t)u, hi = (uint32_t)(u >> 32);
-    lo = m == 32 ? xor32_u(lo) : xor16_u(lo);
-    hi = m == 32 ? xor32_u(hi) : xor16_u(hi);
+    const uint32_t lo = dpp_i<CTRL>(0, (int)(uint32_t)u), hi = dpp_i<CTRL>(0, (int)(uint32_t)(u >> 32));
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+X100_DEV double xor16_d(double v)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)xor16_u((uint32_t)(u >> 32)) << 32 | xor16_u((uint32_t)u));
+}
+X100_DEV double xor32_d(double v)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)xor32_u((uint32_t)(u >> 32)) << 32 | xor32_u((uint32_t)u));
+}
+// sum over each group of L = 8 or 16 lanes, in all of them
+template <int L> X100_DEV double sum_lanes(double v)
+{
+    v += dpp_d<0xB1>(v);
+    v += dpp_d<0x4E>(v);
+    v += dpp_d<0x141>(v);
+    if constexpr (L == 16) v += dpp_d<0x140>(v);
+    return v;
 }
 
 // 8 elements of a head row as floats: as they are stored, or the 4-bit numbers' values (d2, m2: d and m twice).
@@ -40,36 +57,57 @@ X100_DEV void elems_q4(uint32_t w, uint32_t dm, float (&v)[8])
     }
 }
 
-// Mean keys.  A block looks at 16 rows of the batch; a wave takes every fourth of those that end a page.  Lane l has the
-// elements 8 (l % L) .. + 7 of rows l / L, l / L + 64 / L, ... of the page (L lanes per row), 8 loads on their way.
+// Mean keys.  A block looks at 16 rows of the batch and one KV head.  Its lanes look the rows up side by side: one search
+// for the first one's sequence, the other rows' by how many of the next 64 sequences end before them.  A single page (a
+// prompt's, or one of a batch of single tokens) is shared by the block's waves, of several each wave takes every fourth.  Lane l
+// has the elements 8 (l % L) .. + 7 of every (64 / L)-th row of its part (L lanes per row), 4 loads on their way.
 // Bound by the chain row -> sequence -> page -> keys for single tokens, by the keys' bytes for prompts.
 constexpr int MEAN_ROWS = 16;
 template <int HD, int AT, bool Q4>
 __global__ __launch_bounds__(256) void k_kv_means(const x100_kv_cfg c, const x100_kv_batch b, const uint8_t *kp, uint16_t *means)
 {
     constexpr int L = HD / 8, RS = 64 / L;   // lanes of a row, rows of a step
+    __shared__ double s_sum[3][HD];
     const int lane = threadIdx.x & 63, w = wave_id(), kvh = blockIdx.x % c.n_head_kv, row0 = blockIdx.x / c.n_head_kv * MEAN_ROWS;
-    const int psh = __builtin_ctz(c.page);
-    // lane i: page of row row0 + i, if that row is the last of a page
-    int pg = -1;
-    for (int i = 0; i < MEAN_ROWS && row0 + i < b.n_rows; i += 1) {
-        if ((i & 3) != w) continue;
-        const int row = row0 + i, s = paged_find(b, row);
-        if (s >= b.n_seq) break;
+    // lane i < 16: page of row row0 + i, if that row is the last of a page (else -1)
+    const int s0 = paged_find(b, row0);
+    if (s0 >= b.n_seq) return;
+    const int row = row0 + min(lane, MEAN_ROWS - 1);
+    const int end = s0 + lane < b.n_seq ? b.q_start[s0 + lane + 1] : 0x7fffffff;   // of the lane's sequence
+    int s = s0;
+#pragma unroll
+    for (int i = 0; i < MEAN_ROWS; i++) {
+        const int past = __popcll(__ballot(end <= row0 + i));
+        if (row == row0 + i) s = s0 + past;
+    }
+    // more than 64 sequences without rows in between, or q_start in disorder: each row by itself
+    if (__any(s - s0 >= 64 || (s < b.n_seq && !paged_seq(b, s).holds(row)))) {
+        for (int i = 0; i < MEAN_ROWS; i++) {
+            const int f = paged_find(b, row0 + i);
+            if (row == row0 + i) s = f;
+        }
+    }
+    int page = -1;
+    if (lane < MEAN_ROWS && s < b.n_seq) {
         const PagedSeq q = paged_seq(b, s);
-        if (!q.holds(row)) continue;
-        const int pos = q.position(row);
-        if (pos < 0 || (pos & (c.page - 1)) != c.page - 1) continue;
-        pg = paged_page(c, b, s, pos);
-        if (pg < 0) continue;
+        const int pos = q.holds(row) ? q.position(row) : -1;
+        if (pos >= 0 && (pos & (c.page - 1)) == c.page - 1) page = paged_page(c, b, s, pos);
+    }
+    uint64_t todo = __ballot(page >= 0);
+    const bool one = __popcll(todo) == 1;
+    const int r0 = one ? w * (c.page / 4) : 0, r1 = one ? r0 + c.page / 4 : c.page;   // rows of the page
+    for (int n = 0; todo; n++) {
+        const int i = __ffsll((unsigned long long)todo) - 1, pg = __shfl(page, i, 64);
+        todo &= todo - 1;
+        if (!one && (n & 3) != w) continue;
         const uint8_t *kb = kp + ((size_t)pg * c.n_head_kv + kvh) * page_head_bytes<HD, Q4>(c.page);
         double sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        const int r0 = lane / L, e0 = lane % L;
-        for (int r = r0; r < c.page; r += 4 * RS) {   // a page has at least 16 rows: some lanes' steps may lie behind it
+        const int e0 = lane % L;
+        for (int r = r0 + lane / L; r < r1; r += 4 * RS) {   // a part has at least 4 rows: some lanes' steps may lie behind it
             float v[4][8];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                const int rr = min(r + u * RS, c.page - 1);
+                const int rr = min(r + u * RS, r1 - 1);
                 if constexpr (!Q4) elems16<AT>(*(const v4u *)(kb + ((size_t)rr * HD + 8 * e0) * 2), v[u]);
                 else
                     elems_q4(((const uint32_t *)kb)[rr * L + e0],
@@ -77,20 +115,30 @@ __global__ __launch_bounds__(256) void k_kv_means(const x100_kv_cfg c, const x10
             }
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                if (r + u * RS >= c.page) continue;
+                if (r + u * RS >= r1) continue;
 #pragma unroll
                 for (int e = 0; e < 8; e++) sum[e] += (double)v[u][e];
             }
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            if constexpr (L == 8) {   // rows of lanes l and l ^ 8 too
-                const uint64_t u = __builtin_bit_cast(uint64_t, sum[e]);
-                const uint32_t lo = dpp_i<0x128>(0, (int)(uint32_t)u), hi = dpp_i<0x128>(0, (int)(uint32_t)(u >> 32));
-                sum[e] += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+            if constexpr (L == 8) sum[e] += dpp_d<0x128>(sum[e]);   // rows of lanes l and l ^ 8 too
+            sum[e] += xor16_d(sum[e]);
+            sum[e] += xor32_d(sum[e]);
+        }
+        if (one) {   // every wave comes here, once
+            if (w > 0 && lane < L) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) s_sum[w - 1][8 * lane + e] = sum[e];
             }
-            sum[e] += xor_d(sum[e], 16);
-            sum[e] += xor_d(sum[e], 32);
+            __syncthreads();
+            if (w > 0) return;
+            if (lane < L) {
+#pragma unroll
+                for (int k = 0; k < 3; k++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) sum[e] += s_sum[k][8 * lane + e];
+            }
         }
         if (lane < L) {
             const double f = 1.0 / c.page;   // a power of two
@@ -122,22 +170,26 @@ struct SelectArgs {
     int64_t ldq;
     const uint16_t *means;
     int *sel;
+    bool apart;   // sequences of MANY rows are k_attn_select_rows's, the others k_attn_select's
 };
 
-constexpr int ST = 256;   // threads of a block
+// Sequences of so many rows in a batch go to the kernel that takes rows together, the others' rows are taken one by one.
+constexpr int MANY = 8;
 
-template <int HD, int R, int CAP> struct SelectLds {
-    uint64_t key[R][CAP];
-    double q[R][HD];
+// ---- one row of few: a block per row and KV head
+
+template <int NT, int CAP> struct SelectLds {
+    uint64_t key[CAP];           // first the pages
     int hist[256];
     int bin, above, same;        // the digit of the list's last key, keys above it, keys with it
-    int gt[ST / 64], eq[ST / 64];
+    int gt[NT / 64], eq[NT / 64];
 };
 
-// The list of the n keys k (n > 0): the n_sel largest that are not KEY_NONE, lowest index first among equal ones,
-// ascending.  The smallest of them is found 8 bits at a time, until a digit's keys are all in or all digits are known.
-template <class Lds> X100_DEV void select_keys(Lds &sh, const uint64_t *k, int n, int n_sel, int *out)
+// The list of n keys (n > 0): the n_sel largest that are not KEY_NONE, lowest index first among equal ones, ascending.  The
+// smallest of them is found 8 bits at a time, until a digit's keys are all in or all digits are known.
+template <int NT, int CAP> X100_DEV void select_keys(SelectLds<NT, CAP> &sh, int n, int n_sel, int *out)
 {
+    const uint64_t *k = sh.key;
     const int t = threadIdx.x, lane = t & 63, w = wave_id();
     uint64_t low = 1;      // selected: keys >= low,
     int ties = 0;          // or, if ties > 0, keys > low and the first `ties` keys that are low
@@ -145,9 +197,9 @@ template <class Lds> X100_DEV void select_keys(Lds &sh, const uint64_t *k, int n
         uint64_t prefix = 0, mask = 0;
         int need = n_sel;
         for (int shift = 56; shift >= 0; shift -= 8) {
-            sh.hist[t] = 0;
+            if (t < 256) sh.hist[t] = 0;
             __syncthreads();
-            for (int i = t; i < n; i += ST)
+            for (int i = t; i < n; i += NT)
                 if ((k[i] & mask) == prefix) atomicAdd(&sh.hist[(int)(k[i] >> shift) & 255], 1);
             __syncthreads();
             if (w == 0) {   // lane l: bins 255 - 4 l .. 252 - 4 l
@@ -155,11 +207,12 @@ template <class Lds> X100_DEV void select_keys(Lds &sh, const uint64_t *k, int n
 #pragma unroll
                 for (int e = 0; e < 4; e++) s += c[e] = sh.hist[255 - 4 * lane - e];
                 int upto = s;   // of the lanes up to this one
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) {
-                    const int y = __shfl_up(upto, d, 64);
-                    if (lane >= d) upto += y;
-                }
+                upto += dpp_i<0x111>(0, upto);
+                upto += dpp_i<0x112>(0, upto);
+                upto += dpp_i<0x114>(0, upto);
+                upto += dpp_i<0x118>(0, upto);
+                upto += dpp_i<0x142, 0xa>(0, upto);
+                upto += dpp_i<0x143, 0xc>(0, upto);
                 int before = upto - s;
                 if (before < need && need <= upto) {
 #pragma unroll
@@ -173,28 +226,22 @@ template <class Lds> X100_DEV void select_keys(Lds &sh, const uint64_t *k, int n
                     }
                 }
             }
-            __syncthreads();
+            __syncthreads();   // the next pass's first barrier lies behind these reads
             prefix |= (uint64_t)sh.bin << shift;
             mask |= 255ull << shift;
             need -= sh.above;
-            const bool all = sh.same == need;
-            __syncthreads();   // bin, above and same are read
-            if (all) {
-                low = prefix;
-                break;
-            }
-            if (shift == 0) {
-                low = prefix;
-                ties = need;
-            }
+            low = prefix;
+            if (sh.same == need) break;   // all keys with these digits
+            if (shift == 0) ties = need;
         }
         if (low == KEY_NONE) {   // blocks without a page would be among them
             low = 1;
             ties = 0;
         }
     }
-    // wave w has the w-th quarter of the keys, in order
-    const int part = (n + 4 * 64 - 1) / (4 * 64) * 64, i0 = min(n, w * part), i1 = min(n, i0 + part);
+    // wave w has the w-th part of the keys, in order
+    constexpr int NW = NT / 64;
+    const int part = (n + NT - 1) / NT * 64, i0 = min(n, w * part), i1 = min(n, i0 + part);
     int gt = 0, eq = 0;
     for (int i = i0 + lane; i - lane < i1; i += 64) {
         const uint64_t x = i < i1 ? k[i] : 0;
@@ -208,7 +255,7 @@ template <class Lds> X100_DEV void select_keys(Lds &sh, const uint64_t *k, int n
     __syncthreads();
     int at = 0, eq0 = 0, total = 0;
 #pragma unroll
-    for (int v = 0, e = 0; v < ST / 64; v++) {
+    for (int v = 0, e = 0; v < NW; v++) {
         const int take = sh.gt[v] + (ties > 0 ? min(max(ties - e, 0), sh.eq[v]) : 0);
         if (v == w) eq0 = e;
         if (v < w) at += take;
@@ -225,16 +272,142 @@ template <class Lds> X100_DEV void select_keys(Lds &sh, const uint64_t *k, int n
         at += __popcll(bt);
         eq0 += __popcll(bq);
     }
-    for (int i = total + t; i < n_sel; i += ST) out[i] = -1;
+    for (int i = total + t; i < n_sel; i += NT) out[i] = -1;
 }
 
-// A block: R rows of the batch and one KV head.  Rows of one sequence read its means together: thread t has blocks t, t +
-// 256, ... of the sequence, whose mean it loads once for the rows.  Bound by the means' bytes for single tokens
-// (each row and KV head reads its own), by the fp64 unit for prompts.
-template <int HD, int AT, int R, int CAP> __global__ __launch_bounds__(ST) void k_attn_select(const SelectArgs a)
+// L lanes have a mean, 8 elements each, 64 / L means per load of a wave, 4 loads on their way; each row and KV head reads its
+// own means.  Bound by latency: row -> sequence -> pages -> means -> the list's four barriers per digit.
+template <int HD, int AT, int NT, int CAP> __global__ __launch_bounds__(NT) void k_attn_select(const SelectArgs a)
 {
-    __shared__ SelectLds<HD, R, CAP> sh;
-    const int t = threadIdx.x, n_kv = a.c.n_head_kv, kvh = blockIdx.x % n_kv, row0 = blockIdx.x / n_kv * R;
+    constexpr int L = HD / 8, GR = 64 / L, NG = NT / L, U = 4;
+    __shared__ SelectLds<NT, CAP> sh;
+    const int t = threadIdx.x, lane = t & 63, n_kv = a.c.n_head_kv, kvh = blockIdx.x % n_kv, row = blockIdx.x / n_kv;
+    const int G = a.c.n_head / n_kv, psh = __builtin_ctz(a.c.page), l = lane % L;
+    const int s = paged_find(a.b, row);
+    if (s >= a.b.n_seq) return;
+    const PagedSeq q = paged_seq(a.b, s);
+    if (!q.holds(row) || (a.apart && q.q_len >= MANY)) return;
+    const int pos = q.position(row), own = pos >> psh;   // below 0: no position
+    int *out = a.sel + ((size_t)row * n_kv + kvh) * a.pick.n_sel;
+    if (pos < 0) {
+        for (int i = t; i < a.pick.n_sel; i += NT) out[i] = -1;
+        return;
+    }
+    const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
+    for (int i = t; i <= own; i += NT) sh.key[i] = (uint32_t)tab[i];
+    double x[8] = {0, 0, 0, 0, 0, 0, 0, 0};   // the sum of the queries
+    for (int h = 0; h < G; h++) {
+        float v[8];
+        elems16<AT>(*(const v4u *)(a.q + (size_t)row * a.ldq + (size_t)(kvh * G + h) * HD + 8 * l), v);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] += (double)v[e];
+    }
+    __syncthreads();
+    const v4u *means = (const v4u *)(a.means + (size_t)kvh * HD) + l;
+    for (int b0 = t / L; b0 - lane / L <= own; b0 += U * NG) {   // the lanes of a wave together
+        v4u m[U];
+        int pg[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            pg[u] = b0 + u * NG <= own ? (int)(uint32_t)sh.key[b0 + u * NG] : -1;
+            if (pg[u] < 0 || pg[u] >= a.c.n_pages) pg[u] = -1;
+            m[u] = means[(size_t)max(pg[u], 0) * n_kv * L];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int b = b0 + u * NG;
+            float v[8];
+            elems16<AT>(m[u], v);
+            double y = 0.0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) y = __builtin_fma(x[e], (double)v[e], y);
+            y = sum_lanes<L>(y);
+            const bool always = b < a.pick.n_first || b > own - a.pick.n_last;
+            if (l == 0 && b <= own) sh.key[b] = pg[u] < 0 ? KEY_NONE : (always ? KEY_ALWAYS : score_key(y));
+        }
+    }
+    __syncthreads();
+    select_keys(sh, own + 1, a.pick.n_sel, out);
+}
+
+// ---- rows of a prompt: a block per R rows and KV head
+
+typedef double v4d __attribute__((ext_vector_type(4)));
+constexpr int RT = 512;   // threads
+
+// The list of a row's n keys by one wave, key i in lane i % 64: the threshold one bit at a time, until as many keys are
+// left as the list takes.
+template <int CAP> X100_DEV void select_row(const uint64_t *key, int n, int n_sel, int *out)
+{
+    constexpr int KL = CAP / 64;
+    const int lane = threadIdx.x & 63, used = (n + 63) >> 6;
+    uint64_t k[KL < 16 ? KL : 16];   // of up to 1024 keys in registers
+    auto at = [&](int u) __attribute__((always_inline)) {
+        if constexpr (KL <= 16) return k[u];
+        else return 64 * u + lane < n ? key[64 * u + lane] : KEY_NONE;
+    };
+    if constexpr (KL <= 16) {
+#pragma unroll
+        for (int u = 0; u < KL; u++) k[u] = 64 * u + lane < n ? key[64 * u + lane] : KEY_NONE;
+    }
+    auto count = [&](uint64_t from) __attribute__((always_inline)) {   // keys >= from
+        int c = 0;
+        if constexpr (KL <= 16) {
+#pragma unroll
+            for (int u = 0; u < KL; u++)
+                if (u < used) c += __popcll(__ballot(k[u] >= from));
+        } else {
+            for (int u = 0; u < used; u++) c += __popcll(__ballot(at(u) >= from));
+        }
+        return c;
+    };
+    uint64_t low = 1;
+    int ties = 0;
+    if (n > n_sel) {
+        uint64_t y = 0;
+        bool exact = false;
+        for (int bit = 63; bit >= 0 && !exact; bit--) {
+            const uint64_t from = y | 1ull << bit;
+            const int c = count(from);
+            if (c >= n_sel) y = from;
+            exact = c == n_sel;
+        }
+        low = y;
+        if (!exact) ties = n_sel - (y == ~0ull ? 0 : count(y + 1));   // no key is in the list for its value alone
+        if (low == KEY_NONE) {
+            low = 1;
+            ties = 0;
+        }
+    }
+    int at_out = 0, eq = 0;
+    const uint64_t below = (1ull << lane) - 1;
+    auto emit = [&](int u, uint64_t x) __attribute__((always_inline)) {
+        const uint64_t bq = __ballot(x == low);
+        const bool take = ties > 0 ? x > low || (x == low && eq + __popcll(bq & below) < ties) : x >= low;
+        const uint64_t bt = __ballot(take);
+        if (take) out[at_out + __popcll(bt & below)] = 64 * u + lane;
+        at_out += __popcll(bt);
+        eq += __popcll(bq);
+    };
+    if constexpr (KL <= 16) {
+#pragma unroll
+        for (int u = 0; u < KL; u++)
+            if (u < used) emit(u, k[u]);
+    } else {
+        for (int u = 0; u < used; u++) emit(u, at(u));
+    }
+    for (int i = at_out + lane; i < n_sel; i += 64) out[i] = -1;
+}
+
+// Scores of 16 blocks and 16 rows by the fp64 matrix instruction, 4 elements each time: lane (c, g) has elements HD / 4 * g ..
+// of row c's query sum (in registers) and of block c's mean; every sum adds its terms in the same order.  Waves take every
+// eighth tile of blocks, the next one's means on their way, then every eighth row's list.
+template <int HD, int AT, int R, int CAP> __global__ __launch_bounds__(RT) void k_attn_select_rows(const SelectArgs a)
+{
+    constexpr int KS = HD / 4, LD = CAP + 1, NW = RT / 64;   // steps; keys of a row, off the banks of the one before
+    __shared__ uint64_t key[R * LD];
+    const int lane = threadIdx.x & 63, w = wave_id(), c = lane & 15, g = lane >> 4;
+    const int n_kv = a.c.n_head_kv, kvh = blockIdx.x % n_kv, row0 = blockIdx.x / n_kv * R;
     const int G = a.c.n_head / n_kv, psh = __builtin_ctz(a.c.page), rows = min(R, a.b.n_rows - row0);
     for (int j = 0; j < rows;) {
         const int s = paged_find(a.b, row0 + j);
@@ -244,79 +417,100 @@ template <int HD, int AT, int R, int CAP> __global__ __launch_bounds__(ST) void 
             j++;
             continue;
         }
-        const int n = min(rows - j, q.q0 + q.q_len - (row0 + j));   // rows of this sequence
-        const int own_last = q.position(row0 + j + n - 1) >> psh;   // the last row's own block (below 0: no position)
-        __syncthreads();   // the rows before are done with sh
-        for (int u = t; u < n * HD; u += ST) {
-            const int r = u / HD, e = u % HD;
-            const uint16_t *x = a.q + (size_t)(row0 + j + r) * a.ldq + (size_t)kvh * G * HD + e;
-            double y = 0.0;
-            for (int h = 0; h < G; h++) y += (double)act2f<AT>(x[h * HD]);
-            sh.q[r][e] = y;
-        }
-        __syncthreads();
-        const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
-        for (int blk = t; blk <= own_last; blk += ST) {
-            const int pg = tab[blk];
-            const bool ok = pg >= 0 && pg < a.c.n_pages;
-            double y[R];
-#pragma unroll
-            for (int r = 0; r < R; r++) y[r] = 0.0;
-            if (ok) {
-                const v4u *m = (const v4u *)(a.means + ((size_t)pg * n_kv + kvh) * HD);
-                v4u x[HD / 8];
-#pragma unroll
-                for (int i = 0; i < HD / 8; i++) x[i] = m[i];
-#pragma unroll
-                for (int i = 0; i < HD / 8; i++) {
-                    float v[8];
-                    elems16<AT>(x[i], v);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const double d = (double)v[e];
-#pragma unroll
-                        for (int r = 0; r < R; r++) y[r] = __builtin_fma(sh.q[r][8 * i + e], d, y[r]);
-                    }
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < R; r++) {
-                if (r >= n) continue;
-                const int own = q.position(row0 + j + r) >> psh;
-                const bool always = blk < a.pick.n_first || blk > own - a.pick.n_last;
-                sh.key[r][blk] = !ok ? KEY_NONE : (always ? KEY_ALWAYS : score_key(y[r]));
-            }
-        }
-        __syncthreads();
-        for (int r = 0; r < n; r++) {
-            const int pos = q.position(row0 + j + r);
-            int *out = a.sel + ((size_t)(row0 + j + r) * n_kv + kvh) * a.pick.n_sel;
-            if (pos < 0) {
-                for (int i = t; i < a.pick.n_sel; i += ST) out[i] = -1;
-                continue;
-            }
-            if (r) __syncthreads();   // the counts of the row before are read
-            select_keys(sh, sh.key[r], (pos >> psh) + 1, a.pick.n_sel, out);
-        }
+        const int n = min(rows - j, q.q0 + q.q_len - (row0 + j)), first = row0 + j;   // rows of this sequence
         j += n;
+        if (a.apart && q.q_len < MANY) continue;
+        const int own_last = q.position(first + n - 1) >> psh;   // the last row's own block (below 0: no position)
+        const int own = q.position(first + min(c, n - 1)) >> psh;
+        double x[KS];
+#pragma unroll
+        for (int e = 0; e < KS; e++) x[e] = 0.0;
+        for (int h = 0; h < G; h++) {
+            const v4u *p = (const v4u *)(a.q + (size_t)(first + min(c, n - 1)) * a.ldq + (size_t)(kvh * G + h) * HD + KS * g);
+#pragma unroll
+            for (int i = 0; i < KS / 8; i++) {
+                float v[8];
+                elems16<AT>(p[i], v);
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[8 * i + e] += (double)v[e];
+            }
+        }
+        const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
+        const uint16_t *means = a.means + (size_t)kvh * HD + KS * g;
+        auto page = [&](int t) __attribute__((always_inline)) {
+            const int b = 16 * t + c, pg = b <= own_last ? tab[b] : -1;
+            return pg >= 0 && pg < a.c.n_pages ? pg : -1;
+        };
+        v4u m[KS / 8];
+        auto load = [&](int pg) __attribute__((always_inline)) {
+            const v4u *p = (const v4u *)(means + (size_t)max(pg, 0) * n_kv * HD);
+#pragma unroll
+            for (int i = 0; i < KS / 8; i++) m[i] = p[i];
+        };
+        __syncthreads();   // the lists of the rows before are made
+        int pg = page(w), pn = page(w + NW);
+        load(pg);
+        for (int t = w; 16 * t <= own_last; t += NW) {
+            const uint64_t ok = __ballot(pg >= 0);
+            v4u now[KS / 8];
+#pragma unroll
+            for (int i = 0; i < KS / 8; i++) now[i] = m[i];
+            load(pn);
+            pg = pn;
+            pn = page(t + 2 * NW);
+            v4d y[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};   // two sums, so that an instruction need not wait for the one before
+#pragma unroll
+            for (int i = 0; i < KS / 8; i++) {
+                float v[8];
+                elems16<AT>(now[i], v);
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e & 1] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)v[e], x[8 * i + e], y[e & 1], 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {   // blocks 4 e + g, row c
+                const int b = 16 * t + 4 * e + g;
+                const bool always = b < a.pick.n_first || b > own - a.pick.n_last;
+                const double z = y[0][e] + y[1][e];
+                if (c < n && b < CAP) key[c * LD + b] = !(ok >> (4 * e + g) & 1) ? KEY_NONE : (always ? KEY_ALWAYS : score_key(z));
+            }
+        }
+        __syncthreads();
+        for (int r = w; r < n; r += NW) {
+            const int pos = q.position(first + r);
+            int *out = a.sel + ((size_t)(first + r) * n_kv + kvh) * a.pick.n_sel;
+            if (pos < 0) {
+                for (int i = lane; i < a.pick.n_sel; i += 64) out[i] = -1;
+            } else {
+                select_row<CAP>(key + r * LD, (pos >> psh) + 1, a.pick.n_sel, out);
+            }
+        }
     }
 }
 
-template <int HD, int AT, int R, int CAP> hipError_t select(const SelectArgs &a, hipStream_t s)
+template <int HD, int AT, int R, int CAP> hipError_t select_rows(const SelectArgs &a, hipStream_t s)
 {
     const unsigned grid = (unsigned)(((int64_t)a.b.n_rows + R - 1) / R * a.c.n_head_kv);
-    k_attn_select<HD, AT, R, CAP><<<grid, ST, 0, s>>>(a);
+    k_attn_select_rows<HD, AT, R, CAP><<<grid, RT, 0, s>>>(a);
     return hipGetLastError();
 }
 
-// Rows of a block by whether sequences have several, and what their keys take in LDS.
-template <int HD, int AT> hipError_t select_by_size(const SelectArgs &a, hipStream_t s)
+// Which kernels a batch takes: rows together, where a sequence can have MANY (and their keys find room in LDS); one by one,
+// where none can.  Where the bounds leave room for both, both run and leave the other's sequences alone; where every
+// sequence may have max_q rows, the first takes whatever there is.
+template <int HD, int AT> hipError_t select_by_size(SelectArgs a, hipStream_t s)
 {
     const int n = (a.b.max_kv - 1) / a.c.page + 1;
-    if (a.b.max_q >= 4 && n <= 1024) return select<HD, AT, 4, 1024>(a, s);
-    if (a.b.max_q >= 4 && n <= 4096) return select<HD, AT, 4, 4096>(a, s);
-    if (n <= 1024) return select<HD, AT, 1, 1024>(a, s);
-    return select<HD, AT, 1, X100_SPARSE_MAX_BLOCKS>(a, s);
+    if (a.b.max_q >= MANY && n <= 4096) {
+        a.apart = (int64_t)a.b.n_seq * a.b.max_q > a.b.n_rows;
+        const hipError_t e = n <= 512 ? select_rows<HD, AT, 16, 512>(a, s) : n <= 1024 ? select_rows<HD, AT, 16, 1024>(a, s) : select_rows<HD, AT, 4, 4096>(a, s);
+        if (e != hipSuccess || !a.apart) return e;
+    }
+    const unsigned grid = (unsigned)((int64_t)a.b.n_rows * a.c.n_head_kv);
+    // few rows: more waves for each (16 x 938 blocks 18.4 us with 4, less with 16)
+    if (n <= 1024 && grid <= 512) k_attn_select<HD, AT, 1024, 1024><<<grid, 1024, 0, s>>>(a);
+    else if (n <= 1024) k_attn_select<HD, AT, 256, 1024><<<grid, 256, 0, s>>>(a);
+    else k_attn_select<HD, AT, 1024, X100_SPARSE_MAX_BLOCKS><<<grid, 1024, 0, s>>>(a);
+    return hipGetLastError();
 }
 
 template <int HD, int AT> hipError_t means_as(const x100_kv_cfg &c, const x100_kv_batch &b, const void *kp, void *means, hipStream_t s)
@@ -339,7 +533,7 @@ hipError_t x100_kv_means_launch(const x100_kv_cfg &c, const x100_kv_batch &b, co
 hipError_t x100_attn_select_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const x100_kv_sel &pick, const void *q,
                                    int64_t ldq, const void *means, int *sel, hipStream_t s)
 {
-    const SelectArgs a = {c, b, pick, (const uint16_t *)q, ldq, (const uint16_t *)means, sel};
+    const SelectArgs a = {c, b, pick, (const uint16_t *)q, ldq, (const uint16_t *)means, sel, false};
     if (c.head_dim == 64) return c.act_type == X100_T_F16 ? select_by_size<64, X100_T_F16>(a, s) : select_by_size<64, X100_T_BF16>(a, s);
     return c.act_type == X100_T_F16 ? select_by_size<128, X100_T_F16>(a, s) : select_by_size<128, X100_T_BF16>(a, s);
 }
