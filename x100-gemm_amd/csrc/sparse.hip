@@ -180,6 +180,7 @@ constexpr int MANY = 8;
 
 template <int NT, int CAP> struct SelectLds {
     uint64_t key[CAP];           // first the pages
+    double q[128];               // the sum of the queries
     int hist[256];
     int bin, above, same;        // the digit of the list's last key, keys above it, keys with it
     int gt[NT / 64], eq[NT / 64];
@@ -275,14 +276,21 @@ template <int NT, int CAP> X100_DEV void select_keys(SelectLds<NT, CAP> &sh, int
     for (int i = total + t; i < n_sel; i += NT) out[i] = -1;
 }
 
-// L lanes have a mean, 8 elements each, 64 / L means per load of a wave, 4 loads on their way; each row and KV head reads its
-// own means.  Bound by latency: row -> sequence -> pages -> means -> the list's four barriers per digit.
-template <int HD, int AT, int NT, int CAP> __global__ __launch_bounds__(NT) void k_attn_select(const SelectArgs a)
+// L lanes have a mean, 8 elements each, 64 / L means per load of a wave, U loads on their way; each row and KV head reads its
+// own means.  Bound by latency: row -> sequence -> pages -> means -> digits.  us, 16 rows of up to 938 blocks: 4.1 to the
+// position, 16 with the scores, 19.3 with the lists (by one wave, a bit at a time, 21).  Scores in fp32 by the 16-bit
+// matrix cores with bounds of their error, and fp64 for what the bounds leave, were no faster (20).
+template <int HD, int AT, int NT, int CAP, int U> __global__ __launch_bounds__(NT) void k_attn_select(const SelectArgs a)
 {
-    constexpr int L = HD / 8, GR = 64 / L, NG = NT / L, U = 4;
+    constexpr int L = HD / 8, NG = NT / L;
     __shared__ SelectLds<NT, CAP> sh;
     const int t = threadIdx.x, lane = t & 63, n_kv = a.c.n_head_kv, kvh = blockIdx.x % n_kv, row = blockIdx.x / n_kv;
     const int G = a.c.n_head / n_kv, psh = __builtin_ctz(a.c.page), l = lane % L;
+    for (int e = t; e < HD; e += NT) {   // the sum of the queries
+        double y = 0.0;
+        for (int h = 0; h < G; h++) y += (double)act2f<AT>(a.q[(size_t)row * a.ldq + (size_t)(kvh * G + h) * HD + e]);
+        sh.q[e] = y;
+    }
     const int s = paged_find(a.b, row);
     if (s >= a.b.n_seq) return;
     const PagedSeq q = paged_seq(a.b, s);
@@ -295,20 +303,17 @@ template <int HD, int AT, int NT, int CAP> __global__ __launch_bounds__(NT) void
     }
     const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
     for (int i = t; i <= own; i += NT) sh.key[i] = (uint32_t)tab[i];
-    double x[8] = {0, 0, 0, 0, 0, 0, 0, 0};   // the sum of the queries
-    for (int h = 0; h < G; h++) {
-        float v[8];
-        elems16<AT>(*(const v4u *)(a.q + (size_t)row * a.ldq + (size_t)(kvh * G + h) * HD + 8 * l), v);
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] += (double)v[e];
-    }
     __syncthreads();
+    double x[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = sh.q[8 * l + e];
     const v4u *means = (const v4u *)(a.means + (size_t)kvh * HD) + l;
     for (int b0 = t / L; b0 - lane / L <= own; b0 += U * NG) {   // the lanes of a wave together
         v4u m[U];
         int pg[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
+            if (b0 - lane / L + u * NG > own) continue;   // all lanes'
             pg[u] = b0 + u * NG <= own ? (int)(uint32_t)sh.key[b0 + u * NG] : -1;
             if (pg[u] < 0 || pg[u] >= a.c.n_pages) pg[u] = -1;
             m[u] = means[(size_t)max(pg[u], 0) * n_kv * L];
@@ -316,6 +321,7 @@ template <int HD, int AT, int NT, int CAP> __global__ __launch_bounds__(NT) void
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int b = b0 + u * NG;
+            if (b - lane / L > own) continue;
             float v[8];
             elems16<AT>(m[u], v);
             double y = 0.0;
@@ -335,46 +341,61 @@ template <int HD, int AT, int NT, int CAP> __global__ __launch_bounds__(NT) void
 typedef double v4d __attribute__((ext_vector_type(4)));
 constexpr int RT = 512;   // threads
 
-// The list of a row's n keys by one wave, key i in lane i % 64: the threshold one bit at a time, until as many keys are
-// left as the list takes.
-template <int CAP> X100_DEV void select_row(const uint64_t *key, int n, int n_sel, int *out)
+// The list of a row's n keys by one wave, key i in lane i % 64: the threshold one bit at a time, the upper half of the keys
+// first, until as many keys are left as the list takes.  Counts are kept per lane and summed once per bit (a ballot and a
+// scalar count per key cost three times as much).  put(place, key's number, or -1).
+template <int CAP, class Put> X100_DEV void select_row(const uint64_t *key, int n, int n_sel, Put &&put)
 {
     constexpr int KL = CAP / 64;
+    constexpr bool REGS = KL <= 16;   // up to 1024 keys in registers
     const int lane = threadIdx.x & 63, used = (n + 63) >> 6;
-    uint64_t k[KL < 16 ? KL : 16];   // of up to 1024 keys in registers
-    auto at = [&](int u) __attribute__((always_inline)) {
-        if constexpr (KL <= 16) return k[u];
-        else return 64 * u + lane < n ? key[64 * u + lane] : KEY_NONE;
-    };
-    if constexpr (KL <= 16) {
+    uint32_t kh[REGS ? KL : 1], kl[REGS ? KL : 1];
+    auto at = [&](int u) __attribute__((always_inline)) { return 64 * u + lane < n ? key[64 * u + lane] : KEY_NONE; };
+    if constexpr (REGS) {
 #pragma unroll
-        for (int u = 0; u < KL; u++) k[u] = 64 * u + lane < n ? key[64 * u + lane] : KEY_NONE;
-    }
-    auto count = [&](uint64_t from) __attribute__((always_inline)) {   // keys >= from
-        int c = 0;
-        if constexpr (KL <= 16) {
-#pragma unroll
-            for (int u = 0; u < KL; u++)
-                if (u < used) c += __popcll(__ballot(k[u] >= from));
-        } else {
-            for (int u = 0; u < used; u++) c += __popcll(__ballot(at(u) >= from));
+        for (int u = 0; u < KL; u++) {
+            const uint64_t x = at(u);
+            kh[u] = (uint32_t)(x >> 32);
+            kl[u] = (uint32_t)x;
         }
-        return c;
+    }
+    auto count = [&](auto &&is) __attribute__((always_inline)) {
+        int c = 0;
+        if constexpr (REGS) {
+#pragma unroll
+            for (int u = 0; u < KL; u++) c += is(kh[u], kl[u]) ? 1 : 0;
+        } else {
+            for (int u = 0; u < used; u++) {
+                const uint64_t x = at(u);
+                c += is((uint32_t)(x >> 32), (uint32_t)x) ? 1 : 0;
+            }
+        }
+        return wave_sum_u(c);
     };
     uint64_t low = 1;
     int ties = 0;
     if (n > n_sel) {
-        uint64_t y = 0;
+        uint32_t yh = 0, yl = 0;
         bool exact = false;
-        for (int bit = 63; bit >= 0 && !exact; bit--) {
-            const uint64_t from = y | 1ull << bit;
-            const int c = count(from);
-            if (c >= n_sel) y = from;
+        for (int bit = 31; bit >= 0 && !exact; bit--) {
+            const uint32_t from = yh | 1u << bit;
+            const int c = count([&](uint32_t h, uint32_t) __attribute__((always_inline)) { return h >= from; });
+            if (c >= n_sel) yh = from;
             exact = c == n_sel;
         }
-        low = y;
-        if (!exact) ties = n_sel - (y == ~0ull ? 0 : count(y + 1));   // no key is in the list for its value alone
-        if (low == KEY_NONE) {
+        if (!exact) {   // more keys have yh's upper half or a larger one: the first of them by their lower halves
+            const int above = yh == ~0u ? 0 : count([&](uint32_t h, uint32_t) __attribute__((always_inline)) { return h > yh; });
+            int c = 0;
+            for (int bit = 31; bit >= 0 && !exact; bit--) {
+                const uint32_t from = yl | 1u << bit;
+                c = above + count([&](uint32_t h, uint32_t l) __attribute__((always_inline)) { return h == yh && l >= from; });
+                if (c >= n_sel) yl = from;
+                exact = c == n_sel;
+            }
+            if (!exact) ties = n_sel - above - (yl == ~0u ? 0 : count([&](uint32_t h, uint32_t l) __attribute__((always_inline)) { return h == yh && l > yl; }));
+        }
+        low = (uint64_t)yh << 32 | yl;
+        if (low == KEY_NONE) {   // blocks without a page would be among them
             low = 1;
             ties = 0;
         }
@@ -385,18 +406,18 @@ template <int CAP> X100_DEV void select_row(const uint64_t *key, int n, int n_se
         const uint64_t bq = __ballot(x == low);
         const bool take = ties > 0 ? x > low || (x == low && eq + __popcll(bq & below) < ties) : x >= low;
         const uint64_t bt = __ballot(take);
-        if (take) out[at_out + __popcll(bt & below)] = 64 * u + lane;
+        if (take) put(at_out + __popcll(bt & below), 64 * u + lane);
         at_out += __popcll(bt);
         eq += __popcll(bq);
     };
-    if constexpr (KL <= 16) {
+    if constexpr (REGS) {
 #pragma unroll
         for (int u = 0; u < KL; u++)
-            if (u < used) emit(u, k[u]);
+            if (u < used) emit(u, (uint64_t)kh[u] << 32 | kl[u]);
     } else {
         for (int u = 0; u < used; u++) emit(u, at(u));
     }
-    for (int i = at_out + lane; i < n_sel; i += 64) out[i] = -1;
+    for (int i = at_out + lane; i < n_sel; i += 64) put(i, -1);
 }
 
 // Scores of 16 blocks and 16 rows by the fp64 matrix instruction, 4 elements each time: lane (c, g) has elements HD / 4 * g ..
@@ -481,7 +502,7 @@ template <int HD, int AT, int R, int CAP> __global__ __launch_bounds__(RT) void 
             if (pos < 0) {
                 for (int i = lane; i < a.pick.n_sel; i += 64) out[i] = -1;
             } else {
-                select_row<CAP>(key + r * LD, (pos >> psh) + 1, a.pick.n_sel, out);
+                select_row<CAP>(key + r * LD, (pos >> psh) + 1, a.pick.n_sel, [&](int i, int k) __attribute__((always_inline)) { out[i] = k; });
             }
         }
     }
@@ -502,14 +523,14 @@ template <int HD, int AT> hipError_t select_by_size(SelectArgs a, hipStream_t s)
     const int n = (a.b.max_kv - 1) / a.c.page + 1;
     if (a.b.max_q >= MANY && n <= 4096) {
         a.apart = (int64_t)a.b.n_seq * a.b.max_q > a.b.n_rows;
-        const hipError_t e = n <= 512 ? select_rows<HD, AT, 16, 512>(a, s) : n <= 1024 ? select_rows<HD, AT, 16, 1024>(a, s) : select_rows<HD, AT, 4, 4096>(a, s);
+        const hipError_t e = n <= 512 ? select_rows<HD, AT, 16, 512>(a, s) : n <= 1024 ? select_rows<HD, AT, 16, 1024>(a, s) : n <= 2048 ? select_rows<HD, AT, 8, 2048>(a, s) : select_rows<HD, AT, 4, 4096>(a, s);
         if (e != hipSuccess || !a.apart) return e;
     }
     const unsigned grid = (unsigned)((int64_t)a.b.n_rows * a.c.n_head_kv);
-    // few rows: more waves for each (16 x 938 blocks 18.4 us with 4, less with 16)
-    if (n <= 1024 && grid <= 512) k_attn_select<HD, AT, 1024, 1024><<<grid, 1024, 0, s>>>(a);
-    else if (n <= 1024) k_attn_select<HD, AT, 256, 1024><<<grid, 256, 0, s>>>(a);
-    else k_attn_select<HD, AT, 1024, X100_SPARSE_MAX_BLOCKS><<<grid, 1024, 0, s>>>(a);
+    // few rows: more waves for each (16 rows of 938 blocks 19 / 26 us with 16 / 4 waves)
+    if (n <= 1024 && grid <= 512) k_attn_select<HD, AT, 1024, 1024, 8><<<grid, 1024, 0, s>>>(a);
+    else if (n <= 1024) k_attn_select<HD, AT, 256, 1024, 8><<<grid, 256, 0, s>>>(a);
+    else k_attn_select<HD, AT, 1024, X100_SPARSE_MAX_BLOCKS, 8><<<grid, 1024, 0, s>>>(a);
     return hipGetLastError();
 }
 
