@@ -59,7 +59,8 @@ def test_gemm_refusals():
     for M, N in ((0, 300), (8, 0)):
         assert ok_or_no_device(x.gemm_fp8, M, N, 256, fp8(), fp8(), x.T_F32, P, 300, None)
     assert g(M=-1) and g(N=-1) and g(K=0) and g(K=8) and g(K=24) and g(K=-16) and g(K=(1 << 24) + 16)
-    assert g(M=1 << 30, N=1 << 20, a=fp8(ls=1 << 30), ldc=1 << 20)
+    for M, N in ((1 << 18, (1 << 18) + 1), ((1 << 26) + 1, 1), (1, (1 << 26) + 1), (1 << 30, 1 << 20), (2 ** 31 - 1, 2 ** 31 - 1)):
+        assert g(M=M, N=N, a=fp8(ls=1 << 31), ldc=1 << 31)
     for bad in (dict(p=None), dict(p=P + 8), dict(ld=240), dict(ld=264), dict(ld=(1 << 24) + 16), dict(scale=None),
                 dict(scale=P + 1), dict(ls=BIG)):
         assert g(a=fp8(**bad)) and g(w=fp8(**bad))

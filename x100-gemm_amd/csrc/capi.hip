@@ -896,7 +896,9 @@ static bool fp8_operand_ok(const x100_fp8 *x, int K, int64_t least_scales)
 int x100_gemm_fp8_hip(int M, int N, int K, const x100_fp8 *a, const x100_fp8 *w, int c_type, void *c, int64_t ldc,
                       void *stream)
 {
-    if (M < 0 || N < 0 || K < 16 || K % 16 || K > 1 << 24 || (int64_t)M * N / 256 >= (int64_t)1 << 31) return X100_EINVAL;
+    // launches of less than 2^32 threads, for every kind of tile
+    if (M < 0 || N < 0 || M > 1 << 26 || N > 1 << 26 || (int64_t)M * N > (int64_t)1 << 36) return X100_EINVAL;
+    if (K < 16 || K % 16 || K > 1 << 24) return X100_EINVAL;
     if (!fp8_operand_ok(a, K, M) || !fp8_operand_ok(w, K, (K + 127) / 128)) return X100_EINVAL;
     const int e = c_type == X100_T_I32 ? 0 : type_bytes(c_type);
     if (!e || !c || (uintptr_t)c % e || ldc < N || ldc > FP8_MAX_LD) return X100_EINVAL;

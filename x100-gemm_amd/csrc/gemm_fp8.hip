@@ -196,10 +196,10 @@ __global__ __launch_bounds__(64 * WM *WN *WK) void k_fp8_tile(const Fp8Args g, i
 {
     constexpr int NW = WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN;
     constexpr int OA = BM / 8 / NW, OW = BN / 8 / NW, OPS = OA + OW + 1;   // DMA operations of a wave per stage
-    constexpr int WOFF = BM * 128, SOFF = (BM + BN) * 128, SLOT = SOFF + BM * 4;
+    constexpr int WOFF = BM * 128, SOFF = (BM + BN) * 128, SLOT = SOFF + (BM < 64 ? 64 : BM) * 4;
     constexpr int HEAD = FM > 4 ? 3 : 1;   // A operands beside whose products they are issued
-    static_assert(OA * NW * 8 == BM && OW * NW * 8 == BN && BM % 64 == 0 && 128 % (16 * FN) == 0 && NW % 2 == 0 && FN % 2 == 0 &&
-                      FM % 2 == 0 && (WK == 1 || NS > 2), "");
+    static_assert(OA * NW * 8 == BM && OW * NW * 8 == BN && BM % 32 == 0 && 128 % (16 * FN) == 0 && NW % 2 == 0 && FM % 2 == 0 &&
+                      (WK == 1 || NS > 2), "");
     __shared__ __attribute__((aligned(256))) uint8_t smem[WK * NS * SLOT];
     const int lane = threadIdx.x & 63, wk = wave_id() / NW, w = wave_id() % NW, wm = w / WN, wn = w % WN, r = lane & 15, q = lane >> 4;
     // blocks of k, the group's stages, and the block of its last one (beyond the end: a group without one multiplies the
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(64 * WM *WN *WK) void k_fp8_tile(const Fp8Args g, i
     const uint32_t sb = lds_addr(ring);
 
     // DMA: operation p of a wave has tile rows 8 (NW p + w) .. + 7, lane l row l / 8 of them and place l % 8.
-    const int seg = w % (BM / 64);   // the wave's 64 row scales
+    const int seg = w % (BM < 64 ? 1 : BM / 64);   // the wave's 64 row scales
     const uint8_t *ga, *gw;
     const float *gs;
     uint32_t va[OA], vw[OW], vs;
@@ -369,13 +369,13 @@ __global__ __launch_bounds__(64 * WM *WN *WK) void k_fp8_tile(const Fp8Args g, i
     auto store = [&](int sm, int sn) __attribute__((always_inline)) {
         hold();
         const int m = sm + wm * FM * 16 + r, n = sn + wn * FN * 16;
-        if (CT != X100_T_F32 && g.vec8 && n + 16 * FN <= g.N) {
+        if (CT != X100_T_F32 && FN % 2 == 0 && g.vec8 && n + 16 * FN <= g.N) {
             uint16_t *row = (uint16_t *)g.c + (size_t)m * g.ldc + n + 16 * (q & 1) + 8 * (q >> 1);
 #pragma unroll
             for (int i = 0; i < FM; i++) {
 #pragma unroll
                 for (int j = 0; j < FN; j += 2) {
-                    const v4f x = acc[i][j], y = acc[i][j + 1];
+                    const v4f x = acc[i][j], y = acc[i][(j + 1) % FN];
                     uint32_t u[4];
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
@@ -469,17 +469,18 @@ template <int FN, int WK, int WN, int U, int CT> hipError_t few_rows(const Fp8Ar
 // The tiles that there are, and what they cost: us of a round of blocks (one per CU, or `occ`) with s stages, start + s * stage,
 // and, where a CU holds several, of a block's stage in the midst of others.  Fitted to all of them timed at M 17 .. 4096 by
 // N x K of 5120 x 2048, 2048 x 4096, 4096 x 4096 and 4096 x 7168 (bf16; f32 takes 1.6 to 1.8 times as long in all).  us, the others beside the
-// fastest: 64 x 2048 x 4096  64x32 7.1 (64x64 halves 9.0, 64x64 11.0);  128 x 5120 x 2048  64x64 halves 6.6 (64x32 9.5, 64x64 7.4);
-// 512 x 5120 x 2048  64x64 12.5 (128x128 12.4, 64x64 halves 16.8);  1024 x 4096 x 7168  128x128 37 (64x64 49, 128x256 49);
-// 1500 x 5120 x 2048  128x256 20 (128x128 24, 256x256 28);  2048 x 5120 x 2048  256x256 29 (128x128 34, 128x256 35).
+// fastest: 64 x 2048 x 4096  32x32 5.9 (64x32 7.0, 64x64 halves 9.0, 64x64 10.7);  64 x 5120 x 2048  64x32 5.5 (32x32 7.8);
+// 128 x 5120 x 2048  64x64 halves 6.5 (64x32 9.5, 64x64 7.4);  512 x 5120 x 2048  64x64 12.5 (128x128 12.4, 64x64 halves 16.8);
+// 1024 x 4096 x 7168  128x128 37 (64x64 49, 128x256 49);  1500 x 5120 x 2048  128x256 20 (128x128 24, 256x256 28);
+// 2048 x 5120 x 2048  256x256 29 (128x128 34, 128x256 35).
 struct TileCost {
     int bm, bn, wk, occ;
     float start, stage, shared;
 };
-enum { T64X32, T64X64_HALVES, T64X64, T128X128, T128X256, T256X256, TILES };
+enum { T32X32, T64X32, T64X64_HALVES, T64X64, T128X128, T128X256, T256X256, TILES };
 constexpr TileCost TILE_COST[TILES] = {
-    {64, 32, 4, 1, 1.8f, 0.575f, 0.575f}, {64, 64, 2, 1, 1.5f, 0.43f, 0.43f}, {64, 64, 1, 3, 1.2f, 0.29f, 0.215f},
-    {128, 128, 1, 1, 1.7f, 0.6f, 0.6f},   {128, 256, 1, 1, 1.7f, 1.0f, 1.0f}, {256, 256, 1, 1, 2.4f, 1.7f, 1.7f},
+    {32, 32, 4, 1, 1.3f, 0.4f, 0.4f},     {64, 32, 4, 1, 1.8f, 0.575f, 0.575f}, {64, 64, 2, 1, 1.5f, 0.43f, 0.43f}, {64, 64, 1, 3, 1.2f, 0.29f, 0.215f},
+    {128, 128, 1, 1, 1.7f, 0.6f, 0.6f},   {128, 256, 1, 1, 1.7f, 1.0f, 1.0f},   {256, 256, 1, 1, 2.4f, 1.7f, 1.7f},
 };
 
 int best_tile(const Fp8Args &g, bool exact)
@@ -508,6 +509,7 @@ template <int CT> hipError_t gemm(const Fp8Args &g, hipStream_t s)
     // 2048 62 / 55, 8 x 5120 x 2048 5.2 / 5.0, 16 x 2048 x 4096 5.9 / 7.8) and rows to read (1 x 151936 x 2048: 49 / 55).
     if (g.M <= 16) return g.M > 4 && g.N >= 8192 ? few_rows<2, 8, 1, 1, CT>(g, s) : few_rows<1, 8, 1, 1, CT>(g, s);
     switch (best_tile(g, EXACT)) {
+    case T32X32: return tile<2, 1, 1, 2, 4, 4, EXACT, CT>(g, s);
     case T64X32: return tile<2, 2, 2, 1, 4, 3, EXACT, CT>(g, s);
     case T64X64_HALVES: return tile<2, 2, 2, 2, 2, 4, EXACT, CT>(g, s);
     case T64X64: return tile<2, 2, 2, 2, 1, 3, EXACT, CT>(g, s);
