@@ -170,7 +170,8 @@ GEMM = [(1, 1, 16), (1, 16, 128), (1, 5120, 2048), (3, 17, 48), (2, 130, 144), (
 GEMM += [(33, 70, 1808), (18, 33, 656), (64, 4096, 656), (128, 5120, 656), (130, 5100, 400), (17, 64, 400), (300, 5120, 400),
          (130, 5100, 272), (700, 5120, 400), (900, 5130, 1296), (1500, 5120, 400), (2300, 4400, 112), (2048, 5120, 144),
          (2047, 5111, 656), (4100, 4300, 272), (5, 8208, 1040), (16, 9000, 144), (4, 8200, 272), (64, 4200, 1040),
-         (200, 1500, 912), (250, 2000, 1808), (60, 5120, 656)]
+         (200, 1500, 912), (250, 2000, 1808), (60, 5120, 656), (3000, 5120, 144), (2900, 5130, 400), (1550, 5130, 528),
+         (3400, 2100, 1040)]
 
 
 @pytest.mark.parametrize("ct", [ref.F32, ref.F16, ref.BF16])

@@ -467,33 +467,37 @@ template <int FN, int WK, int WN, int U, int CT> hipError_t few_rows(const Fp8Ar
 }
 
 // The tiles that there are, and what they cost: us of a round of blocks (one per CU, or `occ`) with s stages, start + s * stage,
-// and, where a CU holds several, of a block's stage in the midst of others.  Fitted to all of them timed at M 17 .. 4096 by
-// N x K of 5120 x 2048, 2048 x 4096, 4096 x 4096 and 4096 x 7168 (bf16; f32 takes 1.6 to 1.8 times as long in all).  us, the others beside the
-// fastest: 64 x 2048 x 4096  32x32 5.9 (64x32 7.0, 64x64 halves 9.0, 64x64 10.7);  64 x 5120 x 2048  64x32 5.5 (32x32 7.8);
-// 128 x 5120 x 2048  64x64 halves 6.5 (64x32 9.5, 64x64 7.4);  512 x 5120 x 2048  64x64 12.5 (128x128 12.4, 64x64 halves 16.8);
-// 1024 x 4096 x 7168  128x128 37 (64x64 49, 128x256 49);  1500 x 5120 x 2048  128x256 20 (128x128 24, 256x256 28);
-// 2048 x 5120 x 2048  256x256 29 (128x128 34, 128x256 35).
+// and, where a CU holds several, of a block's stage in the midst of others.  From 128 rows on, a stage of a chip that is
+// full takes half as long again as one of a few CUs (the clock).  Fitted to all of them timed at M 17 .. 16381 by N x K of
+// 5120 x 2048, 2048 x 4096, 4096 x 4096 and 4096 x 7168 (bf16; f32 takes 1.6 to 1.8 times as long in all); of 21 sizes from
+// M = 1536 on it takes the fastest each time, of smaller ones one within 5%.  us, the others beside the fastest:
+//   64 x 2048 x 4096    32x32 5.9 (64x32 7.0, 64x64 halves 9.0, 64x64 10.7)     64 x 5120 x 2048   64x32 5.5 (32x32 7.8)
+//   128 x 5120 x 2048   64x64 halves 6.5 (64x32 9.5, 64x64 7.4)                 512 x 5120 x 2048  64x64 12.5 (64x64 halves 16.8)
+//   1024 x 4096 x 7168  128x128 37 (64x64 49, 128x256 49)                       1536 x 5120 x 2048 128x256 22 (128x128 25, 256x256 31)
+//   4096 x 5120 x 2048  192x256 51 (128x256 58, 256x256 58)                     6000 x 5120 x 2048 256x256 67 (192x256 74, 128x256 82)
 struct TileCost {
     int bm, bn, wk, occ;
     float start, stage, shared;
 };
-enum { T32X32, T64X32, T64X64_HALVES, T64X64, T128X128, T128X256, T256X256, TILES };
+enum { T32X32, T64X32, T64X64_HALVES, T64X64, T128X128, T128X256, T192X256, T256X256, TILES };
 constexpr TileCost TILE_COST[TILES] = {
-    {32, 32, 4, 1, 1.3f, 0.4f, 0.4f},     {64, 32, 4, 1, 1.8f, 0.575f, 0.575f}, {64, 64, 2, 1, 1.5f, 0.43f, 0.43f}, {64, 64, 1, 3, 1.2f, 0.29f, 0.215f},
-    {128, 128, 1, 1, 1.7f, 0.6f, 0.6f},   {128, 256, 1, 1, 1.7f, 1.0f, 1.0f},   {256, 256, 1, 1, 2.4f, 1.7f, 1.7f},
+    {32, 32, 4, 1, 1.3f, 0.4f, 0.4f},      {64, 32, 4, 1, 1.8f, 0.575f, 0.575f}, {64, 64, 2, 1, 1.5f, 0.43f, 0.43f},
+    {64, 64, 1, 3, 1.2f, 0.29f, 0.215f},   {128, 128, 1, 1, 1.9f, 0.7f, 0.7f},   {128, 256, 1, 1, 3.0f, 1.12f, 1.12f},
+    {192, 256, 1, 1, 3.3f, 1.5f, 1.5f},    {256, 256, 1, 1, 4.0f, 1.9f, 1.9f},
 };
 
 int best_tile(const Fp8Args &g, bool exact)
 {
-    int best = T64X64;
+    int best = 0;
     float least = 0.0f;
     for (int i = 0; i < TILES; i++) {
-        if (i == T256X256 && (exact || g.K <= 128)) continue;   // its registers; its stream of stages
+        if (i >= T192X256 && (exact || g.K <= 128)) continue;   // their registers; their stream of stages
         const TileCost &t = TILE_COST[i];
-        const int64_t tiles = (int64_t)((g.M + t.bm - 1) / t.bm) * ((g.N + t.bn - 1) / t.bn);
-        const float per_cu = (float)((tiles + 255) / 256), s = (float)(((g.K + 127) / 128 + t.wk - 1) / t.wk);
-        const float rounds = (float)((tiles + 256 * t.occ - 1) / (256 * t.occ));
-        const float a = rounds * (t.start + s * t.stage), b = t.start + per_cu * s * t.shared, us = a > b ? a : b;
+        const int64_t tiles = (int64_t)((g.M + t.bm - 1) / t.bm) * ((g.N + t.bn - 1) / t.bn), round = 256 * t.occ;
+        const int64_t rounds = (tiles + round - 1) / round, per_cu = (tiles + 255) / 256;
+        const float full = i >= T128X128 ? 0.65f + 0.35f * (float)tiles / (float)(rounds * round) : 1.0f;
+        const float s = full * (float)(((g.K + 127) / 128 + t.wk - 1) / t.wk);
+        const float a = (float)rounds * (t.start + s * t.stage), b = t.start + (float)per_cu * s * t.shared, us = a > b ? a : b;
         if (i == 0 || us < least) {
             best = i;
             least = us;
@@ -515,8 +519,13 @@ template <int CT> hipError_t gemm(const Fp8Args &g, hipStream_t s)
     case T64X64: return tile<2, 2, 2, 2, 1, 3, EXACT, CT>(g, s);
     case T128X128: return tile<4, 2, 2, 4, 1, 3, EXACT, CT>(g, s);
     case T128X256: return tile<4, 4, 2, 4, 1, 3, EXACT, CT>(g, s);
+    case T192X256:
+        if constexpr (!EXACT) return tile<6, 4, 2, 4, 1, 2, false, CT>(g, s);
+        break;
+    case T256X256:
+        if constexpr (!EXACT) return tile<8, 4, 2, 4, 1, 2, false, CT>(g, s);
+        break;
     }
-    if constexpr (!EXACT) return tile<8, 4, 2, 4, 1, 2, false, CT>(g, s);
     return hipErrorInvalidValue;
 }
 
