@@ -473,3 +473,39 @@ def test_means_of_refused_sequences(dev):
     K, _ = t.c.decode(t.kb, t.vb)
     want = sp.means(t.c, K, rows_of(t), t.table, old)
     assert len(rows_of(t)) == 19 and np.array_equal(d.cpu().numpy().view(np.uint16), want)
+
+
+@acts
+def test_select_prompts_ties_and_odd_scores(dev, act):
+    """As test_select_ties_and_odd_scores and the blocks without a page, for rows that are taken together."""
+    inf = 0x7c00 if act == ref.F16 else 0x7f80
+    for seed, n_head, n_kv, hd in ((30, 4, 2, 64), (31, 3, 1, 128)):
+        p = Pick(seed, n_head, n_kv, hd, 16, act, [20, 17, 8, 33, 40], [640, 300, 900, 33, 560])
+        m = p.mean.reshape(p.c.n_pages, n_kv, hd)
+        m[p.table[0, 5:20]] = m[p.table[0, 5]]
+        m[p.table[1, :18]] = 0
+        m[p.table[1, 3:15:2], :, 0] = 0x8000
+        m[p.table[2, 4], :, 3], m[p.table[2, 9], :, 3], m[p.table[2, 11], :, 3] = inf, inf | 0x8000, inf | 0x200
+        m[p.table[4, :30]] = inf | 0x200
+        p.table[2, 20:40] = -1
+        p.table[3, 0] = p.c.n_pages
+        p.table[4, 32] = 1 << 30
+        for n_sel, first, last in ((1, 0, 1), (4, 0, 1), (5, 2, 3), (9, 1, 1), (20, 1, 2), (39, 0, 1), (40, 1, 1), (64, 30, 34)):
+            p.check(n_sel, first, last)
+
+
+@acts
+def test_select_prompts_of_close_scores(dev, act):
+    """Scores that share their upper bits: all digits of the keys are needed."""
+    p = Pick(32, 2, 1, 64, 16, act, [24], [1600])
+    m = p.mean.reshape(p.c.n_pages, 64)
+    base = m[p.table[0, 0]].copy()
+    for i in range(100):
+        m[p.table[0, i]] = base
+        m[p.table[0, i], 7] = (0x0001 if act == ref.F16 else 0x2000) + i % 23      # tiny next to the others
+    for n_sel in (3, 10, 50):
+        p.check(n_sel, 0, 1)
+    p.q_start, p.q_lens, p.kv_lens, p.n_rows, p.max_q = np.array([0, 1]), [1], [1600], 1, 1
+    p.qbits = p.qbits[:1]
+    for n_sel in (3, 10, 50):
+        p.check(n_sel, 0, 1)

@@ -377,7 +377,32 @@ template <int CAP, class Put> X100_DEV void select_row(const uint64_t *key, int 
     if (n > n_sel) {
         uint32_t yh = 0, yl = 0;
         bool exact = false;
-        for (int bit = 31; bit >= 0 && !exact; bit--) {
+        // The upper 12 bits (a score's sign and exponent) lie at or little below those of the largest key that is not
+        // always taken: these few values first, instead of 12 bits.
+        int top = 31;
+        {
+            uint32_t mx = 0;
+            if constexpr (REGS) {
+#pragma unroll
+                for (int u = 0; u < KL; u++) mx = kh[u] != ~0u ? max(mx, kh[u]) : mx;
+            } else {
+                for (int u = 0; u < used; u++) {
+                    const uint32_t h = (uint32_t)(at(u) >> 32);
+                    mx = h != ~0u ? max(mx, h) : mx;
+                }
+            }
+            uint32_t from = ((uint32_t)wave_max_iu((int)(mx ^ 0x80000000u)) ^ 0x80000000u) & 0xfff00000u;
+            for (int k = 0; k < 4 && from; k++, from -= 0x00100000u) {
+                const int c = count([&](uint32_t h, uint32_t) __attribute__((always_inline)) { return h >= from; });
+                exact = c == n_sel;
+                if (c >= n_sel) {
+                    yh = from;
+                    top = 19;
+                    break;
+                }
+            }
+        }
+        for (int bit = top; bit >= 0 && !exact; bit--) {
             const uint32_t from = yh | 1u << bit;
             const int c = count([&](uint32_t h, uint32_t) __attribute__((always_inline)) { return h >= from; });
             if (c >= n_sel) yh = from;
