@@ -84,9 +84,8 @@ template <int HD, int AT, bool Q4, bool SP> __global__ __launch_bounds__(256, Q4
             entry[k] = i < a.n_sel ? list[i] : -1;
             before[k] = i < a.n_sel && i ? list[i - 1] : -1;
         }
-        s = paged_find(a.b, row0);
-        if (s >= a.b.n_seq) return;
-        const PagedSeq q = paged_seq(a.b, s);
+        PagedSeq q;
+        s = paged_find(a.b, row0, q);
         if (!q.holds(row0)) return;
         const int at = q.position(row0), own = at >> psh;   // below 0: no block
         const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;

@@ -33,6 +33,24 @@ X100_DEV int paged_find(const x100_kv_batch &b, int r)
     return paged_search(b.n_seq, [&](int s) { return b.q_start[s] <= r; });
 }
 
+// The same with the sequence's entries (q_len < 0 where there is none).  Of up to 64 sequences a lane has one, so that the
+// search and the entries are one trip to memory.
+X100_DEV int paged_find(const x100_kv_batch &b, int r, PagedSeq &q)
+{
+    if (b.n_seq > 64) {
+        const int s = paged_find(b, r);
+        q = s < b.n_seq ? paged_seq(b, s) : PagedSeq{0, -1, 0};
+        return s;
+    }
+    const int lane = threadIdx.x & 63, i = min(lane, b.n_seq - 1);
+    const int q0 = b.q_start[i], q1 = b.q_start[i + 1], kv = b.kv_len[i];
+    const int s = __popcll(__ballot(lane < b.n_seq && q1 <= r));
+    const int at = min(s, b.n_seq - 1);
+    q = paged_checked(__builtin_amdgcn_readlane(q0, at), __builtin_amdgcn_readlane(q1, at), __builtin_amdgcn_readlane(kv, at), b.n_rows, b.max_q, b.max_kv);
+    if (s >= b.n_seq) q.q_len = -1;
+    return s;
+}
+
 // Bytes of one head's part of a page, K or V.
 template <int HD, bool Q4> X100_DEV constexpr int page_head_bytes(int page) { return Q4 ? page * HD * 5 / 8 : page * HD * 2; }
 

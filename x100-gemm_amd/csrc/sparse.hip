@@ -57,8 +57,8 @@ X100_DEV void elems_q4(uint32_t w, uint32_t dm, float (&v)[8])
     }
 }
 
-// Mean keys.  A block looks at 16 rows of the batch and one KV head.  Its lanes look the rows up side by side: one search
-// for the first one's sequence, the other rows' by how many of the next 64 sequences end before them.  A single page (a
+// Mean keys.  A block looks at 16 rows of the batch and one KV head.  Its lanes look the rows up side by side: by how many of
+// 64 sequences end before them, from the first row's on (one search) where there are more.  A single page (a
 // prompt's, or one of a batch of single tokens) is shared by the block's waves, of several each wave takes every fourth.  Lane l
 // has the elements 8 (l % L) .. + 7 of every (64 / L)-th row of its part (L lanes per row), 4 loads on their way.
 // Bound by the chain row -> sequence -> page -> keys for single tokens, by the keys' bytes for prompts.
@@ -70,26 +70,33 @@ __global__ __launch_bounds__(256) void k_kv_means(const x100_kv_cfg c, const x10
     __shared__ double s_sum[3][HD];
     const int lane = threadIdx.x & 63, w = wave_id(), kvh = blockIdx.x % c.n_head_kv, row0 = blockIdx.x / c.n_head_kv * MEAN_ROWS;
     // lane i < 16: page of row row0 + i, if that row is the last of a page (else -1)
-    const int s0 = paged_find(b, row0);
+    const int s0 = b.n_seq <= 64 ? 0 : paged_find(b, row0);
     if (s0 >= b.n_seq) return;
     const int row = row0 + min(lane, MEAN_ROWS - 1);
-    const int end = s0 + lane < b.n_seq ? b.q_start[s0 + lane + 1] : 0x7fffffff;   // of the lane's sequence
+    // sequence s0 + lane, and by its end the sequence of each row
+    const int i0 = min(s0 + lane, b.n_seq - 1);
+    const int start = b.q_start[i0], end = b.q_start[i0 + 1], kv = b.kv_len[i0];
     int s = s0;
 #pragma unroll
     for (int i = 0; i < MEAN_ROWS; i++) {
-        const int past = __popcll(__ballot(end <= row0 + i));
+        const int past = __popcll(__ballot(s0 + lane < b.n_seq && end <= row0 + i));
         if (row == row0 + i) s = s0 + past;
     }
+    const int from = min(s - s0, 63);
+    PagedSeq q = paged_checked(__shfl(start, from, 64), __shfl(end, from, 64), __shfl(kv, from, 64), b.n_rows, b.max_q, b.max_kv);
     // more than 64 sequences without rows in between, or q_start in disorder: each row by itself
-    if (__any(s - s0 >= 64 || (s < b.n_seq && !paged_seq(b, s).holds(row)))) {
+    if (__any(s < b.n_seq && (s - s0 >= 64 || !q.holds(row)))) {
         for (int i = 0; i < MEAN_ROWS; i++) {
-            const int f = paged_find(b, row0 + i);
-            if (row == row0 + i) s = f;
+            PagedSeq f;
+            const int at = paged_find(b, row0 + i, f);
+            if (row == row0 + i) {
+                s = at;
+                q = f;
+            }
         }
     }
     int page = -1;
     if (lane < MEAN_ROWS && s < b.n_seq) {
-        const PagedSeq q = paged_seq(b, s);
         const int pos = q.holds(row) ? q.position(row) : -1;
         if (pos >= 0 && (pos & (c.page - 1)) == c.page - 1) page = paged_page(c, b, s, pos);
     }
@@ -291,9 +298,8 @@ template <int HD, int AT, int NT, int CAP, int U> __global__ __launch_bounds__(N
         for (int h = 0; h < G; h++) y += (double)act2f<AT>(a.q[(size_t)row * a.ldq + (size_t)(kvh * G + h) * HD + e]);
         sh.q[e] = y;
     }
-    const int s = paged_find(a.b, row);
-    if (s >= a.b.n_seq) return;
-    const PagedSeq q = paged_seq(a.b, s);
+    PagedSeq q;
+    const int s = paged_find(a.b, row, q);
     if (!q.holds(row) || (a.apart && q.q_len >= MANY)) return;
     const int pos = q.position(row), own = pos >> psh;   // below 0: no position
     int *out = a.sel + ((size_t)row * n_kv + kvh) * a.pick.n_sel;
@@ -456,9 +462,9 @@ template <int HD, int AT, int R, int CAP> __global__ __launch_bounds__(RT) void 
     const int n_kv = a.c.n_head_kv, kvh = blockIdx.x % n_kv, row0 = blockIdx.x / n_kv * R;
     const int G = a.c.n_head / n_kv, psh = __builtin_ctz(a.c.page), rows = min(R, a.b.n_rows - row0);
     for (int j = 0; j < rows;) {
-        const int s = paged_find(a.b, row0 + j);
+        PagedSeq q;
+        const int s = paged_find(a.b, row0 + j, q);
         if (s >= a.b.n_seq) return;
-        const PagedSeq q = paged_seq(a.b, s);
         if (!q.holds(row0 + j)) {
             j++;
             continue;
