@@ -25,12 +25,12 @@ X100_DEV double xor32_d(double v)
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
     return __builtin_bit_cast(double, (uint64_t)xor32_u((uint32_t)(u >> 32)) << 32 | xor32_u((uint32_t)u));
 }
-// sum over each group of L = 8 or 16 lanes, in all of them
+// sum over each group of L = 4, 8 or 16 lanes, in all of them
 template <int L> X100_DEV double sum_lanes(double v)
 {
     v += dpp_d<0xB1>(v);
     v += dpp_d<0x4E>(v);
-    v += dpp_d<0x141>(v);
+    if constexpr (L > 4) v += dpp_d<0x141>(v);
     if constexpr (L == 16) v += dpp_d<0x140>(v);
     return v;
 }
@@ -283,13 +283,14 @@ template <int NT, int CAP> X100_DEV void select_keys(SelectLds<NT, CAP> &sh, int
     for (int i = total + t; i < n_sel; i += NT) out[i] = -1;
 }
 
-// L lanes have a mean, 8 elements each, 64 / L means per load of a wave, U loads on their way; each row and KV head reads its
-// own means.  Bound by latency: row -> sequence -> pages -> means -> digits.  us, 16 rows of up to 938 blocks: 4.1 to the
-// position, 16 with the scores, 19.3 with the lists (by one wave, a bit at a time, 21).  Scores in fp32 by the 16-bit
-// matrix cores with bounds of their error, and fp64 for what the bounds leave, were no faster (20).
+// L lanes have a mean, 16 elements each, 64 / L means of a wave at a time, U times on their way; each row and KV head reads its
+// own means.  Bound by latency (row -> sequence -> pages -> means -> digits) and, on the few CUs that few rows keep busy, by
+// fp64: 16 rows of up to 938 blocks 17.4 us (8 elements per lane and a longer sum over lanes 19.1), of which 4 to the
+// position and 4 for the lists.  Scores in fp32 by the 16-bit matrix cores with bounds of their error, and fp64 for what the bounds
+// leave, were no faster (20).
 template <int HD, int AT, int NT, int CAP, int U> __global__ __launch_bounds__(NT) void k_attn_select(const SelectArgs a)
 {
-    constexpr int L = HD / 8, NG = NT / L;
+    constexpr int L = HD / 16, NG = NT / L;
     __shared__ SelectLds<NT, CAP> sh;
     const int t = threadIdx.x, lane = t & 63, n_kv = a.c.n_head_kv, kvh = blockIdx.x % n_kv, row = blockIdx.x / n_kv;
     const int G = a.c.n_head / n_kv, psh = __builtin_ctz(a.c.page), l = lane % L;
@@ -310,29 +311,34 @@ template <int HD, int AT, int NT, int CAP, int U> __global__ __launch_bounds__(N
     const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
     for (int i = t; i <= own; i += NT) sh.key[i] = (uint32_t)tab[i];
     __syncthreads();
-    double x[8];
+    double x[16];
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = sh.q[8 * l + e];
-    const v4u *means = (const v4u *)(a.means + (size_t)kvh * HD) + l;
+    for (int e = 0; e < 16; e++) x[e] = sh.q[16 * l + e];
+    const v4u *means = (const v4u *)(a.means + (size_t)kvh * HD) + 2 * l;
     for (int b0 = t / L; b0 - lane / L <= own; b0 += U * NG) {   // the lanes of a wave together
-        v4u m[U];
+        v4u m[U][2];
         int pg[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (b0 - lane / L + u * NG > own) continue;   // all lanes'
             pg[u] = b0 + u * NG <= own ? (int)(uint32_t)sh.key[b0 + u * NG] : -1;
             if (pg[u] < 0 || pg[u] >= a.c.n_pages) pg[u] = -1;
-            m[u] = means[(size_t)max(pg[u], 0) * n_kv * L];
+            m[u][0] = means[(size_t)max(pg[u], 0) * n_kv * (HD / 8)];
+            m[u][1] = means[(size_t)max(pg[u], 0) * n_kv * (HD / 8) + 1];
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int b = b0 + u * NG;
             if (b - lane / L > own) continue;
             float v[8];
-            elems16<AT>(m[u], v);
-            double y = 0.0;
+            elems16<AT>(m[u][0], v);
+            double y = 0.0, z = 0.0;
 #pragma unroll
             for (int e = 0; e < 8; e++) y = __builtin_fma(x[e], (double)v[e], y);
+            elems16<AT>(m[u][1], v);
+#pragma unroll
+            for (int e = 0; e < 8; e++) z = __builtin_fma(x[8 + e], (double)v[e], z);
+            y += z;
             y = sum_lanes<L>(y);
             const bool always = b < a.pick.n_first || b > own - a.pick.n_last;
             if (l == 0 && b <= own) sh.key[b] = pg[u] < 0 ? KEY_NONE : (always ? KEY_ALWAYS : score_key(y));
@@ -558,10 +564,10 @@ template <int HD, int AT> hipError_t select_by_size(SelectArgs a, hipStream_t s)
         if (e != hipSuccess || !a.apart) return e;
     }
     const unsigned grid = (unsigned)((int64_t)a.b.n_rows * a.c.n_head_kv);
-    // few rows: more waves for each (16 rows of 938 blocks 19 / 26 us with 16 / 4 waves)
-    if (n <= 1024 && grid <= 512) k_attn_select<HD, AT, 1024, 1024, 8><<<grid, 1024, 0, s>>>(a);
-    else if (n <= 1024) k_attn_select<HD, AT, 256, 1024, 8><<<grid, 256, 0, s>>>(a);
-    else k_attn_select<HD, AT, 1024, X100_SPARSE_MAX_BLOCKS, 8><<<grid, 1024, 0, s>>>(a);
+    // few rows: more waves for each (16 rows of 938 blocks 17 us with 16 waves, half as much again with 4)
+    if (n <= 1024 && grid <= 512) k_attn_select<HD, AT, 1024, 1024, 2><<<grid, 1024, 0, s>>>(a);
+    else if (n <= 1024) k_attn_select<HD, AT, 256, 1024, 2><<<grid, 256, 0, s>>>(a);
+    else k_attn_select<HD, AT, 1024, X100_SPARSE_MAX_BLOCKS, 4><<<grid, 1024, 0, s>>>(a);
     return hipGetLastError();
 }
 
