@@ -13,8 +13,8 @@
  *
  * All pointers are device pointers unless they are the argument structures; every call is asynchronous on
  * stream and capturable.  All arguments that the host can see are checked before anything is enqueued.
- * X100_EINVAL also for a batch that no launch can hold: n_rows * n_head_kv of 2^28 and more in the means, of 2^24 in the
- * selection, and n_rows * n_head_kv * splits of 2^24 in the attention (splits: 1 where there are many rows).
+ * X100_EINVAL also for a batch that no launch can hold: n_rows * n_head_kv above 2^28 - 2^14 in the means, of 2^24 and
+ * more in the selection, and n_rows * n_head_kv * splits of 2^24 in the attention (splits: 1 where there are many rows).
  * Outputs overlap no input.
  */
 #ifndef X100_HIP_SPARSE_H

@@ -97,3 +97,10 @@ def test_workspace():
     assert x.kv_means(cfg(), batch(n_rows=0), A, A) == 0
     assert x.attn_select(cfg(), batch(n_seq=0), pick(), A, LD, A, A) == 0
     assert x.attn_sparse(cfg(), batch(n_rows=0), A, LD, A, 2 * A, 1.0, A, 4, A, LD) == 0
+
+
+def test_means_of_a_full_launch():
+    """Blocks of 16 rows: n_rows is rounded up before it meets the launch's limit (262143 rows by 1024 heads)."""
+    c = cfg(n_head=1024, n_head_kv=1024, head_dim=64)
+    for n in (262129, 262143, 262144):
+        means(c, batch(n_rows=n, max_q=n, max_kv=256, table_ld=4))

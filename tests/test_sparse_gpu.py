@@ -509,3 +509,31 @@ def test_select_prompts_of_close_scores(dev, act):
     p.qbits = p.qbits[:1]
     for n_sel in (3, 10, 50):
         p.check(n_sel, 0, 1)
+
+
+def test_select_of_more_blocks_than_a_launch_holds(dev):
+    """4097 rows by 1024 KV heads, with tables of more than 1024 pages: 2^22 + 2^10 lists of blocks of 1024 threads."""
+    n, nh, pages = 4097, 1024, 3
+    g = np.random.default_rng(27)
+    cfg = x.KvCfg(nh, nh, 64, 16, pages, x.T_BF16, x.T_BF16)
+    kv_lens = g.integers(1, 49, n)
+    table = np.full((n, 1025), -1)
+    table[:, :3] = np.argsort(g.random((n, 3)), axis=1)
+    torch.manual_seed(27)
+    q = torch.randn(n, nh, 64, dtype=torch.bfloat16, device=dev)
+    means = torch.randn(pages, nh, 64, dtype=torch.bfloat16, device=dev)
+    sel = torch.full((n, nh, 2), -99, dtype=torch.int32, device=dev)
+    qs, kl, tab = dev_i32(np.arange(n + 1)), dev_i32(kv_lens), dev_i32(table)
+    b = x.KvBatch(n, n, 1, 16 * 1025, 1025, qs.data_ptr(), kl.data_ptr(), tab.data_ptr())
+    x.attn_select(cfg, b, x.KvSel(2, 0, 1), q.data_ptr(), nh * 64, means.data_ptr(), sel.data_ptr(), stream())
+    torch.cuda.synchronize()
+    # of blocks 0 and 1 the better one, where the row's own is 2
+    better = torch.empty(n, nh, dtype=torch.int32, device=dev)
+    for r in range(0, n, 512):
+        pg = tab[r:r + 512, :2].long()
+        y = [(q[r:r + 512].double() * means[pg[:, i]].double()).sum(-1) for i in (0, 1)]
+        better[r:r + 512] = (y[1] > y[0]).int()
+    own = dev_i32((kv_lens - 1) // 16)[:, None].expand(n, nh)
+    zero = torch.zeros_like(better)
+    want = torch.stack([torch.where(own == 2, better, zero), torch.where(own == 0, zero - 1, own)], -1)
+    assert torch.equal(sel, want)

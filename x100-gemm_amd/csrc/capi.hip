@@ -1087,7 +1087,7 @@ int x100_kv_means_hip(const x100_kv_cfg *c, const x100_kv_batch *b, const void *
 {
     if (!kv_cfg_ok(c) || !kv_batch_ok(c, b) || !k_pool || ((uintptr_t)k_pool & 255) || !means || ((uintptr_t)means & 15))
         return X100_EINVAL;
-    if ((int64_t)b->n_rows * c->n_head_kv >= (int64_t)1 << 28) return X100_EINVAL;   // past one launch
+    if ((int64_t)b->n_rows * c->n_head_kv > (1 << 28) - (1 << 14)) return X100_EINVAL;   // one launch, also with n_rows rounded up to 16
     if (b->n_seq == 0 || b->n_rows == 0) return X100_OK;
     int rc = check_device();
     if (rc) return rc;

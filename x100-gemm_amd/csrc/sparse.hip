@@ -4,6 +4,8 @@
 // mean of their scores with the block's keys.  It is summed in fp64 (a product of two 16-bit numbers is exact there): two
 // blocks change places only where their scores differ by 1e-16 of their terms, so the lists do not depend on an order
 // of sums, and equal blocks tie.
+#include <algorithm>
+
 #include "paged.h"
 #include "x100_internal.h"
 
@@ -178,6 +180,7 @@ struct SelectArgs {
     const uint16_t *means;
     int *sel;
     bool apart;   // sequences of MANY rows are k_attn_select_rows's, the others k_attn_select's
+    unsigned block0;   // first block of this launch
 };
 
 // Sequences of so many rows in a batch go to the kernel that takes rows together, the others' rows are taken one by one.
@@ -292,8 +295,8 @@ template <int HD, int AT, int NT, int CAP, int U> __global__ __launch_bounds__(N
 {
     constexpr int L = HD / 16, NG = NT / L;
     __shared__ SelectLds<NT, CAP> sh;
-    const int t = threadIdx.x, lane = t & 63, n_kv = a.c.n_head_kv, kvh = blockIdx.x % n_kv, row = blockIdx.x / n_kv;
-    const int G = a.c.n_head / n_kv, psh = __builtin_ctz(a.c.page), l = lane % L;
+    const int t = threadIdx.x, lane = t & 63, n_kv = a.c.n_head_kv, kvh = (a.block0 + blockIdx.x) % n_kv;
+    const int row = (a.block0 + blockIdx.x) / n_kv, G = a.c.n_head / n_kv, psh = __builtin_ctz(a.c.page), l = lane % L;
     for (int e = t; e < HD; e += NT) {   // the sum of the queries
         double y = 0.0;
         for (int h = 0; h < G; h++) y += (double)act2f<AT>(a.q[(size_t)row * a.ldq + (size_t)(kvh * G + h) * HD + e]);
@@ -564,10 +567,12 @@ template <int HD, int AT> hipError_t select_by_size(SelectArgs a, hipStream_t s)
         if (e != hipSuccess || !a.apart) return e;
     }
     const unsigned grid = (unsigned)((int64_t)a.b.n_rows * a.c.n_head_kv);
-    // few rows: more waves for each (16 rows of 938 blocks 17 us with 16 waves, half as much again with 4)
+    // few rows: more waves for each (16 rows of 938 blocks, 8 elements per lane: 19 / 26 us with 16 / 4 waves)
     if (n <= 1024 && grid <= 512) k_attn_select<HD, AT, 1024, 1024, 2><<<grid, 1024, 0, s>>>(a);
     else if (n <= 1024) k_attn_select<HD, AT, 256, 1024, 2><<<grid, 256, 0, s>>>(a);
-    else k_attn_select<HD, AT, 1024, X100_SPARSE_MAX_BLOCKS, 4><<<grid, 1024, 0, s>>>(a);
+    else
+        for (constexpr unsigned MOST = 1u << 21; a.block0 < grid; a.block0 += MOST)   // launches of less than 2^32 threads
+            k_attn_select<HD, AT, 1024, X100_SPARSE_MAX_BLOCKS, 4><<<std::min(MOST, grid - a.block0), 1024, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -591,7 +596,7 @@ hipError_t x100_kv_means_launch(const x100_kv_cfg &c, const x100_kv_batch &b, co
 hipError_t x100_attn_select_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const x100_kv_sel &pick, const void *q,
                                    int64_t ldq, const void *means, int *sel, hipStream_t s)
 {
-    const SelectArgs a = {c, b, pick, (const uint16_t *)q, ldq, (const uint16_t *)means, sel, false};
+    const SelectArgs a = {c, b, pick, (const uint16_t *)q, ldq, (const uint16_t *)means, sel, false, 0};
     if (c.head_dim == 64) return c.act_type == X100_T_F16 ? select_by_size<64, X100_T_F16>(a, s) : select_by_size<64, X100_T_BF16>(a, s);
     return c.act_type == X100_T_F16 ? select_by_size<128, X100_T_F16>(a, s) : select_by_size<128, X100_T_BF16>(a, s);
 }
