@@ -537,3 +537,19 @@ def test_select_of_more_blocks_than_a_launch_holds(dev):
     zero = torch.zeros_like(better)
     want = torch.stack([torch.where(own == 2, better, zero), torch.where(own == 0, zero - 1, own)], -1)
     assert torch.equal(sel, want)
+
+
+@acts
+@pytest.mark.parametrize("blocks", [40, 1500, 3000, 5000])
+def test_select_few_sequences_under_wide_bounds(dev, act, blocks):
+    """Prompts and single tokens of few sequences, some empty, refused or before position 0, in a batch of many rows."""
+    kv = 16 * blocks
+    q_lens = [1, 9, 0, 7, 30, 2, 8, 20, 5, 1]
+    kv_lens = [kv, kv - 5, 33, 300, kv - 17, -1, 5, kv + 1, 3, 170]
+    p = Pick(28, 4, 2, 64, 16, act, q_lens, kv_lens, tail_rows=30, max_q=25, max_kv=kv)
+    got = p.check(6, 1, 2)
+    first = [int(n) for n in p.q_start]
+    assert (got[first[4]:first[5]] == -99).all()          # 30 rows > max_q
+    assert (got[first[5]:first[6]] == -99).all() and (got[first[7]:first[8]] == -99).all()
+    assert (got[first[6]:first[6] + 3] == -1).all() and (got[first[8]:first[8] + 2] == -1).all()
+    assert (got[first[-1]:] == -99).all()

@@ -180,6 +180,7 @@ struct SelectArgs {
     const uint16_t *means;
     int *sel;
     bool apart;   // sequences of MANY rows are k_attn_select_rows's, the others k_attn_select's
+    bool by_seq;  // k_attn_select's units are MANY - 1 rows of each sequence (else the batch's rows)
     unsigned block0;   // first block of this launch
 };
 
@@ -295,16 +296,25 @@ template <int HD, int AT, int NT, int CAP, int U> __global__ __launch_bounds__(N
 {
     constexpr int L = HD / 16, NG = NT / L;
     __shared__ SelectLds<NT, CAP> sh;
-    const int t = threadIdx.x, lane = t & 63, n_kv = a.c.n_head_kv, kvh = (a.block0 + blockIdx.x) % n_kv;
-    const int row = (a.block0 + blockIdx.x) / n_kv, G = a.c.n_head / n_kv, psh = __builtin_ctz(a.c.page), l = lane % L;
+    const int t = threadIdx.x, lane = t & 63, l = lane % L, n_kv = a.c.n_head_kv, unit = (a.block0 + blockIdx.x) / n_kv;
+    const int kvh = (a.block0 + blockIdx.x) % n_kv, G = a.c.n_head / n_kv, psh = __builtin_ctz(a.c.page);
+    int row = unit, s = 0;
+    PagedSeq q;
+    if (a.by_seq) {
+        s = unit / (MANY - 1);
+        q = paged_seq(a.b, s);
+        row = q.q0 + unit % (MANY - 1);
+        if (!q.holds(row) || q.q_len >= MANY) return;
+    }
     for (int e = t; e < HD; e += NT) {   // the sum of the queries
         double y = 0.0;
         for (int h = 0; h < G; h++) y += (double)act2f<AT>(a.q[(size_t)row * a.ldq + (size_t)(kvh * G + h) * HD + e]);
         sh.q[e] = y;
     }
-    PagedSeq q;
-    const int s = paged_find(a.b, row, q);
-    if (!q.holds(row) || (a.apart && q.q_len >= MANY)) return;
+    if (!a.by_seq) {
+        s = paged_find(a.b, row, q);
+        if (!q.holds(row) || (a.apart && q.q_len >= MANY)) return;
+    }
     const int pos = q.position(row), own = pos >> psh;   // below 0: no position
     int *out = a.sel + ((size_t)row * n_kv + kvh) * a.pick.n_sel;
     if (pos < 0) {
@@ -362,29 +372,18 @@ constexpr int RT = 512;   // threads
 template <int CAP, class Put> X100_DEV void select_row(const uint64_t *key, int n, int n_sel, Put &&put)
 {
     constexpr int KL = CAP / 64;
-    constexpr bool REGS = KL <= 16;   // up to 1024 keys in registers
     const int lane = threadIdx.x & 63, used = (n + 63) >> 6;
-    uint32_t kh[REGS ? KL : 1], kl[REGS ? KL : 1];
-    auto at = [&](int u) __attribute__((always_inline)) { return 64 * u + lane < n ? key[64 * u + lane] : KEY_NONE; };
-    if constexpr (REGS) {
+    uint32_t kh[KL], kl[KL];
 #pragma unroll
-        for (int u = 0; u < KL; u++) {
-            const uint64_t x = at(u);
-            kh[u] = (uint32_t)(x >> 32);
-            kl[u] = (uint32_t)x;
-        }
+    for (int u = 0; u < KL; u++) {
+        const uint64_t x = 64 * u + lane < n ? key[64 * u + lane] : KEY_NONE;
+        kh[u] = (uint32_t)(x >> 32);
+        kl[u] = (uint32_t)x;
     }
     auto count = [&](auto &&is) __attribute__((always_inline)) {
         int c = 0;
-        if constexpr (REGS) {
 #pragma unroll
-            for (int u = 0; u < KL; u++) c += is(kh[u], kl[u]) ? 1 : 0;
-        } else {
-            for (int u = 0; u < used; u++) {
-                const uint64_t x = at(u);
-                c += is((uint32_t)(x >> 32), (uint32_t)x) ? 1 : 0;
-            }
-        }
+        for (int u = 0; u < KL; u++) c += is(kh[u], kl[u]) ? 1 : 0;
         return wave_sum_u(c);
     };
     uint64_t low = 1;
@@ -397,15 +396,8 @@ template <int CAP, class Put> X100_DEV void select_row(const uint64_t *key, int 
         int top = 31;
         {
             uint32_t mx = 0;
-            if constexpr (REGS) {
 #pragma unroll
-                for (int u = 0; u < KL; u++) mx = kh[u] != ~0u ? max(mx, kh[u]) : mx;
-            } else {
-                for (int u = 0; u < used; u++) {
-                    const uint32_t h = (uint32_t)(at(u) >> 32);
-                    mx = h != ~0u ? max(mx, h) : mx;
-                }
-            }
+            for (int u = 0; u < KL; u++) mx = kh[u] != ~0u ? max(mx, kh[u]) : mx;
             uint32_t from = ((uint32_t)wave_max_iu((int)(mx ^ 0x80000000u)) ^ 0x80000000u) & 0xfff00000u;
             for (int k = 0; k < 4 && from; k++, from -= 0x00100000u) {
                 const int c = count([&](uint32_t h, uint32_t) __attribute__((always_inline)) { return h >= from; });
@@ -450,19 +442,18 @@ template <int CAP, class Put> X100_DEV void select_row(const uint64_t *key, int 
         at_out += __popcll(bt);
         eq += __popcll(bq);
     };
-    if constexpr (REGS) {
 #pragma unroll
-        for (int u = 0; u < KL; u++)
-            if (u < used) emit(u, (uint64_t)kh[u] << 32 | kl[u]);
-    } else {
-        for (int u = 0; u < used; u++) emit(u, at(u));
-    }
+    for (int u = 0; u < KL; u++)
+        if (u < used) emit(u, (uint64_t)kh[u] << 32 | kl[u]);
     for (int i = at_out + lane; i < n_sel; i += 64) put(i, -1);
 }
 
 // Scores of 16 blocks and 16 rows by the fp64 matrix instruction, 4 elements each time: lane (c, g) has elements HD / 4 * g ..
 // of row c's query sum (in registers) and of block c's mean; every sum adds its terms in the same order.  Waves take every
-// eighth tile of blocks, the next one's means on their way, then every eighth row's list.
+// eighth tile of blocks, the next one's means on their way, then every eighth row's list, its keys in registers.  2001 rows on 500
+// blocks, 4 KV heads: 42 us, of which 8 to the query sums (each wave its own: 21), 22 scores (13 of them the matrix
+// instructions'), 11 lists.  Of 1025 .. 2048 blocks a block has room for 8 rows' keys, up to 4096 for 4: the rest of the 16
+// columns is idle (2000 rows on 1024 / 1032 / 2063 blocks 72 / 134 / 576 us).
 template <int HD, int AT, int R, int CAP> __global__ __launch_bounds__(RT) void k_attn_select_rows(const SelectArgs a)
 {
     constexpr int KS = HD / 4, LD = CAP + 1, NW = RT / 64;   // steps; keys of a row, off the banks of the one before
@@ -483,19 +474,6 @@ template <int HD, int AT, int R, int CAP> __global__ __launch_bounds__(RT) void 
         if (a.apart && q.q_len < MANY) continue;
         const int own_last = q.position(first + n - 1) >> psh;   // the last row's own block (below 0: no position)
         const int own = q.position(first + min(c, n - 1)) >> psh;
-        double x[KS];
-#pragma unroll
-        for (int e = 0; e < KS; e++) x[e] = 0.0;
-        for (int h = 0; h < G; h++) {
-            const v4u *p = (const v4u *)(a.q + (size_t)(first + min(c, n - 1)) * a.ldq + (size_t)(kvh * G + h) * HD + KS * g);
-#pragma unroll
-            for (int i = 0; i < KS / 8; i++) {
-                float v[8];
-                elems16<AT>(p[i], v);
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[8 * i + e] += (double)v[e];
-            }
-        }
         const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
         const uint16_t *means = a.means + (size_t)kvh * HD + KS * g;
         auto page = [&](int t) __attribute__((always_inline)) {
@@ -508,9 +486,35 @@ template <int HD, int AT, int R, int CAP> __global__ __launch_bounds__(RT) void 
 #pragma unroll
             for (int i = 0; i < KS / 8; i++) m[i] = p[i];
         };
-        __syncthreads();   // the lists of the rows before are made
         int pg = page(w), pn = page(w + NW);
         load(pg);
+        // The sums of the queries by all threads, E elements each, through LDS where the keys will be.
+        constexpr int E = 16 * HD / RT, LQ = HD + 2;
+        static_assert(R * LQ <= R * LD && (E == 2 || E == 4), "");
+        double *const qsum = (double *)key;
+        __syncthreads();   // the lists of the rows before are made
+        if (const int qr = threadIdx.x / (HD / E), e0 = threadIdx.x % (HD / E) * E; qr < n) {
+            const uint16_t *p = a.q + (size_t)(first + qr) * a.ldq + (size_t)kvh * G * HD + e0;
+            double y[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) y[e] = 0.0;
+#pragma unroll 4
+            for (int h = 0; h < G; h++, p += HD) {
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    const uint32_t u = ((const uint32_t *)p)[e / 2];
+                    y[e] += (double)act2f<AT>(u & 0xffffu);
+                    y[e + 1] += (double)act2f<AT>(u >> 16);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < E; e++) qsum[qr * LQ + e0 + e] = y[e];
+        }
+        __syncthreads();
+        double x[KS];
+#pragma unroll
+        for (int e = 0; e < KS; e++) x[e] = qsum[min(c, n - 1) * LQ + KS * g + e];
+        __syncthreads();
         for (int t = w; 16 * t <= own_last; t += NW) {
             const uint64_t ok = __ballot(pg >= 0);
             v4u now[KS / 8];
@@ -556,7 +560,8 @@ template <int HD, int AT, int R, int CAP> hipError_t select_rows(const SelectArg
 }
 
 // Which kernels a batch takes: rows together, where a sequence can have MANY (and their keys find room in LDS); one by one,
-// where none can.  Where the bounds leave room for both, both run and leave the other's sequences alone; where every
+// where none can.  Where the bounds leave room for both, both run and leave the other's sequences alone (with few sequences,
+// the second looks at MANY - 1 rows of each: by rows of the batch, 2 x 1000 rows on 1563 blocks took 65 us more); where every
 // sequence may have max_q rows, the first takes whatever there is.
 template <int HD, int AT> hipError_t select_by_size(SelectArgs a, hipStream_t s)
 {
@@ -566,7 +571,8 @@ template <int HD, int AT> hipError_t select_by_size(SelectArgs a, hipStream_t s)
         const hipError_t e = n <= 512 ? select_rows<HD, AT, 16, 512>(a, s) : n <= 1024 ? select_rows<HD, AT, 16, 1024>(a, s) : n <= 2048 ? select_rows<HD, AT, 8, 2048>(a, s) : select_rows<HD, AT, 4, 4096>(a, s);
         if (e != hipSuccess || !a.apart) return e;
     }
-    const unsigned grid = (unsigned)((int64_t)a.b.n_rows * a.c.n_head_kv);
+    a.by_seq = a.apart && (int64_t)a.b.n_seq * (MANY - 1) < a.b.n_rows;
+    const unsigned grid = (unsigned)((int64_t)(a.by_seq ? a.b.n_seq * (MANY - 1) : a.b.n_rows) * a.c.n_head_kv);
     // few rows: more waves for each (16 rows of 938 blocks, 8 elements per lane: 19 / 26 us with 16 / 4 waves)
     if (n <= 1024 && grid <= 512) k_attn_select<HD, AT, 1024, 1024, 2><<<grid, 1024, 0, s>>>(a);
     else if (n <= 1024) k_attn_select<HD, AT, 256, 1024, 2><<<grid, 256, 0, s>>>(a);
@@ -596,7 +602,7 @@ hipError_t x100_kv_means_launch(const x100_kv_cfg &c, const x100_kv_batch &b, co
 hipError_t x100_attn_select_launch(const x100_kv_cfg &c, const x100_kv_batch &b, const x100_kv_sel &pick, const void *q,
                                    int64_t ldq, const void *means, int *sel, hipStream_t s)
 {
-    const SelectArgs a = {c, b, pick, (const uint16_t *)q, ldq, (const uint16_t *)means, sel, false, 0};
+    const SelectArgs a = {c, b, pick, (const uint16_t *)q, ldq, (const uint16_t *)means, sel, false, false, 0};
     if (c.head_dim == 64) return c.act_type == X100_T_F16 ? select_by_size<64, X100_T_F16>(a, s) : select_by_size<64, X100_T_BF16>(a, s);
     return c.act_type == X100_T_F16 ? select_by_size<128, X100_T_F16>(a, s) : select_by_size<128, X100_T_BF16>(a, s);
 }
