@@ -553,3 +553,21 @@ def test_select_few_sequences_under_wide_bounds(dev, act, blocks):
     assert (got[first[5]:first[6]] == -99).all() and (got[first[7]:first[8]] == -99).all()
     assert (got[first[6]:first[6] + 3] == -1).all() and (got[first[8]:first[8] + 2] == -1).all()
     assert (got[first[-1]:] == -99).all()
+
+
+@acts
+@pytest.mark.parametrize("blocks", [1100, 2100])
+def test_select_prompts_of_many_blocks_with_ties(dev, act, blocks):
+    """Equal scores, scores that share their upper bits, and blocks without a page, on long contexts."""
+    p = Pick(33, 4, 2, 64, 16, act, [18, 9], [16 * blocks, 16 * blocks - 100])
+    m = p.mean.reshape(p.c.n_pages, 2, 64)
+    m[p.table[0, 100:900]] = m[p.table[0, 100]]
+    base = m[p.table[1, 0]].copy()
+    for i in range(1000):
+        m[p.table[1, i]] = base
+        m[p.table[1, i], :, 7] = (0x0001 if act == ref.F16 else 0x2000) + i % 23      # tiny next to the others
+    p.table[1, 1000:blocks - 7] = -1
+    for n_sel, first, last in ((3, 0, 1), (60, 1, 2), (300, 0, 1), (512, 2, 2)):
+        p.check(n_sel, first, last)
+    p.qbits[:] = 0
+    p.check(40, 1, 1)

@@ -366,31 +366,30 @@ template <int HD, int AT, int NT, int CAP, int U> __global__ __launch_bounds__(N
 typedef double v4d __attribute__((ext_vector_type(4)));
 constexpr int RT = 512;   // threads
 
-// The list of a row's n keys by one wave, key i in lane i % 64: the threshold one bit at a time, the upper half of the keys
-// first, until as many keys are left as the list takes.  Counts are kept per lane and summed once per bit (a ballot and a
-// scalar count per key cost three times as much).  put(place, key's number, or -1).
-template <int CAP, class Put> X100_DEV void select_row(const uint64_t *key, int n, int n_sel, Put &&put)
+// The list of a row by one wave from the upper halves of its n keys, key i in lane i % 64: the threshold one bit at a time,
+// until as many keys are left as the list takes.  Counts are kept per lane and summed once per bit (a ballot and a scalar
+// count per key cost three times as much).  Where keys with the threshold's upper half are in the list and others are not
+// (their scores differ by less than 1e-6, one row in thousands, or are equal), low(i) gives the lower halves of
+// these keys, which take the places of the upper ones.  put(place, key's number, or -1).
+template <int CAP, class Low, class Put> X100_DEV void select_row(uint32_t *key, int n, int n_sel, Low &&low, Put &&put)
 {
     constexpr int KL = CAP / 64;
     const int lane = threadIdx.x & 63, used = (n + 63) >> 6;
-    uint32_t kh[KL], kl[KL];
+    uint32_t kh[KL];
 #pragma unroll
-    for (int u = 0; u < KL; u++) {
-        const uint64_t x = 64 * u + lane < n ? key[64 * u + lane] : KEY_NONE;
-        kh[u] = (uint32_t)(x >> 32);
-        kl[u] = (uint32_t)x;
-    }
-    auto count = [&](auto &&is) __attribute__((always_inline)) {
+    for (int u = 0; u < KL; u++) kh[u] = 64 * u + lane < n ? key[64 * u + lane] : (uint32_t)(KEY_NONE >> 32);
+    auto count = [&](uint32_t from) __attribute__((always_inline)) {   // keys >= from
         int c = 0;
 #pragma unroll
-        for (int u = 0; u < KL; u++) c += is(kh[u], kl[u]) ? 1 : 0;
+        for (int u = 0; u < KL; u++) c += kh[u] >= from ? 1 : 0;
         return wave_sum_u(c);
     };
-    uint64_t low = 1;
+    uint32_t yh = 1, yl = 0;   // selected: keys > yh, and of those that are yh all (exact), or by their lower halves those > yl
+    bool exact = true;         // and the first `ties` that are yl
     int ties = 0;
     if (n > n_sel) {
-        uint32_t yh = 0, yl = 0;
-        bool exact = false;
+        yh = 0;
+        exact = false;
         // The upper 12 bits (a score's sign and exponent) lie at or little below those of the largest key that is not
         // always taken: these few values first, instead of 12 bits.
         int top = 31;
@@ -400,7 +399,7 @@ template <int CAP, class Put> X100_DEV void select_row(const uint64_t *key, int 
             for (int u = 0; u < KL; u++) mx = kh[u] != ~0u ? max(mx, kh[u]) : mx;
             uint32_t from = ((uint32_t)wave_max_iu((int)(mx ^ 0x80000000u)) ^ 0x80000000u) & 0xfff00000u;
             for (int k = 0; k < 4 && from; k++, from -= 0x00100000u) {
-                const int c = count([&](uint32_t h, uint32_t) __attribute__((always_inline)) { return h >= from; });
+                const int c = count(from);
                 exact = c == n_sel;
                 if (c >= n_sel) {
                     yh = from;
@@ -411,53 +410,65 @@ template <int CAP, class Put> X100_DEV void select_row(const uint64_t *key, int 
         }
         for (int bit = top; bit >= 0 && !exact; bit--) {
             const uint32_t from = yh | 1u << bit;
-            const int c = count([&](uint32_t h, uint32_t) __attribute__((always_inline)) { return h >= from; });
+            const int c = count(from);
             if (c >= n_sel) yh = from;
             exact = c == n_sel;
         }
-        if (!exact) {   // more keys have yh's upper half or a larger one: the first of them by their lower halves
-            const int above = yh == ~0u ? 0 : count([&](uint32_t h, uint32_t) __attribute__((always_inline)) { return h > yh; });
-            int c = 0;
-            for (int bit = 31; bit >= 0 && !exact; bit--) {
-                const uint32_t from = yl | 1u << bit;
-                c = above + count([&](uint32_t h, uint32_t l) __attribute__((always_inline)) { return h == yh && l >= from; });
-                if (c >= n_sel) yl = from;
-                exact = c == n_sel;
-            }
-            if (!exact) ties = n_sel - above - (yl == ~0u ? 0 : count([&](uint32_t h, uint32_t l) __attribute__((always_inline)) { return h == yh && l > yl; }));
+        if (yh == 0) {   // fewer blocks with a page than the list takes
+            yh = 1;
+            exact = true;
         }
-        low = (uint64_t)yh << 32 | yl;
-        if (low == KEY_NONE) {   // blocks without a page would be among them
-            low = 1;
-            ties = 0;
+        if (!exact) {   // a lower half is at least 1 here, 0: not one of these keys
+            const int need = n_sel - count(yh + 1);   // yh is not all ones: those keys are no more than n_sel
+            for (int i = lane; i < n; i += 64) key[i] = key[i] == yh ? max(low(i, yh), 1u) : 0;
+            auto count_low = [&](uint32_t from) __attribute__((always_inline)) {
+                int c = 0;
+                for (int i = lane; i < n; i += 64) c += key[i] >= from ? 1 : 0;
+                return wave_sum_u(c);
+            };
+            int c = 0;
+            for (int bit = 31; bit >= 0 && c != need; bit--) {
+                const uint32_t from = yl | 1u << bit;
+                c = count_low(from);
+                if (c >= need) yl = from;
+            }
+            ties = c == need ? n : need - (yl == ~0u ? 0 : count_low(yl + 1));
         }
     }
     int at_out = 0, eq = 0;
     const uint64_t below = (1ull << lane) - 1;
-    auto emit = [&](int u, uint64_t x) __attribute__((always_inline)) {
-        const uint64_t bq = __ballot(x == low);
-        const bool take = ties > 0 ? x > low || (x == low && eq + __popcll(bq & below) < ties) : x >= low;
+#pragma unroll
+    for (int u = 0; u < KL; u++) {
+        if (u >= used) continue;
+        bool take = kh[u] >= yh;
+        if (!exact) {
+            const uint32_t l = 64 * u + lane < n ? key[64 * u + lane] : 0;
+            const bool tied = kh[u] == yh && l == yl;
+            const uint64_t bq = __ballot(tied);
+            take = kh[u] > yh || (kh[u] == yh && l > yl) || (tied && eq + __popcll(bq & below) < ties);
+            eq += __popcll(bq);
+        }
         const uint64_t bt = __ballot(take);
         if (take) put(at_out + __popcll(bt & below), 64 * u + lane);
         at_out += __popcll(bt);
-        eq += __popcll(bq);
-    };
-#pragma unroll
-    for (int u = 0; u < KL; u++)
-        if (u < used) emit(u, (uint64_t)kh[u] << 32 | kl[u]);
+    }
     for (int i = at_out + lane; i < n_sel; i += 64) put(i, -1);
 }
 
 // Scores of 16 blocks and 16 rows by the fp64 matrix instruction, 4 elements each time: lane (c, g) has elements HD / 4 * g ..
 // of row c's query sum (in registers) and of block c's mean; every sum adds its terms in the same order.  Waves take every
-// eighth tile of blocks, the next one's means on their way, then every eighth row's list, its keys in registers.  2001 rows on 500
-// blocks, 4 KV heads: 42 us, of which 8 to the query sums (each wave its own: 21), 22 scores (13 of them the matrix
-// instructions'), 11 lists.  Of 1025 .. 2048 blocks a block has room for 8 rows' keys, up to 4096 for 4: the rest of the 16
-// columns is idle (2000 rows on 1024 / 1032 / 2063 blocks 72 / 134 / 576 us).
+// eighth tile of blocks, the next one's means on their way, then every eighth row's list.  The upper halves of the keys are kept:
+// whole ones of more than 1024 blocks would leave no room for 16 rows, and the rest of the 16 columns idle (2000 rows on 1032 /
+// 2063 blocks, 4 KV heads: 80 / 241 us, with whole keys 134 / 576).  2001 rows on 500 blocks: 40 us, of which 8 to the
+// query sums (21 where each wave makes its own), 22 scores (13 of them the matrix instructions'), 10 lists (all scores equal: 200;
+// whole keys 40).
 template <int HD, int AT, int R, int CAP> __global__ __launch_bounds__(RT) void k_attn_select_rows(const SelectArgs a)
 {
     constexpr int KS = HD / 4, LD = CAP + 1, NW = RT / 64;   // steps; keys of a row, off the banks of the one before
-    __shared__ uint64_t key[R * LD];
+    constexpr int E = 16 * HD / RT, LQ = HD + 2;             // a thread's elements of the query sums, and their rows in LDS
+    static_assert(E == 2 || E == 4, "");
+    __shared__ uint32_t key[R * LD];   // upper halves
+    __shared__ double qsum[R * LQ];
     const int lane = threadIdx.x & 63, w = wave_id(), c = lane & 15, g = lane >> 4;
     const int n_kv = a.c.n_head_kv, kvh = blockIdx.x % n_kv, row0 = blockIdx.x / n_kv * R;
     const int G = a.c.n_head / n_kv, psh = __builtin_ctz(a.c.page), rows = min(R, a.b.n_rows - row0);
@@ -488,10 +499,7 @@ template <int HD, int AT, int R, int CAP> __global__ __launch_bounds__(RT) void 
         };
         int pg = page(w), pn = page(w + NW);
         load(pg);
-        // The sums of the queries by all threads, E elements each, through LDS where the keys will be.
-        constexpr int E = 16 * HD / RT, LQ = HD + 2;
-        static_assert(R * LQ <= R * LD && (E == 2 || E == 4), "");
-        double *const qsum = (double *)key;
+        // the sums of the queries, by all threads
         __syncthreads();   // the lists of the rows before are made
         if (const int qr = threadIdx.x / (HD / E), e0 = threadIdx.x % (HD / E) * E; qr < n) {
             const uint16_t *p = a.q + (size_t)(first + qr) * a.ldq + (size_t)kvh * G * HD + e0;
@@ -514,7 +522,6 @@ template <int HD, int AT, int R, int CAP> __global__ __launch_bounds__(RT) void 
         double x[KS];
 #pragma unroll
         for (int e = 0; e < KS; e++) x[e] = qsum[min(c, n - 1) * LQ + KS * g + e];
-        __syncthreads();
         for (int t = w; 16 * t <= own_last; t += NW) {
             const uint64_t ok = __ballot(pg >= 0);
             v4u now[KS / 8];
@@ -536,7 +543,7 @@ template <int HD, int AT, int R, int CAP> __global__ __launch_bounds__(RT) void 
                 const int b = 16 * t + 4 * e + g;
                 const bool always = b < a.pick.n_first || b > own - a.pick.n_last;
                 const double z = y[0][e] + y[1][e];
-                if (c < n && b < CAP) key[c * LD + b] = !(ok >> (4 * e + g) & 1) ? KEY_NONE : (always ? KEY_ALWAYS : score_key(z));
+                if (c < n && b < CAP) key[c * LD + b] = (uint32_t)((!(ok >> (4 * e + g) & 1) ? KEY_NONE : (always ? KEY_ALWAYS : score_key(z))) >> 32);
             }
         }
         __syncthreads();
@@ -546,7 +553,21 @@ template <int HD, int AT, int R, int CAP> __global__ __launch_bounds__(RT) void 
             if (pos < 0) {
                 for (int i = lane; i < a.pick.n_sel; i += 64) out[i] = -1;
             } else {
-                select_row<CAP>(key + r * LD, (pos >> psh) + 1, a.pick.n_sel, [&](int i, int k) __attribute__((always_inline)) { out[i] = k; });
+                // the lower half of block b's key; its upper half, summed in another order, may be the next one to yh
+                auto low = [&](int b, uint32_t yh) {
+                    const v4u *p = (const v4u *)(a.means + ((size_t)tab[b] * n_kv + kvh) * HD);
+                    double y = 0.0;
+                    for (int i = 0; i < HD / 8; i++) {
+                        float v[8];
+                        elems16<AT>(p[i], v);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) y = __builtin_fma(qsum[r * LQ + 8 * i + e], (double)v[e], y);
+                    }
+                    const uint64_t x = score_key(y);
+                    const uint32_t h = (uint32_t)(x >> 32);
+                    return h == yh ? (uint32_t)x : (h > yh ? ~0u : 0u);
+                };
+                select_row<CAP>(key + r * LD, (pos >> psh) + 1, a.pick.n_sel, low, [&](int i, int k) __attribute__((always_inline)) { out[i] = k; });
             }
         }
     }
@@ -568,7 +589,7 @@ template <int HD, int AT> hipError_t select_by_size(SelectArgs a, hipStream_t s)
     const int n = (a.b.max_kv - 1) / a.c.page + 1;
     if (a.b.max_q >= MANY && n <= 4096) {
         a.apart = (int64_t)a.b.n_seq * a.b.max_q > a.b.n_rows;
-        const hipError_t e = n <= 512 ? select_rows<HD, AT, 16, 512>(a, s) : n <= 1024 ? select_rows<HD, AT, 16, 1024>(a, s) : n <= 2048 ? select_rows<HD, AT, 8, 2048>(a, s) : select_rows<HD, AT, 4, 4096>(a, s);
+        const hipError_t e = n <= 512 ? select_rows<HD, AT, 16, 512>(a, s) : n <= 1024 ? select_rows<HD, AT, 16, 1024>(a, s) : n <= 2048 ? select_rows<HD, AT, 16, 2048>(a, s) : select_rows<HD, AT, 8, 4096>(a, s);
         if (e != hipSuccess || !a.apart) return e;
     }
     a.by_seq = a.apart && (int64_t)a.b.n_seq * (MANY - 1) < a.b.n_rows;
