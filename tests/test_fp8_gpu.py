@@ -236,3 +236,64 @@ def test_same_bits_and_graph(dev, M, N, K):
         x.gemm_fp8(M, N, K, fa, fw, x.T_F32, c[0].data_ptr(), N, stream())
         torch.cuda.synchronize()
         assert torch.equal(c[0], c[2])
+
+
+@pytest.mark.parametrize("ct", [ref.F32, ref.F16, ref.BF16])
+@pytest.mark.parametrize("M", [1, 9, 17, 40, 72, 129, 137, 1505, 1537, 2057, 3080, 4097, 6009])
+def test_gemm_rows_behind_are_left(dev, M, ct):
+    """Rows that end inside every kind of tile: those behind M keep what they held, and the last ones are right."""
+    N, K = 5120, 272
+    g = np.random.default_rng(M)
+    a, da, sa, w, dw, sw = operands(g, M, N, K)
+    if ct == ref.F16:
+        sw = sw * np.float32(1.0 / 4096)
+    dsa, dsw = torch.from_numpy(sa).cuda(), torch.from_numpy(sw).cuda()
+    c = torch.full((M + 300, N), 77.0, dtype=fr.TT[ct], device=dev)
+    x.gemm_fp8(M, N, K, x.Fp8(da.data_ptr(), K, dsa.data_ptr(), M), x.Fp8(dw.data_ptr(), K, dsw.data_ptr(), sw.shape[1]), ct,
+               c.data_ptr(), N, stream())
+    assert (c[M:] == 77).all()
+    r = slice(max(0, M - 40), M)
+    want, size = fr.product(a[r], np.ascontiguousarray(sa[:, r]), w, sw)
+    far = np.abs(c[r].double().cpu().numpy() - want)
+    assert (far <= fr.product_bound(K, want, size, ct)).all()
+
+
+@pytest.mark.parametrize("ct", [ref.F16, ref.BF16])
+@pytest.mark.parametrize("M,N,K", [(1, 40, 144), (20, 40, 144), (300, 5120, 400), (1500, 5120, 400), (2900, 5120, 400), (6000, 5120, 272)])
+def test_gemm_nan_16_bits(dev, M, N, K, ct):
+    """A NaN code reaches its row or column, also by the 8-bit instruction, and nothing else."""
+    g = np.random.default_rng(4)
+    a, da, sa, w, dw, sw = operands(g, M, N, K)
+    m, n = M - 1, N // 2
+    da[m, K - 1] = 0x7f
+    dw[n, 3] = 0xff
+    dsa, dsw = torch.from_numpy(sa).cuda(), torch.from_numpy(sw / 4096).cuda()
+    c = torch.zeros(M, N, dtype=fr.TT[ct], device=dev)
+    x.gemm_fp8(M, N, K, x.Fp8(da.data_ptr(), K, dsa.data_ptr(), M), x.Fp8(dw.data_ptr(), K, dsw.data_ptr(), sw.shape[1]), ct,
+               c.data_ptr(), N, stream())
+    want = torch.zeros(M, N, dtype=torch.bool, device=dev)
+    want[m, :] = True
+    want[:, n] = True
+    assert torch.equal(torch.isnan(c), want)
+
+
+def test_a_large_product_captured(dev):
+    """The persistent tiles in a graph, replayed over new codes beside eager calls on two streams: the same bits."""
+    M, N, K = 6001, 5120, 400
+    g = np.random.default_rng(9)
+    a, da, sa, w, dw, sw = operands(g, M, N, K)
+    dsa, dsw = torch.from_numpy(sa).cuda(), torch.from_numpy(sw).cuda()
+    fa, fw = x.Fp8(da.data_ptr(), K, dsa.data_ptr(), M), x.Fp8(dw.data_ptr(), K, dsw.data_ptr(), sw.shape[1])
+    c = [torch.zeros(M, N, dtype=torch.bfloat16, device=dev) for _ in range(3)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x.gemm_fp8(M, N, K, fa, fw, x.T_BF16, c[2].data_ptr(), N, torch.cuda.current_stream().cuda_stream)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        da.copy_(da.flip(0).contiguous())
+        torch.cuda.synchronize()
+        x.gemm_fp8(M, N, K, fa, fw, x.T_BF16, c[1].data_ptr(), N, side.cuda_stream)
+        graph.replay()
+        x.gemm_fp8(M, N, K, fa, fw, x.T_BF16, c[0].data_ptr(), N, stream())
+        torch.cuda.synchronize()
+        assert torch.equal(c[0], c[1]) and torch.equal(c[0], c[2]) and not torch.isnan(c[0]).any()

@@ -365,26 +365,45 @@ __global__ __launch_bounds__(64 * WM *WN *WK) void k_fp8_tile(const Fp8Args g, i
         to = to + SLOT == NS * SLOT ? 0 : to + SLOT;
     };
     // The tile's results from row sm, column sn.  16 bits: a lane has columns 4 q .. + 3 of its row of every product; lane
-    // groups of two neighbouring products exchange theirs, so that a lane has 8 consecutive columns of one.
+    // groups of two neighbouring products exchange theirs, so that a lane has 8 consecutive columns of one.  Of 64 columns
+    // (a line of 128 bytes) lanes r and r + 8 then exchange half lines, so that a store has whole lines of 8 rows, which the
+    // L2s need not keep (16381 x 5120 x 2048: 168 us with half lines, 162 with half lines past the L2s, 155 so, and 135 without
+    // results; with what reads them next 16384 x 2048 x 4096 173 -> 169, 4096 x 2048 x 4096 as before).  32 bits are
+    // stored as they lie: lines were 5% slower (4096^3), past the L2s 5 to 9%.
     auto store = [&](int sm, int sn) __attribute__((always_inline)) {
         hold();
         const int m = sm + wm * FM * 16 + r, n = sn + wn * FN * 16;
         if (CT != X100_T_F32 && FN % 2 == 0 && g.vec8 && n + 16 * FN <= g.N) {
-            uint16_t *row = (uint16_t *)g.c + (size_t)m * g.ldc + n + 16 * (q & 1) + 8 * (q >> 1);
+            constexpr int T = CT == X100_T_F32 ? X100_T_F16 : CT, HALVES = (FN + 1) / 2;   // 32 columns each
+            constexpr bool LINES = HALVES == 2;
+            const bool up = LINES && r >= 8;
+            const int ms = up ? m - 8 : m;
+            uint16_t *row = (uint16_t *)g.c + (size_t)ms * g.ldc + n + 16 * (q & 1) + 8 * (q >> 1) + (up ? 32 : 0);
 #pragma unroll
             for (int i = 0; i < FM; i++) {
+                v4u o[HALVES];
 #pragma unroll
-                for (int j = 0; j < FN; j += 2) {
-                    const v4f x = acc[i][j], y = acc[i][(j + 1) % FN];
-                    uint32_t u[4];
+                for (int h = 0; h < HALVES; h++) {
+                    const v4f x = acc[i][2 * h], y = acc[i][(2 * h + 1) % FN];
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        constexpr int T = CT == X100_T_F32 ? X100_T_F16 : CT;
                         const auto z = __builtin_amdgcn_permlane16_swap(pack2<T>(x[2 * e], x[2 * e + 1]), pack2<T>(y[2 * e], y[2 * e + 1]), false, false);
-                        u[e] = z[0];
-                        u[2 + e] = z[1];
+                        o[h][e] = z[0];
+                        o[h][2 + e] = z[1];
                     }
-                    if (m + 16 * i < g.M) *(v4u *)(row + 16 * j) = v4u{u[0], u[1], u[2], u[3]};
+                }
+                if constexpr (LINES) {
+                    v4u a, b;   // of rows ms and ms + 8
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const uint32_t t = (uint32_t)dpp_i<0x128>(0, (int)(up ? o[0][e] : o[1][e]));   // lane l ^ 8's
+                        a[e] = up ? t : o[0][e];
+                        b[e] = up ? o[1][e] : t;
+                    }
+                    if (ms + 16 * i < g.M) __builtin_nontemporal_store(a, (v4u *)row);
+                    if (ms + 16 * i + 8 < g.M) __builtin_nontemporal_store(b, (v4u *)(row + 8 * g.ldc));
+                } else {
+                    if (m + 16 * i < g.M) *(v4u *)row = o[0];
                 }
                 row += 16 * g.ldc;
                 __builtin_amdgcn_sched_barrier(0);
