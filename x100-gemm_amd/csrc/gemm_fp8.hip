@@ -488,12 +488,12 @@ template <int FN, int WK, int WN, int U, int CT> hipError_t few_rows(const Fp8Ar
 // The tiles that there are, and what they cost: us of a round of blocks (one per CU, or `occ`) with s stages, start + s * stage,
 // and, where a CU holds several, of a block's stage in the midst of others.  From 128 rows on, a stage of a chip that is
 // full takes half as long again as one of a few CUs (the clock).  Fitted to all of them timed at M 17 .. 16381 by N x K of
-// 5120 x 2048, 2048 x 4096, 4096 x 4096 and 4096 x 7168 (bf16; f32 takes 1.6 to 1.8 times as long in all); of 21 sizes from
-// M = 1536 on it takes the fastest each time, of smaller ones one within 5%.  us, the others beside the fastest:
-//   64 x 2048 x 4096    32x32 5.9 (64x32 7.0, 64x64 halves 9.0, 64x64 10.7)     64 x 5120 x 2048   64x32 5.5 (32x32 7.8)
-//   128 x 5120 x 2048   64x64 halves 6.5 (64x32 9.5, 64x64 7.4)                 512 x 5120 x 2048  64x64 12.5 (64x64 halves 16.8)
-//   1024 x 4096 x 7168  128x128 37 (64x64 49, 128x256 49)                       1536 x 5120 x 2048 128x256 22 (128x128 25, 256x256 31)
-//   4096 x 5120 x 2048  192x256 51 (128x256 58, 256x256 58)                     6000 x 5120 x 2048 256x256 67 (192x256 74, 128x256 82)
+// 5120 x 2048, 2048 x 4096, 4096 x 4096 and 4096 x 7168 (bf16; f32 takes 1.6 to 1.8 times as long in all); of 38 sizes from
+// M = 256 on it takes the fastest of those timed each time (f32: within 3%), of smaller ones one within 5%.  us, the others beside it:
+//   64 x 2048 x 4096    32x32 5.9 (64x32 7.0, 64x64 halves 9.0, 64x64 10.7)      64 x 5120 x 2048   64x32 5.5 (32x32 7.8)
+//   128 x 5120 x 2048   64x64 halves 6.5 (64x32 9.5, 64x64 7.4)                  384 x 5120 x 2048  64x64 9.4 (64x64 halves 12, 128x128 12)
+//   768 x 5120 x 2048   128x128 12.8 (64x64 18, 128x256 18)                      1280 x 5120 x 2048 128x256 19 (128x128 23, 192x256 24)
+//   4096 x 5120 x 2048  192x256 48 (128x256 54, 256x256 56)                      6000 x 5120 x 2048 256x256 62 (192x256 71, 128x256 74)
 struct TileCost {
     int bm, bn, wk, occ;
     float start, stage, shared;
@@ -501,8 +501,8 @@ struct TileCost {
 enum { T32X32, T64X32, T64X64_HALVES, T64X64, T128X128, T128X256, T192X256, T256X256, TILES };
 constexpr TileCost TILE_COST[TILES] = {
     {32, 32, 4, 1, 1.3f, 0.4f, 0.4f},      {64, 32, 4, 1, 1.8f, 0.575f, 0.575f}, {64, 64, 2, 1, 1.5f, 0.43f, 0.43f},
-    {64, 64, 1, 3, 1.2f, 0.29f, 0.215f},   {128, 128, 1, 1, 1.9f, 0.7f, 0.7f},   {128, 256, 1, 1, 3.0f, 1.12f, 1.12f},
-    {192, 256, 1, 1, 3.3f, 1.5f, 1.5f},    {256, 256, 1, 1, 4.0f, 1.9f, 1.9f},
+    {64, 64, 1, 3, 1.2f, 0.29f, 0.215f},   {128, 128, 1, 1, 1.9f, 0.6f, 0.6f},   {128, 256, 1, 1, 2.6f, 1.05f, 1.05f},
+    {192, 256, 1, 1, 3.0f, 1.38f, 1.38f},  {256, 256, 1, 1, 3.4f, 1.72f, 1.72f},
 };
 
 int best_tile(const Fp8Args &g, bool exact)
@@ -536,7 +536,7 @@ template <int CT> hipError_t gemm(const Fp8Args &g, hipStream_t s)
     case T64X32: return tile<2, 2, 2, 1, 4, 3, EXACT, CT>(g, s);
     case T64X64_HALVES: return tile<2, 2, 2, 2, 2, 4, EXACT, CT>(g, s);
     case T64X64: return tile<2, 2, 2, 2, 1, 3, EXACT, CT>(g, s);
-    case T128X128: return tile<4, 2, 2, 4, 1, 3, EXACT, CT>(g, s);
+    case T128X128: return tile<2, 4, 4, 2, 1, 3, EXACT, CT>(g, s);
     case T128X256: return tile<4, 4, 2, 4, 1, 3, EXACT, CT>(g, s);
     case T192X256:
         if constexpr (!EXACT) return tile<6, 4, 2, 4, 1, 2, false, CT>(g, s);
