@@ -297,3 +297,11 @@ def test_a_large_product_captured(dev):
         x.gemm_fp8(M, N, K, fa, fw, x.T_BF16, c[0].data_ptr(), N, stream())
         torch.cuda.synchronize()
         assert torch.equal(c[0], c[1]) and torch.equal(c[0], c[2]) and not torch.isnan(c[0]).any()
+
+
+@pytest.mark.parametrize("ct", [ref.F32, ref.BF16])
+@pytest.mark.parametrize("M,N,K", [(6300, 5120, 144), (6301, 5120, 256), (4700, 5120, 144), (4711, 5100, 256), (6090, 4088, 16),
+                                   (6081, 4096, 128), (2022, 2048, 112), (751, 5120, 16), (4650, 2048, 384)])
+def test_gemm_large_and_short(dev, M, N, K, ct):
+    """Large tiles over one to three blocks of k, several tiles to a CU."""
+    run_gemm(dev, np.random.default_rng(M + K), M, N, K, ct)
