@@ -571,3 +571,26 @@ def test_select_prompts_of_many_blocks_with_ties(dev, act, blocks):
         p.check(n_sel, first, last)
     p.qbits[:] = 0
     p.check(40, 1, 1)
+
+
+@acts
+@pytest.mark.parametrize("blocks", [30, 600, 1100, 2100])
+@pytest.mark.parametrize("score", [-1.0, -2.0, 2.0 - 2.0 ** -24, "one"])
+def test_select_of_forced_blocks_alone(dev, act, blocks, score):
+    """Lists that the first and last blocks fill, on prompts and single rows, where the other blocks' scores have keys that end in
+    ones: no other block is listed, and nothing behind the lists is written."""
+    p = Pick(34, 4, 2, 64, 16, act, [21, 1, 9], [16 * blocks, 16 * blocks - 9, 16 * blocks - 40], tail_rows=5)
+    q = np.zeros((p.n_rows, 4, 64))
+    q[:, :, :2] = 0.5                                      # two heads: sums of 1
+    p.qbits = ref.to_bits(q.reshape(p.n_rows, -1).astype(np.float32), act)
+    m = np.zeros((p.c.n_pages, 2, 64))
+    if score == "one":
+        m[:, :, 0] = -7
+        m[p.table[0, 5]] = m[p.table[1, 5]] = m[p.table[2, 5]] = -0.5
+    elif score > 0:
+        m[:, :, 0], m[:, :, 1] = 2, -2.0 ** -24
+    else:
+        m[:, :, 0] = score
+    p.mean = ref.to_bits(m.astype(np.float32), act)
+    for n_sel, first, last in ((1, 0, 1), (3, 1, 2), (16, 4, 12), (20, 0, 20), (4, 1, 2)):
+        p.check(n_sel, first, last)

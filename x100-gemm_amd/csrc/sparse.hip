@@ -7,6 +7,7 @@
 #include <algorithm>
 
 #include "paged.h"
+#include "select_cut.h"
 #include "x100_internal.h"
 
 namespace {
@@ -160,16 +161,6 @@ __global__ __launch_bounds__(256) void k_kv_means(const x100_kv_cfg c, const x10
 }
 
 // ---- selection -----------------------------------------------------------------------------------
-
-// Keys are compared as unsigned numbers, in the order of the scores.  0: not to be selected; all ones: always.
-constexpr uint64_t KEY_NONE = 0, KEY_ALWAYS = ~0ull;
-X100_DEV uint64_t score_key(double s)
-{
-    if (!(s == s)) s = -__builtin_inf();
-    s += 0.0;   // -0 is 0
-    const uint64_t u = __builtin_bit_cast(uint64_t, s);
-    return u >> 63 ? ~u : u | 1ull << 63;
-}
 
 struct SelectArgs {
     x100_kv_cfg c;
@@ -366,11 +357,9 @@ template <int HD, int AT, int NT, int CAP, int U> __global__ __launch_bounds__(N
 typedef double v4d __attribute__((ext_vector_type(4)));
 constexpr int RT = 512;   // threads
 
-// The list of a row by one wave from the upper halves of its n keys, key i in lane i % 64: the threshold one bit at a time,
-// until as many keys are left as the list takes.  Counts are kept per lane and summed once per bit (a ballot and a scalar
-// count per key cost three times as much).  Where keys with the threshold's upper half are in the list and others are not
-// (their scores differ by less than 1e-6, one row in thousands, or are equal), low(i) gives the lower halves of
-// these keys, which take the places of the upper ones.  put(place, key's number, or -1).
+// The list of a row by one wave from the upper halves of its n keys, key i in lane i % 64 (select_cut.h).  Counts are kept per
+// lane and summed once per bit (a ballot and a scalar count per key cost three times as much).  low(i, upper) gives the lower
+// halves that are needed, which take the places of the upper ones.  put(place, key's number, or -1).
 template <int CAP, class Low, class Put> X100_DEV void select_row(uint32_t *key, int n, int n_sel, Low &&low, Put &&put)
 {
     constexpr int KL = CAP / 64;
@@ -384,68 +373,34 @@ template <int CAP, class Low, class Put> X100_DEV void select_row(uint32_t *key,
         for (int u = 0; u < KL; u++) c += kh[u] >= from ? 1 : 0;
         return wave_sum_u(c);
     };
-    uint32_t yh = 1, yl = 0;   // selected: keys > yh, and of those that are yh all (exact), or by their lower halves those > yl
-    bool exact = true;         // and the first `ties` that are yl
-    int ties = 0;
+    SelectCut cut = {1, 0, true, 0};
     if (n > n_sel) {
-        yh = 0;
-        exact = false;
-        // The upper 12 bits (a score's sign and exponent) lie at or little below those of the largest key that is not
-        // always taken: these few values first, instead of 12 bits.
-        int top = 31;
-        {
-            uint32_t mx = 0;
+        uint32_t mx = 0;
 #pragma unroll
-            for (int u = 0; u < KL; u++) mx = kh[u] != ~0u ? max(mx, kh[u]) : mx;
-            uint32_t from = ((uint32_t)wave_max_iu((int)(mx ^ 0x80000000u)) ^ 0x80000000u) & 0xfff00000u;
-            for (int k = 0; k < 4 && from; k++, from -= 0x00100000u) {
-                const int c = count(from);
-                exact = c == n_sel;
-                if (c >= n_sel) {
-                    yh = from;
-                    top = 19;
-                    break;
-                }
-            }
-        }
-        for (int bit = top; bit >= 0 && !exact; bit--) {
-            const uint32_t from = yh | 1u << bit;
-            const int c = count(from);
-            if (c >= n_sel) yh = from;
-            exact = c == n_sel;
-        }
-        if (yh == 0) {   // fewer blocks with a page than the list takes
-            yh = 1;
-            exact = true;
-        }
-        if (!exact) {   // a lower half is at least 1 here, 0: not one of these keys
-            const int need = n_sel - count(yh + 1);   // yh is not all ones: those keys are no more than n_sel
-            for (int i = lane; i < n; i += 64) key[i] = key[i] == yh ? max(low(i, yh), 1u) : 0;
-            auto count_low = [&](uint32_t from) __attribute__((always_inline)) {
+        for (int u = 0; u < KL; u++) mx = kh[u] != ~0u ? max(mx, kh[u]) : mx;
+        mx = (uint32_t)wave_max_iu((int)(mx ^ 0x80000000u)) ^ 0x80000000u;
+        cut = select_cut(
+            n, n_sel, mx, count,
+            [&](uint32_t upper) __attribute__((always_inline)) {   // a lower half is at least 1 here, 0: not one of these keys
+                for (int i = lane; i < n; i += 64) key[i] = key[i] == upper ? max(low(i, upper), 1u) : 0;
+            },
+            [&](uint32_t from) __attribute__((always_inline)) {
                 int c = 0;
                 for (int i = lane; i < n; i += 64) c += key[i] >= from ? 1 : 0;
                 return wave_sum_u(c);
-            };
-            int c = 0;
-            for (int bit = 31; bit >= 0 && c != need; bit--) {
-                const uint32_t from = yl | 1u << bit;
-                c = count_low(from);
-                if (c >= need) yl = from;
-            }
-            ties = c == need ? n : need - (yl == ~0u ? 0 : count_low(yl + 1));
-        }
+            });
     }
     int at_out = 0, eq = 0;
     const uint64_t below = (1ull << lane) - 1;
 #pragma unroll
     for (int u = 0; u < KL; u++) {
         if (u >= used) continue;
-        bool take = kh[u] >= yh;
-        if (!exact) {
+        bool take = kh[u] >= cut.upper;
+        if (!cut.exact) {
             const uint32_t l = 64 * u + lane < n ? key[64 * u + lane] : 0;
-            const bool tied = kh[u] == yh && l == yl;
+            const bool tied = cut.tied(kh[u], l);
             const uint64_t bq = __ballot(tied);
-            take = kh[u] > yh || (kh[u] == yh && l > yl) || (tied && eq + __popcll(bq & below) < ties);
+            take = cut.above(kh[u], l) || (tied && eq + __popcll(bq & below) < cut.ties);
             eq += __popcll(bq);
         }
         const uint64_t bt = __ballot(take);
