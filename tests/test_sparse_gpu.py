@@ -594,3 +594,33 @@ def test_select_of_forced_blocks_alone(dev, act, blocks, score):
     p.mean = ref.to_bits(m.astype(np.float32), act)
     for n_sel, first, last in ((1, 0, 1), (3, 1, 2), (16, 4, 12), (20, 0, 20), (4, 1, 2)):
         p.check(n_sel, first, last)
+
+
+@kinds
+@pytest.mark.parametrize("n_sel", [4, 70, 300, 512])
+def test_own_block_behind_a_list_s_end(dev, act, kv, n_sel):
+    """Entries behind a list's end that name the own block again, beside the end, 64 and 256 entries away and in every place: the
+    positions behind the row's own stay out.  They hold NaN, or keys of later rows."""
+    t = Setup(35, 4, 2, 64, 16, act, kv, [1] * 6 + [9], [150, 145, 159, 145, 9, 97, 157])
+    sel = np.full((t.n_rows, 2, n_sel), -1, np.int64)
+    for r, s, pos in rows_of(t):
+        own = pos // 16
+        for h in range(2):
+            sel[r, h, :2] = [0, own] if own and (r + h) % 4 else [own, -1]
+            end = 2 if own and (r + h) % 4 else 1
+            for at in {0: [end + 1], 1: range(end + 1, n_sel, 2), 2: [n_sel - 1], 3: range(end, n_sel), 4: [end + 63],
+                       5: [end + 255], 6: [end + 1, n_sel - 1]}[(r + 2 * h) % 7]:
+                sel[r, h, min(at, n_sel - 1)] = own
+    check(t, n_sel, sel)
+
+
+@kinds
+def test_a_list_repeated(dev, act, kv):
+    """Short lists repeated to fill n_sel end where they begin again; also of one block, the own one."""
+    t = Setup(36, 8, 2, 128, 32, act, kv, [1, 1, 6], [300, 70, 203])
+    sel = np.full((t.n_rows, 2, 12), -1, np.int64)
+    for r, s, pos in rows_of(t):
+        own = pos // 32
+        sel[r, 0] = ([own, 0, own] if r % 2 else [own, 1, 0]) * 4
+        sel[r, 1] = [0, own] * 6 if own else [0] * 12
+    check(t, 12, sel)

@@ -91,18 +91,18 @@ template <int HD, int AT, bool Q4, bool SP> __global__ __launch_bounds__(256, Q4
         const int *tab = a.b.block_table + (size_t)s * a.b.table_ld;
         // the list's pages, up to the first entry that breaks its order
         __shared__ int s_cnt[NW], s_own[NW];
-        int end = a.n_sel, own_at = -1;
+        int end = a.n_sel, own_at = a.n_sel;
 #pragma unroll
         for (int k = 0; k < LE; k++) {
             const int i = threadIdx.x + 64 * NW * k, e = entry[k];
             if (i >= a.n_sel) continue;
             const bool ok = e > before[k] && e >= 0 && e <= own;
             if (!ok) end = min(end, i);
-            if (ok && e == own) own_at = i;
+            if (ok && e == own) own_at = min(own_at, i);
             sh.pg[i] = ok ? valid(tab[e]) : -1;
         }
         end = -wave_max_iu(-end);
-        own_at = wave_max_iu(own_at);
+        own_at = -wave_max_iu(-own_at);
         if (lane == 0) {
             s_cnt[w] = end;
             s_own[w] = own_at;
@@ -112,8 +112,8 @@ template <int HD, int AT, bool Q4, bool SP> __global__ __launch_bounds__(256, Q4
         for (int k = 0; k < NW; k++) end = min(end, s_cnt[k]);
         vis = end * page;
 #pragma unroll
-        for (int k = 0; k < NW; k++)   // only the last entry can be the own block: an entry is above all before it
-            if (s_own[k] >= 0 && s_own[k] == end - 1) vis = end * page - (page - 1 - (at & (page - 1)));
+        for (int k = 0; k < NW; k++)   // entries ascend up to the end, so only the last one, and a wave's first such, can be the own block
+            if (s_own[k] == end - 1) vis = end * page - (page - 1 - (at & (page - 1)));
         kv_len = vis;
         pos0 = vis - 1;
         per = a.tile.positions(a.n_sel << psh);
