@@ -83,14 +83,14 @@ template <int CT> X100_DEV void store_c4(const Fp8Args &g, int m, int n, v4f v)
         }
 }
 
-// Few rows (M <= 16): bound by W's bytes.  A wave has 16 FN columns and takes every WK-th block of k; the WK waves of its columns
-// are summed through LDS.  Operands go from memory to registers, U blocks of k at a time, W's as it streams by and A's
-// out of the caches, once for FN of W's.
-template <int FN, int WK, int WN, int U, int CT> __global__ __launch_bounds__(64 * WK *WN) void k_fp8_rows(const Fp8Args g)
+// Few rows (M <= 16): bound by W's bytes.  A block's WK waves have the same 16 FN columns, each takes every WK-th block of k, and
+// they are summed through LDS.  Operands go from memory to registers, W's as it streams by and A's out of the caches, once for
+// FN of W's.
+template <int FN, int WK, int CT> __global__ __launch_bounds__(64 * WK) void k_fp8_rows(const Fp8Args g)
 {
-    __shared__ v4f part[WK > 1 ? (WK - 1) * WN * FN * 64 : 1];
-    const int lane = threadIdx.x & 63, w = wave_id(), wk = w % WK, wn = w / WK, r = lane & 15, q = lane >> 4;
-    const int n0 = (blockIdx.x * WN + wn) * 16 * FN, m = min(r, g.M - 1);
+    __shared__ v4f part[(WK - 1) * FN * 64];
+    const int lane = threadIdx.x & 63, wk = wave_id(), r = lane & 15, q = lane >> 4;
+    const int n0 = blockIdx.x * 16 * FN, m = min(r, g.M - 1);
     const int nb = (g.K + 127) >> 7, full = g.K >> 7;
     const uint8_t *ap = g.a + (size_t)m * g.lda + 16 * q, *wp[FN];
     const float *sa = g.as + m, *sw[FN];
@@ -103,44 +103,39 @@ template <int FN, int WK, int WN, int U, int CT> __global__ __launch_bounds__(64
 #pragma unroll
     for (int j = 0; j < FN; j++) acc[j] = v4f{0, 0, 0, 0};
 
-    v4i wf[U][FN][2], af[U][2];
-    float s[U], t[U][FN];
-    auto load = [&](int u, int b) __attribute__((always_inline)) {
+    v4i wf[FN][2], af[2];
+    float s, t[FN];
+    auto scales = [&](int b) __attribute__((always_inline)) {
+        s = sa[b * g.ld_as];
 #pragma unroll
-        for (int j = 0; j < FN; j++) {
-            wf[u][j][0] = *(const v4i *)(wp[j] + 128 * (size_t)b);
-            wf[u][j][1] = *(const v4i *)(wp[j] + 128 * (size_t)b + 64);
-            t[u][j] = sw[j][b];
-        }
-        af[u][0] = *(const v4i *)(ap + 128 * (size_t)b);
-        af[u][1] = *(const v4i *)(ap + 128 * (size_t)b + 64);
-        s[u] = sa[b * g.ld_as];
+        for (int j = 0; j < FN; j++) t[j] = sw[j][b];
     };
-    auto add = [&](int u) __attribute__((always_inline)) {
+    auto add = [&]() __attribute__((always_inline)) {
         Frag<true> x;
-        x.set(0, af[u][0]);
-        x.set(1, af[u][1]);
+        x.set(0, af[0]);
+        x.set(1, af[1]);
 #pragma unroll
         for (int j = 0; j < FN; j++) {
             Frag<true> y;
-            y.set(0, wf[u][j][0]);
-            y.set(1, wf[u][j][1]);
+            y.set(0, wf[j][0]);
+            y.set(1, wf[j][1]);
             const v4f d = Frag<true>::mul(y, x);
-            const float f = s[u] * t[u][j];
+            const float f = s * t[j];
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[j][e] = __builtin_fmaf(d[e], f, acc[j][e]);
         }
     };
     int b = wk;
-    for (; b + (U - 1) * WK < full; b += U * WK) {
-#pragma unroll
-        for (int u = 0; u < U; u++) load(u, b + u * WK);
-#pragma unroll
-        for (int u = 0; u < U; u++) add(u);
-    }
     for (; b < full; b += WK) {
-        load(0, b);
-        add(0);
+#pragma unroll
+        for (int j = 0; j < FN; j++) {
+            wf[j][0] = *(const v4i *)(wp[j] + 128 * (size_t)b);
+            wf[j][1] = *(const v4i *)(wp[j] + 128 * (size_t)b + 64);
+        }
+        af[0] = *(const v4i *)(ap + 128 * (size_t)b);
+        af[1] = *(const v4i *)(ap + 128 * (size_t)b + 64);
+        scales(b);
+        add();
     }
     if (b < nb) {   // the short block
         const int left = g.K - 128 * b;
@@ -148,27 +143,23 @@ template <int FN, int WK, int WN, int U, int CT> __global__ __launch_bounds__(64
         for (int h = 0; h < 2; h++) {
             const int k = 16 * q + 64 * h, at = min(k, left - 16) - 16 * q;
             const v4i x = *(const v4i *)(ap + 128 * (size_t)b + at);
-            af[0][h] = k < left ? x : v4i{0, 0, 0, 0};
+            af[h] = k < left ? x : v4i{0, 0, 0, 0};
 #pragma unroll
-            for (int j = 0; j < FN; j++) wf[0][j][h] = *(const v4i *)(wp[j] + 128 * (size_t)b + at);
+            for (int j = 0; j < FN; j++) wf[j][h] = *(const v4i *)(wp[j] + 128 * (size_t)b + at);
         }
-        s[0] = sa[b * g.ld_as];
-#pragma unroll
-        for (int j = 0; j < FN; j++) t[0][j] = sw[j][b];
-        add(0);
+        scales(b);
+        add();
     }
-    if constexpr (WK > 1) {
-        if (wk > 0) {
+    if (wk > 0) {
 #pragma unroll
-            for (int j = 0; j < FN; j++) part[(((wk - 1) * WN + wn) * FN + j) * 64 + lane] = acc[j];
-        }
-        __syncthreads();
-        if (wk > 0) return;
-#pragma unroll
-        for (int k = 0; k < WK - 1; k++)
-#pragma unroll
-            for (int j = 0; j < FN; j++) acc[j] += part[((k * WN + wn) * FN + j) * 64 + lane];
+        for (int j = 0; j < FN; j++) part[((wk - 1) * FN + j) * 64 + lane] = acc[j];
     }
+    __syncthreads();
+    if (wk > 0) return;
+#pragma unroll
+    for (int k = 0; k < WK - 1; k++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[j] += part[(k * FN + j) * 64 + lane];
 #pragma unroll
     for (int j = 0; j < FN; j++) {
         const int n = n0 + 16 * j + 4 * q;
@@ -479,9 +470,9 @@ template <int FM, int FN, int WM, int WN, int WK, int NS, bool EXACT, int CT> hi
     return hipGetLastError();
 }
 
-template <int FN, int WK, int WN, int U, int CT> hipError_t few_rows(const Fp8Args &g, hipStream_t s)
+template <int FN, int CT> hipError_t few_rows(const Fp8Args &g, hipStream_t s)
 {
-    k_fp8_rows<FN, WK, WN, U, CT><<<(g.N + 16 * FN * WN - 1) / (16 * FN * WN), 64 * WK * WN, 0, s>>>(g);
+    k_fp8_rows<FN, 8, CT><<<(g.N + 16 * FN - 1) / (16 * FN), 64 * 8, 0, s>>>(g);
     return hipGetLastError();
 }
 
@@ -530,7 +521,7 @@ template <int CT> hipError_t gemm(const Fp8Args &g, hipStream_t s)
     constexpr bool EXACT = CT == X100_T_F32;
     // Two 16-column tiles of W per wave halve A's reads, where there are waves enough for it (us with one / two: 8 x 151936 x
     // 2048 62 / 55, 8 x 5120 x 2048 5.2 / 5.0, 16 x 2048 x 4096 5.9 / 7.8) and rows to read (1 x 151936 x 2048: 49 / 55).
-    if (g.M <= 16) return g.M > 4 && g.N >= 8192 ? few_rows<2, 8, 1, 1, CT>(g, s) : few_rows<1, 8, 1, 1, CT>(g, s);
+    if (g.M <= 16) return g.M > 4 && g.N >= 8192 ? few_rows<2, CT>(g, s) : few_rows<1, CT>(g, s);
     switch (best_tile(g, EXACT)) {
     case T32X32: return tile<2, 1, 1, 2, 4, 4, EXACT, CT>(g, s);
     case T64X32: return tile<2, 2, 2, 1, 4, 3, EXACT, CT>(g, s);
