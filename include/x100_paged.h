@@ -114,6 +114,8 @@ int x100_kv_read_hip(const x100_kv_cfg *cfg, const x100_kv_batch *batch, const v
  * reads KV head h / (n_head / n_head_kv).  Scores, softmax and sums in fp32, the weights divided by
  * their sum at the end (so bf16 V up to 2^100 in size); for the product with V they are rounded to 16
  * bits (act_type, or fp16 for 4-bit pages), and in fp16 a weight below 2^-29 of the largest is zero.
+ * bf16 queries meet 4-bit pages as fp16 times a power of two per row: exact for elements down to 2^-17 of
+ * the row's largest, others off by 2^-25 of it at most.
  * A row that attends to nothing (no position, no valid page, or every score -inf) gives zeros; one
  * with a score that is NaN gives NaN.  Infinities and NaN in positions that a row does not attend to
  * do not reach it.

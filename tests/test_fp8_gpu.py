@@ -305,3 +305,21 @@ def test_a_large_product_captured(dev):
 def test_gemm_large_and_short(dev, M, N, K, ct):
     """Large tiles over one to three blocks of k, several tiles to a CU."""
     run_gemm(dev, np.random.default_rng(M + K), M, N, K, ct)
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 200, 272), (40, 200, 272), (400, 300, 272)])
+@pytest.mark.parametrize("ea,ew", [(-63, -62), (100, -100), (-110, 90), (60, 40), (-70, -66)])
+def test_gemm_scales_of_any_size(dev, M, N, K, ea, ew):
+    """Scales far from 1 whose product is a number of fp32, down to its subnormal ones."""
+    g = np.random.default_rng(M)
+    a, da, _, w, dw, _ = operands(g, M, N, K)
+    sa = np.full((fr.blocks(K), M), 2.0 ** ea, np.float32)
+    sw = np.full((fr.blocks(N), fr.blocks(K)), 2.0 ** ew, np.float32)
+    dsa, dsw = torch.from_numpy(sa).cuda(), torch.from_numpy(sw).cuda()
+    c = torch.zeros(M, N, device=dev)
+    x.gemm_fp8(M, N, K, x.Fp8(da.data_ptr(), K, dsa.data_ptr(), M), x.Fp8(dw.data_ptr(), K, dsw.data_ptr(), sw.shape[1]),
+               x.T_F32, c.data_ptr(), N, stream())
+    want, size = fr.product(a, sa, w, sw)
+    # an addition per block may end among fp32's subnormal numbers: a step of these each
+    bound = fr.product_bound(K, want, size, ref.F32) + fr.blocks(K) * 2.0 ** -149
+    assert (np.abs(c.double().cpu().numpy() - want) <= bound).all()
